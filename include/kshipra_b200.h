@@ -48,6 +48,8 @@ extern "C" {
 #define KSH_FLAG_BAD_TOKEN    16   /* token id outside [0, vocab) */
 #define KSH_FLAG_BAD_LENGTH   32   /* sequence longer than its block table */
 #define KSH_FLAG_TIMEOUT      64   /* a bounded device wait gave up */
+#define KSH_FLAG_BAD_PARENT  128   /* drafted node whose parent is not an earlier node */
+#define KSH_FLAG_BAD_PROBS   256   /* probability row without mass */
 
 int ksh_abi_version(void);
 const char* ksh_status_string(int status);
@@ -325,6 +327,96 @@ int64_t ksh_peer_allreduce_epoch_words(void);
 int ksh_peer_allreduce_f32(const uint64_t* peer_buffers, int rank, int world, int64_t n,
                            int64_t n_max, int parity, float* out, uint32_t* epochs,
                            int32_t* flags, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Speculative decoding over the block pool (the reference's
+ * engine/speculative.py drafts and verifies on a mock model only; these
+ * serve KshipraModel).  A sequence of a batch brings n drafted nodes: node 0
+ * is the token emitted last (the root, not yet in the cache), the others are
+ * drafted continuations, each with an earlier node as its parent.  Rows of a
+ * batch lie one sequence after the other (q_start); a node's K/V stands in
+ * the slot of position prefix + (its index).  At most 256 nodes a sequence.
+ * ---------------------------------------------------------------------- */
+
+/* Tables of a batch from request lengths, all on the device (replaces the
+ * host lists of generate, engine/model.py:154-205).  Sequence s holds
+ * prefix_lens[s] cached positions and brings new_lens[s] rows; block_ids
+ * [num_block_ids] holds every sequence's blocks one after the other, sequence
+ * s's at block_start[s] .. block_start[s + 1] (both NULL: block_tables is an
+ * input).  parents [total] (own sequence's node index, negative: a root) or
+ * NULL for plain chunks.  Writes q_start [S + 1], block_tables [S,
+ * max_blocks] (padded with 0), positions [total] (prefix + depth in the tree;
+ * without parents prefix + index), slots [total] and, with parents, mask
+ * [total, mask_words]: bit j of a row's 64-bit words is set where node j is
+ * an ancestor or the node itself.  total is the host's sum of new_lens; rows
+ * that the lengths do not cover get position 0, slot -1 and no mask bits,
+ * and raise KSH_FLAG_BAD_LENGTH, as does a sequence longer than its blocks.
+ * A parent that is no earlier node raises KSH_FLAG_BAD_PARENT and counts as
+ * a root.  mask_words <= 4. */
+int ksh_tree_tables(const int32_t* prefix_lens, const int32_t* new_lens, int64_t num_seqs,
+                    int64_t total, int64_t block_size, const int32_t* block_ids,
+                    int64_t num_block_ids, const int32_t* block_start, int64_t max_blocks,
+                    const int32_t* parents, int64_t mask_words, int32_t* q_start,
+                    int32_t* block_tables, int64_t* positions, int64_t* slots, uint64_t* mask,
+                    int32_t* flags, void* stream);
+
+/* Attention of the drafted nodes (chunked_attention, engine/chunked_prefill.py:
+ * 93-140, with the causal order replaced by the tree's).  q [total, hq, d];
+ * pool, block_tables and layer as for ksh_paged_attention.  Node i attends
+ * every cached position and the nodes of its mask row (mask NULL: nodes
+ * 0 .. i); one that may see no key gives zeros, and what a node may not see
+ * does not reach its sums, NaN and infinity included.  max_nodes and
+ * max_total_len are host-side upper bounds.  The workspace, of
+ * ksh_tree_attention_workspace_size bytes and 256-byte aligned, needs no
+ * initialisation.  d <= 256. */
+int64_t ksh_tree_attention_workspace_size(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d,
+                                          int64_t max_nodes);
+int ksh_tree_attention(const float* q, int64_t total, int64_t hq, int64_t d, const float* pool,
+                       int64_t num_blocks, int64_t num_layers, int64_t layer, int64_t hkv,
+                       int64_t block_size, const int32_t* block_tables, int64_t max_blocks,
+                       const int32_t* q_start, const int32_t* prefix_lens, int64_t num_seqs,
+                       const uint64_t* mask, int64_t mask_words, int64_t max_nodes,
+                       int64_t max_total_len, float* out, void* workspace,
+                       int64_t workspace_bytes, int32_t* flags, void* stream);
+
+/* Probabilities of m rows of logits at a temperature per row (NULL: 1):
+ * p = exp((x - max) / T) / sum; T <= 0 puts one at the first maximum.  Rows
+ * logits_stride / probs_stride floats apart; probs may be logits. */
+int ksh_target_probs(const float* logits, int64_t m, int64_t vocab, int64_t logits_stride,
+                     const float* temperature, float* probs, int64_t probs_stride, void* stream);
+
+/* Drafted tokens against the target's distribution (the accept / residual
+ * resampling rule of engine/speculative.py, on trees).  Row q_start[s] + i of
+ * target_probs is the target's distribution after node i, the same row of
+ * draft_probs the one that node i's children were drawn from.  From the root
+ * on, with r = P_root and Z = 1, child i of the current node (in node order)
+ * is accepted iff u_accept[i] * Z * Q(token) < r(token); then it becomes the
+ * current node with r = P_i, Z = 1.  Otherwise r = max(r - Z * Q, 0), Z =
+ * sum r.  draft_probs NULL: the children are fixed proposals, Q(token) = 1
+ * and a refused token's r becomes 0.  next is the first t with cumsum(r)[t] >
+ * u_sample * sum r (r = P of the node where nothing is left).  With
+ * target_tokens [total] (the target's greedy token after each node) instead
+ * of target_probs, a child is accepted iff it is that token, and next is the
+ * last node's.  path [S, max_nodes]: the accepted nodes from the root on,
+ * padded with -1; path_len [S] counts them (the root included; 0 and next -1
+ * for a sequence without nodes).  Random numbers are in [0, 1).  Sums are
+ * held in 64 bits. */
+int ksh_verify_tree(const int64_t* tokens, const int32_t* parents, const int32_t* q_start,
+                    int64_t num_seqs, int64_t total, int64_t max_nodes, int64_t vocab,
+                    const float* target_probs, int64_t target_stride, const float* draft_probs,
+                    int64_t draft_stride, const int64_t* target_tokens, const float* u_accept,
+                    const float* u_sample, int32_t* path, int32_t* path_len,
+                    int64_t* next_tokens, int32_t* flags, void* stream);
+
+/* Moves the accepted nodes' K/V of every layer to consecutive positions: for
+ * j < path_len[s], position prefix + path[j] goes to prefix + j.  A path rises
+ * (an entry that does not stays where it is and raises KSH_FLAG_BAD_LENGTH).
+ * new_lens [S] (NULL: not wanted) gets prefix + path_len. */
+int ksh_tree_commit(float* pool, int64_t num_blocks, int64_t num_layers, int64_t hkv,
+                    int64_t block_size, int64_t d, const int32_t* block_tables,
+                    int64_t max_blocks, const int32_t* prefix_lens, int64_t num_seqs,
+                    const int32_t* path, int64_t path_stride, const int32_t* path_len,
+                    int32_t* new_lens, int32_t* flags, void* stream);
 
 /* ------------------------------------------------------------------------
  * Failure-path check of the device waits (no counterpart in the reference;

@@ -39,6 +39,7 @@ from ._lib import call, ptr, stream_ptr
 from .chunked_prefill import AttentionWorkspace, paged_attention
 from .config import ModelConfig
 from .prefix_cache import BlockAllocator
+from .speculative import tree_attention
 from .tensor_parallel import (down_col_range, gate_up_row_ranges, merge_argmax, o_col_range,
                               qkv_row_ranges, take_cols, take_rows, tp_shape)
 from .quantization import (QuantizedLinear, QuantizedWeight, Workspace, linear_launch,
@@ -46,7 +47,9 @@ from .quantization import (QuantizedLinear, QuantizedWeight, Workspace, linear_l
 
 FLAG_NAMES = {1: "non-finite weight", 2: "block id out of range", 4: "slot out of range",
               8: "position outside the RoPE table", 16: "token id out of range",
-              32: "sequence longer than its block table", 64: "a bounded device wait gave up"}
+              32: "sequence longer than its block table", 64: "a bounded device wait gave up",
+              128: "drafted node whose parent is not an earlier node",
+              256: "probability row without mass"}
 FLAG_TIMEOUT = 64
 LM_GEMV_ROWS = 16            # lm_head rows served by the fp32 GEMV; more go to tensor cores
 PEER_AR_ROWS = 256           # token rows of a row-parallel sum done over peer memory
@@ -297,7 +300,9 @@ class KshipraModel:
 
     def _run_layers(self, acts, ids, positions, slots, block_tables, q_start, prefix_lens,
                     num_seqs: int, max_q_len: int, max_total_len: int, pool: torch.Tensor,
-                    lin_ws: Workspace, attn_ws: AttentionWorkspace) -> torch.Tensor:
+                    lin_ws: Workspace, attn_ws: AttentionWorkspace, tree=None) -> torch.Tensor:
+        """``tree``: (ancestor mask, TreeWorkspace) of drafted trees, whose nodes
+        attend their ancestors instead of every earlier row of the pass."""
         T = ids.shape[0]
         s = stream_ptr()
         hid, xn, qkv, q, attn, h = (acts[k] for k in ("hidden", "xn", "qkv", "q", "attn", "h"))
@@ -310,7 +315,8 @@ class KshipraModel:
         eps = self.eps
         # decode step (one token per sequence, position == prefix length): the
         # fused RoPE + K/V write + attention kernel
-        fused = (max_q_len == 1 and T == num_seqs and self.fused_decode and bs % 16 == 0
+        fused = (tree is None and max_q_len == 1 and T == num_seqs and self.fused_decode
+                 and bs % 16 == 0
                  and d in (64, 128) and self.n_heads // self.n_kv_heads in _DECODE_GROUPS[d])
         if fused:   # key-split partial states (zeroed once; the kernels leave the counters at 0)
             dec_ws = attn_ws.decode(int(_lib.lib().ksh_decode_attention_workspace_size(
@@ -327,8 +333,12 @@ class KshipraModel:
                 call("ksh_rope_kv_write", ptr(qkv), T, self.n_heads, self.n_kv_heads,
                      self.head_dim, ptr(positions), ptr(slots), ptr(rc), ptr(rs), rc.shape[0],
                      ptr(q), ptr(pool), nb, L, i, bs, ptr(self.flags), s)
-                paged_attention(q, pool, i, block_tables, q_start, prefix_lens, max_q_len,
-                                max_total_len, attn, self.flags, ws=attn_ws)
+                if tree is None:
+                    paged_attention(q, pool, i, block_tables, q_start, prefix_lens, max_q_len,
+                                    max_total_len, attn, self.flags, ws=attn_ws)
+                else:
+                    tree_attention(q, pool, i, block_tables, q_start, prefix_lens, tree[0],
+                                   max_q_len, max_total_len, attn, self.flags, ws=tree[1])
             self._row_parallel(attn.view(T, -1), Ly.o, hid, lin_ws)
             swiglu_launch(hid, Ly.gate_up.qw, Ly.gate_up.w, self.inter, h, ws=lin_ws,
                           norm_w=Ly.ln2, eps=eps)

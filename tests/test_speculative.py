@@ -1,0 +1,89 @@
+"""Host side of speculative decoding: drafts, argument errors of the C entries
+(detected before any launch) and workspace sizes."""
+
+import pytest
+
+from kshipra_b200 import _lib
+from kshipra_b200.speculative import PromptLookup
+
+FAKE = 256          # never dereferenced: the arguments are checked before any launch
+
+
+def walk(tokens, parents, node):
+    out = []
+    while node > 0:
+        out.append(tokens[node])
+        node = parents[node]
+    return out[::-1]
+
+
+def test_prompt_lookup_merges_continuations():
+    toks, par = PromptLookup(ngram=2, depth=3, branches=3, max_nodes=8).propose(
+        [1, 2, 9, 8, 1, 2, 9, 7, 1, 2])
+    assert toks[0] == 2 and par[0] == -1
+    assert all(0 <= p < i for i, p in enumerate(par) if i)
+    paths = {tuple(walk(toks, par, i)) for i in range(1, len(toks))}
+    assert {(9, 7, 1), (9, 8, 1)} <= paths
+    # no child of a node twice
+    assert len({(p, t) for p, t in zip(par, toks)}) == len(toks)
+
+
+def test_prompt_lookup_limits():
+    assert PromptLookup().propose([4]) == ([4], [-1])
+    assert PromptLookup().propose([1, 2, 3]) == ([3], [-1])
+    toks, par = PromptLookup(ngram=1, depth=50, branches=50, max_nodes=5).propose([7] * 40)
+    assert len(toks) == 5 and par == [-1, 0, 1, 2, 3]
+    for bad in (dict(ngram=0), dict(max_nodes=0), dict(max_nodes=257), dict(depth=-1)):
+        with pytest.raises(ValueError):
+            PromptLookup(**bad)
+
+
+def test_workspace_size_needs_no_device():
+    h = _lib.lib()
+    assert h.ksh_tree_attention_workspace_size(64, 32, 8, 128, 16) > 0
+    assert h.ksh_tree_attention_workspace_size(1, 3, 2, 64, 4) == 0        # bad GQA ratio
+    assert h.ksh_tree_attention_workspace_size(0, 4, 2, 64, 4) == 0
+
+
+def attention(h, **kw):
+    a = dict(q=FAKE, total=4, hq=4, d=64, pool=FAKE, nb=4, layers=1, layer=0, hkv=2, bs=16, bt=FAKE,
+             maxb=2, qs=FAKE, pre=FAKE, seqs=1, mask=FAKE, words=1, nodes=4, tot=20, out=FAKE, ws=FAKE,
+             wsb=1 << 30, flags=None)
+    a.update(kw)
+    return h.ksh_tree_attention(*a.values(), None)
+
+
+def test_argument_errors_are_reported_without_a_launch():
+    h = _lib.lib()
+    for kw, st in ((dict(hq=5), -1), (dict(layer=1), -1), (dict(bs=0), -1), (dict(q=None), -1),
+                   (dict(mask=FAKE, words=0), -1), (dict(d=257), -4), (dict(nodes=257), -4),
+                   (dict(words=5), -4), (dict(total=-1), -1)):
+        assert attention(h, **kw) == st, kw
+    # nothing to do is no error
+    for kw in (dict(seqs=0), dict(total=0), dict(nodes=0)):
+        assert attention(h, **kw) == 0
+
+    def tables(seqs=1, total=4, bs=16, ids=FAKE, start=FAKE, maxb=2, par=FAKE, words=1, qs=FAKE,
+               bt=FAKE, pos=FAKE, mask=FAKE):
+        return h.ksh_tree_tables(FAKE, FAKE, seqs, total, bs, ids, 2, start, maxb, par, words, qs, bt,
+                                 pos, FAKE, mask, None, None)
+    for kw, st in ((dict(seqs=0), -1), (dict(bs=0), -1), (dict(start=None), -1), (dict(maxb=0), -1),
+                   (dict(words=5), -4), (dict(words=0), -1), (dict(mask=None), -1), (dict(pos=None), -1),
+                   (dict(qs=None), -1)):
+        assert tables(**kw) == st, kw
+
+    def verify(seqs=1, nodes=4, vocab=10, tp=FAKE, ts=10, dp=None, ds=10, tt=None, u=FAKE, path=FAKE):
+        return h.ksh_verify_tree(FAKE, FAKE, FAKE, seqs, 4, nodes, vocab, tp, ts, dp, ds, tt, u, FAKE,
+                                 path, FAKE, FAKE, None, None)
+    for kw, st in ((dict(seqs=0), -1), (dict(nodes=0), -1), (dict(nodes=257), -4), (dict(vocab=0), -1),
+                   (dict(ts=9), -1), (dict(tp=None), -1), (dict(tt=FAKE), -1), (dict(u=None), -1),
+                   (dict(dp=FAKE, ds=9), -1), (dict(tp=None, tt=FAKE, dp=FAKE), -1), (dict(path=None), -1)):
+        assert verify(**kw) == st, kw
+
+    assert h.ksh_target_probs(FAKE, 2, 10, 9, None, FAKE, 10, None) == -1
+    assert h.ksh_target_probs(FAKE, 2, 0, 9, None, FAKE, 10, None) == -1
+    assert h.ksh_target_probs(None, 2, 10, 10, None, FAKE, 10, None) == -1
+    assert h.ksh_target_probs(None, 0, 10, 10, None, None, 10, None) == 0
+    assert h.ksh_tree_commit(FAKE, 4, 1, 2, 16, 64, FAKE, 2, FAKE, 0, FAKE, 4, FAKE, None, None, None) == -1
+    assert h.ksh_tree_commit(FAKE, 4, 1, 2, 16, 64, FAKE, 2, FAKE, 1, FAKE, 0, FAKE, None, None, None) == -1
+    assert h.ksh_tree_commit(None, 4, 1, 2, 16, 64, FAKE, 2, FAKE, 1, FAKE, 4, FAKE, None, None, None) == -1
