@@ -23,14 +23,22 @@
 // uneven lengths leave no SM idle; an item cut between CTAs leaves its
 // (m, l, acc) pieces in the workspace and tree_merge_kernel joins them in key
 // order (the same bits in every run).  Warps of a CTA:
-//   0..3   rows: thread = query row.  Scores from TMEM, running softmax in
-//          32 bits, P split into hi / lo back into TMEM (over the scores), and
-//          every tile's P V added into fp32 registers (adding a long context
-//          up inside the tensor core would round toward zero at each step)
-//   4..11  K/V: global -> registers (one tile ahead) -> scaled hi / lo fp16 in
-//          shared memory, 128-byte swizzle; block table per key, any block size
-//   12     MMAs: S = Q K^T (A = Q in TMEM, B = K), O = P V (A = P in TMEM, B =
-//          V with the keys along K, so no transpose is stored)
+//   17      block table lookups and bulk copies of K / V rows into raw
+//           shared-memory slots: a copy per eight keys where they stand one
+//           after the other, else one per key (any block size)
+//   8..15   widening: raw rows -> scaled hi / lo fp16 tiles, 128-byte swizzle
+//   16      MMAs: S = Q K^T (A = Q in TMEM, B = K), O = P V (A = P in TMEM,
+//           B = V with the keys along K, so no transpose is stored)
+//   0..7    rows: thread = query row, and half of the tile's keys and of D.
+//           Scores from TMEM, running softmax in 32 bits, P as hi / lo into
+//           TMEM, and every tile's P V added into fp32 registers (a long
+//           context added up inside the tensor core would lose low bits at
+//           each step).  Both halves take the whole row's maximum, so neither
+//           waits for the other.
+// Registers decide the split: 128 x 128 accumulators are a quarter of the
+// file, so K / V in flight stay in shared memory and the code of each role is
+// kept short (an earlier form with the copies in registers spilled and missed
+// the instruction cache).
 
 #include <math.h>
 
@@ -73,9 +81,11 @@ struct SplitItem {
 
 constexpr int kTK = 64;                  // keys per tile
 constexpr int kRows = 128;               // query rows per tile (MMA M)
-constexpr int kRowWarps = 4, kLoadWarps = 8;
-constexpr int kTcThreads = 512;          // rows 128, loaders 256, MMA warp + 3 idle
-constexpr int kKeysPerWarp = kTK / kLoadWarps;
+constexpr int kRowWarps = 8, kWideWarps = 8;
+constexpr int kMmaWarp = kRowWarps + kWideWarps, kCopyWarp = kMmaWarp + 1;
+constexpr int kTcThreads = 32 * (kRowWarps + kWideWarps + 4);   // two idle warps fill the last warpgroup
+constexpr int kGroup = kTK / kWideWarps; // keys per widening warp, one scale for them
+constexpr int kMeta = 16;                // tiles whose scales are kept: more than the stages let run apart
 
 // floats of one partial state: m [128], l [128], acc [D / 4][128][4]
 template <int D>
@@ -83,22 +93,26 @@ constexpr int64_t part_floats() { return 2 * kRows + static_cast<int64_t>(D) * k
 
 template <int D>
 struct TreeLayout {
-  static constexpr int TERM = kTK * D * 2;           // one fp16 term of a K or V tile
-  static constexpr int HALF = kTK * 128;             // 64 columns of it: 128-byte rows
-  static constexpr int NST = D == 128 ? 3 : 6;       // stages of K and of V
-  static constexpr int K_OFF = 0;
-  static constexpr int V_OFF = NST * 2 * TERM;
-  static constexpr int META = 2 * V_OFF;             // kinv, vinv [NST][64]
-  static constexpr int BITS = META + 2 * NST * kTK * 4;    // valid, kpois, vpois [NST][8] bytes
-  static constexpr int BAR = BITS + 3 * NST * 8;
-  static constexpr int NBAR = 4 * NST + 2 * 3 + 2;
+  static constexpr int RAW = kTK * D * 4;            // raw K (or V) rows of a tile
+  static constexpr int TERM = kTK * D * 2;           // one fp16 term of them
+  static constexpr int HALF = kTK * 128;             // 64 columns of a term: 128-byte rows
+  static constexpr int NRAW = D == 128 ? 1 : 2;      // raw slots of K and of V
+  static constexpr int NST = D == 128 ? 2 : 4;       // widened stages of K and of V
+  static constexpr int RK_OFF = 0, RV_OFF = NRAW * RAW;
+  static constexpr int K_OFF = 2 * RV_OFF, V_OFF = K_OFF + NST * 2 * TERM;
+  // per tile (ring of kMeta): inverse scales of K and V per group of eight
+  // keys, and per key relative to that (tiles with drafted nodes)
+  static constexpr int META = V_OFF + NST * 2 * TERM;    // kinv, vinv [8], krel, vrel [64]
+  static constexpr int BITS = META + 2 * kMeta * (kWideWarps + kTK) * 4;   // valid, kpois, vpois, tree [8]
+  static constexpr int BAR = BITS + 4 * kMeta * 8;
+  static constexpr int NBAR = 4 * NRAW + 4 * NST + 2 * 2 + 5;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int BYTES = MISC + 64 + 1024;
-  // TMEM columns: Q hi, Q lo (D / 2 each), two S / P buffers, two O buffers
-  static constexpr uint32_t Q_COL = 0, S_COL = D, O_COL = D + 2 * kTK;
+  // TMEM columns: Q hi, Q lo (D / 2 each), two S, two P buffers, O
+  static constexpr uint32_t Q_COL = 0, S_COL = D, P_COL = D + 2 * kTK, O_COL = D + 4 * kTK;
   static constexpr uint32_t COLS = 512;
-  static_assert(O_COL + 2 * D <= COLS, "TMEM columns");
-  static_assert(BYTES <= 227 * 1024, "shared memory");
+  static_assert(O_COL + D <= COLS, "TMEM columns");
+  static_assert(BYTES <= 220 * 1024, "shared memory");
 };
 
 // One sequence's share of the work.
@@ -148,8 +162,9 @@ __device__ __forceinline__ bool next_piece(const TreeArgs& a, Walk* wk, Piece* p
     k.base += w.units(a.hkv);
     w = seq_work(a, ++k.s);
   }
-  const int item = static_cast<int>((k.u - k.base) / w.ntiles);
-  p->t0 = static_cast<int>((k.u - k.base) - static_cast<int64_t>(item) * w.ntiles);
+  const uint32_t rel = static_cast<uint32_t>(k.u - k.base);    // a sequence's tiles fit 32 bits
+  const int item = static_cast<int>(rel / static_cast<uint32_t>(w.ntiles));
+  p->t0 = static_cast<int>(rel - static_cast<uint32_t>(item) * w.ntiles);
   p->t1 = static_cast<int>(min(static_cast<int64_t>(w.ntiles), p->t0 + (k.u_end - k.u)));
   p->hk = item / w.nqt;
   p->qt = item - p->hk * w.nqt;
@@ -166,28 +181,105 @@ __device__ __forceinline__ bool next_piece(const TreeArgs& a, Walk* wk, Piece* p
   return true;
 }
 
-__device__ __forceinline__ float4 ld_stream(const float* p) {
-  float4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "l"(p));
-  return v;
+// Global -> shared copy, 16-byte aligned, completing on an mbarrier.
+__device__ __forceinline__ void copy_bulk(void* dst, const float* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-// Power of two that brings a row whose largest |x| has these bits into
-// [2^14, 2^15), and its inverse.
-__device__ __forceinline__ void row_scale(uint32_t bits, float* s, float* inv) {
-  const int e = min(268 - static_cast<int>(bits >> 23), 253);
+__device__ __forceinline__ bool not_finite(float x) { return abs_bits(x) >= 0x7f800000u; }
+// largest |x|; NaN wins
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return m;
+}
+__device__ __forceinline__ float warp_amax(float x) {
+  float m;
+  asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+  return m;
+}
+// Power of two that brings values up to `top` into [2^14, 2^15), and its
+// inverse.
+__device__ __forceinline__ void pow2_scale(float top, float* s, float* inv) {
+  const int e = min(268 - static_cast<int>(abs_bits(top) >> 23), 253);
   *s = __uint_as_float(static_cast<uint32_t>(e) << 23);
   *inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 }
+// two floats in one register pair: one instruction for both
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// x = hi + lo as fp16 pairs
-__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  *hi = h2_bits(h);
-  *lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+// x = hi + lo as fp16 pairs: hi the leading 11 bits, lo the next 11
+__device__ __forceinline__ void split2(F2 xy, uint32_t* hi, uint32_t* lo) {
+  const float2 f = unpack(xy);
+  const float hx = __uint_as_float(__float_as_uint(f.x) & 0xffffe000u);
+  const float hy = __uint_as_float(__float_as_uint(f.y) & 0xffffe000u);
+  const float2 r = unpack(fma2(f2(hx, hy), f2(-1.0f, -1.0f), xy));
+  *hi = h2_bits(__floats2half2_rn(hx, hy));
+  *lo = h2_bits(__floats2half2_rn(r.x, r.y));
+}
+// The loads of v have arrived (v as operands: no use may move above this).
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                 "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                 "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]),
+                 "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                 "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -215,10 +307,10 @@ __device__ __forceinline__ void set_regs_dec() {
 
 // Float offset of the K row of a sequence's `pos`, -1 without one.
 __device__ __forceinline__ int64_t key_offset(const TreeArgs& a, int s, int hk, int pos, int D) {
-  const int64_t j = pos / a.bs;
+  const int bs = static_cast<int>(a.bs), j = pos / bs;
   const int64_t blk = a.block_tables[static_cast<int64_t>(s) * a.max_blocks + j];
   if (blk < 0 || blk >= a.num_blocks) return -1;
-  return ((((blk * a.num_layers + a.layer) * 2) * a.hkv + hk) * a.bs + (pos - j * a.bs)) * D;
+  return ((((blk * a.num_layers + a.layer) * 2) * a.hkv + hk) * a.bs + (pos - j * bs)) * D;
 }
 
 template <int D>
@@ -228,49 +320,67 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* kinv_s = reinterpret_cast<float*>(smem + L::META);
-  float* vinv_s = kinv_s + NST * kTK;
-  uint8_t* valid_s = smem + L::BITS;
-  uint8_t* kpois_s = valid_s + NST * 8;
-  uint8_t* vpois_s = kpois_s + NST * 8;
-  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* kempty = kfull + NST;
-  uint64_t* vfull = kempty + NST;
-  uint64_t* vempty = vfull + NST;
+  float* kinv_s = reinterpret_cast<float*>(smem + L::META);    // [kMeta][8]
+  float* vinv_s = kinv_s + kMeta * kWideWarps;
+  float* krel_s = vinv_s + kMeta * kWideWarps;                 // [kMeta][64]
+  float* vrel_s = krel_s + kMeta * kTK;
+  uint8_t* valid_s = smem + L::BITS;                           // [kMeta][8]: bits of the groups' keys
+  uint8_t* kpois_s = valid_s + kMeta * 8;
+  uint8_t* vpois_s = kpois_s + kMeta * 8;
+  uint8_t* tree_s = vpois_s + kMeta * 8;
+  uint64_t* rkfull = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* rvfull = rkfull + L::NRAW;
+  uint64_t* rkempty = rvfull + L::NRAW;
+  uint64_t* rvempty = rkempty + L::NRAW;
+  uint64_t* kfull = rvempty + L::NRAW;
+  uint64_t* vfull = kfull + NST;
+  uint64_t* kempty = vfull + NST;
+  uint64_t* vempty = kempty + NST;
   uint64_t* sfull = vempty + NST;       // [2]
   uint64_t* pready = sfull + 2;         // [2]
-  uint64_t* ofull = pready + 2;         // [2]
-  uint64_t* qready = ofull + 2;
-  uint64_t* drain = qready + 1;
+  uint64_t* ofull = pready + 2;
+  uint64_t* oempty = ofull + 1;
+  uint64_t* qready = oempty + 1;
+  uint64_t* lready = qready + 1;
+  uint64_t* drain = lready + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s0_s = reinterpret_cast<int*>(tmem_slot + 2);
   int64_t* line_s = reinterpret_cast<int64_t*>(tmem_slot + 4);   // U, base of s0
   __shared__ int64_t scan_s[kTcThreads / 32];
   __shared__ Walk walk_s[kTcThreads / 32];
-  __shared__ uint64_t rare_s[2][kRows];     // keys with a V that is not finite, per row
+  __shared__ float lsum_s[2][2][kRows];     // the halves' sums, by piece parity
   __shared__ SplitItem cut_s;
+  __shared__ Piece piece_s[kRowWarps];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
+    for (int i = 0; i < L::NRAW; ++i) {
+      mbar_init(&rkfull[i], 1);
+      mbar_init(&rvfull[i], 1);
+      mbar_init(&rkempty[i], kWideWarps);
+      mbar_init(&rvempty[i], kWideWarps);
+    }
     for (int i = 0; i < NST; ++i) {
-      mbar_init(&kfull[i], kLoadWarps);
-      mbar_init(&kempty[i], 1 + kRowWarps);      // the MMAs and every row warp
-      mbar_init(&vfull[i], kLoadWarps);
-      mbar_init(&vempty[i], 1 + kRowWarps);
+      mbar_init(&kfull[i], kWideWarps);
+      mbar_init(&vfull[i], kWideWarps);
+      mbar_init(&kempty[i], 1);
+      mbar_init(&vempty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pready[i], kRowWarps);
-      mbar_init(&ofull[i], 1);
     }
+    mbar_init(ofull, 1);
+    mbar_init(oempty, kRowWarps);
     mbar_init(qready, kRowWarps);
+    mbar_init(lready, kRowWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
     *s0_s = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, L::COLS);
     tmem_relinquish();
   }
@@ -347,225 +457,308 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     return ok;
   };
 
-  if (warp >= 12) {
-    set_regs_dec<56>();
-    if (warp == 12) {
+  if (warp >= kMmaWarp) {
+    set_regs_dec<64>();
+    if (warp == kMmaWarp) {
       // ---------------- MMAs ----------------
       constexpr uint32_t id_s = idesc_f16_f32(kRows, kTK);
       constexpr uint32_t id_o = idesc_f16_f32(kRows, D) | (1u << 16);   // B: keys along K
       int n = 0, seg = 0;
       bool ok = true;
       const uint32_t kbase = smem_u32(smem + L::K_OFF), vbase = smem_u32(smem + L::V_OFF);
-      auto issue_o = [&](int m) -> bool {            // O = P V of tile m
-        const int st = m % NST, b = m & 1;
-        if (!wait(&vfull[st], (m / NST) & 1) || !wait(&pready[b], (m >> 1) & 1)) return false;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t d = tmem + L::O_COL + static_cast<uint32_t>(b) * D;
-          const uint32_t ph = tmem + L::S_COL + static_cast<uint32_t>(b) * kTK;
-          // columns of 16 keys: [hi 8][hi 8][lo 8][lo 8] per 32 keys
-          auto pcol = [&](int k, int lo) { return ph + static_cast<uint32_t>((k >> 1) * 32 + lo * 16 + (k & 1) * 8); };
-          const uint64_t vh = desc_mn_sw128(vbase + st * 2 * L::TERM, L::HALF);
-          const uint64_t vl = desc_mn_sw128(vbase + st * 2 * L::TERM + L::TERM, L::HALF);
-          // 16 keys: 8 columns of P, 2048 bytes (128 in the address field) of V
-#pragma unroll
-          for (int k = 0; k < kTK / 16; ++k) mma_f16_ts(d, pcol(k, 0), vl + 128 * k, id_o, k > 0);
-#pragma unroll
-          for (int k = 0; k < kTK / 16; ++k) mma_f16_ts(d, pcol(k, 1), vh + 128 * k, id_o, 1u);
-#pragma unroll
-          for (int k = 0; k < kTK / 16; ++k) mma_f16_ts(d, pcol(k, 0), vh + 128 * k, id_o, 1u);
-          mma_commit(&vempty[st]);
-          mma_commit(&ofull[b]);
-        }
-        __syncwarp();
-        return true;
-      };
       while (ok && next_piece(a, wk, &pc)) {
         if (!(ok = wait(qready, seg & 1))) break;
         ++seg;
         tc_fence_after();
-        for (int t = pc.t0; t < pc.t1; ++t, ++n) {
-          const int st = n % NST, b = n & 1;
-          if (!(ok = wait(&kfull[st], (n / NST) & 1))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t d = tmem + L::S_COL + static_cast<uint32_t>(b) * kTK;
-            const uint32_t qh = tmem + L::Q_COL, ql = qh + D / 2;
-            const uint32_t kb = kbase + st * 2 * L::TERM;
-            // the small terms first: the tensor core cuts low bits off at
-            // every step, relative to the sum so far
+        // S of tile t, then O of tile t - 1
+#pragma unroll 1
+        for (int t = pc.t0; t <= pc.t1; ++t, ++n) {
+          if (t < pc.t1) {
+            const int st = n % NST, b = n & 1;
+            if (!(ok = wait(&kfull[st], (n / NST) & 1))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t d = tmem + L::S_COL + static_cast<uint32_t>(b) * kTK;
+              const uint32_t qh = tmem + L::Q_COL, ql = qh + D / 2;
+              const uint64_t kh = desc_k_sw128(kbase + st * 2 * L::TERM);
+              // the small terms first: the tensor core cuts low bits off at
+              // every step, relative to the sum so far
 #pragma unroll
-            for (int term = 0; term < 3; ++term) {
-              const uint32_t qa = term == 1 ? ql : qh;
-              const uint32_t kt = kb + (term == 0 ? L::TERM : 0);
+              for (int term = 0; term < 3; ++term) {
+                const uint32_t qa = term == 1 ? ql : qh;
+                const uint64_t kt = kh + (term == 0 ? L::TERM / 16 : 0);
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint64_t kd = desc_k_sw128(kt + (k / 4) * L::HALF) + 2 * (k % 4);
-                mma_f16_ts(d, qa + 8 * k, kd, id_s, (term > 0 || k > 0) ? 1u : 0u);
+                for (int k = 0; k < D / 16; ++k)
+                  mma_f16_ts(d, qa + 8 * k, kt + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
+                             (term > 0 || k > 0) ? 1u : 0u);
               }
+              mma_commit(&kempty[st]);
+              mma_commit(&sfull[b]);
             }
-            mma_commit(&kempty[st]);
-            mma_commit(&sfull[b]);
+            __syncwarp();
           }
-          __syncwarp();
-          if (t > pc.t0 && !(ok = issue_o(n - 1))) break;
+          if (t > pc.t0) {
+            const int m = n - 1, st = m % NST, b = m & 1;
+            if (!(ok = wait(&vfull[st], (m / NST) & 1) && wait(&pready[b], (m >> 1) & 1) &&
+                       (m == 0 || wait(oempty, (m - 1) & 1))))
+              break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t d = tmem + L::O_COL;
+              const uint32_t p = tmem + L::P_COL + static_cast<uint32_t>(b) * kTK;
+              const uint64_t vh = desc_mn_sw128(vbase + st * 2 * L::TERM, L::HALF);
+              // 16 keys: eight columns of hi pairs of P and eight of lo pairs,
+              // 2048 bytes of V
+#pragma unroll
+              for (int term = 0; term < 3; ++term) {
+                const uint32_t pa = p + (term == 1 ? 8 : 0);
+                const uint64_t vt = vh + (term == 0 ? L::TERM / 16 : 0);
+#pragma unroll
+                for (int k = 0; k < kTK / 16; ++k)
+                  mma_f16_ts(d, pa + 16 * k, vt + 128 * k, id_o, (term > 0 || k > 0) ? 1u : 0u);
+              }
+              mma_commit(&vempty[st]);
+              mma_commit(ofull);
+            }
+            __syncwarp();
+          }
         }
-        if (ok) ok = issue_o(n - 1);
+        --n;                                        // the round after the last tile
       }
       // nothing of this CTA's is in flight when its TMEM goes
       if (elect_one()) mma_commit(drain);
       __syncwarp();
       mbar_wait(drain, 0);
+    } else if (warp == kCopyWarp) {
+      // ---------------- K / V rows into shared memory ----------------
+      const int64_t vstep = a.hkv * a.bs * D;
+      const int bs = static_cast<int>(a.bs);
+      bool have = next_piece(a, wk, &pc), bad = false, ok = true;
+      int t = pc.t0, done = 0;                      // tiles whose copies are on their way
+      while (ok && have) {
+        // two tiles' block table entries in flight together
+        int blk[2][2], rest[2][2], hk[2];
+        bool is[2], tree[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          hk[e] = pc.hk;
+          is[e] = have;
+          tree[e] = (t + 1) * kTK > pc.pre;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int pos = t * kTK + 32 * h + lane;
+            blk[e][h] = -1;
+            rest[e][h] = 0;
+            if (have && pos < pc.keys) {
+              const int j = pos / bs;
+              rest[e][h] = pos - j * bs;
+              blk[e][h] = a.block_tables[static_cast<int64_t>(pc.s) * a.max_blocks + j];
+              if (blk[e][h] < 0) blk[e][h] = INT32_MAX;
+            }
+          }
+          if (have && ++t >= pc.t1) {
+            have = next_piece(a, wk, &pc);
+            t = pc.t0;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (!ok || !is[e]) continue;
+          const int rs = done % L::NRAW, mt = done % kMeta;
+          const uint32_t ph = ((done / L::NRAW) - 1) & 1;
+          int64_t off[2];
+          unsigned there[2], row[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            off[h] = -1;
+            if (blk[e][h] >= 0) {
+              if (blk[e][h] < a.num_blocks)
+                off[h] = ((((blk[e][h] * a.num_layers + a.layer) * 2) * a.hkv + hk[e]) * a.bs + rest[e][h]) * D;
+              else
+                bad = true;
+            }
+            // per group of eight: which keys there are, and whether they
+            // stand one after the other
+            const int64_t first = __shfl_sync(0xffffffffu, off[h], lane & 24);
+            there[h] = __ballot_sync(0xffffffffu, off[h] >= 0);
+            row[h] = __ballot_sync(0xffffffffu, off[h] >= 0 && off[h] == first + (lane & 7) * D);
+          }
+          const uint32_t bytes = static_cast<uint32_t>(__popc(there[0]) + __popc(there[1])) * D * 4;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* bar = (kv ? rvfull : rkfull) + rs;
+            if (done >= L::NRAW && !(ok = wait((kv ? rvempty : rkempty) + rs, ph))) break;
+            if (kv == 0) {
+              if (lane < 8)
+                valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
+              if (lane == 0) tree_s[mt * 8] = tree[e] ? 1 : 0;
+              __syncwarp();
+            }
+            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+            __syncwarp();
+            uint8_t* dst = smem + (kv ? L::RV_OFF : L::RK_OFF) + rs * L::RAW;
+            const float* src = a.pool + (kv ? vstep : 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool run = ((row[h] >> (lane & 24)) & 0xffu) == 0xffu;
+              if (off[h] >= 0 && (!run || (lane & 7) == 0))
+                copy_bulk(dst + (32 * h + lane) * D * 4, src + off[h], (run ? kGroup : 1) * D * 4, bar);
+            }
+          }
+          if (ok) ++done;
+        }
+      }
+      // after an abort, let the copies still in flight land before the CTA exits
+      if (*abort_flag)
+        for (int i = max(0, done - L::NRAW); i < done; ++i) {
+          mbar_wait(&rkfull[i % L::NRAW], (i / L::NRAW) & 1);
+          mbar_wait(&rvfull[i % L::NRAW], (i / L::NRAW) & 1);
+        }
+      if (bad) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
     }
   } else if (warp >= kRowWarps) {
-    // ---------------- K/V ----------------
-    set_regs_dec<120>();
-    const int lw = warp - kRowWarps;
+    // ---------------- widening ----------------
+    set_regs_dec<64>();
+    const int ww = warp - kRowWarps;
     constexpr int RPI = 128 / D;                    // rows per warp-wide load
-    constexpr int NLD = kKeysPerWarp / RPI;         // loads of K (and of V) per tile
+    constexpr int NLD = kGroup / RPI;
     const int sub = D == 128 ? 0 : lane >> 4;       // row of the load
     const int ln = D == 128 ? lane : lane & 15;     // float4 column of the row
-    const int64_t vstep = a.hkv * a.bs * D;
     const uint32_t half_off = static_cast<uint32_t>(ln >> 4) * L::HALF;
     const uint32_t chunk = static_cast<uint32_t>((ln & 15) >> 1), word = static_cast<uint32_t>(ln & 1) * 8;
-    bool have = next_piece(a, wk, &pc);
-    int t = pc.t0;
-    bool bad = false;
-    // offset of key lw * 8 + (lane & 7) of tile t
-    auto offset_of = [&]() -> int64_t {
-      const int pos = t * kTK + lw * kKeysPerWarp + (lane & 7);
-      if (!have || pos >= pc.keys) return -1;
-      const int64_t o = key_offset(a, pc.s, pc.hk, pos, D);
-      bad |= o < 0;
-      return o;
-    };
-    auto step = [&]() {
-      if (++t >= pc.t1) {
-        have = next_piece(a, wk, &pc);
-        t = pc.t0;
-      }
-    };
-    float4 kr[NLD], vr[NLD];
-    auto load = [&](float4 (&r)[NLD], int64_t off, int64_t add) {
+    const int ntl = static_cast<int>(u1 - u0);      // tiles of this CTA
+    bool ok = true;
+#pragma unroll 1
+    for (int i2 = 0; ok && i2 < 2 * ntl; ++i2) {    // K, then V of each tile
+      const int n = i2 >> 1, kv = i2 & 1, rs = n % L::NRAW, st = n % NST, mt = n % kMeta;
+      if (!(ok = wait((kv ? rvfull : rkfull) + rs, (n / L::NRAW) & 1))) break;
+      const uint32_t valid = valid_s[mt * 8 + ww];
+      const bool tree = tree_s[mt * 8] != 0;
+      const float4* raw = reinterpret_cast<const float4*>(smem + (kv ? L::RV_OFF : L::RK_OFF) + rs * L::RAW) +
+                          (ww * kGroup + sub) * (D / 4) + ln;
+      float4 r[NLD];
+      float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const int64_t o = __shfl_sync(0xffffffffu, off, i * RPI + sub);
-        r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (o >= 0) r[i] = ld_stream(a.pool + o + add + 4 * ln);
-      }
-    };
-    // scaled hi / lo terms of the warp's rows into a stage; bits of the rows
-    // that hold something not finite (those elements go in as zeros)
-    auto store = [&](float4 (&r)[NLD], uint8_t* stage, float* inv_s) -> uint32_t {
+      for (int i = 0; i < NLD; ++i) r[i] = raw[i * RPI * (D / 4)];
+#pragma unroll
+      for (int i = 0; i < NLD; ++i) top = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, top);
+      top = warp_amax(top);
+      __syncwarp();
+      if (lane == 0) mbar_arrive((kv ? rvempty : rkempty) + rs);
       uint32_t pois = 0;
+      if (__builtin_expect(valid != 0xffu || not_finite(top), 0)) {
+        // rows that are not there, and elements that are not finite, go in as
+        // zeros; the bits of the latter's rows are kept
+        top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const int key = i * RPI + sub;              // of the warp's eight
-        float4 v = r[i];
-        uint32_t mx = max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
-        if (__any_sync(0xffffffffu, mx >= 0x7f800000u)) {
-          const bool mine = mx >= 0x7f800000u;
-          const unsigned who = __ballot_sync(0xffffffffu, mine);
+        for (int i = 0; i < NLD; ++i) {
+          float4& v = r[i];
+          if (!((valid >> (i * RPI + sub)) & 1)) v = make_float4(0.f, 0.f, 0.f, 0.f);
+          const unsigned who = __ballot_sync(
+              0xffffffffu, not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w));
           if (D == 128) {
-            pois |= 1u << i;
+            if (who) pois |= 1u << i;
           } else {
             if (who & 0xffffu) pois |= 1u << (i * RPI);
             if (who >> 16) pois |= 1u << (i * RPI + 1);
           }
-          v.x = abs_bits(v.x) >= 0x7f800000u ? 0.f : v.x;
-          v.y = abs_bits(v.y) >= 0x7f800000u ? 0.f : v.y;
-          v.z = abs_bits(v.z) >= 0x7f800000u ? 0.f : v.z;
-          v.w = abs_bits(v.w) >= 0x7f800000u ? 0.f : v.w;
-          mx = max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+          v.x = not_finite(v.x) ? 0.f : v.x;
+          v.y = not_finite(v.y) ? 0.f : v.y;
+          v.z = not_finite(v.z) ? 0.f : v.z;
+          v.w = not_finite(v.w) ? 0.f : v.w;
+          top = amax3(amax3(v.x, v.y, v.z), v.w, top);
         }
-        if (D == 128) {
-          mx = __reduce_max_sync(0xffffffffu, mx);
-        } else {
+        top = warp_amax(top);
+      }
+      // one power of two for the eight rows: smaller rows keep 22 bits down to
+      // 2^-16 of the largest
+      float sc, inv;
+      pow2_scale(top, &sc, &inv);
+      if (n >= NST && !(ok = wait((kv ? vempty : kempty) + st, ((n / NST) - 1) & 1))) break;
+      if (lane == 0) {
+        (kv ? vinv_s : kinv_s)[mt * kWideWarps + ww] = inv;
+        (kv ? vpois_s : kpois_s)[mt * 8 + ww] = static_cast<uint8_t>(pois);
+      }
+      if (__builtin_expect(tree, 0)) {
+        // tiles with drafted nodes: each row brought to the size of the
+        // largest, so that a row few nodes see cannot cost the others bits
 #pragma unroll
-          for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        for (int i = 0; i < NLD; ++i) {
+          float m = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, 0.0f);
+#pragma unroll
+          for (int o = D / 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          float s1, inv1;
+          pow2_scale(m, &s1, &inv1);
+          const float up = fminf(s1 * inv, 0x1p120f);
+          r[i].x *= up;
+          r[i].y *= up;
+          r[i].z *= up;
+          r[i].w *= up;
+          if (ln == 0) (kv ? vrel_s : krel_s)[mt * kTK + ww * kGroup + i * RPI + sub] = 1.0f / up;
         }
-        float sc, inv;
-        row_scale(mx, &sc, &inv);
+      }
+      uint8_t* stage = smem + (kv ? L::V_OFF : L::K_OFF) + st * 2 * L::TERM + half_off;
+#pragma unroll
+      for (int i = 0; i < NLD; ++i) {
+        const int row = ww * kGroup + i * RPI + sub;
         uint2 hi, lo;
-        split2(v.x * sc, v.y * sc, &hi.x, &lo.x);
-        split2(v.z * sc, v.w * sc, &hi.y, &lo.y);
-        const int row = lw * kKeysPerWarp + key;
-        const uint32_t at = half_off + static_cast<uint32_t>(row) * 128 +
+        split2(mul2(f2(r[i].x, r[i].y), f2(sc, sc)), &hi.x, &lo.x);
+        split2(mul2(f2(r[i].z, r[i].w), f2(sc, sc)), &hi.y, &lo.y);
+        const uint32_t at = static_cast<uint32_t>(row) * 128 +
                             ((chunk ^ static_cast<uint32_t>(row & 7)) << 4) + word;
         *reinterpret_cast<uint2*>(stage + at) = hi;
         *reinterpret_cast<uint2*>(stage + L::TERM + at) = lo;
-        if (ln == 0) inv_s[row] = inv;
-      }
-      return pois;
-    };
-    int64_t off = offset_of();
-    if (have) {
-      load(kr, off, 0);
-      load(vr, off, vstep);
-    }
-    for (int n = 0; have; ++n) {
-      const int st = n % NST;
-      const uint32_t ph = ((n / NST) - 1) & 1;
-      const unsigned there = __ballot_sync(0xffffffffu, off >= 0) & 0xffu;
-      step();
-      const int64_t off1 = offset_of();
-      if (n >= NST && !wait(&kempty[st], ph)) break;
-      uint32_t pois = store(kr, smem + L::K_OFF + st * 2 * L::TERM, kinv_s + st * kTK);
-      if (lane == 0) {
-        valid_s[st * 8 + lw] = static_cast<uint8_t>(there);
-        kpois_s[st * 8 + lw] = static_cast<uint8_t>(pois);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kfull[st]);
-      if (have) load(kr, off1, 0);
-      if (n >= NST && !wait(&vempty[st], ph)) break;
-      pois = store(vr, smem + L::V_OFF + st * 2 * L::TERM, vinv_s + st * kTK);
-      if (lane == 0) vpois_s[st * 8 + lw] = static_cast<uint8_t>(pois);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&vfull[st]);
-      if (have) load(vr, off1, vstep);
-      off = off1;
+      if (lane == 0) mbar_arrive((kv ? vfull : kfull) + st);
     }
-    if (bad) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
   } else {
     // ---------------- rows ----------------
-    set_regs_inc<216>();
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    int n = 0;
+    set_regs_inc<144>();
+    const int hw = warp >> 2, row = (warp & 3) * 32 + lane;      // half, query row
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    constexpr int DH = D / 2;                       // columns of O per half
+    int n = 0, seg = 0;
     bool ok = true;
+    const Piece& ps = piece_s[warp];                // of the rare paths
     while (ok && next_piece(a, wk, &pc)) {
-      const int R = pc.qt * kRows + tid;            // query row of the kv head
-      const int node = R / a.g;
-      const bool live = node < pc.nq;
-      const bool any = pc.qt * kRows + warp * 32 < pc.nq * a.g;   // the warp has live rows
+      __syncwarp();
+      if (lane == 0) piece_s[warp] = pc;
+      __syncwarp();
+      const int t0 = pc.t0, t1 = pc.t1, pre = pc.pre;
+      const bool live = (pc.qt * kRows + row) / a.g < pc.nq;
+      const bool any = pc.qt * kRows + (warp & 3) * 32 < pc.nq * a.g;     // the warp has live rows
+      auto node_of = [&]() { return (ps.qt * kRows + row) / a.g; };
       auto row_at = [&]() -> int64_t {              // the row's place in q and out
-        return ((pc.a0 + node) * a.hq + static_cast<int64_t>(pc.hk) * a.g + (R - node * a.g)) * D;
+        const int R = ps.qt * kRows + row, node = R / a.g;
+        return ((ps.a0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
       };
-      float acc[D];
-      float qs, qinv;
-      // Q: hi / lo terms into TMEM
+      float qinv;
+      // Q: hi / lo terms of the half's columns into TMEM
       {
         const float* qp = a.q + row_at();
-        uint32_t mx = 0;
-#pragma unroll
+        auto quad = [&](int c) {
+          return live ? *reinterpret_cast<const float4*>(qp + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        float top = 0.0f, qs;
+#pragma unroll 8
         for (int c = 0; c < D; c += 4) {
-          const float4 v = live ? *reinterpret_cast<const float4*>(qp + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-          acc[c] = v.x;
-          acc[c + 1] = v.y;
-          acc[c + 2] = v.z;
-          acc[c + 3] = v.w;
-          mx = max(max(mx, max(abs_bits(v.x), abs_bits(v.y))), max(abs_bits(v.z), abs_bits(v.w)));
+          const float4 v = quad(c);
+          top = amax3(top, amax3(v.x, v.y, v.z), v.w);
         }
-        row_scale(mx, &qs, &qinv);
+        pow2_scale(top, &qs, &qinv);
+#pragma unroll 1
+        for (int c0 = 0; c0 < DH; c0 += 32) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 64) {
-          uint32_t hi[32], lo[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) split2(acc[c0 + 2 * c] * qs, acc[c0 + 2 * c + 1] * qs, &hi[c], &lo[c]);
-          tmem_st_32x32b_x32(lanes + L::Q_COL + c0 / 2, hi);
-          tmem_st_32x32b_x32(lanes + L::Q_COL + D / 2 + c0 / 2, lo);
+          for (int c = 0; c < 32; c += 4) {
+            const float4 v = quad(hw * DH + c0 + c);
+            split2(mul2(f2(v.x, v.y), f2(qs, qs)), &hi[c / 2], &lo[c / 2]);
+            split2(mul2(f2(v.z, v.w), f2(qs, qs)), &hi[c / 2 + 1], &lo[c / 2 + 1]);
+          }
+          tmem_st_32x32b_x16(lanes + L::Q_COL + (hw * DH + c0) / 2, hi);
+          tmem_st_32x32b_x16(lanes + L::Q_COL + DH + (hw * DH + c0) / 2, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -573,193 +766,260 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
         if (lane == 0) mbar_arrive(qready);
       }
       auto word = [&](int i) -> uint64_t {          // nodes 64 i .. 64 i + 63 that the row sees
-        if (a.mask) return live && i < a.words ? a.mask[(pc.a0 + node) * a.words + i] : 0;
+        const int node = node_of();
+        if (a.mask) return live && i < a.words ? a.mask[(ps.a0 + node) * a.words + i] : 0;
         const int bits = node + 1 - 64 * i;
         return bits <= 0 ? 0 : bits >= 64 ? ~0ull : (1ull << bits) - 1;
       };
       const float cq = qinv * (a.scale * 1.44269504088896340736f);   // to powers of two
-      float m = -INFINITY, mref = 0.0f, l = 0.0f;
+      // running state: the reference that the sums stand at (in powers of two;
+      // it follows the maximum once that is 2^8 above it, so most tiles
+      // rescale nothing), the half's sum
+      float mref = -INFINITY, l = 0.0f;
+      F2 acc[DH / 2];
 #pragma unroll
-      for (int c = 0; c < D; ++c) acc[c] = 0.0f;
+      for (int c = 0; c < DH / 2; ++c) acc[c] = f2(0.f, 0.f);
       // of the tile whose P V is still to be added
       float corr_p = 1.0f, vs_p = 0.0f;
-      bool rare_p = false;
+      uint64_t rare_p = 0;
 
-      auto promote = [&](int mt, int tile) -> bool {
-        if (!wait(&ofull[mt & 1], (mt >> 1) & 1)) return false;
-        tc_fence_after();
-        if (any) {
-          const uint32_t o = lanes + L::O_COL + static_cast<uint32_t>(mt & 1) * D;
-          if (__any_sync(0xffffffffu, corr_p != 1.0f)) {
+      // softmax of tile t, then the addition of tile t - 1's P V
+#pragma unroll 1
+      for (int t = t0; t <= t1; ++t, ++n) {
+        float corr = 1.0f, vs = 0.0f;
+        uint64_t rare = 0;
+        if (t < t1) {
+          const int st = n % NST, b = n & 1, mt = n % kMeta;
+          const uint32_t pq = (n >> 1) & 1, pv = (n / NST) & 1;
+          if (!__all_sync(0xffffffffu, mbar_test2(&sfull[b], pq, &vfull[st], pv)))
+            if (!(ok = wait(&sfull[b], pq) && wait(&vfull[st], pv))) break;
+          tc_fence_after();
+          if (any) {
+            const uint64_t kpois = *reinterpret_cast<const uint64_t*>(kpois_s + mt * 8);
+            const uint64_t vpois = *reinterpret_cast<const uint64_t*>(vpois_s + mt * 8);
+            const uint64_t valid = *reinterpret_cast<const uint64_t*>(valid_s + mt * 8);
+            const bool tree = (t + 1) * kTK > pre;
+            const float* kg = kinv_s + mt * kWideWarps;
+            const float* vg = vinv_s + mt * kWideWarps;
+            const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK;
+            const uint32_t pc0 = lanes + L::P_COL + static_cast<uint32_t>(b) * kTK;
+            float x[32], m = -INFINITY;
+            auto top32 = [&](int h) {                // eight keys share a scale
 #pragma unroll
-            for (int c = 0; c < D; ++c) acc[c] *= corr_p;
-          }
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            float v[32];
-            tmem_ld_32x32b_x32(o + c0, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) acc[c0 + c] = fmaf(v[c], vs_p, acc[c0 + c]);
-          }
-          if (rare_p) {        // V elements that are not finite: to the rows that see them
-            for (uint64_t left = live ? rare_s[mt & 1][tid] : 0; left; left &= left - 1) {
-              const int pos = tile * kTK + __ffsll(static_cast<long long>(left)) - 1;
-              const int64_t at = key_offset(a, pc.s, pc.hk, pos, D);
-              if (at < 0) continue;
-              const float* vp = a.pool + at + a.hkv * a.bs * D;
-#pragma unroll
-              for (int c = 0; c < D; ++c) {
-                const float x = vp[c];
-                if (abs_bits(x) >= 0x7f800000u) acc[c] += x;
+              for (int g = 0; g < 4; ++g) {
+                const float* v = x + 8 * g;
+                m = fmaxf(m, fmaxf(max3(max3(v[0], v[1], v[2]), v[3], v[4]), max3(v[5], v[6], v[7])) * kg[4 * h + g]);
               }
+            };
+            uint32_t own = sc + 32 * hw;             // the half's scores
+            if (__builtin_expect(!tree && (valid == ~0ull) && ((kpois | vpois) == 0), 1)) {
+              tmem_ld_32x32b_x32(sc + 32 * (hw ^ 1), x);      // the other half's, for the maximum
+              tmem_wait_ld(x);
+              top32(hw ^ 1);
+            } else {
+              // the tree's part of the keys, keys that are not there
+              uint64_t see = valid;
+              const int n0 = t * kTK - pre;          // node of the tile's first key
+              if (tree) {
+                if (n0 < 0) {
+                  see &= ((1ull << -n0) - 1) | (word(0) << -n0);
+                } else {
+                  const int i = n0 >> 6, sh = n0 & 63;
+                  see &= sh ? (word(i) >> sh) | (word(i + 1) << (64 - sh)) : word(i);
+                }
+              }
+              rare = live ? vpois & see : 0;
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                float y[16];
+                tmem_ld_32x32b_x16(sc + 16 * c, y);
+                tmem_wait_ld(y);
+                if (tree) {
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) y[j] *= krel_s[mt * kTK + 16 * c + j];
+                }
+                // K elements that are not finite went in as zeros
+                for (uint32_t left = static_cast<uint32_t>(kpois >> (16 * c)) & 0xffffu; left && live; left &= left - 1) {
+                  const int j = __ffs(static_cast<int>(left)) - 1;
+                  const int64_t at = key_offset(a, ps.s, ps.hk, t * kTK + 16 * c + j, D);
+                  const float* qp = a.q + row_at();
+                  float add = 0.0f;
+                  if (at >= 0)
+#pragma unroll 1
+                    for (int e = 0; e < D; ++e) {
+                      const float kx = a.pool[at + e];
+                      if (not_finite(kx)) add += qp[e] * kx;
+                    }
+#pragma unroll
+                  for (int e = 0; e < 16; ++e)
+                    if (e == j) y[e] += add;
+                }
+                const uint32_t on = static_cast<uint32_t>(see >> (16 * c));
+                const float k0 = kg[2 * c], k1 = kg[2 * c + 1];
+                uint32_t bits[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  y[j] = (on >> j) & 1 ? y[j] : -INFINITY;
+                  m = fmaxf(m, y[j] * (j < 8 ? k0 : k1));
+                  bits[j] = __float_as_uint(y[j]);
+                }
+                if ((c >> 1) == hw) tmem_st_32x32b_x16(pc0 + 16 * c, bits);    // P's columns are free
+              }
+              tmem_wait_st();
+              own = pc0 + 32 * hw;
+            }
+            tmem_ld_32x32b_x32(own, x);
+            tmem_wait_ld(x);
+            top32(hw);
+            const float mc = m * cq;
+            if (mc > mref + 8.0f) {
+              corr = ex2(mref - mc);
+              mref = mc;
+            }
+            const float ref = mref == -INFINITY ? 0.0f : mref;
+            // V's scales relative to the tile's largest; P is up to 2^8, its
+            // terms up to 2^15
+            const float vm = warp_amax(fmaxf(vg[lane & 7], 0x1p-100f));
+            const float up = __uint_as_float((261u << 23) - (__float_as_uint(vm) & 0x7f800000u));   // 2^7 / vm
+            vs = vm * (1.0f / 128.0f);
+            // P = 2^(x c - ref)
+            F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+            const F2 nref = f2(-ref, -ref);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float c1 = fmaxf(kg[4 * hw + g] * cq, 0x1p-126f);
+              const F2 c2 = f2(c1, c1);
+#pragma unroll
+              for (int j = 8 * g; j < 8 * g + 8; j += 2) {
+                const float2 e = unpack(fma2(f2(x[j], x[j + 1]), c2, nref));
+                x[j] = ex2(e.x);
+                x[j + 1] = ex2(e.y);
+                s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], f2(x[j], x[j + 1]));
+              }
+            }
+            const float2 sa = unpack(s2[0]), sb = unpack(s2[1]);
+            l = fmaf(l, corr, (sa.x + sa.y) + (sb.x + sb.y));
+            if (__builtin_expect(tree, 0)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] *= vrel_s[mt * kTK + 32 * hw + j];
+            }
+            // its terms: columns of 16 keys, eight of hi pairs and eight of lo
+            uint32_t pt[32];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float f1 = vg[4 * hw + g] * up;
+              const F2 w2 = f2(f1, f1);
+#pragma unroll
+              for (int j = 0; j < 8; j += 2) {
+                const int at = (g >> 1) * 16 + (g & 1) * 4 + j / 2;
+                split2(mul2(f2(x[8 * g + j], x[8 * g + j + 1]), w2), &pt[at], &pt[at + 8]);
+              }
+            }
+            tmem_st_32x32b_x32(pc0 + 32 * hw, pt);
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pready[b]);
+        }
+        if (t > t0) {
+          const int mt = n - 1;
+          if (!(ok = wait(ofull, mt & 1))) break;
+          tc_fence_after();
+          if (any) {
+            const uint32_t o = lanes + L::O_COL + hw * DH;
+            if (__any_sync(0xffffffffu, corr_p != 1.0f)) {
+#pragma unroll
+              for (int c = 0; c < DH / 2; ++c) acc[c] = mul2(acc[c], f2(corr_p, corr_p));
+            }
+            if (__builtin_expect(__any_sync(0xffffffffu, rare_p != 0), 0)) {
+              // V elements that are not finite: to the rows that see them
+#pragma unroll 1
+              for (int c0 = 0; c0 < DH; c0 += 16) {
+                float v[16];
+                tmem_ld_32x32b_x16(o + c0, v);
+                tmem_wait_ld(v);
+                for (uint64_t left = rare_p; left; left &= left - 1) {
+                  const int pos = (t - 1) * kTK + __ffsll(static_cast<long long>(left)) - 1;
+                  const int64_t at = key_offset(a, ps.s, ps.hk, pos, D);
+                  if (at < 0) continue;
+                  const float* vp = a.pool + at + a.hkv * a.bs * D + hw * DH + c0;
+#pragma unroll
+                  for (int c = 0; c < 16; ++c)
+                    if (not_finite(vp[c])) v[c] += vp[c];
+                }
+                uint32_t bits[16];
+#pragma unroll
+                for (int c = 0; c < 16; ++c) bits[c] = __float_as_uint(v[c]);
+                __syncwarp();
+                tmem_st_32x32b_x16(o + c0, bits);
+              }
+              tmem_wait_st();
+            }
+            // 16 columns of O arrive while the 16 before them are added
+            float v[2][16];
+            tmem_ld_32x32b_x16(o, v[0]);
+#pragma unroll
+            for (int i = 0; i < DH / 16; ++i) {
+              tmem_wait_ld(v[i & 1]);
+              if (i + 1 < DH / 16) tmem_ld_32x32b_x16(o + 16 * (i + 1), v[(i + 1) & 1]);
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                acc[8 * i + c] = fma2(f2(v[i & 1][2 * c], v[i & 1][2 * c + 1]), f2(vs_p, vs_p), acc[8 * i + c]);
             }
           }
           tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(oempty);
         }
-        return true;
-      };
-
-      for (int t = pc.t0; t < pc.t1; ++t, ++n) {
-        const int st = n % NST, b = n & 1;
-        if (!(ok = wait(&sfull[b], (n >> 1) & 1) && wait(&vfull[st], (n / NST) & 1))) break;
-        tc_fence_after();
-        const uint64_t kpois = *reinterpret_cast<const uint64_t*>(kpois_s + st * 8);
-        float corr = 1.0f, vs = 0.0f;
-        bool rare = false;
-        if (any) {
-          const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK;
-          uint64_t see = *reinterpret_cast<const uint64_t*>(valid_s + st * 8);
-          const int n0 = t * kTK - pc.pre;           // node of the tile's first key
-          if (n0 + kTK > 0) {                        // the tree's part of the keys
-            if (n0 < 0) {
-              see &= ((1ull << -n0) - 1) | (word(0) << -n0);
-            } else {
-              const int i = n0 >> 6, sh = n0 & 63;
-              see &= sh ? (word(i) >> sh) | (word(i + 1) << (64 - sh)) : word(i);
-            }
-          }
-          const uint64_t vpois = *reinterpret_cast<const uint64_t*>(vpois_s + st * 8);
-          rare = vpois != 0;
-          if (rare) rare_s[b][tid] = vpois & see;
-          const bool hide = __any_sync(0xffffffffu, see != ~0ull);
-          // 32 scores of the row at a time, read twice: registers hold the
-          // accumulators
-          float x[32];
-          auto scores = [&](int h) {
-            tmem_ld_32x32b_x32(sc + 32 * h, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 k4 = *reinterpret_cast<const float4*>(kinv_s + st * kTK + 32 * h + j);
-              x[j] *= k4.x;
-              x[j + 1] *= k4.y;
-              x[j + 2] *= k4.z;
-              x[j + 3] *= k4.w;
-            }
-            if (hide || kpois) {
-              for (uint32_t left = static_cast<uint32_t>(kpois >> (32 * h)); left && live; left &= left - 1) {
-                // K elements that are not finite went in as zeros
-                const int j = __ffs(static_cast<int>(left)) - 1;
-                const int64_t at = key_offset(a, pc.s, pc.hk, t * kTK + 32 * h + j, D);
-                const float* qp = a.q + row_at();
-                float add = 0.0f;
-                if (at >= 0)
-                  for (int c = 0; c < D; ++c) {
-                    const float kx = a.pool[at + c];
-                    if (abs_bits(kx) >= 0x7f800000u) add += qp[c] * kx;
-                  }
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (e == j) x[e] += add;
-              }
-              const uint32_t on = static_cast<uint32_t>(see >> (32 * h));
-#pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = (on >> j) & 1 ? x[j] : -INFINITY;
-            }
-          };
-          float m4[4] = {m, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int h = 0; h < kTK / 32; ++h) {
-            scores(h);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], x[j]);
-          }
-          m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          const float ref = m == -INFINITY ? 0.0f : m * cq;
-          corr = l > 0.0f ? ex2(mref - ref) : 1.0f;
-          mref = ref;
-          // P, scaled per key by V's scale relative to the tile's largest
-          float vm = fmaxf(vinv_s[st * kTK + lane], vinv_s[st * kTK + 32 + lane]);
-          vm = fmaxf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vm))), 0x1p-100f);
-          const float up = 32768.0f / vm;           // powers of two
-          vs = vm * (1.0f / 32768.0f);
-          float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int h = 0; h < kTK / 32; ++h) {
-            scores(h);
-            uint32_t pt[32];                        // hi pairs, then lo pairs, over the scores
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 v4 = *reinterpret_cast<const float4*>(vinv_s + st * kTK + 32 * h + j);
-              const float p0 = ex2(fmaf(x[j], cq, -ref)), p1 = ex2(fmaf(x[j + 1], cq, -ref));
-              const float p2 = ex2(fmaf(x[j + 2], cq, -ref)), p3 = ex2(fmaf(x[j + 3], cq, -ref));
-              s4[0] += p0;
-              s4[1] += p1;
-              s4[2] += p2;
-              s4[3] += p3;
-              split2(p0 * (v4.x * up), p1 * (v4.y * up), &pt[j / 2], &pt[16 + j / 2]);
-              split2(p2 * (v4.z * up), p3 * (v4.w * up), &pt[j / 2 + 1], &pt[16 + j / 2 + 1]);
-            }
-            tmem_st_32x32b_x32(sc + 32 * h, pt);
-          }
-          l = fmaf(l, corr, (s4[0] + s4[1]) + (s4[2] + s4[3]));
-          tmem_wait_st();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&pready[b]);
-          mbar_arrive(&kempty[st]);
-          mbar_arrive(&vempty[st]);
-        }
-        if (t > pc.t0 && !(ok = promote(n - 1, t - 1))) break;
         corr_p = corr;
         vs_p = vs;
         rare_p = rare;
       }
-      if (!ok || !(ok = promote(n - 1, pc.t1 - 1))) break;
+      if (!ok) break;
+      --n;                                          // the round after the last tile
 
-      const bool whole = pc.t0 == 0 && pc.t1 == pc.ntiles;
+      // the halves' sums
+      lsum_s[seg & 1][hw][row] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(lready);
+      if (!(ok = wait(lready, seg & 1))) break;
+      l = lsum_s[seg & 1][0][row] + lsum_s[seg & 1][1][row];
+      ++seg;
+      const bool whole = t0 == 0 && t1 == ps.ntiles;
       if (whole) {
         if (live) {
-          const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-          float* op = a.out + row_at();
+          const float inv = 1.0f / l;
+          float* op = a.out + row_at() + hw * DH;
 #pragma unroll
-          for (int c = 0; c < D; c += 4) {
-            float4 v = make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
+          for (int c = 0; c < DH; c += 4) {
+            const float2 p = unpack(acc[c / 2]), q = unpack(acc[c / 2 + 1]);
+            float4 v = make_float4(p.x * inv, p.y * inv, q.x * inv, q.y * inv);
             if (l == 0.0f) v = make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<float4*>(op + c) = v;
           }
         }
       } else {
-        float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (pc.t0 > 0 ? 0 : 1)) * part_floats<D>();
+        float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * part_floats<D>();
         if (live) {
-          part[tid] = m == -INFINITY ? -INFINITY : mref;
-          part[kRows + tid] = l;
+          if (hw == 0) {
+            part[row] = mref;
+            part[kRows + row] = l;
+          }
 #pragma unroll
-          for (int c = 0; c < D; c += 4)
-            reinterpret_cast<float4*>(part + 2 * kRows)[(c / 4) * kRows + tid] =
-                make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+          for (int c = 0; c < DH; c += 4) {
+            const float2 p = unpack(acc[c / 2]), q = unpack(acc[c / 2 + 1]);
+            reinterpret_cast<float4*>(part + 2 * kRows)[(hw * DH + c) / 4 * kRows + row] = make_float4(p.x, p.y, q.x, q.y);
+          }
         }
-        if (pc.t0 == 0 && tid == 0) {              // the share's last piece: joined from here on
-          const int64_t end = wk->u + (pc.ntiles - pc.t1);       // past the item's last unit
+        if (t0 == 0 && tid == 0) {                 // the share's last piece: joined from here on
+          const int64_t end = wk->u + (ps.ntiles - t1);          // past the item's last unit
           cut_s.first = static_cast<int>(blockIdx.x);
           cut_s.last = static_cast<int>((end * G - 1) / U);
-          cut_s.row0 = static_cast<int>(pc.a0);
-          cut_s.rbase = pc.qt * kRows;
-          cut_s.rows = min(kRows, pc.nq * a.g - pc.qt * kRows);
-          cut_s.hk = pc.hk;
+          cut_s.row0 = static_cast<int>(ps.a0);
+          cut_s.rbase = ps.qt * kRows;
+          cut_s.rows = min(kRows, ps.nq * a.g - ps.qt * kRows);
+          cut_s.hk = ps.hk;
         }
       }
     }
@@ -772,7 +1032,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     }
     a.items[blockIdx.x] = cut_s;
   }
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, L::COLS);
   }
