@@ -23,10 +23,9 @@
 // uneven lengths leave no SM idle; an item cut between CTAs leaves its
 // (m, l, acc) pieces in the workspace and tree_merge_kernel joins them in key
 // order (the same bits in every run).  Warps of a CTA:
-//   17      block table lookups and bulk copies of K / V rows into raw
-//           shared-memory slots: a copy per eight keys where they stand one
-//           after the other, else one per key (any block size)
-//   8..15   widening: raw rows -> scaled hi / lo fp16 tiles, 128-byte swizzle
+//   17, 18  block table lookups and bulk copies of K (17) and V (18) rows into
+//           shared memory, a copy per run of keys that stand one after the other
+//   8..15   widening: raw rows -> scaled hi / lo fp16, 128-byte swizzle, in place
 //   16      MMAs: S = Q K^T (A = Q in TMEM, B = K), O = P V (A = P in TMEM,
 //           B = V with the keys along K, so no transpose is stored)
 //   0..7    rows: thread = query row, and half of the tile's keys and of D.
@@ -83,7 +82,7 @@ constexpr int kTK = 64;                  // keys per tile
 constexpr int kRows = 128;               // query rows per tile (MMA M)
 constexpr int kRowWarps = 8, kWideWarps = 8;
 constexpr int kMmaWarp = kRowWarps + kWideWarps, kCopyWarp = kMmaWarp + 1;
-constexpr int kTcThreads = 32 * (kRowWarps + kWideWarps + 4);   // two idle warps fill the last warpgroup
+constexpr int kTcThreads = 32 * (kRowWarps + kWideWarps + 4);   // an idle warp fills the last warpgroup
 constexpr int kGroup = kTK / kWideWarps; // keys per widening warp, one scale for them
 constexpr int kMeta = 16;                // tiles whose scales are kept: more than the stages let run apart
 
@@ -93,19 +92,21 @@ constexpr int64_t part_floats() { return 2 * kRows + static_cast<int64_t>(D) * k
 
 template <int D>
 struct TreeLayout {
-  static constexpr int RAW = kTK * D * 4;            // raw K (or V) rows of a tile
-  static constexpr int TERM = kTK * D * 2;           // one fp16 term of them
-  static constexpr int HALF = kTK * 128;             // 64 columns of a term: 128-byte rows
-  static constexpr int NRAW = D == 128 ? 1 : 2;      // raw slots of K and of V
-  static constexpr int NST = D == 128 ? 2 : 4;       // widened stages of K and of V
-  static constexpr int RK_OFF = 0, RV_OFF = NRAW * RAW;
-  static constexpr int K_OFF = 2 * RV_OFF, V_OFF = K_OFF + NST * 2 * TERM;
+  static constexpr int TERM = kTK * D * 2;           // one fp16 term of a K (or V) tile
+  static constexpr int NST = D == 128 ? 3 : 6;       // stages of K and of V
+  // A stage is first the raw rows, then, in place, their two terms: a widening
+  // warp's eight rows (GRP bytes) become its own hi blocks, 64 columns of
+  // eight 128-byte rows each, and lo blocks.  The groups' stride goes into the
+  // operand descriptors.
+  static constexpr int GRP = kGroup * D * 4;
+  static constexpr int LO = D / 64 * 1024;           // lo blocks of a group, after the hi blocks
+  static constexpr int K_OFF = 0, V_OFF = NST * 2 * TERM;
   // per tile (ring of kMeta): inverse scales of K and V per group of eight
   // keys, and per key relative to that (tiles with drafted nodes)
   static constexpr int META = V_OFF + NST * 2 * TERM;    // kinv, vinv [8], krel, vrel [64]
   static constexpr int BITS = META + 2 * kMeta * (kWideWarps + kTK) * 4;   // valid, kpois, vpois, tree [8]
   static constexpr int BAR = BITS + 4 * kMeta * 8;
-  static constexpr int NBAR = 4 * NRAW + 4 * NST + 2 * 2 + 5;
+  static constexpr int NBAR = 6 * NST + 2 * 2 + 5;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int BYTES = MISC + 64 + 1024;
   // TMEM columns: Q hi, Q lo (D / 2 each), two S, two P buffers, O
@@ -181,6 +182,26 @@ __device__ __forceinline__ bool next_piece(const TreeArgs& a, Walk* wk, Piece* p
   return true;
 }
 
+// Up to 64 polls of an mbarrier's phase, as few instructions as a poll takes
+// (the waiting warps share their schedulers with working ones).
+__device__ __forceinline__ bool mbar_poll64(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 k;\n\t"
+      "mov.u32 k, 64;\n\t"
+      "POLL:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "sub.u32 k, k, 1;\n\t"
+      "setp.ne.u32 q, k, 0;\n\t"
+      "@q bra POLL;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Global -> shared copy, 16-byte aligned, completing on an mbarrier.
 __device__ __forceinline__ void copy_bulk(void* dst, const float* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -287,13 +308,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// MN-major operand, 128-byte swizzle: 64 columns of 2 bytes per 128-byte row,
-// 8 rows (of the K dimension) per 1024-byte group; `lbo` bytes to the next 64
-// columns.
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t smem_addr, uint32_t lbo) {
-  uint64_t d = desc_k_sw128(smem_addr);
-  d &= ~(static_cast<uint64_t>(0x3FFFu) << 16);
-  return d | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16);
+// Operand descriptor, 128-byte swizzle, 1024-byte blocks of eight 128-byte
+// rows.  K-major (K): `groups` bytes from eight rows to the next eight.
+// MN-major (V): a row holds 64 of the N columns; `groups` bytes from eight rows
+// (of the K dimension) to the next, 1024 to the next 64 columns.
+__device__ __forceinline__ uint64_t desc_blocks(uint32_t smem_addr, uint32_t groups) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1024u >> 4) << 16) |
+         (static_cast<uint64_t>(groups >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 template <int N>
@@ -318,8 +339,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   using L = TreeLayout<D>;
   constexpr int NST = L::NST;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem =
-      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // aligned by an offset, so that the compiler still sees shared memory (a
+  // pointer rounded as an integer makes every access a generic one)
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* kinv_s = reinterpret_cast<float*>(smem + L::META);    // [kMeta][8]
   float* vinv_s = kinv_s + kMeta * kWideWarps;
   float* krel_s = vinv_s + kMeta * kWideWarps;                 // [kMeta][64]
@@ -329,10 +351,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   uint8_t* vpois_s = kpois_s + kMeta * 8;
   uint8_t* tree_s = vpois_s + kMeta * 8;
   uint64_t* rkfull = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* rvfull = rkfull + L::NRAW;
-  uint64_t* rkempty = rvfull + L::NRAW;
-  uint64_t* rvempty = rkempty + L::NRAW;
-  uint64_t* kfull = rvempty + L::NRAW;
+  uint64_t* rvfull = rkfull + NST;
+  uint64_t* kfull = rvfull + NST;
   uint64_t* vfull = kfull + NST;
   uint64_t* kempty = vfull + NST;
   uint64_t* vempty = kempty + NST;
@@ -355,13 +375,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < L::NRAW; ++i) {
+    for (int i = 0; i < NST; ++i) {
       mbar_init(&rkfull[i], 1);
       mbar_init(&rvfull[i], 1);
-      mbar_init(&rkempty[i], kWideWarps);
-      mbar_init(&rvempty[i], kWideWarps);
-    }
-    for (int i = 0; i < NST; ++i) {
       mbar_init(&kfull[i], kWideWarps);
       mbar_init(&vfull[i], kWideWarps);
       mbar_init(&kempty[i], 1);
@@ -446,11 +462,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   __syncwarp();
   Piece pc = {};
 
+  // Bounded wait of the whole warp; gives up for all roles together.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     bool ok = false;
-    for (uint32_t i = 0; i < (1u << 22) && !ok; ++i) {
-      ok = mbar_try_wait(bar, parity);
-      if (!ok && (i & 63u) == 63u && *abort_flag) break;
+    for (uint32_t i = 0; i < (1u << 16); ++i) {
+      ok = mbar_poll64(bar, parity);
+      if (ok || *abort_flag) break;
     }
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) *abort_flag = 1;
@@ -480,16 +497,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
             if (elect_one()) {
               const uint32_t d = tmem + L::S_COL + static_cast<uint32_t>(b) * kTK;
               const uint32_t qh = tmem + L::Q_COL, ql = qh + D / 2;
-              const uint64_t kh = desc_k_sw128(kbase + st * 2 * L::TERM);
+              const uint64_t kh = desc_blocks(kbase + st * 2 * L::TERM, L::GRP);
               // the small terms first: the tensor core cuts low bits off at
               // every step, relative to the sum so far
 #pragma unroll
               for (int term = 0; term < 3; ++term) {
                 const uint32_t qa = term == 1 ? ql : qh;
-                const uint64_t kt = kh + (term == 0 ? L::TERM / 16 : 0);
+                const uint64_t kt = kh + (term == 0 ? L::LO / 16 : 0);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                  mma_f16_ts(d, qa + 8 * k, kt + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
+                  mma_f16_ts(d, qa + 8 * k, kt + (k / 4) * 64 + 2 * (k % 4), id_s,
                              (term > 0 || k > 0) ? 1u : 0u);
               }
               mma_commit(&kempty[st]);
@@ -506,16 +523,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
             if (elect_one()) {
               const uint32_t d = tmem + L::O_COL;
               const uint32_t p = tmem + L::P_COL + static_cast<uint32_t>(b) * kTK;
-              const uint64_t vh = desc_mn_sw128(vbase + st * 2 * L::TERM, L::HALF);
+              const uint64_t vh = desc_blocks(vbase + st * 2 * L::TERM, L::GRP);
               // 16 keys: eight columns of hi pairs of P and eight of lo pairs,
-              // 2048 bytes of V
+              // two groups of V
 #pragma unroll
               for (int term = 0; term < 3; ++term) {
                 const uint32_t pa = p + (term == 1 ? 8 : 0);
-                const uint64_t vt = vh + (term == 0 ? L::TERM / 16 : 0);
+                const uint64_t vt = vh + (term == 0 ? L::LO / 16 : 0);
 #pragma unroll
                 for (int k = 0; k < kTK / 16; ++k)
-                  mma_f16_ts(d, pa + 16 * k, vt + 128 * k, id_o, (term > 0 || k > 0) ? 1u : 0u);
+                  mma_f16_ts(d, pa + 16 * k, vt + 2 * L::GRP / 16 * k, id_o, (term > 0 || k > 0) ? 1u : 0u);
               }
               mma_commit(&vempty[st]);
               mma_commit(ofull);
@@ -529,16 +546,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
       if (elect_one()) mma_commit(drain);
       __syncwarp();
       mbar_wait(drain, 0);
-    } else if (warp == kCopyWarp) {
-      // ---------------- K / V rows into shared memory ----------------
-      const int64_t vstep = a.hkv * a.bs * D;
+    } else if (warp <= kCopyWarp + 1) {
+      // ---------------- K (one warp) / V (the next) rows into shared memory ----------------
+      const int kv = warp - kCopyWarp;
+      uint64_t* const rfull = kv ? rvfull : rkfull;
+      uint64_t* const freed = kv ? vempty : kempty;
+      uint8_t* const base = smem + (kv ? L::V_OFF : L::K_OFF);
+      const float* const src = a.pool + (kv ? a.hkv * a.bs * D : 0);
       const int bs = static_cast<int>(a.bs);
       bool have = next_piece(a, wk, &pc), bad = false, ok = true;
       int t = pc.t0, done = 0;                      // tiles whose copies are on their way
-      while (ok && have) {
-        // two tiles' block table entries in flight together
-        int blk[2][2], rest[2][2], hk[2];
-        bool is[2], tree[2];
+      // lane = keys lane and 32 + lane of two tiles; their block table entries
+      // are fetched while the two tiles before are copied
+      int blk[2][2], rest[2][2], hk[2];
+      bool is[2], tree[2];
+      auto fetch = [&]() {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           hk[e] = pc.hk;
@@ -561,59 +583,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
             t = pc.t0;
           }
         }
+      };
+      fetch();
+      while (ok && is[0]) {
+        int64_t off[2][2];
+        bool is1 = is[1], tree_of[2] = {tree[0], tree[1]};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (!ok || !is[e]) continue;
-          const int rs = done % L::NRAW, mt = done % kMeta;
-          const uint32_t ph = ((done / L::NRAW) - 1) & 1;
-          int64_t off[2];
-          unsigned there[2], row[2];
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            off[h] = -1;
+            off[e][h] = -1;
             if (blk[e][h] >= 0) {
               if (blk[e][h] < a.num_blocks)
-                off[h] = ((((blk[e][h] * a.num_layers + a.layer) * 2) * a.hkv + hk[e]) * a.bs + rest[e][h]) * D;
+                off[e][h] = ((((blk[e][h] * a.num_layers + a.layer) * 2) * a.hkv + hk[e]) * a.bs + rest[e][h]) * D;
               else
                 bad = true;
             }
-            // per group of eight: which keys there are, and whether they
-            // stand one after the other
-            const int64_t first = __shfl_sync(0xffffffffu, off[h], lane & 24);
-            there[h] = __ballot_sync(0xffffffffu, off[h] >= 0);
-            row[h] = __ballot_sync(0xffffffffu, off[h] >= 0 && off[h] == first + (lane & 7) * D);
+          }
+        fetch();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (!ok || (e == 1 && !is1)) continue;
+          const int st = done % NST, mt = done % kMeta;
+          const uint32_t ph = ((done / NST) - 1) & 1;
+          // keys that stand one after the other (in a half of the tile) go in
+          // one copy, whatever the block size: bytes from this lane's key on,
+          // 0 where an earlier lane's copy brings it
+          uint32_t len[2], there[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t before = __shfl_up_sync(0xffffffffu, off[e][h], 1);
+            const bool on = off[e][h] >= 0, follows = on && lane > 0 && before >= 0 && off[e][h] == before + D;
+            there[h] = __ballot_sync(0xffffffffu, on);
+            const uint32_t chain = __ballot_sync(0xffffffffu, follows);
+            len[h] = on && !follows ? (lane == 31 ? 1u : static_cast<uint32_t>(__ffs(static_cast<int>(~(chain >> (lane + 1)))))) * (D * 4) : 0u;
           }
           const uint32_t bytes = static_cast<uint32_t>(__popc(there[0]) + __popc(there[1])) * D * 4;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            uint64_t* bar = (kv ? rvfull : rkfull) + rs;
-            if (done >= L::NRAW && !(ok = wait((kv ? rvempty : rkempty) + rs, ph))) break;
-            if (kv == 0) {
-              if (lane < 8)
-                valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
-              if (lane == 0) tree_s[mt * 8] = tree[e] ? 1 : 0;
-              __syncwarp();
-            }
-            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          if (done >= NST && !(ok = wait(freed + st, ph))) continue;
+          if (kv == 0) {
+            if (lane < 8)
+              valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
+            if (lane == 0) tree_s[mt * 8] = tree_of[e] ? 1 : 0;
             __syncwarp();
-            uint8_t* dst = smem + (kv ? L::RV_OFF : L::RK_OFF) + rs * L::RAW;
-            const float* src = a.pool + (kv ? vstep : 0);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool run = ((row[h] >> (lane & 24)) & 0xffu) == 0xffu;
-              if (off[h] >= 0 && (!run || (lane & 7) == 0))
-                copy_bulk(dst + (32 * h + lane) * D * 4, src + off[h], (run ? kGroup : 1) * D * 4, bar);
-            }
           }
-          if (ok) ++done;
+          if (lane == 0) mbar_arrive_expect_tx(rfull + st, bytes);
+          __syncwarp();
+          uint8_t* dst = base + st * 2 * L::TERM + lane * D * 4;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (len[h]) copy_bulk(dst + 32 * h * D * 4, src + off[e][h], len[h], rfull + st);
+          ++done;
         }
       }
       // after an abort, let the copies still in flight land before the CTA exits
       if (*abort_flag)
-        for (int i = max(0, done - L::NRAW); i < done; ++i) {
-          mbar_wait(&rkfull[i % L::NRAW], (i / L::NRAW) & 1);
-          mbar_wait(&rvfull[i % L::NRAW], (i / L::NRAW) & 1);
-        }
+        for (int i = max(0, done - NST); i < done; ++i) mbar_wait(rfull + i % NST, (i / NST) & 1);
       if (bad) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
     }
   } else if (warp >= kRowWarps) {
@@ -624,27 +648,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     constexpr int NLD = kGroup / RPI;
     const int sub = D == 128 ? 0 : lane >> 4;       // row of the load
     const int ln = D == 128 ? lane : lane & 15;     // float4 column of the row
-    const uint32_t half_off = static_cast<uint32_t>(ln >> 4) * L::HALF;
+    const uint32_t block = static_cast<uint32_t>(ln >> 4) * 1024;
     const uint32_t chunk = static_cast<uint32_t>((ln & 15) >> 1), word = static_cast<uint32_t>(ln & 1) * 8;
     const int ntl = static_cast<int>(u1 - u0);      // tiles of this CTA
     bool ok = true;
 #pragma unroll 1
     for (int i2 = 0; ok && i2 < 2 * ntl; ++i2) {    // K, then V of each tile
-      const int n = i2 >> 1, kv = i2 & 1, rs = n % L::NRAW, st = n % NST, mt = n % kMeta;
-      if (!(ok = wait((kv ? rvfull : rkfull) + rs, (n / L::NRAW) & 1))) break;
+      const int n = i2 >> 1, kv = i2 & 1, st = n % NST, mt = n % kMeta;
+      uint8_t* grp = smem + (kv ? L::V_OFF : L::K_OFF) + st * 2 * L::TERM + ww * L::GRP;
+      if (!(ok = wait((kv ? rvfull : rkfull) + st, (n / NST) & 1))) break;
       const uint32_t valid = valid_s[mt * 8 + ww];
       const bool tree = tree_s[mt * 8] != 0;
-      const float4* raw = reinterpret_cast<const float4*>(smem + (kv ? L::RV_OFF : L::RK_OFF) + rs * L::RAW) +
-                          (ww * kGroup + sub) * (D / 4) + ln;
       float4 r[NLD];
       float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) r[i] = raw[i * RPI * (D / 4)];
+      for (int i = 0; i < NLD; ++i)
+        r[i] = *reinterpret_cast<const float4*>(grp + (i * RPI + sub) * (D * 4) + ln * 16);
+      __syncwarp();                                 // the terms go over the rows
 #pragma unroll
       for (int i = 0; i < NLD; ++i) top = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, top);
       top = warp_amax(top);
-      __syncwarp();
-      if (lane == 0) mbar_arrive((kv ? rvempty : rkempty) + rs);
       uint32_t pois = 0;
       if (__builtin_expect(valid != 0xffu || not_finite(top), 0)) {
         // rows that are not there, and elements that are not finite, go in as
@@ -674,7 +697,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
       // 2^-16 of the largest
       float sc, inv;
       pow2_scale(top, &sc, &inv);
-      if (n >= NST && !(ok = wait((kv ? vempty : kempty) + st, ((n / NST) - 1) & 1))) break;
       if (lane == 0) {
         (kv ? vinv_s : kinv_s)[mt * kWideWarps + ww] = inv;
         (kv ? vpois_s : kpois_s)[mt * 8 + ww] = static_cast<uint8_t>(pois);
@@ -697,17 +719,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
           if (ln == 0) (kv ? vrel_s : krel_s)[mt * kTK + ww * kGroup + i * RPI + sub] = 1.0f / up;
         }
       }
-      uint8_t* stage = smem + (kv ? L::V_OFF : L::K_OFF) + st * 2 * L::TERM + half_off;
 #pragma unroll
       for (int i = 0; i < NLD; ++i) {
-        const int row = ww * kGroup + i * RPI + sub;
+        const uint32_t row = i * RPI + sub;
         uint2 hi, lo;
         split2(mul2(f2(r[i].x, r[i].y), f2(sc, sc)), &hi.x, &lo.x);
         split2(mul2(f2(r[i].z, r[i].w), f2(sc, sc)), &hi.y, &lo.y);
-        const uint32_t at = static_cast<uint32_t>(row) * 128 +
-                            ((chunk ^ static_cast<uint32_t>(row & 7)) << 4) + word;
-        *reinterpret_cast<uint2*>(stage + at) = hi;
-        *reinterpret_cast<uint2*>(stage + L::TERM + at) = lo;
+        uint8_t* at = grp + block + row * 128 + ((chunk ^ row) << 4) + word;
+        *reinterpret_cast<uint2*>(at) = hi;
+        *reinterpret_cast<uint2*>(at + L::LO) = lo;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -956,16 +976,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
               }
               tmem_wait_st();
             }
-            // 16 columns of O arrive while the 16 before them are added
-            float v[2][16];
-            tmem_ld_32x32b_x16(o, v[0]);
+            float v[32];
 #pragma unroll
-            for (int i = 0; i < DH / 16; ++i) {
-              tmem_wait_ld(v[i & 1]);
-              if (i + 1 < DH / 16) tmem_ld_32x32b_x16(o + 16 * (i + 1), v[(i + 1) & 1]);
+            for (int i = 0; i < DH; i += 32) {
+              tmem_ld_32x32b_x32(o + i, v);
+              tmem_wait_ld(v);
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                acc[8 * i + c] = fma2(f2(v[i & 1][2 * c], v[i & 1][2 * c + 1]), f2(vs_p, vs_p), acc[8 * i + c]);
+              for (int c = 0; c < 16; ++c)
+                acc[i / 2 + c] = fma2(f2(v[2 * c], v[2 * c + 1]), f2(vs_p, vs_p), acc[i / 2 + c]);
             }
           }
           tc_fence_before();
