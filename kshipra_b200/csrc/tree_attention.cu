@@ -25,7 +25,8 @@
 // order (the same bits in every run).  Warps of a CTA:
 //   17, 18  block table lookups and bulk copies of K (17) and V (18) rows into
 //           shared memory, a copy per run of keys that stand one after the other
-//   8..15   widening: raw rows -> scaled hi / lo fp16, 128-byte swizzle, in place
+//   8..15   widening (four warps for K, four for V): raw rows -> scaled hi / lo
+//           fp16, 128-byte swizzle, in place
 //   16      MMAs: S = Q K^T (A = Q in TMEM, B = K), O = P V (A = P in TMEM,
 //           B = V with the keys along K, so no transpose is stored)
 //   0..7    rows: thread = query row, and half of the tile's keys and of D.
@@ -83,7 +84,7 @@ constexpr int kRows = 128;               // query rows per tile (MMA M)
 constexpr int kRowWarps = 8, kWideWarps = 8;
 constexpr int kMmaWarp = kRowWarps + kWideWarps, kCopyWarp = kMmaWarp + 1;
 constexpr int kTcThreads = 32 * (kRowWarps + kWideWarps + 4);   // an idle warp fills the last warpgroup
-constexpr int kGroup = kTK / kWideWarps; // keys per widening warp, one scale for them
+constexpr int kGroup = 8, kGroups = kTK / kGroup;    // keys that share a scale
 constexpr int kMeta = 16;                // tiles whose scales are kept: more than the stages let run apart
 
 // floats of one partial state: m [128], l [128], acc [D / 4][128][4]
@@ -104,7 +105,7 @@ struct TreeLayout {
   // per tile (ring of kMeta): inverse scales of K and V per group of eight
   // keys, and per key relative to that (tiles with drafted nodes)
   static constexpr int META = V_OFF + NST * 2 * TERM;    // kinv, vinv [8], krel, vrel [64]
-  static constexpr int BITS = META + 2 * kMeta * (kWideWarps + kTK) * 4;   // valid, kpois, vpois, tree [8]
+  static constexpr int BITS = META + 2 * kMeta * (kGroups + kTK) * 4;   // valid, kpois, vpois, tree [8]
   static constexpr int BAR = BITS + 4 * kMeta * 8;
   static constexpr int NBAR = 6 * NST + 2 * 2 + 5;
   static constexpr int MISC = BAR + NBAR * 8;
@@ -343,8 +344,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   // pointer rounded as an integer makes every access a generic one)
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* kinv_s = reinterpret_cast<float*>(smem + L::META);    // [kMeta][8]
-  float* vinv_s = kinv_s + kMeta * kWideWarps;
-  float* krel_s = vinv_s + kMeta * kWideWarps;                 // [kMeta][64]
+  float* vinv_s = kinv_s + kMeta * kGroups;
+  float* krel_s = vinv_s + kMeta * kGroups;                 // [kMeta][64]
   float* vrel_s = krel_s + kMeta * kTK;
   uint8_t* valid_s = smem + L::BITS;                           // [kMeta][8]: bits of the groups' keys
   uint8_t* kpois_s = valid_s + kMeta * 8;
@@ -378,8 +379,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     for (int i = 0; i < NST; ++i) {
       mbar_init(&rkfull[i], 1);
       mbar_init(&rvfull[i], 1);
-      mbar_init(&kfull[i], kWideWarps);
-      mbar_init(&vfull[i], kWideWarps);
+      mbar_init(&kfull[i], kWideWarps / 2);
+      mbar_init(&vfull[i], kWideWarps / 2);
       mbar_init(&kempty[i], 1);
       mbar_init(&vempty[i], 1);
     }
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
           }
           const uint32_t bytes = static_cast<uint32_t>(__popc(there[0]) + __popc(there[1])) * D * 4;
           if (done >= NST && !(ok = wait(freed + st, ph))) continue;
-          if (kv == 0) {
+          {                                         // both warps the same
             if (lane < 8)
               valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
             if (lane == 0) tree_s[mt * 8] = tree_of[e] ? 1 : 0;
@@ -643,7 +644,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   } else if (warp >= kRowWarps) {
     // ---------------- widening ----------------
     set_regs_dec<64>();
-    const int ww = warp - kRowWarps;
+    // four warps for K, four for V, two groups of keys each
+    const int kv = (warp - kRowWarps) >> 2, w2 = ((warp - kRowWarps) & 3) * 2;
+    uint64_t* const rfull = kv ? rvfull : rkfull;
+    uint64_t* const full = kv ? vfull : kfull;
+    uint8_t* const base = smem + (kv ? L::V_OFF : L::K_OFF);
+    float* const inv_s = kv ? vinv_s : kinv_s;
+    float* const rel_s = kv ? vrel_s : krel_s;
+    uint8_t* const pois_s = kv ? vpois_s : kpois_s;
     constexpr int RPI = 128 / D;                    // rows per warp-wide load
     constexpr int NLD = kGroup / RPI;
     const int sub = D == 128 ? 0 : lane >> 4;       // row of the load
@@ -653,85 +661,88 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     const int ntl = static_cast<int>(u1 - u0);      // tiles of this CTA
     bool ok = true;
 #pragma unroll 1
-    for (int i2 = 0; ok && i2 < 2 * ntl; ++i2) {    // K, then V of each tile
-      const int n = i2 >> 1, kv = i2 & 1, st = n % NST, mt = n % kMeta;
-      uint8_t* grp = smem + (kv ? L::V_OFF : L::K_OFF) + st * 2 * L::TERM + ww * L::GRP;
-      if (!(ok = wait((kv ? rvfull : rkfull) + st, (n / NST) & 1))) break;
-      const uint32_t valid = valid_s[mt * 8 + ww];
+    for (int n = 0; n < ntl; ++n) {
+      const int st = n % NST, mt = n % kMeta;
+      if (!(ok = wait(rfull + st, (n / NST) & 1))) break;
       const bool tree = tree_s[mt * 8] != 0;
-      float4 r[NLD];
-      float top = 0.0f;
+#pragma unroll 1
+      for (int ww = w2; ww < w2 + 2; ++ww) {
+        const uint32_t valid = valid_s[mt * 8 + ww];
+        uint8_t* grp = base + st * 2 * L::TERM + ww * L::GRP;
+        float4 r[NLD];
+        float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NLD; ++i)
-        r[i] = *reinterpret_cast<const float4*>(grp + (i * RPI + sub) * (D * 4) + ln * 16);
-      __syncwarp();                                 // the terms go over the rows
+        for (int i = 0; i < NLD; ++i)
+          r[i] = *reinterpret_cast<const float4*>(grp + (i * RPI + sub) * (D * 4) + ln * 16);
+        __syncwarp();                                 // the terms go over the rows
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) top = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, top);
-      top = warp_amax(top);
-      uint32_t pois = 0;
-      if (__builtin_expect(valid != 0xffu || not_finite(top), 0)) {
-        // rows that are not there, and elements that are not finite, go in as
-        // zeros; the bits of the latter's rows are kept
-        top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NLD; ++i) {
-          float4& v = r[i];
-          if (!((valid >> (i * RPI + sub)) & 1)) v = make_float4(0.f, 0.f, 0.f, 0.f);
-          const unsigned who = __ballot_sync(
-              0xffffffffu, not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w));
-          if (D == 128) {
-            if (who) pois |= 1u << i;
-          } else {
-            if (who & 0xffffu) pois |= 1u << (i * RPI);
-            if (who >> 16) pois |= 1u << (i * RPI + 1);
-          }
-          v.x = not_finite(v.x) ? 0.f : v.x;
-          v.y = not_finite(v.y) ? 0.f : v.y;
-          v.z = not_finite(v.z) ? 0.f : v.z;
-          v.w = not_finite(v.w) ? 0.f : v.w;
-          top = amax3(amax3(v.x, v.y, v.z), v.w, top);
-        }
+        for (int i = 0; i < NLD; ++i) top = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, top);
         top = warp_amax(top);
-      }
-      // one power of two for the eight rows: smaller rows keep 22 bits down to
-      // 2^-16 of the largest
-      float sc, inv;
-      pow2_scale(top, &sc, &inv);
-      if (lane == 0) {
-        (kv ? vinv_s : kinv_s)[mt * kWideWarps + ww] = inv;
-        (kv ? vpois_s : kpois_s)[mt * 8 + ww] = static_cast<uint8_t>(pois);
-      }
-      if (__builtin_expect(tree, 0)) {
-        // tiles with drafted nodes: each row brought to the size of the
-        // largest, so that a row few nodes see cannot cost the others bits
+        uint32_t pois = 0;
+        if (__builtin_expect(valid != 0xffu || not_finite(top), 0)) {
+          // rows that are not there, and elements that are not finite, go in as
+          // zeros; the bits of the latter's rows are kept
+          top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < NLD; ++i) {
+            float4& v = r[i];
+            if (!((valid >> (i * RPI + sub)) & 1)) v = make_float4(0.f, 0.f, 0.f, 0.f);
+            const unsigned who = __ballot_sync(
+                0xffffffffu, not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w));
+            if (D == 128) {
+              if (who) pois |= 1u << i;
+            } else {
+              if (who & 0xffffu) pois |= 1u << (i * RPI);
+              if (who >> 16) pois |= 1u << (i * RPI + 1);
+            }
+            v.x = not_finite(v.x) ? 0.f : v.x;
+            v.y = not_finite(v.y) ? 0.f : v.y;
+            v.z = not_finite(v.z) ? 0.f : v.z;
+            v.w = not_finite(v.w) ? 0.f : v.w;
+            top = amax3(amax3(v.x, v.y, v.z), v.w, top);
+          }
+          top = warp_amax(top);
+        }
+        // one power of two for the eight rows: smaller rows keep 22 bits down to
+        // 2^-16 of the largest
+        float sc, inv;
+        pow2_scale(top, &sc, &inv);
+        if (lane == 0) {
+          inv_s[mt * kGroups + ww] = inv;
+          pois_s[mt * 8 + ww] = static_cast<uint8_t>(pois);
+        }
+        if (__builtin_expect(tree, 0)) {
+          // tiles with drafted nodes: each row brought to the size of the
+          // largest, so that a row few nodes see cannot cost the others bits
+#pragma unroll
+          for (int i = 0; i < NLD; ++i) {
+            float m = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, 0.0f);
+#pragma unroll
+            for (int o = D / 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            float s1, inv1;
+            pow2_scale(m, &s1, &inv1);
+            const float up = fminf(s1 * inv, 0x1p120f);
+            r[i].x *= up;
+            r[i].y *= up;
+            r[i].z *= up;
+            r[i].w *= up;
+            if (ln == 0) rel_s[mt * kTK + ww * kGroup + i * RPI + sub] = 1.0f / up;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
-          float m = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, 0.0f);
-#pragma unroll
-          for (int o = D / 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          float s1, inv1;
-          pow2_scale(m, &s1, &inv1);
-          const float up = fminf(s1 * inv, 0x1p120f);
-          r[i].x *= up;
-          r[i].y *= up;
-          r[i].z *= up;
-          r[i].w *= up;
-          if (ln == 0) (kv ? vrel_s : krel_s)[mt * kTK + ww * kGroup + i * RPI + sub] = 1.0f / up;
+          const uint32_t row = i * RPI + sub;
+          uint2 hi, lo;
+          split2(mul2(f2(r[i].x, r[i].y), f2(sc, sc)), &hi.x, &lo.x);
+          split2(mul2(f2(r[i].z, r[i].w), f2(sc, sc)), &hi.y, &lo.y);
+          uint8_t* at = grp + block + row * 128 + ((chunk ^ row) << 4) + word;
+          *reinterpret_cast<uint2*>(at) = hi;
+          *reinterpret_cast<uint2*>(at + L::LO) = lo;
         }
-      }
-#pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const uint32_t row = i * RPI + sub;
-        uint2 hi, lo;
-        split2(mul2(f2(r[i].x, r[i].y), f2(sc, sc)), &hi.x, &lo.x);
-        split2(mul2(f2(r[i].z, r[i].w), f2(sc, sc)), &hi.y, &lo.y);
-        uint8_t* at = grp + block + row * 128 + ((chunk ^ row) << 4) + word;
-        *reinterpret_cast<uint2*>(at) = hi;
-        *reinterpret_cast<uint2*>(at + L::LO) = lo;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive((kv ? vfull : kfull) + st);
+      if (lane == 0) mbar_arrive(full + st);
     }
   } else {
     // ---------------- rows ----------------
@@ -748,7 +759,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
       __syncwarp();
       const int t0 = pc.t0, t1 = pc.t1, pre = pc.pre;
       const bool live = (pc.qt * kRows + row) / a.g < pc.nq;
-      const bool any = pc.qt * kRows + (warp & 3) * 32 < pc.nq * a.g;     // the warp has live rows
       auto node_of = [&]() { return (ps.qt * kRows + row) / a.g; };
       auto row_at = [&]() -> int64_t {              // the row's place in q and out
         const int R = ps.qt * kRows + row, node = R / a.g;
@@ -814,13 +824,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
           if (!__all_sync(0xffffffffu, mbar_test2(&sfull[b], pq, &vfull[st], pv)))
             if (!(ok = wait(&sfull[b], pq) && wait(&vfull[st], pv))) break;
           tc_fence_after();
-          if (any) {
+          {
             const uint64_t kpois = *reinterpret_cast<const uint64_t*>(kpois_s + mt * 8);
             const uint64_t vpois = *reinterpret_cast<const uint64_t*>(vpois_s + mt * 8);
             const uint64_t valid = *reinterpret_cast<const uint64_t*>(valid_s + mt * 8);
             const bool tree = (t + 1) * kTK > pre;
-            const float* kg = kinv_s + mt * kWideWarps;
-            const float* vg = vinv_s + mt * kWideWarps;
+            const float* kg = kinv_s + mt * kGroups;
+            const float* vg = vinv_s + mt * kGroups;
             const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK;
             const uint32_t pc0 = lanes + L::P_COL + static_cast<uint32_t>(b) * kTK;
             float x[32], m = -INFINITY;
@@ -946,7 +956,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
           const int mt = n - 1;
           if (!(ok = wait(ofull, mt & 1))) break;
           tc_fence_after();
-          if (any) {
+          {
             const uint32_t o = lanes + L::O_COL + hw * DH;
             if (__any_sync(0xffffffffu, corr_p != 1.0f)) {
 #pragma unroll
