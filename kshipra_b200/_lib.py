@@ -112,14 +112,19 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-def call(name: str, *args) -> int:
-    st = getattr(lib(), name)(*args)
+def check(name: str, st: int) -> None:
+    """Raise for a non-zero status of the C entry ``name``."""
     if st != 0:
         msg = lib().ksh_status_string(st).decode()
         extra = ""
         if st == -3:
             extra = f" (cudaError {lib().ksh_last_cuda_error()})"
         raise KshipraLibraryError(f"{name} failed: {msg}{extra}")
+
+
+def call(name: str, *args) -> int:
+    st = getattr(lib(), name)(*args)
+    check(name, st)
     return st
 
 

@@ -22,14 +22,34 @@ OR-ed into ``flags`` (int32 [1], KSH_FLAG_* bits) where one is given.
 
 from __future__ import annotations
 
+import functools
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import call, ptr, stream_ptr
+from ._lib import ptr, stream_ptr
 
 MAX_NODES = 256              # nodes of one sequence's tree: four 64-bit mask words
+
+
+# These operators take 5 to 30 us on the GPU, so the host side of a call is kept
+# short: the current stream's handle straight from torch (2 us less than through
+# a Stream object), no device switch where the tensors' device is current.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _run(device: torch.device, name: str, *args) -> None:
+    """The C entry on ``device`` and its current stream (appended to args)."""
+    idx = device.index
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            _run(device, name, *args)
+        return
+    stream = _raw_stream(idx) if _raw_stream is not None else stream_ptr()
+    st = getattr(_lib.lib(), name)(*args, stream)
+    if st != 0:
+        _lib.check(name, st)
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, ndim: int) -> torch.Tensor:
@@ -63,15 +83,22 @@ class TreeWorkspace:
     def __init__(self):
         self.bufs: Dict[tuple, torch.Tensor] = {}
 
-    def get(self, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-        buf = self.bufs.get((device, stream))
+    def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
+        idx = device.index
+        key = (idx, _raw_stream(idx) if _raw_stream is not None else stream_ptr(device))
+        buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             buf = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-            self.bufs[(device, stream)] = buf
+            self.bufs[key] = buf
         return buf
 
 
 _WS = TreeWorkspace()
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(seqs: int, hq: int, hkv: int, d: int, max_nodes: int) -> int:
+    return int(_lib.lib().ksh_tree_attention_workspace_size(seqs, hq, hkv, d, max_nodes))
 
 
 def tree_tables(prefix_lens: torch.Tensor, new_lens: torch.Tensor, total: int, block_size: int,
@@ -102,25 +129,24 @@ def tree_tables(prefix_lens: torch.Tensor, new_lens: torch.Tensor, total: int, b
         _need(block_ids, "block_ids", torch.int32, 1)
         if _need(block_start, "block_start", torch.int32, 1).shape[0] != S + 1:
             raise ValueError("block_start must have one entry more than there are sequences")
-        block_tables = torch.empty((S, max_blocks), dtype=torch.int32, device=dev)
+        block_tables = prefix_lens.new_empty((S, max_blocks))
     elif tuple(_need(block_tables, "block_tables", torch.int32, 2).shape) != (S, max_blocks):
         raise ValueError(f"block_tables must be [{S}, {max_blocks}]")
-    words, mask = 0, None
+    words = 0
     if parents is not None:
         if _need(parents, "parents", torch.int32, 1).shape[0] != total:
             raise ValueError("parents must have one entry per row")
         if not 1 <= max_nodes <= MAX_NODES:
             raise ValueError(f"max_nodes must be 1..{MAX_NODES}, got {max_nodes}")
         words = (max_nodes + 63) >> 6
-        mask = torch.empty((total, words), dtype=torch.int64, device=dev)
-    q_start = torch.empty(S + 1, dtype=torch.int32, device=dev)
-    pos_slot = torch.empty((2, total), dtype=torch.int64, device=dev)
-    positions, slots = pos_slot[0], pos_slot[1]
-    with torch.cuda.device(dev):
-        call("ksh_tree_tables", ptr(prefix_lens), ptr(new_lens), S, total, block_size,
-             ptr(block_ids), 0 if block_ids is None else block_ids.shape[0], ptr(block_start),
-             max_blocks, ptr(parents), words, ptr(q_start), ptr(block_tables), ptr(positions),
-             ptr(slots), ptr(mask), ptr(flags), stream_ptr())
+    q_start = prefix_lens.new_empty(S + 1)
+    positions = torch.empty(total, dtype=torch.int64, device=dev)
+    slots = torch.empty_like(positions)
+    mask = None if parents is None else positions.new_empty((total, words))
+    _run(dev, "ksh_tree_tables", prefix_lens.data_ptr(), new_lens.data_ptr(), S, total, block_size,
+         ptr(block_ids), 0 if block_ids is None else block_ids.shape[0], ptr(block_start),
+         max_blocks, ptr(parents), words, q_start.data_ptr(), block_tables.data_ptr(),
+         positions.data_ptr(), slots.data_ptr(), ptr(mask), ptr(flags))
     return q_start, block_tables, positions, slots, mask
 
 
@@ -158,13 +184,12 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_tables
         out = torch.empty_like(q)
     elif _need(out, "out", torch.float32, 3).shape != q.shape:
         raise ValueError("out must have q's shape")
-    with torch.cuda.device(q.device):
-        s = stream_ptr()
-        n = int(_lib.lib().ksh_tree_attention_workspace_size(S, hq, hkv, d, max_nodes))
-        buf = ws.get(n, q.device, s)
-        call("ksh_tree_attention", ptr(q), T, hq, d, ptr(pool), nb, L, layer, hkv, bs,
-             ptr(block_tables), max_blocks, ptr(q_start), ptr(prefix_lens), S, ptr(mask), words,
-             max_nodes, max_total_len, ptr(out), ptr(buf), buf.numel(), ptr(flags), s)
+    dev = q.device
+    buf = ws.get(_workspace_bytes(S, hq, hkv, d, max_nodes), dev)
+    _run(dev, "ksh_tree_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), nb, L, layer, hkv, bs,
+         block_tables.data_ptr(), max_blocks, q_start.data_ptr(), prefix_lens.data_ptr(), S,
+         ptr(mask), words, max_nodes, max_total_len, out.data_ptr(), buf.data_ptr(), buf.numel(),
+         ptr(flags))
     return out
 
 
@@ -179,9 +204,8 @@ def target_probs(logits: torch.Tensor, temperature: Optional[torch.Tensor] = Non
         out = torch.empty((m, vocab), dtype=torch.float32, device=logits.device)
     elif _rows(out, "out").shape != logits.shape:
         raise ValueError("out must have the logits' shape")
-    with torch.cuda.device(logits.device):
-        call("ksh_target_probs", ptr(logits), m, vocab, _stride(logits), ptr(temperature),
-             ptr(out), _stride(out), stream_ptr())
+    _run(logits.device, "ksh_target_probs", logits.data_ptr(), m, vocab, _stride(logits),
+         ptr(temperature), out.data_ptr(), _stride(out))
     return out
 
 
@@ -228,15 +252,14 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, q_start: torch.Tens
         if _need(target_tokens, "target_tokens", torch.int64, 1).shape[0] != T:
             raise ValueError("target_tokens must have one entry per node")
     dev = tokens.device
-    path = torch.empty((S, max_nodes), dtype=torch.int32, device=dev)
-    path_len = torch.empty(S, dtype=torch.int32, device=dev)
-    nxt = torch.empty(S, dtype=torch.int64, device=dev)
-    with torch.cuda.device(dev):
-        call("ksh_verify_tree", ptr(tokens), ptr(parents), ptr(q_start), S, T, max_nodes, vocab,
-             ptr(target_probs), ps, ptr(draft_probs), qs, ptr(target_tokens),
-             None if target_probs is None else ptr(u_accept),
-             None if target_probs is None else ptr(u_sample), ptr(path), ptr(path_len), ptr(nxt),
-             ptr(flags), stream_ptr())
+    path = q_start.new_empty((S, max_nodes))
+    path_len = q_start.new_empty(S)
+    nxt = tokens.new_empty(S)
+    _run(dev, "ksh_verify_tree", tokens.data_ptr(), parents.data_ptr(), q_start.data_ptr(), S, T,
+         max_nodes, vocab, ptr(target_probs), ps, ptr(draft_probs), qs, ptr(target_tokens),
+         None if target_probs is None else u_accept.data_ptr(),
+         None if target_probs is None else u_sample.data_ptr(), path.data_ptr(),
+         path_len.data_ptr(), nxt.data_ptr(), ptr(flags))
     return path, path_len, nxt
 
 
@@ -256,11 +279,10 @@ def commit_tree(pool: torch.Tensor, block_tables: torch.Tensor, prefix_lens: tor
             or _need(path_len, "path_len", torch.int32, 1).shape[0] != S
             or _need(path, "path", torch.int32, 2).shape[0] != S):
         raise ValueError("prefix_lens, path and path_len must have one entry per sequence")
-    new_lens = torch.empty(S, dtype=torch.int32, device=pool.device)
-    with torch.cuda.device(pool.device):
-        call("ksh_tree_commit", ptr(pool), nb, L, hkv, bs, d, ptr(block_tables), max_blocks,
-             ptr(prefix_lens), S, ptr(path), path.shape[1], ptr(path_len), ptr(new_lens),
-             ptr(flags), stream_ptr())
+    new_lens = prefix_lens.new_empty(S)
+    _run(pool.device, "ksh_tree_commit", pool.data_ptr(), nb, L, hkv, bs, d,
+         block_tables.data_ptr(), max_blocks, prefix_lens.data_ptr(), S, path.data_ptr(),
+         path.shape[1], path_len.data_ptr(), new_lens.data_ptr(), ptr(flags))
     return new_lens
 
 
