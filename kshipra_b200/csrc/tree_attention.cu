@@ -554,87 +554,85 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
       uint64_t* const freed = kv ? vempty : kempty;
       uint8_t* const base = smem + (kv ? L::V_OFF : L::K_OFF);
       const float* const src = a.pool + (kv ? a.hkv * a.bs * D : 0);
-      const int bs = static_cast<int>(a.bs);
-      bool have = next_piece(a, wk, &pc), bad = false, ok = true;
-      int t = pc.t0, done = 0;                      // tiles whose copies are on their way
-      // lane = keys lane and 32 + lane of two tiles; their block table entries
-      // are fetched while the two tiles before are copied
-      int blk[2][2], rest[2][2], hk[2];
-      bool is[2], tree[2];
+      // A lane has the keys lane and 32 + lane of a tile: table column, place in
+      // the block and table entry, the entry fetched one tile ahead.  A tile's
+      // lookups are kept to additions (rows of the pool as 32-bit numbers; the
+      // host checks that they fit): with divisions and 64-bit offsets here the
+      // two warps were the slowest roles, 3270 of 4200 cycles a tile.
+      const int bs = static_cast<int>(a.bs), dj = kTK / bs, dr = kTK - dj * bs;
+      const uint32_t rows_per_block = static_cast<uint32_t>(a.num_layers * 2 * a.hkv * a.bs);
+      bool have = next_piece(a, wk, &pc), bad = false;
+      int t = 0, done = 0;                          // done: tiles whose copies are on their way
+      uint32_t row0 = 0;                            // of the piece's layer and head in block 0
+      const int32_t* table = nullptr;
+      int col[2], rest[2], blk[2];
+      auto begin = [&]() {
+        t = pc.t0;
+        row0 = static_cast<uint32_t>((a.layer * 2 * a.hkv + pc.hk) * a.bs);
+        table = a.block_tables + static_cast<int64_t>(pc.s) * a.max_blocks;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int pos = t * kTK + 32 * h + lane;
+          col[h] = pos / bs;
+          rest[h] = pos - col[h] * bs;
+        }
+      };
       auto fetch = [&]() {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          hk[e] = pc.hk;
-          is[e] = have;
-          tree[e] = (t + 1) * kTK > pc.pre;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int pos = t * kTK + 32 * h + lane;
-            blk[e][h] = -1;
-            rest[e][h] = 0;
-            if (have && pos < pc.keys) {
-              const int j = pos / bs;
-              rest[e][h] = pos - j * bs;
-              blk[e][h] = a.block_tables[static_cast<int64_t>(pc.s) * a.max_blocks + j];
-              if (blk[e][h] < 0) blk[e][h] = INT32_MAX;
-            }
-          }
-          if (have && ++t >= pc.t1) {
-            have = next_piece(a, wk, &pc);
-            t = pc.t0;
+        for (int h = 0; h < 2; ++h) {
+          blk[h] = -1;
+          if (have && t * kTK + 32 * h + lane < pc.keys) {
+            blk[h] = table[col[h]];
+            if (blk[h] < 0) blk[h] = INT32_MAX;
           }
         }
       };
+      if (have) begin();
       fetch();
-      while (ok && is[0]) {
-        int64_t off[2][2];
-        bool is1 = is[1], tree_of[2] = {tree[0], tree[1]};
+      while (have) {
+        uint32_t row[2], there[2], len[2];
+        // keys that stand one after the other (in a half of the tile) go in
+        // one copy, whatever the block size: bytes from this lane's key on,
+        // 0 where an earlier lane's copy brings it
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            off[e][h] = -1;
-            if (blk[e][h] >= 0) {
-              if (blk[e][h] < a.num_blocks)
-                off[e][h] = ((((blk[e][h] * a.num_layers + a.layer) * 2) * a.hkv + hk[e]) * a.bs + rest[e][h]) * D;
-              else
-                bad = true;
-            }
-          }
-        fetch();
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (!ok || (e == 1 && !is1)) continue;
-          const int st = done % NST, mt = done % kMeta;
-          const uint32_t ph = ((done / NST) - 1) & 1;
-          // keys that stand one after the other (in a half of the tile) go in
-          // one copy, whatever the block size: bytes from this lane's key on,
-          // 0 where an earlier lane's copy brings it
-          uint32_t len[2], there[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int64_t before = __shfl_up_sync(0xffffffffu, off[e][h], 1);
-            const bool on = off[e][h] >= 0, follows = on && lane > 0 && before >= 0 && off[e][h] == before + D;
-            there[h] = __ballot_sync(0xffffffffu, on);
-            const uint32_t chain = __ballot_sync(0xffffffffu, follows);
-            len[h] = on && !follows ? (lane == 31 ? 1u : static_cast<uint32_t>(__ffs(static_cast<int>(~(chain >> (lane + 1)))))) * (D * 4) : 0u;
-          }
-          const uint32_t bytes = static_cast<uint32_t>(__popc(there[0]) + __popc(there[1])) * D * 4;
-          if (done >= NST && !(ok = wait(freed + st, ph))) continue;
-          {                                         // both warps the same
-            if (lane < 8)
-              valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
-            if (lane == 0) tree_s[mt * 8] = tree_of[e] ? 1 : 0;
-            __syncwarp();
-          }
-          if (lane == 0) mbar_arrive_expect_tx(rfull + st, bytes);
-          __syncwarp();
-          uint8_t* dst = base + st * 2 * L::TERM + lane * D * 4;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (len[h]) copy_bulk(dst + 32 * h * D * 4, src + off[e][h], len[h], rfull + st);
-          ++done;
+        for (int h = 0; h < 2; ++h) {
+          const bool on = blk[h] >= 0 && blk[h] < a.num_blocks;
+          bad = bad || (blk[h] >= 0 && !on);
+          row[h] = static_cast<uint32_t>(blk[h]) * rows_per_block + row0 + static_cast<uint32_t>(rest[h]);
+          there[h] = __ballot_sync(0xffffffffu, on);
+          const uint32_t before = __shfl_up_sync(0xffffffffu, row[h], 1);
+          const bool follows = on && ((there[h] << 1) >> lane & 1) && row[h] == before + 1;
+          const uint32_t chain = __ballot_sync(0xffffffffu, follows);
+          // the lanes after this one that follow on; none past lane 31
+          len[h] = on && !follows ? static_cast<uint32_t>(__ffs(static_cast<int>(~((chain >> lane) >> 1)))) * (D * 4) : 0u;
         }
+        const bool tree = (t + 1) * kTK > pc.pre;
+        if (++t < pc.t1) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            col[h] += dj;
+            rest[h] += dr;
+            if (rest[h] >= bs) rest[h] -= bs, ++col[h];
+          }
+        } else {
+          have = next_piece(a, wk, &pc);
+          if (have) begin();
+        }
+        fetch();
+        const int st = done % NST, mt = done % kMeta;
+        const uint32_t bytes = static_cast<uint32_t>(__popc(there[0]) + __popc(there[1])) * D * 4;
+        if (done >= NST && !wait(freed + st, ((done / NST) - 1) & 1)) break;
+        if (lane < 8)                               // both warps the same
+          valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
+        if (lane == 0) tree_s[mt * 8] = tree ? 1 : 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(rfull + st, bytes);
+        __syncwarp();
+        uint8_t* dst = base + st * 2 * L::TERM + lane * D * 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (len[h]) copy_bulk(dst + 32 * h * D * 4, src + static_cast<int64_t>(row[h]) * D, len[h], rfull + st);
+        ++done;
       }
       // after an abort, let the copies still in flight land before the CTA exits
       if (*abort_flag)
@@ -1215,6 +1213,10 @@ extern "C" int ksh_tree_attention(const float* q, int64_t total, int64_t hq, int
   if (num_seqs == 0 || total == 0 || max_nodes == 0) return KSH_OK;
   KSH_CHECK_ARG(q && pool && block_tables && q_start && prefix_lens && out);
   if (d > 256 || max_nodes > kMaxWords * 64 || (mask && mask_words > kMaxWords))
+    return KSH_ERR_UNSUPPORTED;
+  // K/V rows are numbered in 32 bits (2^31 rows of 64 floats are 512 GB)
+  if (static_cast<double>(num_blocks) * 2.0 * static_cast<double>(num_layers) * static_cast<double>(hkv) *
+          static_cast<double>(block_size) > static_cast<double>(INT32_MAX))
     return KSH_ERR_UNSUPPORTED;
   TreeArgs a = {};
   a.q = q;
