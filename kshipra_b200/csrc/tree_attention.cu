@@ -66,6 +66,7 @@ struct TreeArgs {
   float* part;                  // [gridDim.x][2] partial states
   int64_t total, num_blocks, num_layers, layer, hkv, hq, bs, max_blocks;
   int num_seqs, words, g, d, max_nodes;
+  int item_cost;                // units an item's start counts for, beside its tiles
   float scale;
 };
 
@@ -85,6 +86,12 @@ constexpr int kRowWarps = 8, kWideWarps = 8;
 constexpr int kMmaWarp = kRowWarps + kWideWarps, kCopyWarp = kMmaWarp + 1;
 constexpr int kTcThreads = 32 * (kRowWarps + kWideWarps + 4);   // an idle warp fills the last warpgroup
 constexpr int kGroup = 8, kGroups = kTK / kGroup;    // keys that share a scale
+// An item's start (its Q, an empty pipeline, the state written out) takes about
+// four tiles' time; counted so in the line, the CTAs with two items are not the
+// last ones.  24 sequences of 20 x 7 rows over up to 3000 keys of D = 64: 44 us,
+// 48 with no such count.  Where there are fewer tiles than SMs can share out
+// (4 a CTA) it would only put more tiles into some CTAs.
+constexpr int kItemCost = 4;
 constexpr int kMeta = 16;                // tiles whose scales are kept: more than the stages let run apart
 
 // floats of one partial state: m [128], l [128], acc [D / 4][128][4]
@@ -122,9 +129,6 @@ struct SeqWork {
   int64_t a0;
   int nq, keys, pre, ntiles, nqt;
   bool bad;                     // lengths that do not fit
-  __device__ __forceinline__ int64_t units(int64_t hkv) const {
-    return hkv * nqt * static_cast<int64_t>(ntiles);
-  }
 };
 
 __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s) {
@@ -144,12 +148,13 @@ __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s) {
   return w;
 }
 
-// The pieces of items in one CTA's share [u, u_end) of the line, one after
-// the other.  Each warp keeps its own walk in shared memory (registers are
-// for the tiles).
+// The pieces of items in one CTA's share of the line, one after the other.
+// Each warp keeps its own walk in shared memory (registers are for the tiles);
+// a step is additions, and loads only where a new sequence begins.
 struct Walk {
-  int64_t u, u_end, base;       // base: first unit of sequence s
-  int s;
+  SeqWork w;                    // of sequence s
+  int64_t left;                 // units of the share still to go
+  int s, item, t;               // t: next tile of the item
 };
 struct Piece {
   int64_t a0;
@@ -158,25 +163,29 @@ struct Piece {
 
 __device__ __forceinline__ bool next_piece(const TreeArgs& a, Walk* wk, Piece* p) {
   Walk k = *wk;
-  if (k.u >= k.u_end) return false;
-  SeqWork w = seq_work(a, k.s);
-  while (k.u >= k.base + w.units(a.hkv)) {
-    k.base += w.units(a.hkv);
-    w = seq_work(a, ++k.s);
+  if (k.left <= 0) return false;
+  if (k.t == k.w.ntiles) {
+    k.t = 0;
+    ++k.item;
+    k.left -= a.item_cost;
+    if (k.left <= 0) return false;
+    if (k.item == static_cast<int>(a.hkv) * k.w.nqt) {
+      k.item = 0;
+      do k.w = seq_work(a, ++k.s);
+      while (k.w.nqt == 0);
+    }
   }
-  const uint32_t rel = static_cast<uint32_t>(k.u - k.base);    // a sequence's tiles fit 32 bits
-  const int item = static_cast<int>(rel / static_cast<uint32_t>(w.ntiles));
-  p->t0 = static_cast<int>(rel - static_cast<uint32_t>(item) * w.ntiles);
-  p->t1 = static_cast<int>(min(static_cast<int64_t>(w.ntiles), p->t0 + (k.u_end - k.u)));
-  p->hk = item / w.nqt;
-  p->qt = item - p->hk * w.nqt;
+  p->t0 = k.t;
+  p->t1 = k.t = static_cast<int>(min(static_cast<int64_t>(k.w.ntiles), k.t + k.left));
+  k.left -= p->t1 - p->t0;
+  p->hk = k.w.nqt == 1 ? k.item : k.item / k.w.nqt;
+  p->qt = k.item - p->hk * k.w.nqt;
   p->s = k.s;
-  p->a0 = w.a0;
-  p->nq = w.nq;
-  p->keys = w.keys;
-  p->pre = w.pre;
-  p->ntiles = w.ntiles;
-  k.u += p->t1 - p->t0;
+  p->a0 = k.w.a0;
+  p->nq = k.w.nq;
+  p->keys = k.w.keys;
+  p->pre = k.w.pre;
+  p->ntiles = k.w.ntiles;
   __syncwarp();
   if ((threadIdx.x & 31) == 0) *wk = k;
   __syncwarp();
@@ -309,6 +318,27 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Four lanes with element k of row i each (i = 0..3 in x[i], k = lane & 3) change
+// to row k's elements in each lane.  Its own inverse.
+__device__ __forceinline__ void exchange4(float4 (&x)[4], int lane) {
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(i & o)) {
+        const bool up = lane & o;
+        float4 s = up ? x[i] : x[i + o];
+        s.x = __shfl_xor_sync(0xffffffffu, s.x, o);
+        s.y = __shfl_xor_sync(0xffffffffu, s.y, o);
+        s.z = __shfl_xor_sync(0xffffffffu, s.z, o);
+        s.w = __shfl_xor_sync(0xffffffffu, s.w, o);
+        if (up)
+          x[i] = s;
+        else
+          x[i + o] = s;
+      }
+}
+
 // Operand descriptor, 128-byte swizzle, 1024-byte blocks of eight 128-byte
 // rows.  K-major (K): `groups` bytes from eight rows to the next eight.
 // MN-major (V): a row holds 64 of the N columns; `groups` bytes from eight rows
@@ -366,10 +396,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   uint64_t* drain = lready + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s0_s = reinterpret_cast<int*>(tmem_slot + 2);
-  int64_t* line_s = reinterpret_cast<int64_t*>(tmem_slot + 4);   // U, base of s0
   __shared__ int64_t scan_s[kTcThreads / 32];
-  __shared__ Walk walk_s[kTcThreads / 32];
+  __shared__ Walk walk_s[kTcThreads / 32], start_s;
   __shared__ float lsum_s[2][2][kRows];     // the halves' sums, by piece parity
   __shared__ SplitItem cut_s;
   __shared__ Piece piece_s[kRowWarps];
@@ -394,7 +422,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     mbar_init(lready, kRowWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
-    *s0_s = 0;
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -405,20 +432,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   grid_dep_wait();
   grid_dep_launch();
 
-  // The line of tiles: its length, and the sequence where this CTA's share
-  // starts.
-  int64_t U = 0, u0 = 0, G = 1;                   // CTAs that get tiles
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t carry = 0;
-    for (int b = 0; b < a.num_seqs; b += kTcThreads) {
-      const int s = b + tid;
-      int64_t v = 0;
-      if (s < a.num_seqs) {
-        const SeqWork w = seq_work(a, s);
-        v = w.units(a.hkv);
-        if (pass == 0 && blockIdx.x == 0 && w.bad) raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
+  // Q into L2 while the memory is idle: behind the K/V copies a row takes
+  // thousands of cycles
+  {
+    const int64_t bytes = a.total * a.hq * D * 4, each = (bytes / gridDim.x + 15) & ~int64_t(15);
+    const int64_t lo = each * blockIdx.x;
+    if (lo < bytes)
+      prefetch_range_l2(reinterpret_cast<const uint8_t*>(a.q) + lo,
+                        static_cast<size_t>(min(each, bytes - lo)), tid, kTcThreads);
+  }
+
+  // The line of tiles: its length, and the place where this CTA's share
+  // starts.  An item's start counts as item_cost units.
+  int64_t u0 = 0, q = 0, r = 0;                   // q units a CTA, one more for the first r
+  {
+    SeqWork w = {};
+    int64_t v = 0, inc = 0, carry = 0;
+    auto scan = [&](int b, bool first) {          // of kTcThreads sequences from b on
+      w = {};
+      v = 0;
+      if (b + tid < a.num_seqs) {
+        w = seq_work(a, b + tid);
+        v = a.hkv * w.nqt * (static_cast<int64_t>(w.ntiles) + a.item_cost);
+        if (first && blockIdx.x == 0 && w.bad) raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
       }
-      int64_t inc = v;
+      inc = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
@@ -427,38 +465,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
       __syncthreads();
       if (lane == 31) scan_s[warp] = inc;
       __syncthreads();
+      const int warps = min(kTcThreads / 32, (a.num_seqs - b + 31) / 32);
       int64_t before = carry;
-      for (int w = 0; w < kTcThreads / 32; ++w) {
-        if (w < warp) before += scan_s[w];
-        carry += scan_s[w];
+      for (int i = 0; i < warps; ++i) {
+        if (i < warp) before += scan_s[i];
+        carry += scan_s[i];
       }
       inc += before;
-      if (pass == 1 && v > 0 && u0 >= inc - v && u0 < inc) {
-        *s0_s = s;
-        line_s[1] = inc - v;
+    };
+    auto find = [&](int b) {
+      if (v > 0 && u0 >= inc - v && u0 < inc) {
+        const int64_t rel = u0 - (inc - v), len = w.ntiles + a.item_cost;
+        const int64_t item = (rel >> 32) ? rel / len : static_cast<uint32_t>(rel) / static_cast<uint32_t>(len);
+        const int at = static_cast<int>(rel - item * len) - a.item_cost;
+        start_s.w = w;
+        start_s.left = q + (blockIdx.x < r ? 1 : 0) + min(at, 0);
+        start_s.s = b + tid;
+        start_s.item = static_cast<int>(item);
+        start_s.t = max(at, 0);
       }
-    }
-    if (pass == 0) {
-      U = carry;
-      G = max(min(static_cast<int64_t>(gridDim.x), U), int64_t(1));
-      u0 = min(static_cast<int64_t>(blockIdx.x), G) * U / G;
+    };
+    if (tid == 0) start_s.left = 0;
+    for (int b = 0; b < a.num_seqs; b += kTcThreads) scan(b, true);
+    const int64_t U = carry, G = max(min(static_cast<int64_t>(gridDim.x), U), int64_t(1));
+    q = (U >> 32) ? U / G : static_cast<uint32_t>(U) / static_cast<uint32_t>(G);
+    r = U - q * G;
+    u0 = blockIdx.x * q + min(static_cast<int64_t>(blockIdx.x), r);
+    if (blockIdx.x < G) {
+      if (a.num_seqs <= kTcThreads) {
+        find(0);
+      } else {
+        carry = 0;
+        for (int b = 0; b < a.num_seqs; b += kTcThreads) scan(b, false), find(b);
+      }
     }
   }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int64_t u1 = min(static_cast<int64_t>(blockIdx.x) + 1, G) * U / G;
   Walk* const wk = &walk_s[warp];
-  if (lane == 0) {
-    Walk k = {};
-    k.u = u0;
-    k.u_end = u1;
-    if (u0 < u1) {
-      k.s = *s0_s;
-      k.base = line_s[1];
-    }
-    *wk = k;
-  }
+  if (lane == 0) *wk = start_s;
   if (tid == 0) cut_s.first = 0, cut_s.last = -1;
   __syncwarp();
   Piece pc = {};
@@ -656,10 +702,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     const int ln = D == 128 ? lane : lane & 15;     // float4 column of the row
     const uint32_t block = static_cast<uint32_t>(ln >> 4) * 1024;
     const uint32_t chunk = static_cast<uint32_t>((ln & 15) >> 1), word = static_cast<uint32_t>(ln & 1) * 8;
-    const int ntl = static_cast<int>(u1 - u0);      // tiles of this CTA
     bool ok = true;
 #pragma unroll 1
-    for (int n = 0; n < ntl; ++n) {
+    for (int n = 0; ok && next_piece(a, wk, &pc);)
+    for (int end = n + pc.t1 - pc.t0; n < end; ++n) {
       const int st = n % NST, mt = n % kMeta;
       if (!(ok = wait(rfull + st, (n / NST) & 1))) break;
       const bool tree = tree_s[mt * 8] != 0;
@@ -763,30 +809,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
         return ((ps.a0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
       };
       float qinv;
-      // Q: hi / lo terms of the half's columns into TMEM
+      // Q: hi / lo terms of the half's columns into TMEM.  Four lanes load 64
+      // bytes of a row, for the rows of the four, and exchange them (a row a
+      // lane took 32 lines a load, 8 K cycles an item)
       {
-        const float* qp = a.q + row_at();
-        auto quad = [&](int c) {
-          return live ? *reinterpret_cast<const float4*>(qp + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        float top = 0.0f, qs;
-#pragma unroll 8
-        for (int c = 0; c < D; c += 4) {
-          const float4 v = quad(c);
-          top = amax3(top, amax3(v.x, v.y, v.z), v.w);
+        const float* qp[4];
+        float m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int R = pc.qt * kRows + (row & ~3) + k, node = R / a.g;
+          qp[k] = node < pc.nq ? a.q + ((pc.a0 + node) * a.hq + static_cast<int64_t>(pc.hk) * a.g + (R - node * a.g)) * D +
+                                     (lane & 3) * 4
+                               : nullptr;
+          m[k] = 0.0f;
         }
+        auto quad = [&](int k, int c) {
+          return qp[k] ? *reinterpret_cast<const float4*>(qp[k] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        float4 v[DH / 4];
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {      // the other half's for the maximum alone
+#pragma unroll
+          for (int c = 0; c < DH / 4; ++c) v[c] = quad(c & 3, (hw ^ half) * DH + (c >> 2) * 16);
+#pragma unroll
+          for (int c = 0; c < DH / 4; ++c)
+            m[c & 3] = amax3(amax3(m[c & 3], v[c].x, v[c].y), v[c].z, v[c].w);
+        }
+        // the four lanes' maxima of the lane's row
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) m[k] = amax3(m[k], __shfl_xor_sync(0xffffffffu, m[k], o), 0.0f);
+        const float top = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
+        float qs;
         pow2_scale(top, &qs, &qinv);
-#pragma unroll 1
-        for (int c0 = 0; c0 < DH; c0 += 32) {
+#pragma unroll
+        for (int c0 = 0; c0 < DH / 4; c0 += 8) {
           uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 v = quad(hw * DH + c0 + c);
-            split2(mul2(f2(v.x, v.y), f2(qs, qs)), &hi[c / 2], &lo[c / 2]);
-            split2(mul2(f2(v.z, v.w), f2(qs, qs)), &hi[c / 2 + 1], &lo[c / 2 + 1]);
+          for (int c = c0; c < c0 + 8; c += 4) {
+            float4 x[4] = {v[c], v[c + 1], v[c + 2], v[c + 3]};
+            exchange4(x, lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = (c - c0 + k) * 2;
+              split2(mul2(f2(x[k].x, x[k].y), f2(qs, qs)), &hi[at], &lo[at]);
+              split2(mul2(f2(x[k].z, x[k].w), f2(qs, qs)), &hi[at + 1], &lo[at + 1]);
+            }
           }
-          tmem_st_32x32b_x16(lanes + L::Q_COL + (hw * DH + c0) / 2, hi);
-          tmem_st_32x32b_x16(lanes + L::Q_COL + DH + (hw * DH + c0) / 2, lo);
+          tmem_st_32x32b_x16(lanes + L::Q_COL + (hw * DH + c0 * 4) / 2, hi);
+          tmem_st_32x32b_x16(lanes + L::Q_COL + DH + (hw * DH + c0 * 4) / 2, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -1014,16 +1086,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
       ++seg;
       const bool whole = t0 == 0 && t1 == ps.ntiles;
       if (whole) {
-        if (live) {
-          const float inv = 1.0f / l;
-          float* op = a.out + row_at() + hw * DH;
+        const float inv = 1.0f / l;
+        float* op[4];
 #pragma unroll
-          for (int c = 0; c < DH; c += 4) {
-            const float2 p = unpack(acc[c / 2]), q = unpack(acc[c / 2 + 1]);
-            float4 v = make_float4(p.x * inv, p.y * inv, q.x * inv, q.y * inv);
-            if (l == 0.0f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(op + c) = v;
+        for (int k = 0; k < 4; ++k) {
+          const int R = ps.qt * kRows + (row & ~3) + k, node = R / a.g;
+          op[k] = node < ps.nq ? a.out + ((ps.a0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D +
+                                     hw * DH + (lane & 3) * 4
+                               : nullptr;
+        }
+#pragma unroll
+        for (int c = 0; c < DH; c += 16) {
+          float4 x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 p = unpack(acc[c / 2 + 2 * k]), u = unpack(acc[c / 2 + 2 * k + 1]);
+            x[k] = make_float4(p.x * inv, p.y * inv, u.x * inv, u.y * inv);
+            if (l == 0.0f) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
+          exchange4(x, lane);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (op[k]) *reinterpret_cast<float4*>(op[k] + c) = x[k];
         }
       } else {
         float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * part_floats<D>();
@@ -1039,9 +1123,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
           }
         }
         if (t0 == 0 && tid == 0) {                 // the share's last piece: joined from here on
-          const int64_t end = wk->u + (ps.ntiles - t1);          // past the item's last unit
+          const int64_t x = u0 + q + (blockIdx.x < r ? 1 : 0) + (ps.ntiles - t1) - 1;   // the item's last unit
           cut_s.first = static_cast<int>(blockIdx.x);
-          cut_s.last = static_cast<int>((end * G - 1) / U);
+          cut_s.last = static_cast<int>(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
           cut_s.row0 = static_cast<int>(ps.a0);
           cut_s.rbase = ps.qt * kRows;
           cut_s.rows = min(kRows, ps.nq * a.g - ps.qt * kRows);
@@ -1249,12 +1333,14 @@ extern "C" int ksh_tree_attention(const float* q, int64_t total, int64_t hq, int
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return KSH_ERR_ALIGN;
     a.items = static_cast<SplitItem*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + items_bytes());
-    // no more CTAs than there can be tiles
+    // No more CTAs than there can be tiles.
     const int64_t tiles = std::max<int64_t>(1, (max_total_len + kTK - 1) / kTK);
     const int64_t qtiles = (max_nodes * a.g + kRows - 1) / kRows;
     const int grid = static_cast<int>(std::min<double>(
         num_sms(), static_cast<double>(num_seqs) * static_cast<double>(hkv) * static_cast<double>(qtiles) *
                        static_cast<double>(tiles)));
+    a.item_cost = static_cast<double>(num_seqs) * static_cast<double>(hkv) * static_cast<double>(qtiles) *
+                      static_cast<double>(tiles) >= 4.0 * num_sms() ? kItemCost : 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return d == 64 ? launch_tree_tc<64>(a, grid, st) : launch_tree_tc<128>(a, grid, st);
   }
