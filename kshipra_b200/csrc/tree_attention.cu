@@ -872,6 +872,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
         return bits <= 0 ? 0 : bits >= 64 ? ~0ull : (1ull << bits) - 1;
       };
       const float cq = qinv * (a.scale * 1.44269504088896340736f);   // to powers of two
+      if ((pc.qt * kRows + (warp & 3) * 32) / a.g >= pc.nq) {
+        // No row of the warp's is live: zeros for P once (multiplying them costs
+        // the tensor cores no power, and power bounds long runs), then it only
+        // keeps step.
+        uint32_t zero[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) zero[c] = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int c = 0; c < 32; c += 16) tmem_st_32x32b_x16(lanes + L::P_COL + b * kTK + 32 * hw + c, zero);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+#pragma unroll 1
+        for (int t = t0; t <= t1; ++t, ++n) {
+          if (t < t1) {
+            if (!(ok = wait(&sfull[n & 1], (n >> 1) & 1))) break;
+            if (lane == 0) mbar_arrive(&pready[n & 1]);
+          }
+          if (t > t0) {
+            if (!(ok = wait(ofull, (n - 1) & 1))) break;
+            if (lane == 0) mbar_arrive(oempty);
+          }
+        }
+        if (!ok) break;
+        --n;
+        if (lane == 0) mbar_arrive(lready);
+        if (!(ok = wait(lready, seg & 1))) break;
+        ++seg;
+        continue;
+      }
       // running state: the reference that the sums stand at (in powers of two;
       // it follows the maximum once that is 2^8 above it, so most tiles
       // rescale nothing), the half's sum
