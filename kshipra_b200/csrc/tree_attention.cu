@@ -112,7 +112,7 @@ struct TreeLayout {
   // per tile (ring of kMeta): inverse scales of K and V per group of eight
   // keys, and per key relative to that (tiles with drafted nodes)
   static constexpr int META = V_OFF + NST * 2 * TERM;    // kinv, vinv [8], krel, vrel [64]
-  static constexpr int BITS = META + 2 * kMeta * (kGroups + kTK) * 4;   // valid, kpois, vpois, tree [8]
+  static constexpr int BITS = META + 2 * kMeta * (kGroups + kTK) * 4;   // valid, kpois, vpois, tile [8]
   static constexpr int BAR = BITS + 4 * kMeta * 8;
   static constexpr int NBAR = 6 * NST + 2 * 2 + 5;
   static constexpr int MISC = BAR + NBAR * 8;
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   uint8_t* valid_s = smem + L::BITS;                           // [kMeta][8]: bits of the groups' keys
   uint8_t* kpois_s = valid_s + kMeta * 8;
   uint8_t* vpois_s = kpois_s + kMeta * 8;
-  uint8_t* tree_s = vpois_s + kMeta * 8;
+  uint8_t* tile_s = vpois_s + kMeta * 8;                   // 1: drafted nodes, 2: the CTA's last
   uint64_t* rkfull = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* rvfull = rkfull + NST;
   uint64_t* kfull = rvfull + NST;
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
         if (done >= NST && !wait(freed + st, ((done / NST) - 1) & 1)) break;
         if (lane < 8)                               // both warps the same
           valid_s[mt * 8 + lane] = static_cast<uint8_t>((lane < 4 ? there[0] : there[1]) >> (8 * (lane & 3)));
-        if (lane == 0) tree_s[mt * 8] = tree ? 1 : 0;
+        if (lane == 0) tile_s[mt * 8] = static_cast<uint8_t>((tree ? 1 : 0) | (have ? 0 : 2));
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(rfull + st, bytes);
         __syncwarp();
@@ -702,13 +702,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     const int ln = D == 128 ? lane : lane & 15;     // float4 column of the row
     const uint32_t block = static_cast<uint32_t>(ln >> 4) * 1024;
     const uint32_t chunk = static_cast<uint32_t>((ln & 15) >> 1), word = static_cast<uint32_t>(ln & 1) * 8;
-    bool ok = true;
+    bool more = wk->left > 0;
 #pragma unroll 1
-    for (int n = 0; ok && next_piece(a, wk, &pc);)
-    for (int end = n + pc.t1 - pc.t0; n < end; ++n) {
+    for (int n = 0; more; ++n) {
       const int st = n % NST, mt = n % kMeta;
-      if (!(ok = wait(rfull + st, (n / NST) & 1))) break;
-      const bool tree = tree_s[mt * 8] != 0;
+      if (!wait(rfull + st, (n / NST) & 1)) break;
+      more = !(tile_s[mt * 8] & 2);
+      const bool tree = tile_s[mt * 8] & 1;
 #pragma unroll 1
       for (int ww = w2; ww < w2 + 2; ++ww) {
         const uint32_t valid = valid_s[mt * 8 + ww];
