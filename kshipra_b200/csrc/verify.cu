@@ -394,10 +394,10 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) 
   };
   int turn = 0;
   // Sums of every piece into all CTAs' part_s[turn], of the piece's 512-element
-  // steps into step_s; the row's sum.
+  // steps into step_s where the search will need them; the row's sum.
   double cum[4];                            // lane: sums up to its (size / 2) pieces
   const int per_slot = (a.chunk + 512 * kSlots - 1) / (512 * kSlots);   // steps that share a slot
-  auto total = [&]() -> double {
+  auto total = [&](bool steps) -> double {
     int lo, hi;
     piece(static_cast<int>(rank) * kVerWarps + warp, &lo, &hi);
     const bool vec = aligned();
@@ -406,8 +406,9 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) 
     for (int i = lo; i < hi; i += 512) {
       double v[16];
       rest16(i + 4 * lane, 128, hi, vec, v);
-      slot += warp_sum_f64(sum16(v));
-      if (++n_in == per_slot || i + 512 >= hi) {
+      slot += sum16(v);
+      if (steps && (++n_in == per_slot || i + 512 >= hi)) {
+        slot = warp_sum_f64(slot);
         if (lane == 0) step_s[warp][at] = slot;
         sum += slot;
         slot = 0.0;
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) 
         ++at;
       }
     }
+    if (!steps) sum = warp_sum_f64(slot);
     turn ^= 1;
     if (!joined) cluster_joined();
     joined = true;
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) 
       yes = u_s[i] != 0.0f;
     } else {
       if (MODE == MODE_DRAWN && stale) {
-        z = total();
+        z = total(false);
         stale = false;
       }
       const int t = tok_s[i];
@@ -496,10 +498,10 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) 
     if (first && tid == 0) a.next[s] = a.greedy[a0 + cur];
     return;
   }
-  double sum = total();
+  double sum = total(true);
   if (!(sum > 0.0)) {                       // nothing left: the node's own row
     row_of(cur);
-    sum = total();
+    sum = total(true);
   }
   if (!(sum > 0.0)) {
     if (first && tid == 0) {
