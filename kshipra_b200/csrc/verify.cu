@@ -283,6 +283,11 @@ struct Rest {
 // cluster's warps, each with a contiguous piece, and the pieces' sums go to
 // every CTA through distributed shared memory.  Only the rows that a sum is
 // needed of are read, 512 elements of the last one twice.
+// 64 sequences x 128256, drawn proposals, 8 nodes: 27 us back to back against
+// 10 us for one reading of each final pair of rows: a refusal's sum needs the one
+// before it, and each is a pass of about 4 us over the row (now in L2) and the
+// cluster.  One sequence x 151936, fixed proposals: 12 us, latency; the call's
+// 15 us are the host's.
 template <int MODE>
 __global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) {
   __shared__ int tok_s[kMaxNodes], par_s[kMaxNodes], path_s[kMaxNodes], gone_s[kMaxNodes];

@@ -402,6 +402,37 @@ def test_target_probs(vocab):
     assert torch.equal(sp.target_probs(xd, t.cuda(), out=xd).cpu().double(), got)
 
 
+@pytest.mark.parametrize("m,vocab", [(601, 1000), (1300, 3), (2400, 6), (600, 20483), (151, 39998), (83, 151936)])
+def test_target_probs_many_rows(m, vocab):
+    """Rows on 16-byte boundaries and not give the same bits, however many."""
+    g = torch.Generator().manual_seed(m)
+    width = (vocab + 3) // 4 * 4 + 4
+    x = (torch.randn((m, width), generator=g) * 5).cuda()
+    x[3, :vocab] = float("-inf")
+    x[4, vocab // 2] = float("nan")
+    x[5, :vocab // 2] = float("-inf")
+    t = (torch.rand(m, generator=g) + 0.5).cuda()
+    t[::7] = 0.0
+    out = torch.full_like(x, -1.0)
+    sp.target_probs(x[:, :vocab], t, out=out[:, :vocab])
+    assert (out[:, vocab:] == -1).all()
+    off = torch.empty((m, width + 1), device="cuda")
+    off[:, 1:1 + vocab] = x[:, :vocab]
+    want = sp.target_probs(off[:, 1:1 + vocab], t)
+    assert torch.equal(out[:, :vocab].nan_to_num(7.0), want.nan_to_num(7.0))
+    for r in (0, 1, 2, 5, 14, m - 2, m - 1):
+        row = x[r, :vocab].cpu().double()
+        if float(t[r]) > 0:
+            ref = torch.softmax((row - row.max()) / t[r].cpu().double(), 0)
+            assert ((out[r, :vocab].cpu().double() - ref).abs() <= 1e-5 * ref + 1e-37).all(), r
+        else:
+            assert out[r, :vocab].nonzero().view(-1).tolist() == [int(row.argmax())]
+    assert torch.isnan(out[3, :vocab]).all() and torch.isnan(out[4, :vocab]).all()
+    same = x.clone()
+    sp.target_probs(same[:, :vocab], t, out=same[:, :vocab])
+    assert torch.equal(same[:, :vocab].nan_to_num(7.0), want.nan_to_num(7.0))
+
+
 def test_target_probs_not_finite_rows():
     x = torch.zeros((4, 200))
     x[0, 5] = float("nan")
