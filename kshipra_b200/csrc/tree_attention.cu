@@ -185,8 +185,10 @@ __device__ __forceinline__ bool next_piece(const TreeArgs& a, Walk* wk, Piece* p
     if (k.left <= 0) return false;
     if (k.item == static_cast<int>(a.hkv) * k.w.nqt) {
       k.item = 0;
-      do k.w = seq_work(a, ++k.s);
-      while (k.w.nqt == 0);
+      do {
+        if (++k.s >= a.num_seqs) return false;    // lengths that changed on the way
+        k.w = seq_work(a, k.s);
+      } while (k.w.nqt == 0);
     }
   }
   p->t0 = k.t;

@@ -57,7 +57,8 @@ def test_argument_errors_are_reported_without_a_launch():
     h = _lib.lib()
     for kw, st in ((dict(hq=5), -1), (dict(layer=1), -1), (dict(bs=0), -1), (dict(q=None), -1),
                    (dict(mask=FAKE, words=0), -1), (dict(d=257), -4), (dict(nodes=257), -4),
-                   (dict(words=5), -4), (dict(total=-1), -1)):
+                   (dict(words=5), -4), (dict(total=-1), -1), (dict(bs=1 << 31), -1),
+                   (dict(nb=1 << 30), -4)):     # K/V rows numbered in 32 bits
         assert attention(h, **kw) == st, kw
     # nothing to do is no error
     for kw in (dict(seqs=0), dict(total=0), dict(nodes=0)):

@@ -357,6 +357,19 @@ def test_tree_attention_offsets_past_32_bits():
     assert torch.equal(pool[blocks[2], :, :, :, 151 % 64], before)
 
 
+@pytest.mark.parametrize("seqs,hq,hkv,d,deep,nodes", [
+    (130, 6, 2, 64, 200, 5), (700, 4, 2, 64, 90, 3), (700, 2, 1, 128, 90, 3), (24, 16, 2, 64, 900, 30),
+    (9, 16, 2, 128, 1900, 40)])
+def test_tree_attention_many_items(seqs, hq, hkv, d, deep, nodes):
+    """Lines of many items, cut anywhere; sequences without nodes among them."""
+    rs = np.random.RandomState(seqs + d)
+    pre, lens = rs.randint(0, deep, seqs), rs.randint(0, nodes + 1, seqs)
+    lens[seqs // 2] = nodes
+    c = Case(pre.tolist(), lens.tolist(), hq, hkv, d, 16, seed=seqs, layers=1)
+    c.check()
+    assert torch.equal(c.run()[0], c.run()[0])
+
+
 def test_tree_attention_graph_replay_follows_device_lengths():
     c = Case([200, 90], [8, 8], 8, 2, 64, 16, seed=6)
     args = [c.q.cuda(), c.pool.nan_to_num(0.0).cuda(), c.layer, i32(c.bt), i32(c.qs), i32(c.pre), c.mask.cuda(), 8, 208]
