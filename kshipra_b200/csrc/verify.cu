@@ -58,14 +58,17 @@ __device__ __forceinline__ int head_of(const float* row) {
 // ---------------------------------------------------------------------------
 // One row per cluster: each CTA keeps its part of the row in shared memory,
 // so the row is read once and written once; the maximum and the sum cross the
-// cluster through distributed shared memory.  512 x 128256: 123 us, 4.3 TB/s,
-// 65 % of measured HBM; its waves of clusters read, wait for each other and
-// write, and three CTAs of 384 threads per SM overlap these best (512 threads
-// 147 us, 256 threads 133; exponentials four at a time change nothing).  One
-// CTA per row reading it three times: 23 %.
+// cluster through distributed shared memory.  512 x 128256: 109 us, 4.8 TB/s,
+// 74 % of measured HBM; clusters read, wait for each other and write in waves,
+// and three CTAs per SM overlap these.  The part comes by bulk copies (through
+// registers, where three CTAs of 384 threads hold two thirds of it in flight:
+// 110 us, with half of those 131; CTAs of 416 threads, of which two fit: 149);
+// streaming hints on loads and stores cost 2 us; clusters of 16 with parts half
+// as large: 115 us.  One CTA per row reading it three times: 23 %.
 
 constexpr int kProbThreads = 384;
 constexpr int kProbWarps = kProbThreads / 32;
+constexpr int kProbCopy = 1024;           // float4 of one bulk copy
 constexpr int kProbSlice = 50 * 1024;      // floats of a part, at most
 
 struct ProbArgs {
@@ -89,9 +92,15 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
   __shared__ uint64_t redk[kProbWarps];
   __shared__ float redg[kProbWarps];
   __shared__ uint64_t top_s[kMaxCluster];
+  __shared__ __align__(8) uint64_t full;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int64_t r = blockIdx.x / size;
+  if (tid == 0) {
+    mbar_init(&full, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
   cluster_join();
   grid_dep_wait();
   grid_dep_launch();
@@ -104,27 +113,32 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
   const int lo = min(a.vocab, static_cast<int>(rank) * a.chunk), hi = min(a.vocab, lo + a.chunk);
   const int a0 = min(lo + head_of(xr + lo), hi), n4 = (hi - a0) / 4, rest = a0 + 4 * n4;
   float* const s = slice + 4 - a0;
+  // all of the part on its way at once
+  if (tid < 32) {
+    if (tid == 0) mbar_arrive_expect_tx(&full, static_cast<uint32_t>(n4) * 16);
+    __syncwarp();
+    for (int i = tid * kProbCopy; i < n4; i += 32 * kProbCopy)
+      asm volatile(
+          "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+              smem_u32(s + a0 + 4 * i)),
+          "l"(xr + a0 + 4 * i), "r"(min(kProbCopy, n4 - i) * 16), "r"(smem_u32(&full))
+          : "memory");
+  }
   float m = -INFINITY;
   {
-    const float4* x4 = reinterpret_cast<const float4*>(xr + a0);
-    float4* s4 = reinterpret_cast<float4*>(s + a0);
-    for (int i0 = tid; i0 < n4; i0 += 8 * kProbThreads) {
-      float4 v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i0 + u * kProbThreads < n4) v[u] = __ldcs(x4 + i0 + u * kProbThreads);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i0 + u * kProbThreads < n4) {
-          s4[i0 + u * kProbThreads] = v[u];
-          m = fmaxf(m, fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w)));
-        }
-    }
-    // up to three elements before and after
     const int e = tid < a0 - lo ? lo + tid : (tid >= 4 && tid - 4 < hi - rest ? rest + tid - 4 : -1);
     if (e >= 0) {
       s[e] = xr[e];
-      m = fmaxf(m, s[e]);
+      m = s[e];
+    }
+  }
+  const bool came = mbar_wait(&full, 0);
+  {
+    const float4* s4 = reinterpret_cast<const float4*>(s + a0);
+#pragma unroll 4
+    for (int i = tid; i < n4; i += kProbThreads) {
+      const float4 v = s4[i];
+      m = fmaxf(m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
   }
   if (!(t <= 0.0f)) {
@@ -164,7 +178,8 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
       sum += sg * pow2((mg - M) * c);
     }
     // a row of nothing but -inf stays NaN
-    const float inv = m == -INFINITY && M != -INFINITY ? 0.0f : pow2((m - M) * c) / sum;
+    float inv = m == -INFINITY && M != -INFINITY ? 0.0f : pow2((m - M) * c) / sum;
+    if (!came) inv = NAN;
     if (((reinterpret_cast<uintptr_t>(pr) ^ reinterpret_cast<uintptr_t>(xr)) & 15) == 0) {
       float4* p4 = reinterpret_cast<float4*>(pr + a0);
       const float4* s4 = reinterpret_cast<const float4*>(s + a0);
@@ -172,7 +187,7 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
 #pragma unroll 4
       for (int i = tid; i < n4; i += kProbThreads) {
         const float4 v = s4[i];
-        __stcs(p4 + i, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        p4[i] = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       }
       if (e >= 0) pr[e] = s[e] * inv;
     } else {
@@ -194,7 +209,7 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
   cluster_sync();
   for (uint32_t c = 0; c < size; ++c) key = max(key, top_s[c]);
   const int at = static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-  for (int i = lo + tid; i < hi; i += kProbThreads) pr[i] = i == at ? 1.0f : 0.0f;
+  for (int i = lo + tid; i < hi; i += kProbThreads) pr[i] = !came ? NAN : i == at ? 1.0f : 0.0f;
 }
 
 // Rows too long for a cluster's shared memory: one CTA each, three readings.
