@@ -68,7 +68,7 @@ __device__ __forceinline__ int head_of(const float* row) {
 
 constexpr int kProbThreads = 384;
 constexpr int kProbWarps = kProbThreads / 32;
-constexpr int kProbCopy = 1024;           // float4 of one bulk copy
+constexpr int kProbCopy = 1024;            // float4 of one bulk copy
 constexpr int kProbSlice = 50 * 1024;      // floats of a part, at most
 
 struct ProbArgs {
