@@ -52,7 +52,8 @@
 // No faster: two stages of K and four of V for three and three; S and O issued
 // by two warps; one thread instead of a warp waiting and issuing (slower);
 // up to 64 rows standing twice in the lanes with half of the keys each; a
-// softmax state per half with alternating tiles (slower).
+// softmax state per half with alternating tiles (slower); at D = 64 sixteen row
+// warps, each with a quarter of the keys and of D (24 x 3000: 39 us for 35).
 
 #include <math.h>
 
