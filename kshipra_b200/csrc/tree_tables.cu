@@ -19,8 +19,8 @@
 // prefix + j in every layer.  A valid path rises, so path[j] >= j and no
 // destination is a later source: loads of several entries are in flight
 // before the first store and nothing needs a second buffer.  HBM bound: two
-// times the moved bytes; 48 sequences x 32 layers, 8 heads x 128: 19 us for
-// 84 MB, 4.4 TB/s, 68 % of measured HBM (a launch this short spends the rest
+// times the moved bytes; 48 sequences x 32 layers, 8 heads x 128: 84 MB in
+// 16 us, 5.2 TB/s, 80 % of measured HBM (a launch this short spends the rest
 // on starting and on its tail).
 
 #include "common.cuh"
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(CommitArgs 
     const int n = n_s;
     constexpr int E = sizeof(V) / 4;
     const int64_t per = a.d / E, rows = 2 * a.hkv;
-    for (int64_t x = tid; x < rows * per; x += kCommitThreads) {
+    for (int64_t x = tid; x < rows * per; x += blockDim.x) {
       const int64_t r = x / per, c = x - r * per;
       const int64_t at = r * a.bs * a.d + c * E;
       for (int k0 = 0; k0 < n; k0 += 8) {
@@ -317,7 +317,12 @@ extern "C" int ksh_tree_commit(float* pool, int64_t num_blocks, int64_t num_laye
   a.path_stride = path_stride;
   const dim3 grid(static_cast<unsigned>(num_layers), static_cast<unsigned>(num_seqs));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // More CTAs than eight per SM: half as wide, so that they still run at once
+  // (48 sequences x 32 layers, 8 heads x 128: 11.2 us from L2, 13.8 with 256
+  // threads).  With few of them the wide ones finish a token sooner (4
+  // sequences: 10.2 us cold, 12.3 with 128).
+  const dim3 block(num_layers * num_seqs > 8 * static_cast<int64_t>(num_sms()) ? kCommitThreads / 2 : kCommitThreads);
   if (d % 4 == 0 && (reinterpret_cast<uintptr_t>(pool) & 15) == 0)
-    return launch(tree_commit_kernel<float4>, grid, dim3(kCommitThreads), 0, st, a);
-  return launch(tree_commit_kernel<float>, grid, dim3(kCommitThreads), 0, st, a);
+    return launch(tree_commit_kernel<float4>, grid, block, 0, st, a);
+  return launch(tree_commit_kernel<float>, grid, block, 0, st, a);
 }

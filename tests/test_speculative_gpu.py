@@ -632,10 +632,11 @@ def test_verify_tree_edges():
 # commit
 # --------------------------------------------------------------------------- #
 
-@pytest.mark.parametrize("hkv,d,block", [(2, 64, 16), (8, 128, 16), (1, 6, 7), (3, 5, 1)])
-def test_commit_tree(hkv, d, block):
+@pytest.mark.parametrize("hkv,d,block,layers", [(2, 64, 16, 3), (8, 128, 16, 3), (1, 6, 7, 3), (3, 5, 1, 3),
+                                                (2, 24, 16, 260), (2, 6, 16, 260)])
+def test_commit_tree(hkv, d, block, layers):
     rs = np.random.RandomState(d)
-    lens, layers = [8, 1, 40, 5, 0], 3
+    lens = [8, 1, 40, 5, 0]
     pre = [13, 0, 50, 16, 4]
     need = [max(1, -(-(p + n) // block)) for p, n in zip(pre, lens)]
     nb = sum(need) + 1
