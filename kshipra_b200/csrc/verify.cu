@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_long_kernel(ProbArg
 // ---------------------------------------------------------------------------
 
 constexpr int kMaxNodes = 256;
-constexpr int kVerThreads = 512, kSlots = 32;
+constexpr int kVerThreads = 256, kSlots = 32;
 constexpr int kVerWarps = kVerThreads / 32;
 enum { MODE_GREEDY = 0, MODE_FIXED = 1, MODE_DRAWN = 2 };
 
@@ -298,13 +298,13 @@ struct Rest {
 // cluster's warps, each with a contiguous piece, and the pieces' sums go to
 // every CTA through distributed shared memory.  Only the rows that a sum is
 // needed of are read, 512 elements of the last one twice.
-// 64 sequences x 128256, drawn proposals, 8 nodes: 27 us back to back against
+// 64 sequences x 128256, drawn proposals, 8 nodes: 25 us back to back against
 // 10 us for one reading of each final pair of rows: a refusal's sum needs the one
 // before it, and each is a pass of about 4 us over the row (now in L2) and the
 // cluster.  One sequence x 151936, fixed proposals: 12 us, latency; the call's
 // 15 us are the host's.
 template <int MODE>
-__global__ void __launch_bounds__(kVerThreads, 2) verify_tree_kernel(VerArgs a) {
+__global__ void __launch_bounds__(kVerThreads, 4) verify_tree_kernel(VerArgs a) {
   __shared__ int tok_s[kMaxNodes], par_s[kMaxNodes], path_s[kMaxNodes], gone_s[kMaxNodes];
   __shared__ float u_s[kMaxNodes], p_s[kMaxNodes], q_s[kMaxNodes];
   __shared__ double part_s[2][kMaxCluster * kVerWarps], step_s[kVerWarps][kSlots];
@@ -697,10 +697,11 @@ extern "C" int ksh_verify_tree(const int64_t* tokens, const int32_t* parents,
   a.max_nodes = static_cast<int>(max_nodes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (target_tokens) return launch_cluster(verify_tree_kernel<MODE_GREEDY>, num_seqs, 1, kVerThreads, 0, st, a);
-  // CTAs per sequence: as many as run at once (two per SM), pieces of at least
-  // 128 elements a warp.  64 x 128256 drawn: 39 us with 4, 45 us with 8.
+  // CTAs per sequence: as many as run at once (four per SM), pieces of at least
+  // 256 elements a warp.  64 x 128256 drawn: 25.0 us with 8 (more even over the
+  // SMs), 27.2 with 4 of 512 threads, 31.8 with 4 of 256.
   int cluster = 1;
-  while (cluster < kMaxCluster && num_seqs * cluster <= num_sms() && vocab >= 4096LL * cluster) cluster *= 2;
+  while (cluster < kMaxCluster && num_seqs * cluster <= 2 * num_sms() && vocab >= 4096LL * cluster) cluster *= 2;
   if (num_seqs * cluster > INT32_MAX) return KSH_ERR_UNSUPPORTED;
   a.chunk = static_cast<int>(((vocab + cluster * kVerWarps - 1) / (cluster * kVerWarps) + 3) / 4 * 4);
   if (draft_probs) return launch_cluster(verify_tree_kernel<MODE_DRAWN>, num_seqs, cluster, kVerThreads, 0, st, a);
