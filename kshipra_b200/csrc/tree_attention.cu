@@ -978,6 +978,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
                 }
               }
               rare = live ? vpois & see : 0;
+              __syncwarp();                          // word() loads for live rows only
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 float y[16];
@@ -1003,6 +1004,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
                   for (int e = 0; e < 16; ++e)
                     if (e == j) y[e] += add;
                 }
+                __syncwarp();                        // lanes without a live row skipped the loop
                 const uint32_t on = static_cast<uint32_t>(see >> (16 * c));
                 const float k0 = kg[2 * c], k1 = kg[2 * c + 1];
                 uint32_t bits[16];

@@ -275,6 +275,23 @@ def test_tree_attention_nan_stays_where_it_may_be_seen(d):
         c.check(got)
 
 
+@pytest.mark.parametrize("nodes,hq,hkv,d", [(5, 7, 1, 64), (5, 14, 2, 128), (19, 7, 1, 64), (3, 4, 4, 128)])
+def test_tree_attention_nan_keys_beside_lanes_without_rows(nodes, hq, hkv, d):
+    """Warps of which only some lanes have a query row: their slow path for keys
+    that are not finite must not keep the others from the warp's TMEM accesses."""
+    g = hq // hkv
+    for pos in (3, 66, 70):                     # cached, cached in the tree's tile, the root
+        c = Case([70], [nodes], hq, hkv, d, 16, seed=nodes + d)
+        clean = c.plain()
+        c.pool[c.bt[0, pos // 16], c.layer, 0, hkv - 1, pos % 16, 5] = float("nan")
+        got, f = c.run()
+        assert f == 0
+        sees = torch.tensor([pos < 70 or bool(c.see[0][i][pos - 70]) for i in range(nodes)])
+        assert torch.isnan(got[sees][:, hq - g:]).all()
+        got[:, hq - g:][sees] = clean[:, hq - g:][sees].float()
+        c.check(got)
+
+
 @pytest.mark.parametrize("k,v", [(1e-6, 1e6), (1e5, 1e-5), (1e12, 1e-12), (1e-20, 1e20)])
 def test_tree_attention_value_ranges(k, v):
     Case([100], [9], 8, 2, 128, 16, seed=1, scale=(k, v)).check()
