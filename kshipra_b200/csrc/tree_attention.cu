@@ -447,7 +447,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
   }
   tc_fence_before();
   grid_dep_wait();
-  grid_dep_launch();
 
   // Q into L2 while the memory is idle: behind the K/V copies a row takes
   // thousands of cycles
@@ -518,6 +517,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
     }
   }
   __syncthreads();
+  // the next kernel's CTAs may take TMEM before they wait for this one: not
+  // before this CTA has its own
+  grid_dep_launch();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Walk* const wk = &walk_s[warp];

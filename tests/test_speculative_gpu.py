@@ -355,6 +355,27 @@ def test_tree_attention_on_another_stream():
         assert torch.equal(o.cpu(), want)       # the same bits, whatever ran beside it
 
 
+def test_tree_attention_of_one_cta_between_other_tensor_core_kernels():
+    """A call of a single CTA has no second launch: the kernels right before and
+    after it in the stream allocate TMEM as it does."""
+    from kshipra_b200.quantization import QuantizedLinear
+    c = Case([20], [4], 2, 1, 64, 16, seed=3)
+    want = c.check().cuda()
+    g = torch.Generator().manual_seed(0)
+    lin = torch.nn.Linear(256, 256, bias=False)
+    lin.weight.data = torch.randn((256, 256), generator=g)
+    lin = QuantizedLinear(lin.cuda(), "int8")
+    x = torch.randn((64, 256), generator=g).cuda()
+    ref = lin(x)
+    args = [c.q.cuda(), c.pool.cuda(), c.layer, i32(c.bt), i32(c.qs), i32(c.pre), c.mask.cuda(), 4, 24]
+    got = []
+    for _ in range(20):
+        got += [(sp.tree_attention(*args), want), (lin(x), ref), (sp.tree_attention(*args), want),
+                (sp.tree_attention(*args), want)]
+    for a, b in got:
+        assert torch.equal(a, b)
+
+
 def test_tree_attention_offsets_past_32_bits():
     """Blocks whose float offsets lie past 2^31 (and 2^32 bytes past that)."""
     hq, hkv, d, bs, layers = 4, 2, 128, 64, 40
