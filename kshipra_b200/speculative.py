@@ -15,8 +15,8 @@ of earlier occurrences of the last tokens); its greedy stream is
 ``KshipraModel.generate``'s.  The reference's engine/speculative.py drafts and
 verifies against a mock model only (speculative.py:51-81, 154-270).
 
-All tensors are CUDA tensors on one device; calls run on the current stream
-and allocate only their outputs.  Errors that only the device can see are
+All tensors are CUDA tensors on one device, which is checked; calls run on its
+current stream and allocate only their outputs.  Errors that only the device can see are
 OR-ed into ``flags`` (int32 [1], KSH_FLAG_* bits) where one is given.
 """
 
@@ -52,24 +52,46 @@ def _run(device: torch.device, name: str, *args) -> None:
         _lib.check(name, st)
 
 
-def _need(t: torch.Tensor, name: str, dtype: torch.dtype, ndim: int) -> torch.Tensor:
-    if not t.is_cuda:
-        raise _lib.KshipraLibraryError(f"{name} must be a CUDA tensor (no CPU path)")
+def _wrong_device(name: str, at: int, dev: Optional[int]) -> Exception:
+    if at < 0:
+        return _lib.KshipraLibraryError(f"{name} must be a CUDA tensor (no CPU path)")
+    return ValueError(f"{name} is on cuda:{at}, the call's other tensors on cuda:{dev}")
+
+
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, ndim: int,
+          dev: Optional[int] = None) -> torch.Tensor:
+    """``t`` if it fits and is on CUDA device ``dev`` (None: on any)."""
+    at = t.get_device()
+    if at < 0 or (at != dev and dev is not None):
+        raise _wrong_device(name, at, dev)
     if t.dtype is not dtype or t.dim() != ndim or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {ndim}-D {dtype} tensor, got "
                          f"{t.dtype} {tuple(t.shape)}")
     return t
 
 
-def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+def _rows(t: torch.Tensor, name: str, dev: Optional[int] = None) -> torch.Tensor:
     """A 2-D fp32 tensor whose rows are contiguous (they may lie further apart)."""
-    if not t.is_cuda:
-        raise _lib.KshipraLibraryError(f"{name} must be a CUDA tensor (no CPU path)")
+    at = t.get_device()
+    if at < 0 or (at != dev and dev is not None):
+        raise _wrong_device(name, at, dev)
     if (t.dtype is not torch.float32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1)
             or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         raise ValueError(f"{name} must be fp32 [rows, vocab] with contiguous rows, got "
                          f"{t.dtype} {tuple(t.shape)} strides {t.stride()}")
     return t
+
+
+def _flags(t: Optional[torch.Tensor], dev: int) -> Optional[int]:
+    """Address of the status word, or None."""
+    if t is None:
+        return None
+    at = t.get_device()
+    if at != dev:
+        raise _wrong_device("flags", at, dev)
+    if t.dtype is not torch.int32 or t.numel() < 1:
+        raise ValueError(f"flags must be an int32 tensor of one element, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def _stride(t: torch.Tensor) -> int:
@@ -118,23 +140,23 @@ def tree_tables(prefix_lens: torch.Tensor, new_lens: torch.Tensor, total: int, b
     [total, ceil(max_nodes / 64)] or None), as ``KshipraModel`` takes them.
     """
     S = prefix_lens.shape[0]
-    _need(prefix_lens, "prefix_lens", torch.int32, 1)
-    _need(new_lens, "new_lens", torch.int32, 1)
+    at = _need(prefix_lens, "prefix_lens", torch.int32, 1).get_device()
+    _need(new_lens, "new_lens", torch.int32, 1, at)
     if new_lens.shape[0] != S:
         raise ValueError("prefix_lens and new_lens differ in length")
     if (block_ids is None) != (block_start is None) or (block_ids is None) == (block_tables is None):
         raise ValueError("pass block_ids with block_start, or block_tables")
     dev = prefix_lens.device
     if block_ids is not None:
-        _need(block_ids, "block_ids", torch.int32, 1)
-        if _need(block_start, "block_start", torch.int32, 1).shape[0] != S + 1:
+        _need(block_ids, "block_ids", torch.int32, 1, at)
+        if _need(block_start, "block_start", torch.int32, 1, at).shape[0] != S + 1:
             raise ValueError("block_start must have one entry more than there are sequences")
         block_tables = prefix_lens.new_empty((S, max_blocks))
-    elif tuple(_need(block_tables, "block_tables", torch.int32, 2).shape) != (S, max_blocks):
+    elif tuple(_need(block_tables, "block_tables", torch.int32, 2, at).shape) != (S, max_blocks):
         raise ValueError(f"block_tables must be [{S}, {max_blocks}]")
     words = 0
     if parents is not None:
-        if _need(parents, "parents", torch.int32, 1).shape[0] != total:
+        if _need(parents, "parents", torch.int32, 1, at).shape[0] != total:
             raise ValueError("parents must have one entry per row")
         if not 1 <= max_nodes <= MAX_NODES:
             raise ValueError(f"max_nodes must be 1..{MAX_NODES}, got {max_nodes}")
@@ -146,7 +168,7 @@ def tree_tables(prefix_lens: torch.Tensor, new_lens: torch.Tensor, total: int, b
     _run(dev, "ksh_tree_tables", prefix_lens.data_ptr(), new_lens.data_ptr(), S, total, block_size,
          ptr(block_ids), 0 if block_ids is None else block_ids.shape[0], ptr(block_start),
          max_blocks, ptr(parents), words, q_start.data_ptr(), block_tables.data_ptr(),
-         positions.data_ptr(), slots.data_ptr(), ptr(mask), ptr(flags))
+         positions.data_ptr(), slots.data_ptr(), ptr(mask), _flags(flags, at))
     return q_start, block_tables, positions, slots, mask
 
 
@@ -160,9 +182,9 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_tables
     slots of positions prefix .. prefix + n - 1, mask int64 [T, words] from
     ``tree_tables`` (None: node i attends nodes 0 .. i).  Returns [T, Hq, D];
     a node that may see no key gives zeros."""
-    _need(q, "q", torch.float32, 3)
-    _need(pool, "pool", torch.float32, 6)
-    _need(block_tables, "block_tables", torch.int32, 2)
+    at = _need(q, "q", torch.float32, 3).get_device()
+    _need(pool, "pool", torch.float32, 6, at)
+    _need(block_tables, "block_tables", torch.int32, 2, at)
     T, hq, d = q.shape
     nb, L, two, hkv, bs, dp = pool.shape
     S, max_blocks = block_tables.shape
@@ -170,26 +192,26 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_tables
         raise ValueError(f"q {tuple(q.shape)} does not fit the pool {tuple(pool.shape)}")
     if not 0 <= layer < L:
         raise ValueError(f"layer {layer} outside the pool's {L}")
-    if (_need(q_start, "q_start", torch.int32, 1).shape[0] != S + 1
-            or _need(prefix_lens, "prefix_lens", torch.int32, 1).shape[0] != S):
+    if (_need(q_start, "q_start", torch.int32, 1, at).shape[0] != S + 1
+            or _need(prefix_lens, "prefix_lens", torch.int32, 1, at).shape[0] != S):
         raise ValueError("q_start must have S + 1 and prefix_lens S entries")
     if not 0 <= max_nodes <= MAX_NODES:
         raise ValueError(f"max_nodes must be 0..{MAX_NODES}, got {max_nodes}")
     words = 0
     if mask is not None:
-        if _need(mask, "mask", torch.int64, 2).shape[0] != T:
+        if _need(mask, "mask", torch.int64, 2, at).shape[0] != T:
             raise ValueError("mask must have one row per node")
         words = mask.shape[1]
     if out is None:
         out = torch.empty_like(q)
-    elif _need(out, "out", torch.float32, 3).shape != q.shape:
+    elif _need(out, "out", torch.float32, 3, at).shape != q.shape:
         raise ValueError("out must have q's shape")
     dev = q.device
     buf = ws.get(_workspace_bytes(S, hq, hkv, d, max_nodes), dev)
     _run(dev, "ksh_tree_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), nb, L, layer, hkv, bs,
          block_tables.data_ptr(), max_blocks, q_start.data_ptr(), prefix_lens.data_ptr(), S,
          ptr(mask), words, max_nodes, max_total_len, out.data_ptr(), buf.data_ptr(), buf.numel(),
-         ptr(flags))
+         _flags(flags, at))
     return out
 
 
@@ -198,11 +220,12 @@ def target_probs(logits: torch.Tensor, temperature: Optional[torch.Tensor] = Non
     """Probabilities of logits [m, vocab] at temperature fp32 [m] (None: 1; 0:
     one at the first maximum).  ``out`` may be ``logits``."""
     m, vocab = _rows(logits, "logits").shape
-    if temperature is not None and _need(temperature, "temperature", torch.float32, 1).shape[0] != m:
+    at = logits.get_device()
+    if temperature is not None and _need(temperature, "temperature", torch.float32, 1, at).shape[0] != m:
         raise ValueError("temperature must have one entry per row")
     if out is None:
         out = torch.empty((m, vocab), dtype=torch.float32, device=logits.device)
-    elif _rows(out, "out").shape != logits.shape:
+    elif _rows(out, "out", at).shape != logits.shape:
         raise ValueError("out must have the logits' shape")
     _run(logits.device, "ksh_target_probs", logits.data_ptr(), m, vocab, _stride(logits),
          ptr(temperature), out.data_ptr(), _stride(out))
@@ -225,8 +248,9 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, q_start: torch.Tens
     target_tokens int64 [T] (greedy).  Returns (path int32 [S, max_nodes]
     padded with -1, path_len int32 [S], next int64 [S])."""
     T = _need(tokens, "tokens", torch.int64, 1).shape[0]
-    S = _need(q_start, "q_start", torch.int32, 1).shape[0] - 1
-    if _need(parents, "parents", torch.int32, 1).shape[0] != T or S < 1:
+    at = tokens.get_device()
+    S = _need(q_start, "q_start", torch.int32, 1, at).shape[0] - 1
+    if _need(parents, "parents", torch.int32, 1, at).shape[0] != T or S < 1:
         raise ValueError("parents must have one entry per token, q_start S + 1 >= 2")
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError(f"max_nodes must be 1..{MAX_NODES}, got {max_nodes}")
@@ -236,20 +260,20 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, q_start: torch.Tens
     if target_probs is not None:
         if u_accept is None or u_sample is None:
             raise ValueError("target_probs needs u_accept and u_sample")
-        if _rows(target_probs, "target_probs").shape[0] != T:
+        if _rows(target_probs, "target_probs", at).shape[0] != T:
             raise ValueError("target_probs must have one row per node")
-        if (_need(u_accept, "u_accept", torch.float32, 1).shape[0] != T
-                or _need(u_sample, "u_sample", torch.float32, 1).shape[0] != S):
+        if (_need(u_accept, "u_accept", torch.float32, 1, at).shape[0] != T
+                or _need(u_sample, "u_sample", torch.float32, 1, at).shape[0] != S):
             raise ValueError("u_accept must have one entry per node, u_sample per sequence")
         vocab, ps = target_probs.shape[1], _stride(target_probs)
         if draft_probs is not None:
-            if _rows(draft_probs, "draft_probs").shape != target_probs.shape:
+            if _rows(draft_probs, "draft_probs", at).shape != target_probs.shape:
                 raise ValueError("draft_probs must have target_probs' shape")
             qs = _stride(draft_probs)
     else:
         if draft_probs is not None:
             raise ValueError("draft_probs needs target_probs")
-        if _need(target_tokens, "target_tokens", torch.int64, 1).shape[0] != T:
+        if _need(target_tokens, "target_tokens", torch.int64, 1, at).shape[0] != T:
             raise ValueError("target_tokens must have one entry per node")
     dev = tokens.device
     path = q_start.new_empty((S, max_nodes))
@@ -259,7 +283,7 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, q_start: torch.Tens
          max_nodes, vocab, ptr(target_probs), ps, ptr(draft_probs), qs, ptr(target_tokens),
          None if target_probs is None else u_accept.data_ptr(),
          None if target_probs is None else u_sample.data_ptr(), path.data_ptr(),
-         path_len.data_ptr(), nxt.data_ptr(), ptr(flags))
+         path_len.data_ptr(), nxt.data_ptr(), _flags(flags, at))
     return path, path_len, nxt
 
 
@@ -270,19 +294,19 @@ def commit_tree(pool: torch.Tensor, block_tables: torch.Tensor, prefix_lens: tor
     path_len int32 [S], from ``verify_tree``) to positions prefix, prefix + 1,
     ... in every layer of the pool, in place, and returns the new lengths
     prefix_lens + path_len (int32 [S])."""
-    _need(pool, "pool", torch.float32, 6)
+    at = _need(pool, "pool", torch.float32, 6).get_device()
     nb, L, two, hkv, bs, d = pool.shape
-    S, max_blocks = _need(block_tables, "block_tables", torch.int32, 2).shape
+    S, max_blocks = _need(block_tables, "block_tables", torch.int32, 2, at).shape
     if two != 2:
         raise ValueError(f"pool must be [nb, L, 2, Hkv, B, D], got {tuple(pool.shape)}")
-    if (_need(prefix_lens, "prefix_lens", torch.int32, 1).shape[0] != S
-            or _need(path_len, "path_len", torch.int32, 1).shape[0] != S
-            or _need(path, "path", torch.int32, 2).shape[0] != S):
+    if (_need(prefix_lens, "prefix_lens", torch.int32, 1, at).shape[0] != S
+            or _need(path_len, "path_len", torch.int32, 1, at).shape[0] != S
+            or _need(path, "path", torch.int32, 2, at).shape[0] != S):
         raise ValueError("prefix_lens, path and path_len must have one entry per sequence")
     new_lens = prefix_lens.new_empty(S)
     _run(pool.device, "ksh_tree_commit", pool.data_ptr(), nb, L, hkv, bs, d,
          block_tables.data_ptr(), max_blocks, prefix_lens.data_ptr(), S, path.data_ptr(),
-         path.shape[1], path_len.data_ptr(), new_lens.data_ptr(), ptr(flags))
+         path.shape[1], path_len.data_ptr(), new_lens.data_ptr(), _flags(flags, at))
     return new_lens
 
 

@@ -3,7 +3,10 @@
 
 import pytest
 
+import torch
+
 from kshipra_b200 import _lib
+from kshipra_b200 import speculative as sp
 from kshipra_b200.speculative import PromptLookup
 
 FAKE = 256          # never dereferenced: the arguments are checked before any launch
@@ -88,3 +91,44 @@ def test_argument_errors_are_reported_without_a_launch():
     assert h.ksh_tree_commit(FAKE, 4, 1, 2, 16, 64, FAKE, 2, FAKE, 0, FAKE, 4, FAKE, None, None, None) == -1
     assert h.ksh_tree_commit(FAKE, 4, 1, 2, 16, 64, FAKE, 2, FAKE, 1, FAKE, 0, FAKE, None, None, None) == -1
     assert h.ksh_tree_commit(None, 4, 1, 2, 16, 64, FAKE, 2, FAKE, 1, FAKE, 4, FAKE, None, None, None) == -1
+
+
+class On:
+    """What the checks look at of a tensor on some device."""
+
+    is_cuda = True
+
+    def __init__(self, device, shape, dtype=torch.int32):
+        self.t = torch.empty(shape, dtype=dtype)
+        self.device_index = device
+
+    def get_device(self):
+        return self.device_index
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def test_tensors_of_one_call_are_on_one_device():
+    ok = On(1, (4,))
+    assert sp._need(ok, "x", torch.int32, 1) is ok and sp._need(ok, "x", torch.int32, 1, 1) is ok
+    rows = On(1, (2, 3), torch.float32)
+    assert sp._rows(rows, "x", 1) is rows and sp._flags(None, 1) is None
+    assert sp._flags(ok, 1) == ok.data_ptr()
+    for bad in (lambda: sp._need(ok, "x", torch.int32, 1, 0), lambda: sp._rows(rows, "x", 0),
+                lambda: sp._flags(ok, 0),
+                lambda: sp._flags(On(1, (1,), torch.int64), 1), lambda: sp._flags(On(1, (0,)), 1),
+                # no launch follows: the first tensors differ
+                lambda: sp.tree_tables(ok, On(0, (4,)), 4, 16, 4, 1, block_tables=On(1, (4, 1))),
+                lambda: sp.tree_attention(On(0, (2, 2, 64), torch.float32), On(1, (1, 1, 2, 2, 16, 64), torch.float32),
+                                          0, ok, ok, ok, None, 1, 1),
+                lambda: sp.target_probs(rows, On(0, (2,), torch.float32)),
+                lambda: sp.verify_tree(On(0, (4,), torch.int64), ok, ok, 2, target_tokens=ok),
+                lambda: sp.commit_tree(On(0, (1, 1, 2, 2, 16, 64), torch.float32), On(1, (1, 1)), ok, ok, ok)):
+        with pytest.raises(ValueError):
+            bad()
+    cpu = torch.zeros(4, dtype=torch.int32)
+    for bad in (lambda: sp._need(cpu, "x", torch.int32, 1), lambda: sp._flags(cpu, 0),
+                lambda: sp._rows(torch.zeros(2, 3), "x")):
+        with pytest.raises(_lib.KshipraLibraryError):
+            bad()

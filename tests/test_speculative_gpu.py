@@ -747,6 +747,23 @@ def test_refusals():
             bad()
 
 
+def test_status_words_are_checked_before_the_launch():
+    c = Case([10], [4], 4, 2, 64, 16)
+    q, pool, bt, qs, pre, mask = c.q.cuda(), c.pool.cuda(), i32(c.bt), i32(c.qs), i32(c.pre), c.mask.cuda()
+    par, tok = i32([-1, 0, 0, 1]), torch.zeros(4, dtype=torch.int64, device="cuda")
+    path, ln = sp.verify_tree(tok, par, qs, 4, target_tokens=tok)[:2]
+    calls = (lambda f: sp.tree_tables(pre, i32([4]), 4, 16, 4, bt.shape[1], block_tables=bt, parents=par, flags=f),
+             lambda f: sp.tree_attention(q, pool, 0, bt, qs, pre, mask, 4, 14, flags=f),
+             lambda f: sp.verify_tree(tok, par, qs, 4, target_tokens=tok, flags=f),
+             lambda f: sp.commit_tree(pool, bt, pre, path, ln, flags=f))
+    for call in calls:
+        call(new_flags())
+        with pytest.raises(_lib.KshipraLibraryError):
+            call(torch.zeros(1, dtype=torch.int32))
+        with pytest.raises(ValueError):
+            call(torch.zeros(1, dtype=torch.int64, device="cuda"))
+
+
 @pytest.fixture(scope="module")
 def tiny():
     from kshipra_b200.config import TINY_LLAMA
