@@ -28,6 +28,9 @@ namespace {
 using namespace tc;
 
 constexpr int kMaxCluster = 8;
+// A row's elements are numbered in 32 bits, and loops go one stride past its
+// end: rows up to 2^30 leave room for that.
+constexpr int64_t kMaxVocab = 1 << 30;
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
@@ -641,6 +644,7 @@ extern "C" int ksh_target_probs(const float* logits, int64_t m, int64_t vocab,
                 logits_stride >= vocab && probs_stride >= vocab);
   if (m == 0) return KSH_OK;
   KSH_CHECK_ARG(logits && probs);
+  if (vocab > kMaxVocab) return KSH_ERR_UNSUPPORTED;
   ProbArgs a = {logits, temperature, probs, logits_stride, probs_stride, static_cast<int>(vocab), 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // CTAs per row: parts of at most 80 KB, so that two or three CTAs share an
@@ -676,7 +680,7 @@ extern "C" int ksh_verify_tree(const int64_t* tokens, const int32_t* parents,
   } else {
     KSH_CHECK_ARG(!draft_probs);
   }
-  if (max_nodes > kMaxNodes) return KSH_ERR_UNSUPPORTED;
+  if (max_nodes > kMaxNodes || vocab > kMaxVocab) return KSH_ERR_UNSUPPORTED;
   VerArgs a = {};
   a.tokens = tokens;
   a.parents = parents;

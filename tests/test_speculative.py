@@ -132,3 +132,11 @@ def test_tensors_of_one_call_are_on_one_device():
                 lambda: sp._rows(torch.zeros(2, 3), "x")):
         with pytest.raises(_lib.KshipraLibraryError):
             bad()
+
+
+def test_rows_past_32_bit_element_numbers_are_refused():
+    h = _lib.lib()
+    for v in ((1 << 30) + 1, (1 << 31) - 1):
+        assert h.ksh_target_probs(FAKE, 1, v, v, None, FAKE, v, None) == -4
+        assert h.ksh_verify_tree(FAKE, FAKE, FAKE, 1, 4, 4, v, FAKE, v, None, 0, None, FAKE, FAKE, FAKE, FAKE,
+                                 FAKE, None, None) == -4
