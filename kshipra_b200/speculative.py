@@ -99,19 +99,30 @@ def _stride(t: torch.Tensor) -> int:
 
 
 class TreeWorkspace:
-    """Grow-only scratch of the tree attention, one buffer per device and
-    stream (calls on different streams may overlap).  Needs no initialisation."""
+    """Scratch of the tree attention, one buffer per device and stream (calls on
+    different streams may overlap).  Needs no initialisation.
+
+    A captured graph keeps the address that it was captured with, so a buffer is
+    never replaced: it is allocated at the largest size of any head dimension
+    (19.6 MB on 148 SMs).  And a call under capture gets a buffer of its own from
+    the capture's memory pool, which lives as long as the graph: graphs captured
+    on one stream may be replayed on several at once.
+    """
 
     def __init__(self):
         self.bufs: Dict[tuple, torch.Tensor] = {}
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
         idx = device.index
+        if idx != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self.get(nbytes, device)
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
         key = (idx, _raw_stream(idx) if _raw_stream is not None else stream_ptr(device))
         buf = self.bufs.get(key)
-        if buf is None or buf.numel() < nbytes:
-            buf = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-            self.bufs[key] = buf
+        if buf is None:
+            buf = self.bufs[key] = torch.empty(_largest_workspace(), dtype=torch.uint8, device=device)
         return buf
 
 
@@ -121,6 +132,11 @@ _WS = TreeWorkspace()
 @functools.lru_cache(maxsize=None)
 def _workspace_bytes(seqs: int, hq: int, hkv: int, d: int, max_nodes: int) -> int:
     return int(_lib.lib().ksh_tree_attention_workspace_size(seqs, hq, hkv, d, max_nodes))
+
+
+@functools.lru_cache(maxsize=None)
+def _largest_workspace() -> int:
+    return max(_workspace_bytes(1, 1, 1, d, 1) for d in (64, 128))
 
 
 def tree_tables(prefix_lens: torch.Tensor, new_lens: torch.Tensor, total: int, block_size: int,

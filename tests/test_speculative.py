@@ -140,3 +140,24 @@ def test_rows_past_32_bit_element_numbers_are_refused():
         assert h.ksh_target_probs(FAKE, 1, v, v, None, FAKE, v, None) == -4
         assert h.ksh_verify_tree(FAKE, FAKE, FAKE, 1, 4, 4, v, FAKE, v, None, 0, None, FAKE, FAKE, FAKE, FAKE,
                                  FAKE, None, None) == -4
+
+
+def test_workspace_is_kept_by_what_may_still_use_it(monkeypatch):
+    """A captured graph holds the buffer's address: no later call may replace the
+    buffer, and a capture takes one of its own."""
+    real, capturing = torch.empty, [False]
+    monkeypatch.setattr(torch, "empty", lambda n, dtype, device: real(n, dtype=dtype))
+    monkeypatch.setattr(sp, "_raw_stream", lambda idx: 7 + idx)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    size = {d: _lib.lib().ksh_tree_attention_workspace_size(4, 8, 2, d, 8) for d in (64, 80, 128)}
+    assert size[80] < size[64] < size[128]
+    dev, ws = torch.device("cuda", 0), sp.TreeWorkspace()
+    first = ws.get(size[80], dev)
+    assert ws.get(size[64], dev) is first and ws.get(size[128], dev) is first
+    capturing[0] = True
+    a, b = ws.get(size[64], dev), ws.get(size[128], dev)
+    assert len({t.data_ptr() for t in (first, a, b)}) == 3
+    assert a.numel() >= size[64] and b.numel() >= size[128]
+    capturing[0] = False
+    assert ws.get(size[128], dev) is first

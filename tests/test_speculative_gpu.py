@@ -421,6 +421,50 @@ def test_tree_attention_graph_replay_follows_device_lengths():
     assert torch.equal(out, sp.tree_attention(*args))
 
 
+def test_tree_attention_graphs_replayed_side_by_side():
+    """Two graphs of one capture stream, replayed on two streams with a larger
+    call of the ordinary workspace in between: each has scratch of its own."""
+    class Recorder(sp.TreeWorkspace):
+        def __init__(self):
+            super().__init__()
+            self.at = []
+
+        def get(self, nbytes, device):
+            buf = super().get(nbytes, device)
+            self.at.append(buf.data_ptr())
+            return buf
+
+    ws = Recorder()
+    cap = torch.cuda.Stream()
+    runs = []
+    with torch.cuda.stream(cap):
+        for d, seed in ((64, 6), (128, 7), (64, 8)):
+            c = Case([900, 300], [8, 8], 8, 2, d, 16, seed=seed)
+            args = [c.q.cuda(), c.pool.cuda(), c.layer, i32(c.bt), i32(c.qs), i32(c.pre), c.mask.cuda(), 8, 908]
+            want = sp.tree_attention(*args, ws=ws)
+            out = torch.zeros_like(want)
+            cap.synchronize()
+            c.check(want.cpu())
+            runs.append((args, out, want, torch.cuda.CUDAGraph()))
+        for args, out, _, graph in runs:
+            with torch.cuda.graph(graph, stream=cap):
+                sp.tree_attention(*args, out=out, ws=ws)
+                sp.tree_attention(*args, out=out, ws=ws)
+        after = sp.tree_attention(*runs[1][0], ws=ws)
+    torch.cuda.synchronize()
+    eager, held = ws.at[:3] + ws.at[-1:], [set(ws.at[3 + 2 * i:5 + 2 * i]) for i in range(3)]
+    assert len(set(eager)) == 1 and torch.equal(after, runs[1][2])
+    assert not (held[0] & held[1] or held[0] & held[2] or held[1] & held[2] or set(eager) & set.union(*held))
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(30):
+        for stream, (_, _, _, graph) in zip(streams, runs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _ in runs:
+        assert torch.equal(out, want)
+
+
 # --------------------------------------------------------------------------- #
 # probabilities
 # --------------------------------------------------------------------------- #
