@@ -14,9 +14,12 @@
 // the kernel (4 R D operations for 8 D bytes); the products go to the tensor
 // cores at fp32 accuracy by splitting each operand into two fp16 terms,
 // x * 2^e = hi + lo (22 bits; one power of two per row), and taking
-// hi*lo + lo*hi + hi*hi.  With 128 query rows on the MMA's M side that is
-// 1.6 K tensor cycles per 64 keys of D = 128, while the SM's share of HBM
-// takes 2.5 K cycles to bring their 64 KB.
+// hi*lo + lo*hi + hi*hi.  P goes in relative to the largest V row that the
+// query row sees in a tile, so an output is held to 2^-22 of its weighted values
+// and, beside that, to about 2^-32 of that V row whatever its weight (a cached row
+// 2^16 times its neighbours, with no weight: 1.5e-5).  With 128 query rows on
+// the MMA's M side that is 1.6 K tensor cycles per 64 keys of D = 128, while the
+// SM's share of HBM takes 2.5 K cycles to bring their 64 KB.
 //
 // One persistent CTA per SM.  The (sequence, kv head, 128-row tile) items'
 // 64-key tiles form one line that is cut into equal pieces, one per CTA, so
@@ -380,6 +383,17 @@ __device__ __forceinline__ int64_t key_offset(const TreeArgs& a, int s, int hk, 
   const int64_t blk = a.block_tables[static_cast<int64_t>(s) * a.max_blocks + j];
   if (blk < 0 || blk >= a.num_blocks) return -1;
   return ((((blk * a.num_layers + a.layer) * 2) * a.hkv + hk) * a.bs + (pos - j * bs)) * D;
+}
+
+// The largest of the V scales of a tile with drafted nodes (each key's is
+// relative to its group's) that a row sees.  Out of line: seldom called, and
+// with the loop in the row warps' code 64 x 4096 keys took 1 % longer.
+__device__ __noinline__ float seen_scale(const float* vg, const float* rv, uint64_t see) {
+  float mine = 0.0f;
+#pragma unroll 1
+  for (int j = 0; j < kTK; ++j)
+    if ((see >> j) & 1) mine = fmaxf(mine, rv[j] * vg[j >> 3]);
+  return mine;
 }
 
 template <int D>
@@ -776,7 +790,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
         }
         if (__builtin_expect(tree, 0)) {
           // tiles with drafted nodes: each row brought to the size of the
-          // largest, so that a row few nodes see cannot cost the others bits
+          // largest, so that a row few nodes see cannot cost the others bits;
+          // the scores and P take the factors back, by what each query row sees
 #pragma unroll
           for (int i = 0; i < NLD; ++i) {
             float m = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, 0.0f);
@@ -980,6 +995,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
                 }
               }
               rare = live ? vpois & see : 0;
+              if (tree) {
+                // P goes in relative to the largest V scale of the tile; where its V
+                // rows are 2^8 apart, to the largest that the row sees (both halves
+                // alike), so that rows of V that it does not see cost it no bits.
+                // Not further down than 2^-119 of the tile's: P of a key that is not
+                // seen is 0 times a finite factor.
+                const float* rv = vrel_s + mt * kTK;
+                const float s0 = rv[lane] * vg[lane >> 3], s1 = rv[lane + 32] * vg[4 + (lane >> 3)];
+                const float big = fmaxf(warp_amax(fmaxf(s0, s1)), 0x1p-100f), low = big * 0x1p-8f;
+                float mine = big;
+                if (__any_sync(0xffffffffu, ((valid >> lane) & 1 && s0 < low) || ((valid >> lane >> 32) & 1 && s1 < low)))
+                  mine = fmaxf(seen_scale(vg, rv, see), big * 0x1p-119f);
+                vs = fmaxf(mine, 0x1p-100f);
+              }
               __syncwarp();                          // word() loads for live rows only
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {
@@ -1032,7 +1061,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
             const float ref = mref == -INFINITY ? 0.0f : mref;
             // V's scales relative to the tile's largest; P is up to 2^8, its
             // terms up to 2^15
-            const float vm = warp_amax(fmaxf(vg[lane & 7], 0x1p-100f));
+            float vm = warp_amax(fmaxf(vg[lane & 7], 0x1p-100f));
+            vm = vs != 0.0f ? vs : vm;               // a tile with drafted nodes: the row's own
             const float up = __uint_as_float((261u << 23) - (__float_as_uint(vm) & 0x7f800000u));   // 2^7 / vm
             vs = vm * (1.0f / 128.0f);
             // P = 2^(x c - ref)

@@ -308,6 +308,44 @@ def test_tree_attention_mixed_magnitudes_in_one_tile():
     c.check()
 
 
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("what", [0, 1])
+@pytest.mark.parametrize("factor", [1e4, 1e8, 1e30])
+@pytest.mark.parametrize("pre,nodes,big", [(70, 12, [5]), (0, 9, [3, 8]), (100, 90, [7, 40, 41, 80]), (200, 5, [0])])
+def test_tree_attention_large_finite_rows_that_nodes_may_not_see(d, what, factor, pre, nodes, big):
+    """K or V rows that no node sees, as large as fp32 holds, beside rows that all
+    see.  Row by row: a weight is off by 4e-6 of itself and P and V by 2^-22, so
+    an output is within 1e-5 of its values' weighted magnitudes."""
+    see = [ancestors(p) for p in trees([nodes], np.random.RandomState(d))]
+    see[0][:, big] = False
+    c = Case([pre], [nodes], 4, 2, d, 16, seed=d + nodes, see=see)
+    for b in big:
+        t = pre + b
+        c.kv[0][what][:, t] *= factor
+        c.pool[c.bt[0, t // 16], c.layer, :, :, t % 16] = c.kv[0][:, :, t]
+    want = c.plain()
+    got, f = c.run()
+    assert f == 0
+    c.kv[0][1] = c.kv[0][1].abs()
+    assert ((got.double() - want).norm(dim=2) <= 1e-5 * c.plain().norm(dim=2)).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_tree_attention_large_values_reach_only_their_descendants(d):
+    """One node's V is 1e6 times the others': its descendants' outputs are of that
+    size, everyone else's are held to their own."""
+    c = Case([40], [20], 8, 2, d, 16, seed=d)
+    node, t = 4, 44
+    c.kv[0][1][:, t] *= 1e6
+    c.pool[c.bt[0, t // 16], c.layer, :, :, t % 16] = c.kv[0][:, :, t]
+    want = c.plain()
+    got, f = c.run()
+    assert f == 0
+    c.kv[0][1] = c.kv[0][1].abs()
+    assert 0 < c.see[0][:, node].sum() < 20
+    assert ((got.double() - want).norm(dim=2) <= 1e-5 * c.plain().norm(dim=2)).all()
+
+
 def test_tree_attention_peaked_scores():
     """Scores of hundreds: nearly every row has one key's weight.  A score of
     500 held to 2^-22 moves a weight by 1.2e-4 where two keys come close."""
