@@ -371,6 +371,27 @@ class PromptLookup:
         return out, parents
 
 
+def cut_tree(tokens: Sequence[int], parents: Sequence[int], depth: int
+             ) -> Tuple[List[int], List[int]]:
+    """The nodes at most ``depth`` below their root, renumbered.  A parent that
+    is no earlier node becomes -1 (which the verification reports)."""
+    if not tokens or len(tokens) != len(parents):
+        raise ValueError(f"a tree needs a token and a parent per node, got {len(tokens)} and {len(parents)}")
+    if depth >= len(tokens) - 1:                 # a chain of all of them is no deeper
+        return list(tokens), list(parents)
+    below: List[int] = []
+    at: List[int] = []
+    toks, ups = [], []
+    for i, (t, p) in enumerate(zip(tokens, parents)):
+        inner = 0 <= p < i
+        below.append(below[p] + 1 if inner else 0)
+        at.append(len(toks))
+        if below[i] <= depth:
+            toks.append(t)
+            ups.append(at[p] if inner else -1)
+    return toks, ups
+
+
 class SpeculativeDecoder:
     """Batched decoding of drafted trees through a ``KshipraModel``.
 
@@ -486,6 +507,11 @@ class SpeculativeDecoder:
         for i in live:
             have = list(prompts[i]) + out[i]
             t, p = self.proposer.propose(have)
+            if len(t) > self.proposer.max_nodes:
+                raise ValueError(f"{len(t)} drafted nodes, max_nodes is {self.proposer.max_nodes}")
+            # a step emits one token more than it accepts; nothing past the
+            # position table can be accepted
+            t, p = cut_tree(t, p, max(0, min(most - len(out[i]) - 1, self.m.max_positions - len(have))))
             prefix.append(len(have) - 1)
             toks.append(t)
             parents.append(p)

@@ -161,3 +161,16 @@ def test_workspace_is_kept_by_what_may_still_use_it(monkeypatch):
     assert a.numel() >= size[64] and b.numel() >= size[128]
     capturing[0] = False
     assert ws.get(size[128], dev) is first
+
+
+def test_cut_keeps_the_nodes_down_to_a_depth():
+    toks, par = [9, 1, 2, 3, 4, 5, 6], [-1, 0, 1, 0, 2, 3, 5]
+    assert sp.cut_tree(toks, par, 3) == (toks, par)
+    assert sp.cut_tree(toks, par, 2) == ([9, 1, 2, 3, 5], [-1, 0, 1, 0, 3])
+    assert sp.cut_tree(toks, par, 1) == ([9, 1, 3], [-1, 0, 0])
+    assert sp.cut_tree(toks, par, 0) == ([9], [-1])
+    # a parent that is no earlier node stays one for the device to report
+    assert sp.cut_tree([9, 1, 2, 3], [-1, 3, 0, 2], 1) == ([9, 1, 2], [-1, -1, 0])
+    for bad in (([], []), ([1, 2], [-1])):
+        with pytest.raises(ValueError):
+            sp.cut_tree(*bad, 1)

@@ -894,6 +894,46 @@ def test_decoder_greedy_stream_is_generates(tiny):
     assert sp.SpeculativeDecoder(tiny).generate(prompts, 20, eos_token_id=eos) == cut
 
 
+def test_decoder_drafts_only_what_can_be_emitted(tiny, monkeypatch):
+    """A prompt that repeats itself up to the end of the position table: generate
+    feeds the table's last position, and no draft lies behind it."""
+    a = np.random.RandomState(7).randint(0, tiny.vocab_size, 12).tolist()
+    prompts = [(a * 200)[:tiny.max_positions - 8], a * 3, a]
+    want = [tiny.generate(p, 9, block_size=16) for p in prompts]
+    last = []
+    real = sp.tree_tables
+
+    def spy(prefix, new, *args, **kw):
+        out = real(prefix, new, *args, **kw)
+        last.extend((out[2][out[0][1:].long() - 1]).tolist())
+        last.append(int(out[2].max()))
+        return out
+
+    monkeypatch.setattr(sp, "tree_tables", spy)
+    assert sp.SpeculativeDecoder(tiny).generate(prompts, 9) == want
+    assert max(last) == tiny.max_positions - 1
+    last.clear()
+    drafts = Oracle([p + w for p, w in zip(prompts, want)], tiny.vocab_size)
+    assert sp.SpeculativeDecoder(tiny, drafts).generate(prompts[:1], 9) == want[:1]
+    assert max(last) == tiny.max_positions - 1
+    # the model's own limit still holds, as it does for generate
+    from kshipra_b200.model import KshipraDeviceError
+    for run in (tiny.generate, lambda p, n: sp.SpeculativeDecoder(tiny).generate([p], n)):
+        with pytest.raises(KshipraDeviceError):
+            run(prompts[0], 12)
+
+
+def test_decoder_refuses_trees_past_the_proposers_limit(tiny):
+    class Many:
+        max_nodes = 2
+
+        def propose(self, tokens):
+            return [tokens[-1], 1, 2, 3], [-1, 0, 1, 2]
+
+    with pytest.raises(ValueError):
+        sp.SpeculativeDecoder(tiny, Many()).generate([[1, 2, 3]], 9)
+
+
 def test_decoder_sampling(tiny):
     """Temperature: the stream is the generator's, and a tiny temperature is greedy."""
     prompts = prompts_of(tiny.vocab_size)
