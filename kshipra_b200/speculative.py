@@ -420,6 +420,7 @@ class SpeculativeDecoder:
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 20,
                  eos_token_id: Optional[int] = None,
                  prefill_chunk: Optional[int] = None) -> List[List[int]]:
+        from .model import _check_flags
         m, bs = self.m, self.block_size
         if max_new_tokens < 1 or any(len(p) < 1 for p in prompts):
             raise ValueError("prompts need a token and max_new_tokens must be positive")
@@ -435,6 +436,7 @@ class SpeculativeDecoder:
             out: List[List[int]] = []
             for p, bt in zip(prompts, tables):
                 out.append([self._first(p, pool, bt, prefill_chunk)])
+            _check_flags(m.flags)
             self.emitted = len(out)
             live = [i for i in range(len(out)) if not self._done(out[i], max_new_tokens, eos_token_id)]
             while live:

@@ -923,6 +923,16 @@ def test_decoder_drafts_only_what_can_be_emitted(tiny, monkeypatch):
             run(prompts[0], 12)
 
 
+def test_decoder_reports_what_the_prefill_found(tiny):
+    """A prompt token outside the vocabulary, also where no step follows."""
+    from kshipra_b200.model import KshipraDeviceError
+    for n in (1, 4):
+        for dec in (sp.SpeculativeDecoder(tiny), sp.SpeculativeDecoder(tiny, temperature=0.7)):
+            with pytest.raises(KshipraDeviceError):
+                dec.generate([[1, 2], [tiny.vocab_size + 5, 3]], n)
+            assert int(tiny.flags) == 0
+
+
 def test_decoder_refuses_trees_past_the_proposers_limit(tiny):
     class Many:
         max_nodes = 2
