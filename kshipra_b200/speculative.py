@@ -440,16 +440,13 @@ class SpeculativeDecoder:
             self.emitted = len(out)
             live = [i for i in range(len(out)) if not self._done(out[i], max_new_tokens, eos_token_id)]
             while live:
-                self._step(prompts, out, tables, pool, live, max_new_tokens)
+                self._step(prompts, out, tables, pool, live, max_new_tokens, eos_token_id)
                 live = [i for i in live if not self._done(out[i], max_new_tokens, eos_token_id)]
-            for i, toks in enumerate(out):
-                if eos_token_id is not None and eos_token_id in toks:
-                    out[i] = toks[:toks.index(eos_token_id) + 1]
         return out
 
     @staticmethod
     def _done(toks: List[int], most: int, eos: Optional[int]) -> bool:
-        return len(toks) >= most or (eos is not None and eos in toks)
+        return len(toks) >= most or (eos is not None and toks[-1] == eos)
 
     def _rand(self, n: int) -> torch.Tensor:
         return torch.rand(n, generator=self.generator, device=self.m.device)
@@ -504,7 +501,7 @@ class SpeculativeDecoder:
         _check_flags(m.flags)
         return path, path_len, nxt
 
-    def _step(self, prompts, out, tables, pool, live, most: int) -> None:
+    def _step(self, prompts, out, tables, pool, live, most: int, eos: Optional[int]) -> None:
         prefix, toks, parents = [], [], []
         for i in live:
             have = list(prompts[i]) + out[i]
@@ -521,6 +518,8 @@ class SpeculativeDecoder:
         for i, t, row, n, last in zip(live, toks, path.tolist(), path_len.tolist(), nxt.tolist()):
             new = [t[j] for j in row[1:n]] + [last]
             new = new[:most - len(out[i])]
+            if eos is not None and eos in new:
+                new = new[:new.index(eos) + 1]
             out[i].extend(new)
             self.emitted += len(new)
         self.steps += 1

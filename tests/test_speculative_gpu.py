@@ -923,6 +923,18 @@ def test_decoder_drafts_only_what_can_be_emitted(tiny, monkeypatch):
             run(prompts[0], 12)
 
 
+def test_decoder_counts_the_tokens_that_it_returns(tiny):
+    """An end token amid accepted drafts: what comes after it is not emitted."""
+    prompts = prompts_of(tiny.vocab_size)
+    want = [tiny.generate(p, max_new_tokens=20, block_size=16) for p in prompts]
+    drafts = Oracle([p + w for p, w in zip(prompts, want)], tiny.vocab_size)
+    for eos in {w[2] for w in want} | {w[7] for w in want}:
+        cut = [w[:w.index(eos) + 1] if eos in w else w for w in want]
+        dec = sp.SpeculativeDecoder(tiny, drafts)
+        assert dec.generate(prompts, 20, eos_token_id=eos) == cut
+        assert dec.emitted == sum(len(w) for w in cut)
+
+
 def test_decoder_reports_what_the_prefill_found(tiny):
     """A prompt token outside the vocabulary, also where no step follows."""
     from kshipra_b200.model import KshipraDeviceError
