@@ -82,9 +82,9 @@ struct ProbArgs {
   int vocab, chunk;             // chunk: floats of a part, a multiple of four
 };
 
-// Order-preserving key of (value, first index); NaN loses to everything.
+// Order-preserving key of (value, first index); -0 == +0; NaN loses to everything.
 __device__ __forceinline__ uint64_t top_key(float v, int i) {
-  const uint32_t u = __float_as_uint(v);
+  const uint32_t u = __float_as_uint(v + 0.0f);
   const uint32_t k = v == v ? ((u & 0x80000000u) ? ~u : u | 0x80000000u) : 0u;
   return (static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
 }

@@ -566,6 +566,17 @@ def test_target_probs_many_rows(m, vocab):
     assert torch.equal(same[:, :vocab].nan_to_num(7.0), want.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("vocab", [8, 5000, 151936, 420001])
+def test_target_probs_greedy_ties_of_signed_zeros(vocab):
+    """-0 and +0 are one value: the first of them is the maximum."""
+    x = torch.full((3, vocab), -1.0)
+    x[0, 2], x[0, vocab - 2] = -0.0, 0.0
+    x[1, 3], x[1, vocab - 3] = 0.0, -0.0
+    x[2] = -0.0
+    got = sp.target_probs(x.cuda(), torch.zeros(3, device="cuda")).cpu()
+    assert [r.nonzero().view(-1).tolist() for r in got] == [[2], [3], [0]] and got.max() == 1
+
+
 def test_target_probs_not_finite_rows():
     x = torch.zeros((4, 200))
     x[0, 5] = float("nan")
