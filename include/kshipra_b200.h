@@ -380,9 +380,9 @@ int ksh_tree_attention(const float* q, int64_t total, int64_t hq, int64_t d, con
                        int64_t workspace_bytes, int32_t* flags, void* stream);
 
 /* Probabilities of m rows of logits at a temperature per row (NULL: 1):
- * p = exp((x - max) / T) / sum; T <= 0 puts one at the first maximum.  Rows
- * logits_stride / probs_stride floats apart; probs may be logits.  vocab up
- * to 2^30, here and in ksh_verify_tree. */
+ * p = exp((x - max) / T) / sum; T <= 0 puts one at the first maximum (NaN is the
+ * largest).  Rows logits_stride / probs_stride floats apart; probs may be
+ * logits.  vocab up to 2^30, here and in ksh_verify_tree. */
 int ksh_target_probs(const float* logits, int64_t m, int64_t vocab, int64_t logits_stride,
                      const float* temperature, float* probs, int64_t probs_stride, void* stream);
 

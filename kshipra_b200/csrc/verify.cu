@@ -82,10 +82,11 @@ struct ProbArgs {
   int vocab, chunk;             // chunk: floats of a part, a multiple of four
 };
 
-// Order-preserving key of (value, first index); -0 == +0; NaN loses to everything.
+// Order-preserving key of (value, first index); -0 == +0; NaN above +inf, as in
+// torch.argmax and the tensor-core lm_head.
 __device__ __forceinline__ uint64_t top_key(float v, int i) {
   const uint32_t u = __float_as_uint(v + 0.0f);
-  const uint32_t k = v == v ? ((u & 0x80000000u) ? ~u : u | 0x80000000u) : 0u;
+  const uint32_t k = v == v ? ((u & 0x80000000u) ? ~u : u | 0x80000000u) : 0xffffffffu;
   return (static_cast<uint64_t>(k) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
 }
 

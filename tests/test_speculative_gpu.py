@@ -577,6 +577,20 @@ def test_target_probs_greedy_ties_of_signed_zeros(vocab):
     assert [r.nonzero().view(-1).tolist() for r in got] == [[2], [3], [0]] and got.max() == 1
 
 
+@pytest.mark.parametrize("vocab", [8, 5000, 151936, 420001])
+def test_target_probs_greedy_rows_with_nan(vocab):
+    """NaN is the largest, as torch.argmax and the batch lm_head take it; its sign
+    does not matter."""
+    x = torch.randn((4, vocab), generator=torch.Generator().manual_seed(vocab))
+    x[0, vocab - 2] = float("nan")
+    x[0, 1] = float("inf")
+    x[1, 3] = x[1, 5] = float("nan")
+    x[2] = float("nan")
+    x.view(torch.int32)[3, 4] = -1
+    got = sp.target_probs(x.cuda(), torch.zeros(4, device="cuda")).cpu()
+    assert [r.nonzero().view(-1).tolist() for r in got] == [[vocab - 2], [3], [0], [4]] and got.max() == 1
+
+
 def test_target_probs_not_finite_rows():
     x = torch.zeros((4, 200))
     x[0, 5] = float("nan")
