@@ -1,8 +1,9 @@
 """Host side of speculative decoding: drafts, argument errors of the C entries
 (detected before any launch) and workspace sizes."""
 
-import pytest
+import random
 
+import pytest
 import torch
 
 from kshipra_b200 import _lib
@@ -174,3 +175,61 @@ def test_cut_keeps_the_nodes_down_to_a_depth():
     for bad in (([], []), ([1, 2], [-1])):
         with pytest.raises(ValueError):
             sp.cut_tree(*bad, 1)
+
+
+@pytest.mark.parametrize("ngram,depth,branches,nodes", [(3, 6, 3, 16), (1, 4, 9, 40), (4, 2, 1, 3), (2, 0, 3, 8),
+                                                        (3, 5, 0, 8), (2, 7, 5, 1)])
+def test_lookup_of_a_growing_sequence_is_the_scans(ngram, depth, branches, nodes):
+    lookup = PromptLookup(ngram, depth, branches, nodes)
+    for seed in range(6):
+        r = random.Random(seed)
+        tokens = [r.randrange(2 + seed) for _ in range(r.choice([1, 2, 9, 60]))]
+        seq = lookup.sequence(tokens)
+        for _ in range(25):
+            assert seq.propose() == lookup.propose(tokens)
+            new = [r.randrange(2 + seed) for _ in range(r.randrange(4))]
+            tokens = tokens + new
+            seq.extend(new)
+
+
+def test_lookup_reads_what_it_drafts_not_the_history():
+    class Counted(list):
+        reads = 0
+
+        def __getitem__(self, i):
+            got = super().__getitem__(i)
+            Counted.reads += len(got) if isinstance(i, slice) else 1
+            return got
+
+        def __iter__(self):
+            Counted.reads += len(self)
+            return super().__iter__()
+
+    lookup = PromptLookup(ngram=3, depth=6, branches=3, max_nodes=16)
+    for tokens in (list(range(30000)), [i % 997 for i in range(30000)], [5] * 30000):
+        seq = lookup.sequence(tokens)
+        seq.tokens = Counted(seq.tokens)
+        for step in range(5):
+            Counted.reads = 0
+            seq.extend([7, 8])
+            seq.propose()
+            assert Counted.reads <= 2 * (1 + 2 + 3) + 6 + 1 + 3 * 6
+
+
+def test_a_proposers_own_propose_is_called():
+    class Mine(PromptLookup):
+        def propose(self, tokens):
+            return [tokens[-1], len(tokens)], [-1, 0]
+
+    class Plain:
+        max_nodes = 2
+
+        def propose(self, tokens):
+            tokens.append(99)                   # its own copy
+            return [tokens[-2], len(tokens) - 1], [-1, 0]
+
+    for proposer in (Mine(), Plain()):
+        seq = sp.sequence_of(proposer, [4, 6])
+        assert seq.propose() == ([6, 2], [-1, 0])
+        seq.extend([3])
+        assert seq.propose() == ([3, 3], [-1, 0])
