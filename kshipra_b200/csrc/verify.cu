@@ -16,6 +16,7 @@
 // whole number, and a sum that depends on its order in the last bits of 32
 // would move it for one sample in a hundred at 128 K tokens.
 
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -42,6 +43,12 @@ __device__ __forceinline__ float pow2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Scale of (x - max) / t to powers of two.  Finite, so that the maxima of a row
+// at a temperature below 2^-127 keep their 0; a temperature of NaN stays NaN.
+__device__ __forceinline__ float to_pow2(float t) {
+  const float c = 1.44269504088896340736f / t;
+  return c > FLT_MAX ? FLT_MAX : c;
 }
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
@@ -154,7 +161,7 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
 #pragma unroll
     for (int w = 0; w < kProbWarps; ++w) m = fmaxf(m, redf[w]);
     const float ref = m == -INFINITY ? 0.0f : m;    // a part of nothing but -inf
-    const float c = 1.44269504088896340736f / t;    // to powers of two
+    const float c = to_pow2(t);
     float sum = 0.0f;
 #pragma unroll 8
     for (int i = lo + tid; i < hi; i += kProbThreads) {
@@ -249,7 +256,7 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_long_kernel(ProbArg
     for (int i = tid; i < a.vocab; i += kProbThreads) pr[i] = i == at ? 1.0f : 0.0f;
     return;
   }
-  const float c = 1.44269504088896340736f / t;
+  const float c = to_pow2(t);
   float sum = 0.0f;
   for (int i = tid; i < a.vocab; i += kProbThreads) sum += pow2((xr[i] - m) * c);
   sum = warp_sum(sum);

@@ -591,6 +591,24 @@ def test_target_probs_greedy_rows_with_nan(vocab):
     assert [r.nonzero().view(-1).tolist() for r in got] == [[vocab - 2], [3], [0], [4]] and got.max() == 1
 
 
+@pytest.mark.parametrize("vocab", [7, 5000, 420001])
+def test_target_probs_at_the_smallest_temperatures(vocab):
+    """1 / T overflows below 2^-127: what is left is the softmax's limit, all on the
+    maxima alike."""
+    x = torch.randn((4, vocab), generator=torch.Generator().manual_seed(vocab))
+    x[:, 2] = x[:, 5] = 9.0
+    x[1, 5] = 9.0 - 1e-6                        # the next fp32 below 9
+    x[2, 3] = float("-inf")
+    t = torch.tensor([1e-40, 1e-45, 3e-39, 1e-38])
+    assert (t > 0).all()
+    got = sp.target_probs(x.cuda(), t.cuda()).cpu()
+    want = torch.zeros_like(got)
+    want[:, 2] = want[:, 5] = 0.5
+    want[1, 2], want[1, 5] = 1.0, 0.0
+    assert torch.equal(got, want)
+    assert torch.isnan(sp.target_probs(x[:1].cuda(), torch.full((1,), float("nan"), device="cuda"))).all()
+
+
 def test_target_probs_not_finite_rows():
     x = torch.zeros((4, 200))
     x[0, 5] = float("nan")
