@@ -233,3 +233,32 @@ def test_a_proposers_own_propose_is_called():
         assert seq.propose() == ([6, 2], [-1, 0])
         seq.extend([3])
         assert seq.propose() == ([3, 3], [-1, 0])
+
+
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    """From another current device the entry runs under the tensors' one, on its
+    current stream."""
+    now, log = [0], []
+
+    class Under:
+        def __init__(self, device):
+            self.to = device.index
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.to
+
+        def __exit__(self, *exc):
+            now[0] = self.was
+
+    class Entries:
+        def ksh_some_entry(self, *args):
+            log.append((now[0],) + args)
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Under)
+    monkeypatch.setattr(sp, "_raw_stream", lambda idx: 100 + idx)
+    monkeypatch.setattr(sp._lib, "lib", Entries)
+    for idx in (0, 3):
+        sp._run(torch.device("cuda", idx), "ksh_some_entry", 5, None)
+    assert log == [(0, 5, None, 100), (3, 5, None, 103)] and now == [0]

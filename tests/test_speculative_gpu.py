@@ -232,6 +232,26 @@ def test_tree_attention_sequences_without_nodes():
     Case([10, 50, 0, 20], [3, 0, 2, 0], 4, 2, 64, 16, seed=9).check()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_tree_attention_of_tensors_off_16_byte_boundaries(d):
+    """The same call on a pool, a q or an out that starts in the middle of 16 bytes."""
+    c = Case([70, 3], [9, 4], 4, 2, d, 16, seed=d)
+    want = c.check()
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        buf[1:] = t.reshape(-1).cuda()
+        return buf[1:].view(t.shape)
+
+    q, pool, out = c.q.cuda(), c.pool.cuda(), torch.empty_like(c.q, device="cuda")
+    rest = [c.layer, i32(c.bt), i32(c.qs), i32(c.pre), c.mask.cuda(), 9, 79]
+    for args, o in (((off(q), pool), out), ((q, off(pool)), out), ((q, pool), off(out))):
+        assert sum(t.data_ptr() % 16 for t in (*args, o)) == 4
+        got = sp.tree_attention(*args, *rest, out=o).cpu()
+        c.check(got)
+        assert ((got - want).norm() / want.norm()) <= 2e-5
+
+
 def test_tree_attention_without_mask_is_causal():
     c = Case([50, 3], [20, 70], 8, 2, 64, 16, seed=1, chain=True)
     got, f = c.run(mask=False)
@@ -609,6 +629,20 @@ def test_target_probs_at_the_smallest_temperatures(vocab):
     assert torch.isnan(sp.target_probs(x[:1].cuda(), torch.full((1,), float("nan"), device="cuda"))).all()
 
 
+def test_target_probs_rows_past_a_clusters_shared_memory():
+    """Rows that are read three times; also in place and from odd addresses."""
+    vocab = 500009
+    x = torch.randn((3, vocab + 3), generator=torch.Generator().manual_seed(1)) * 5
+    t = torch.tensor([0.7, 0.0, 1.3])
+    xd = x.cuda()[:, 1:1 + vocab]
+    got = sp.target_probs(xd, t.cuda())
+    for r in (0, 2):
+        want = torch.softmax(x[r, 1:1 + vocab].double() / t[r].double(), 0)
+        assert ((got[r].cpu().double() - want).abs() <= 1e-5 * want + 1e-37).all()
+    assert got[1].nonzero().view(-1).tolist() == [int(x[1, 1:1 + vocab].argmax())]
+    assert torch.equal(sp.target_probs(xd, t.cuda(), out=xd), got)
+
+
 def test_target_probs_not_finite_rows():
     x = torch.zeros((4, 200))
     x[0, 5] = float("nan")
@@ -726,6 +760,37 @@ def test_verify_tree_large_vocabularies_and_row_strides(kind):
     check_verify([6], 151936, kind, seed=2)
     check_verify([9, 4, 1], 4001, kind, seed=3, wide=6)
     check_verify([200, 256], 64, kind, seed=4)
+
+
+@pytest.mark.parametrize("kind", ["drawn", "fixed"])
+def test_verify_tree_many_sequences_over_a_large_vocabulary(kind):
+    """So many sequences that each has one CTA, whose warps' pieces hold more steps
+    than there are slots for their sums."""
+    S, V = 300, 131073
+    g = torch.Generator(device="cuda").manual_seed(5)
+    P = torch.softmax(torch.randn((2 * S, V), generator=g, device="cuda") * 3, 1)
+    Q = torch.softmax(torch.randn((2 * S, V), generator=g, device="cuda") * 3, 1)
+    tok = torch.multinomial(Q, 1, generator=g).view(-1)
+    tok[1::2] = torch.where(torch.arange(S, device="cuda") % 2 == 0, P[::2].argmax(1), tok[::2])
+    u, us = torch.rand(2 * S, generator=g, device="cuda"), torch.rand(S, generator=g, device="cuda")
+    us[:3] = torch.tensor([0.0, 0.9999999, 0.5], device="cuda")
+    path, ln, nxt = sp.verify_tree(tok, i32([-1, 0] * S), i32(np.arange(S + 1) * 2), 2, target_probs=P,
+                                   draft_probs=Q if kind == "drawn" else None, u_accept=u, u_sample=us)
+    for s in range(S):
+        p, t = P[2 * s].double(), int(tok[2 * s + 1])
+        q = Q[2 * s].double() if kind == "drawn" else None
+        if float(u[2 * s + 1].double() * (1.0 if q is None else q[t])) < float(p[t]):
+            want, p = [0, 1], P[2 * s + 1].double()
+        else:
+            want = [0, -1]
+            if q is None:
+                p[t] = 0.0
+            else:
+                p = (p - q).clamp(min=0)
+        c = p.cumsum(0)
+        assert path[s].tolist() == want and int(ln[s]) == 2 + min(want[1], 0)
+        assert int(nxt[s]) == int((c > us[s].double() * c[-1]).to(torch.int8).argmax()), s
+    assert 0 < int((ln == 2).sum()) < S           # both ends were walked
 
 
 @pytest.mark.parametrize("kind", ["drawn", "fixed"])
