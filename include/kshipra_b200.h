@@ -365,7 +365,8 @@ int ksh_tree_tables(const int32_t* prefix_lens, const int32_t* new_lens, int64_t
  * pool, block_tables and layer as for ksh_paged_attention.  Node i attends
  * every cached position and the nodes of its mask row (mask NULL: nodes
  * 0 .. i); one that may see no key gives zeros, and what a node may not see
- * does not reach its sums, NaN and infinity included.  max_nodes and
+ * does not reach its sums, NaN and infinity included; rows of q that no sequence
+ * covers are not written.  max_nodes and
  * max_total_len are host-side upper bounds.  The workspace, of
  * ksh_tree_attention_workspace_size bytes and 256-byte aligned, needs no
  * initialisation.  d <= 256. */

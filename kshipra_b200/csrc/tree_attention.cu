@@ -39,18 +39,19 @@
 //           each step).  Both halves take the whole row's maximum, so neither
 //           waits for the other.
 // Registers decide the split: 128 x 128 accumulators are a quarter of the
-// file, so K / V in flight stay in shared memory and the code of each role is
-// kept short (an earlier form with the copies in registers spilled and missed
-// the instruction cache; unrolling the widening twice costs 12 %).
+// file (the row warps spill 132 bytes a thread at D = 128, 96 at 64), so K / V in
+// flight stay in shared memory and the code of each role is kept short (an
+// earlier form with the copies in registers spilled more and missed the
+// instruction cache; unrolling the widening twice costs 12 %).
 //
 // Measured, 64 sequences x 4096 keys x 16 nodes, 32 / 8 heads, D = 128: 530 us
-// alone (4.1 TB/s, 63 % of measured HBM), 605 us back to back, where the power
-// limit holds the clock at 1.55 GHz.  There the copies by themselves take 354 us
-// (they alone reach the limit), and leaving one part out saves: MMAs 150 us,
+// alone (4.1 TB/s, 63 % of measured HBM), 583 to 617 us back to back, where the
+// power limit holds the clock at 1.55 GHz.  There the copies by themselves take
+// 354 us (they alone reach the limit), and leaving one part out saves: MMAs 150 us,
 // rows 70, widening 65.  Inside a tile (3.9 K cycles) the rows are the longest
 // chain: 1.9 K softmax, 0.7 K for adding O, the rest waits.  3 x 31000 keys x
 // 61 nodes (two row tiles read K and V one after the other, the second time
-// from L2): 314 us alone, 379 back to back.  24 x 3000 x 20 nodes, 14 / 2
+// from L2): 314 us alone, 360 to 380 back to back.  24 x 3000 x 20 nodes, 14 / 2
 // heads, D = 64: 44 us, 2.7 K cycles a tile, of which the rows' chain is 2.3 K.
 // No faster: two stages of K and four of V for three and three; S and O issued
 // by two warps; one thread instead of a warp waiting and issuing (slower);

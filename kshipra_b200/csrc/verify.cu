@@ -313,7 +313,9 @@ struct Rest {
 // 10 us for one reading of each final pair of rows: a refusal's sum needs the one
 // before it, and each is a pass of about 4 us over the row (now in L2) and the
 // cluster.  One sequence x 151936, fixed proposals: 12 us, latency; the call's
-// 15 us are the host's.
+// 15 us are the host's, and so are 16 with 64 sequences x 8 nodes and 13.6 with
+// greedy tokens.  At 64 registers (four CTAs per SM) the drawn form spills 224
+// bytes a thread, the fixed one 64.
 template <int MODE>
 __global__ void __launch_bounds__(kVerThreads, 4) verify_tree_kernel(VerArgs a) {
   __shared__ int tok_s[kMaxNodes], par_s[kMaxNodes], path_s[kMaxNodes], gone_s[kMaxNodes];
