@@ -39,7 +39,7 @@
 //           each step).  Both halves take the whole row's maximum, so neither
 //           waits for the other.
 // Registers decide the split: 128 x 128 accumulators are a quarter of the
-// file (the row warps spill 132 bytes a thread at D = 128, 96 at 64), so K / V in
+// file (the row warps spill 108 bytes a thread at D = 128, 96 at 64), so K / V in
 // flight stay in shared memory and the code of each role is kept short (an
 // earlier form with the copies in registers spilled more and missed the
 // instruction cache; unrolling the widening twice costs 12 %).
@@ -51,7 +51,7 @@
 // rows 70, widening 65.  Inside a tile (3.9 K cycles) the rows are the longest
 // chain: 1.9 K softmax, 0.7 K for adding O, the rest waits.  3 x 31000 keys x
 // 61 nodes (two row tiles read K and V one after the other, the second time
-// from L2): 314 us alone, 360 to 380 back to back.  24 x 3000 x 20 nodes, 14 / 2
+// from L2): 314 us alone, 360 to 385 back to back.  24 x 3000 x 20 nodes, 14 / 2
 // heads, D = 64: 44 us, 2.7 K cycles a tile, of which the rows' chain is 2.3 K.
 // No faster: two stages of K and four of V for three and three; S and O issued
 // by two warps; one thread instead of a warp waiting and issuing (slower);
@@ -129,7 +129,7 @@ struct TreeLayout {
   static constexpr int LO = D / 64 * 1024;           // lo blocks of a group, after the hi blocks
   static constexpr int K_OFF = 0, V_OFF = NST * 2 * TERM;
   // per tile (ring of kMeta): inverse scales of K and V per group of eight
-  // keys, and per key relative to that (tiles with drafted nodes)
+  // keys (1 in tiles with drafted nodes), and per key (in those)
   static constexpr int META = V_OFF + NST * 2 * TERM;    // kinv, vinv [8], krel, vrel [64]
   static constexpr int BITS = META + 2 * kMeta * (kGroups + kTK) * 4;   // valid, kpois, vpois, tile [8]
   static constexpr int BAR = BITS + 4 * kMeta * 8;
@@ -386,15 +386,15 @@ __device__ __forceinline__ int64_t key_offset(const TreeArgs& a, int s, int hk, 
   return ((((blk * a.num_layers + a.layer) * 2) * a.hkv + hk) * a.bs + (pos - j * bs)) * D;
 }
 
-// The largest of the V scales of a tile with drafted nodes (each key's is
-// relative to its group's) that a row sees.  Out of line: seldom called, and
-// with the loop in the row warps' code 64 x 4096 keys took 1 % longer.
-__device__ __noinline__ float seen_scale(const float* vg, const float* rv, uint64_t see) {
-  float mine = 0.0f;
+// The largest of a tile's V scales (with drafted nodes: one per key) that a row
+// sees.  Out of line: seldom called, and with the loop in the row warps' code 64 x
+// 4096 keys took 0.7 % longer.
+__device__ __noinline__ float seen_scale(const float* rel, uint64_t see) {
+  float top = 0.0f;
 #pragma unroll 1
   for (int j = 0; j < kTK; ++j)
-    if ((see >> j) & 1) mine = fmaxf(mine, rv[j] * vg[j >> 3]);
-  return mine;
+    if ((see >> j) & 1) top = fmaxf(top, rel[j]);
+  return top;
 }
 
 template <int D>
@@ -790,9 +790,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
           pois_s[mt * 8 + ww] = static_cast<uint8_t>(pois);
         }
         if (__builtin_expect(tree, 0)) {
-          // tiles with drafted nodes: each row brought to the size of the
-          // largest, so that a row few nodes see cannot cost the others bits;
-          // the scores and P take the factors back, by what each query row sees
+          // tiles with drafted nodes: a power of two for each row, so that a row few
+          // nodes see cannot cost the others bits; the scores and P take them
+          // back, P by what each query row sees
+          if (lane == 0) inv_s[mt * kGroups + ww] = 1.0f;
 #pragma unroll
           for (int i = 0; i < NLD; ++i) {
             float m = amax3(amax3(r[i].x, r[i].y, r[i].z), r[i].w, 0.0f);
@@ -800,12 +801,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
             for (int o = D / 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             float s1, inv1;
             pow2_scale(m, &s1, &inv1);
-            const float up = fminf(s1 * inv, 0x1p120f);
-            r[i].x *= up;
-            r[i].y *= up;
-            r[i].z *= up;
-            r[i].w *= up;
-            if (ln == 0) rel_s[mt * kTK + ww * kGroup + i * RPI + sub] = 1.0f / up;
+            // sc takes inv back below (left out for these tiles there, 64 x 4096 keys
+            // took 1.5 % longer); s1 * inv could overflow, values below 2^15 cannot
+            r[i].x = r[i].x * s1 * inv;
+            r[i].y = r[i].y * s1 * inv;
+            r[i].z = r[i].z * s1 * inv;
+            r[i].w = r[i].w * s1 * inv;
+            if (ln == 0) rel_s[mt * kTK + ww * kGroup + i * RPI + sub] = inv1;
           }
         }
 #pragma unroll
@@ -999,16 +1001,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
               if (tree) {
                 // P goes in relative to the largest V scale of the tile; where its V
                 // rows are 2^8 apart, to the largest that the row sees (both halves
-                // alike), so that rows of V that it does not see cost it no bits.
-                // Not further down than 2^-119 of the tile's: P of a key that is not
-                // seen is 0 times a finite factor.
+                // alike), so that rows of V that it does not see cost it no bits (P of
+                // a key that is not seen is 0 times a finite factor)
                 const float* rv = vrel_s + mt * kTK;
-                const float s0 = rv[lane] * vg[lane >> 3], s1 = rv[lane + 32] * vg[4 + (lane >> 3)];
-                const float big = fmaxf(warp_amax(fmaxf(s0, s1)), 0x1p-100f), low = big * 0x1p-8f;
+                const float s0 = rv[lane], s1 = rv[lane + 32];
+                const float big = warp_amax(fmaxf(s0, s1)), low = big * 0x1p-8f;
                 float mine = big;
                 if (__any_sync(0xffffffffu, ((valid >> lane) & 1 && s0 < low) || ((valid >> lane >> 32) & 1 && s1 < low)))
-                  mine = fmaxf(seen_scale(vg, rv, see), big * 0x1p-119f);
-                vs = fmaxf(mine, 0x1p-100f);
+                  mine = seen_scale(rv, see);
+                vs = fmaxf(mine, 0x1p-119f);
               }
               __syncwarp();                          // word() loads for live rows only
 #pragma unroll 1
@@ -1062,7 +1063,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tree_attn_tc_kernel(TreeArgs a)
             const float ref = mref == -INFINITY ? 0.0f : mref;
             // V's scales relative to the tile's largest; P is up to 2^8, its
             // terms up to 2^15
-            float vm = warp_amax(fmaxf(vg[lane & 7], 0x1p-100f));
+            float vm = warp_amax(fmaxf(vg[lane & 7], 0x1p-119f));
             vm = vs != 0.0f ? vs : vm;               // a tile with drafted nodes: the row's own
             const float up = __uint_as_float((261u << 23) - (__float_as_uint(vm) & 0x7f800000u));   // 2^7 / vm
             vs = vm * (1.0f / 128.0f);

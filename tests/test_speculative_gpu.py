@@ -350,6 +350,26 @@ def test_tree_attention_large_finite_rows_that_nodes_may_not_see(d, what, factor
     assert ((got.double() - want).norm(dim=2) <= 1e-5 * c.plain().norm(dim=2)).all()
 
 
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("what", [0, 1])
+@pytest.mark.parametrize("scale", [1.0, 1e-6, 1e-20])
+@pytest.mark.parametrize("pre,nodes,big", [(70, 12, [5]), (0, 9, [3, 8])])
+def test_tree_attention_the_types_largest_values_that_nodes_may_not_see(d, what, scale, pre, nodes, big):
+    """The same with the largest value that fp32 has, beside V rows of any size."""
+    see = [ancestors(p) for p in trees([nodes], np.random.RandomState(d))]
+    see[0][:, big] = False
+    c = Case([pre], [nodes], 4, 2, d, 16, seed=d + nodes, see=see, scale=(1.0, scale))
+    for b in big:
+        t = pre + b
+        c.kv[0][what][:, t] = torch.finfo(torch.float32).max * c.kv[0][what][:, t].sign()
+        c.pool[c.bt[0, t // 16], c.layer, :, :, t % 16] = c.kv[0][:, :, t]
+    want = c.plain()
+    got, f = c.run()
+    assert f == 0
+    c.kv[0][1] = c.kv[0][1].abs()
+    assert ((got.double() - want).norm(dim=2) <= 1e-5 * c.plain().norm(dim=2)).all()
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_tree_attention_large_values_reach_only_their_descendants(d):
     """One node's V is 1e6 times the others': its descendants' outputs are of that
