@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_kernel(ProbArgs a) 
 // Rows too long for a cluster's shared memory: one CTA each, three readings.
 __global__ void __launch_bounds__(kProbThreads) target_probs_long_kernel(ProbArgs a) {
   __shared__ float redf[kProbWarps];
+  __shared__ double redd[kProbWarps];
   __shared__ uint64_t redk[kProbWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dep_wait();
@@ -257,15 +258,15 @@ __global__ void __launch_bounds__(kProbThreads) target_probs_long_kernel(ProbArg
     return;
   }
   const float c = to_pow2(t);
-  float sum = 0.0f;
-  for (int i = tid; i < a.vocab; i += kProbThreads) sum += pow2((xr[i] - m) * c);
-  sum = warp_sum(sum);
+  // thousands of terms a thread: in 32 bits a flat row's sum was off by 1e-5
+  double sum = 0.0;
+  for (int i = tid; i < a.vocab; i += kProbThreads) sum += static_cast<double>(pow2((xr[i] - m) * c));
+  sum = warp_sum_f64(sum);
+  if (lane == 0) redd[warp] = sum;
   __syncthreads();
-  if (lane == 0) redf[warp] = sum;
-  __syncthreads();
-  sum = 0.0f;
-  for (int w = 0; w < kProbWarps; ++w) sum += redf[w];
-  const float inv = 1.0f / sum;
+  sum = 0.0;
+  for (int w = 0; w < kProbWarps; ++w) sum += redd[w];
+  const float inv = static_cast<float>(1.0 / sum);
   for (int i = tid; i < a.vocab; i += kProbThreads) pr[i] = pow2((xr[i] - m) * c) * inv;
 }
 

@@ -663,6 +663,19 @@ def test_target_probs_rows_past_a_clusters_shared_memory():
     assert torch.equal(sp.target_probs(xd, t.cuda(), out=xd), got)
 
 
+@pytest.mark.parametrize("vocab", [151936, 409600, 409601, 3000001])
+def test_target_probs_of_flat_rows(vocab):
+    """Terms of one size: the sum of hundreds of thousands is good to 1e-6 and a term
+    to 2e-6 (2 ulp, arguments below 1)."""
+    x = torch.randn((3, vocab), generator=torch.Generator().manual_seed(vocab))
+    t = torch.tensor([50.0, 20.0, 1000.0, 3.0, 1.0, 7.0])
+    x = torch.cat([x, torch.full((3, vocab), -1.0)])        # equal terms round the same way at each addition
+    x[3:, 5] = 0.0
+    want = torch.softmax(x.double() / t[:, None].double(), 1)
+    got = sp.target_probs(x.cuda(), t.cuda()).cpu().double()
+    assert ((got - want).abs() <= 3e-6 * want).all()
+
+
 def test_target_probs_not_finite_rows():
     x = torch.zeros((4, 200))
     x[0, 5] = float("nan")
