@@ -448,7 +448,7 @@ def cut_tree(tokens: Sequence[int], parents: Sequence[int], depth: int
              ) -> Tuple[List[int], List[int]]:
     """The nodes at most ``depth`` below their root, renumbered.  A parent that
     is no earlier node becomes -1 (which the verification reports)."""
-    if not tokens or len(tokens) != len(parents):
+    if len(tokens) < 1 or len(tokens) != len(parents):
         raise ValueError(f"a tree needs a token and a parent per node, got {len(tokens)} and {len(parents)}")
     if depth >= len(tokens) - 1:                 # a chain of all of them is no deeper
         return list(tokens), list(parents)

@@ -172,6 +172,9 @@ def test_cut_keeps_the_nodes_down_to_a_depth():
     assert sp.cut_tree(toks, par, 0) == ([9], [-1])
     # a parent that is no earlier node stays one for the device to report
     assert sp.cut_tree([9, 1, 2, 3], [-1, 3, 0, 2], 1) == ([9, 1, 2], [-1, -1, 0])
+    for depth in (1, 9):                        # arrays as well as lists
+        a, b = sp.cut_tree(torch.tensor(toks).numpy(), torch.tensor(par).numpy(), depth)
+        assert (a, b) == sp.cut_tree(toks, par, depth)
     for bad in (([], []), ([1, 2], [-1])):
         with pytest.raises(ValueError):
             sp.cut_tree(*bad, 1)
