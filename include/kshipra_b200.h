@@ -50,6 +50,12 @@ extern "C" {
 #define KSH_FLAG_TIMEOUT      64   /* a bounded device wait gave up */
 #define KSH_FLAG_BAD_PARENT  128   /* drafted node whose parent is not an earlier node */
 #define KSH_FLAG_BAD_PROBS   256   /* probability row without mass */
+#define KSH_FLAG_NO_PAGE     512   /* no free page of the pool was left */
+
+/* ---- element types of a K/V pool ---- */
+#define KSH_TYPE_F32           0
+#define KSH_TYPE_F16           1
+#define KSH_TYPE_BF16          2
 
 int ksh_abi_version(void);
 const char* ksh_status_string(int status);
@@ -419,6 +425,85 @@ int ksh_tree_commit(float* pool, int64_t num_blocks, int64_t num_layers, int64_t
                     int64_t max_blocks, const int32_t* prefix_lens, int64_t num_seqs,
                     const int32_t* path, int64_t path_stride, const int32_t* path_len,
                     int32_t* new_lens, int32_t* flags, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A 16-bit K/V cache: the pool layout of the other entries ([nb, L, 2, Hkv, B,
+ * D]) in fp16 or bf16 (KSH_TYPE_*; fp32 where an entry takes it).  Queries and
+ * outputs stay fp32; K and V are rounded once, when they are stored.
+ * ---------------------------------------------------------------------- */
+
+/* ksh_rope_kv_write (engine/model.py:47-55, 121-129) with norms and a typed
+ * pool: rows of qkv [m, (hq + 2 hkv) d] are split into heads; q and k heads are
+ * normed where a weight [d] is given (y = w * x / sqrt(mean(x^2) + eps)),
+ * rotated at positions[m], and q goes to q_out [m, hq, d], k and v, rounded to
+ * nearest, into the pool's slots.  Without norms and with an fp32 pool the
+ * results are ksh_rope_kv_write's.  Slots of a call are distinct.  A slot
+ * outside the pool raises KSH_FLAG_BAD_SLOT and is skipped, a position outside
+ * the table raises KSH_FLAG_BAD_POSITION and counts as 0. */
+int ksh_rope_cache_write(const float* qkv, int64_t m, int64_t hq, int64_t hkv, int64_t d,
+                         const int64_t* positions, const int64_t* slot_mapping,
+                         const float* rope_cos, const float* rope_sin, int64_t max_pos,
+                         const float* q_norm, const float* k_norm, float eps, float* q_out,
+                         void* pool, int pool_type, int64_t num_blocks, int64_t num_layers,
+                         int64_t layer, int64_t block_size, int32_t* flags, void* stream);
+
+/* Attention of new tokens over a 16-bit pool (chunked_attention,
+ * engine/chunked_prefill.py:93-140, for a batch): sequence s brings rows
+ * q_start[s] .. q_start[s + 1] - 1 of q [total, hq, d], whose K/V stand at
+ * positions prefix_lens[s] .. of its block table; row i attends positions
+ * 0 .. prefix + i.  Softmax statistics and sums are fp32.  What a row may not
+ * see does not reach it, NaN and infinity included; a row that sees a K or V
+ * element that is not finite gives NaN or infinity.  Rows of q that no sequence
+ * covers are not written; a row whose pages are all missing gives zeros.
+ * max_q_len and max_total_len are host-side upper bounds (a longer sequence
+ * raises KSH_FLAG_BAD_LENGTH, its rows past the bound are not written).  d <= 256.
+ * The workspace, of ksh_cache_attention_workspace_size bytes and 256-byte
+ * aligned, needs no initialisation. */
+int64_t ksh_cache_attention_workspace_size(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d,
+                                           int64_t max_q_len);
+int ksh_cache_attention(const float* q, int64_t total, int64_t hq, int64_t d, const void* pool,
+                        int pool_type, int64_t num_blocks, int64_t num_layers, int64_t layer,
+                        int64_t hkv, int64_t block_size, const int32_t* block_tables,
+                        int64_t max_blocks, const int32_t* q_start, const int32_t* prefix_lens,
+                        int64_t num_seqs, int64_t max_q_len, int64_t max_total_len, float* out,
+                        void* workspace, int64_t workspace_bytes, int32_t* flags, void* stream);
+
+/* Sequences continued by others (beams): child i of n continues sequence
+ * parents[i] (negative: none, an empty row) of block_tables [S, max_blocks]
+ * with lens[S] tokens cached, and gets a row of new_tables [n, max_blocks]
+ * (padded with 0), new_lens[i] = lens[parent] and slots[i], the slot of its
+ * next token.  Whole pages are shared.  The page that the next token goes to is
+ * the parent's for the first of its children; for the others it is a free page
+ * into which the filled rows are copied, in every layer, and where a page
+ * begins a free one for each.  ref_counts[nb] counts, for each page, the rows
+ * (of all tables, these or others) that hold it; new_ref is what it is after the
+ * S sequences have given up theirs and the children hold theirs.  Free pages
+ * (count 0 then) are taken from the lowest number up in the children's order.
+ * Without one left a child's slot is -1 and KSH_FLAG_NO_PAGE is raised.
+ * KSH_FLAG_BAD_LENGTH: a length that does not fit its row (slot -1 where the
+ * next token has no place), KSH_FLAG_BAD_PARENT: a parent past S,
+ * KSH_FLAG_BAD_BLOCK: a page outside the pool, or held more often than counted.
+ * n up to 65535.  scratch: ksh_fork_pages_scratch_ints int32. */
+int64_t ksh_fork_pages_scratch_ints(int64_t num_seqs, int64_t n);
+int ksh_fork_pages(void* pool, int pool_type, int64_t num_blocks, int64_t num_layers, int64_t hkv,
+                   int64_t block_size, int64_t d, const int32_t* block_tables, int64_t max_blocks,
+                   const int32_t* lens, int64_t num_seqs, const int32_t* parents, int64_t n,
+                   const int32_t* ref_counts, int32_t* new_tables, int32_t* new_lens,
+                   int64_t* slots, int32_t* new_ref, int32_t* scratch, int64_t scratch_ints,
+                   int32_t* flags, void* stream);
+
+/* The pages in use (ref_counts[nb] > 0), u of them, moved to pages 0 .. u - 1:
+ * the k-th used page from u on goes to the k-th free page below u, in every
+ * layer; pages below u stay.  page_map[nb] is each page's new number (its own
+ * where it did not move), new_ref the counts at the new numbers, used[0] = u,
+ * and new_tables the entries of block_tables renumbered (entries outside the
+ * pool as they are). */
+int64_t ksh_compact_pages_scratch_ints(int64_t num_blocks);
+int ksh_compact_pages(void* pool, int pool_type, int64_t num_blocks, int64_t num_layers,
+                      int64_t hkv, int64_t block_size, int64_t d, const int32_t* block_tables,
+                      int64_t entries, const int32_t* ref_counts, int32_t* new_tables,
+                      int32_t* new_ref, int32_t* page_map, int32_t* used, int32_t* scratch,
+                      int64_t scratch_ints, void* stream);
 
 /* ------------------------------------------------------------------------
  * Failure-path check of the device waits (no counterpart in the reference;

@@ -76,6 +76,16 @@ SIGNATURES = {
     "ksh_verify_tree": (I32, [P, P, P, I64, I64, I64, I64, P, I64, P, I64, P, P, P, P, P, P, P,
                               P]),
     "ksh_tree_commit": (I32, [P, I64, I64, I64, I64, I64, P, I64, P, I64, P, I64, P, P, P, P]),
+    "ksh_rope_cache_write": (I32, [P, I64, I64, I64, I64, P, P, P, P, I64, P, P, F32, P, P, I32,
+                                   I64, I64, I64, I64, P, P]),
+    "ksh_cache_attention_workspace_size": (I64, [I64, I64, I64, I64, I64]),
+    "ksh_cache_attention": (I32, [P, I64, I64, I64, P, I32, I64, I64, I64, I64, I64, P, I64, P, P,
+                                  I64, I64, I64, P, P, I64, P, P]),
+    "ksh_fork_pages_scratch_ints": (I64, [I64, I64]),
+    "ksh_fork_pages": (I32, [P, I32, I64, I64, I64, I64, I64, P, I64, P, I64, P, I64, P, P, P, P, P,
+                             P, I64, P, P]),
+    "ksh_compact_pages_scratch_ints": (I64, [I64]),
+    "ksh_compact_pages": (I32, [P, I32, I64, I64, I64, I64, I64, P, I64, P, P, P, P, P, P, I64, P]),
     "ksh_lm_head_tc_workspace_size": (I64, [I64, I64, I64]),
     "ksh_lm_head_split_weight": (I32, [P, I64, I64, P, P, P, P, P]),
     "ksh_lm_head_argmax_tc": (I32, [P, I64, I64, P, F32, P, P, P, I64, P, P, P, I64, P]),

@@ -49,7 +49,7 @@ FLAG_NAMES = {1: "non-finite weight", 2: "block id out of range", 4: "slot out o
               8: "position outside the RoPE table", 16: "token id out of range",
               32: "sequence longer than its block table", 64: "a bounded device wait gave up",
               128: "drafted node whose parent is not an earlier node",
-              256: "probability row without mass"}
+              256: "probability row without mass", 512: "no free page left"}
 FLAG_TIMEOUT = 64
 LM_GEMV_ROWS = 16            # lm_head rows served by the fp32 GEMV; more go to tensor cores
 PEER_AR_ROWS = 256           # token rows of a row-parallel sum done over peer memory
