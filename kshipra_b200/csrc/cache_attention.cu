@@ -26,9 +26,23 @@ struct CacheArgs {
   const int32_t* prefix;        // [S]
   float* out;                   // [total, hq, d]
   int32_t* flags;
+  struct SplitItem* items;      // [gridDim.x] items cut at the end of a CTA's share
+  float* part;                  // [gridDim.x][2] partial states
   int64_t total, num_blocks, num_layers, layer, hkv, hq, bs, max_blocks;
   int num_seqs, g, d, max_q;
+  int npt;                      // rows of q (all heads of the group) per tile of 128
+  int box;                      // pool rows per copy
+  int item_cost;                // keys that an item's start counts for, beside its own
   float scale;
+};
+
+// An item whose first piece CTA `first` holds: joined from pieces first..last.
+struct SplitItem {
+  int32_t first, last;          // last < first: none
+  int32_t row0;                 // q row of the tile's first token
+  int32_t rows;                 // live rows
+  int32_t hk;
+  int32_t pad[3];
 };
 
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
@@ -89,6 +103,1102 @@ __global__ void __launch_bounds__(32) cache_attn_simple_kernel(CacheArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Tensor cores
+// ---------------------------------------------------------------------------
+
+constexpr int kTK = 128;                 // keys per tile
+constexpr int kRows = 128;               // query rows per tile (MMA M)
+constexpr int kRowWarps = 8;
+constexpr int kMmaWarp = kRowWarps, kCopyWarp = kMmaWarp + 1, kPrepWarp = kCopyWarp + 2;
+constexpr int kItemCost = 512;
+constexpr int kMeta = 16;                // tiles whose notes are kept: more than the stages let run apart
+constexpr int kLag = 2;                  // row by row: tiles on their way behind the one announced
+constexpr int kKeyGroup = 16, kKeyGroups = kTK / kKeyGroup;   // keys that share a scale (bf16)
+
+// floats of one partial state: m [128], l [128], acc [D / 4][128][4]
+template <int D>
+constexpr int64_t part_floats() { return 2 * kRows + static_cast<int64_t>(D) * kRows; }
+
+template <typename T>
+struct Kind {
+  static constexpr bool kBf16 = false;
+  static constexpr int PREP = 1;                     // warps
+};
+template <>
+struct Kind<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
+  static constexpr int PREP = 5;                     // one idle: whole warpgroups
+};
+template <typename T>
+constexpr int cache_threads() { return 32 * (kPrepWarp + Kind<T>::PREP); }
+
+template <int D>
+struct CacheLayout {
+  static constexpr int HALF = kTK * 128;             // bytes of 64 columns of a tile
+  static constexpr int TILE = kTK * D * 2;
+  static constexpr int NST = D == 128 ? 3 : 6;       // stages of K and of V
+  static constexpr int K_OFF = 0, V_OFF = NST * TILE;
+  // notes on a tile: range, four words of keys that are there, four of keys whose
+  // V is not finite, scaled, inverse scales of K and V
+  static constexpr int META = V_OFF + NST * TILE, META_WORDS = 10 + 2 * kKeyGroups;
+  static constexpr int MAX = META + kMeta * META_WORDS * 4;       // row maxima of the halves [2][2][128]
+  static constexpr int BAR = MAX + 4 * kRows * 4;
+  static constexpr int NBAR = 6 * NST + 2 * 2 + 4;
+  static constexpr int MISC = BAR + NBAR * 8;
+  static constexpr int BYTES = MISC + 64 + 1024;
+  // TMEM columns: two S, whose place P takes (16 keys: eight columns of hi and
+  // eight of lo pairs), O, Q hi and lo (D / 2 each)
+  static constexpr uint32_t S_COL = 0, O_COL = 2 * kTK, Q_COL = O_COL + D, COLS = 512;
+  static_assert(Q_COL + D <= COLS, "TMEM columns");
+  static_assert(BYTES <= 222 * 1024, "shared memory");
+};
+// words of a tile's notes
+constexpr int kRange = 0, kThere = 1, kPois = 5, kScaled = 9, kKinv = 10, kVinv = 10 + kKeyGroups;
+// the range word: keys that all rows see | keys that are read << 8, and these bits
+constexpr uint32_t kMissing = 1u << 16, kLast = 1u << 17;
+
+// One sequence's share of the work.
+struct SeqWork {
+  int64_t a0;
+  int nq, pre, nqt;
+  bool bad;                     // lengths that do not fit
+};
+
+__device__ __forceinline__ SeqWork seq_work(const CacheArgs& a, int s) {
+  SeqWork w = {};
+  const int64_t a0 = a.q_start[s], n = a.q_start[s + 1] - a0;
+  const int pre = a.prefix[s];
+  const int64_t cap = min(a.max_blocks * a.bs, static_cast<int64_t>(INT32_MAX - 2 * kTK));
+  w.a0 = a0;
+  w.bad = a0 < 0 || n < 0 || a0 + n > a.total || n > a.max_q || pre < 0 || max(pre, 0) + max(n, int64_t(0)) > cap;
+  if (a0 < 0 || n <= 0 || a0 >= a.total) return w;
+  w.nq = static_cast<int>(min(min(n, static_cast<int64_t>(a.max_q)), min(a.total - a0, cap)));
+  w.pre = static_cast<int>(min(static_cast<int64_t>(max(pre, 0)), cap - w.nq));
+  w.nqt = (w.nq + a.npt - 1) / a.npt;
+  return w;
+}
+// The line's units are keys: an item counts those that its last row sees, and
+// item_cost.  Units of the items of row tiles 0 .. qt - 1, and of all.
+__device__ __forceinline__ int64_t units_before(const CacheArgs& a, const SeqWork& w, int qt) {
+  return a.hkv * (static_cast<int64_t>(qt) * (w.pre + a.item_cost) + static_cast<int64_t>(a.npt) * qt * (qt + 1) / 2);
+}
+__device__ __forceinline__ int64_t units_of(const CacheArgs& a, const SeqWork& w) {
+  return w.nqt == 0 ? 0 : units_before(a, w, w.nqt - 1) + a.hkv * (static_cast<int64_t>(w.pre) + w.nq + a.item_cost);
+}
+
+// The items of one CTA's share [u0, u1) of the line, one after the other; tile t of
+// the item that starts at u belongs to the share that holds u + t * kTK.  Each warp
+// keeps its own walk in shared memory (registers are for the tiles).
+struct Walk {
+  SeqWork w;                    // of sequence s
+  int64_t u, u0, u1;            // u: where the next item starts
+  int s, qt, hk;
+};
+struct Piece {
+  int64_t a0, u;                // of the sequence, of the item
+  int s, hk, t0, t1, nq, pre, ntiles;
+  int node0, keys, kmin;        // first token of the row tile; keys that any row sees, that all see
+};
+
+__device__ __forceinline__ bool next_piece(const CacheArgs& a, Walk* wk, Piece* p) {
+  Walk k = *wk;
+  bool found = false;
+  while (!found && k.u < k.u1) {
+    const int keys = k.w.pre + min(k.w.nq, (k.qt + 1) * a.npt);
+    p->ntiles = (keys + kTK - 1) / kTK;
+    p->t0 = k.u0 > k.u ? static_cast<int>((k.u0 - k.u + kTK - 1) / kTK) : 0;
+    const int64_t to = (k.u1 - k.u + kTK - 1) / kTK;
+    p->t1 = static_cast<int>(min(to, static_cast<int64_t>(p->ntiles)));
+    p->a0 = k.w.a0;
+    p->u = k.u;
+    p->s = k.s;
+    p->hk = k.hk;
+    p->nq = k.w.nq;
+    p->pre = k.w.pre;
+    p->node0 = k.qt * a.npt;
+    p->keys = keys;
+    p->kmin = k.w.pre + p->node0 + 1;
+    found = p->t0 < p->t1;
+    k.u += keys + a.item_cost;
+    if (++k.hk == static_cast<int>(a.hkv)) {
+      k.hk = 0;
+      if (++k.qt == k.w.nqt) {
+        k.qt = 0;
+        do {
+          if (++k.s >= a.num_seqs) {
+            k.u = k.u1;
+            break;
+          }
+          k.w = seq_work(a, k.s);
+        } while (k.w.nqt == 0);
+      }
+    }
+  }
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) *wk = k;
+  __syncwarp();
+  return found;
+}
+
+// Up to 64 polls of an mbarrier's phase, as few instructions as a poll takes
+// (the waiting warps share their schedulers with working ones).
+__device__ __forceinline__ bool mbar_poll64(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 k;\n\t"
+      "mov.u32 k, 64;\n\t"
+      "POLL:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "sub.u32 k, k, 1;\n\t"
+      "setp.ne.u32 q, k, 0;\n\t"
+      "@q bra POLL;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// largest |x|; NaN wins
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return m;
+}
+// Power of two that brings values up to `top` into [2^14, 2^15), and its
+// inverse.
+__device__ __forceinline__ void pow2_scale(float top, float* s, float* inv) {
+  const int e = min(268 - static_cast<int>(abs_bits(top) >> 23), 253);
+  *s = __uint_as_float(static_cast<uint32_t>(e) << 23);
+  *inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+}
+// two floats in one register pair: one instruction for both
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// x = hi + lo as fp16 pairs: hi the leading 11 bits, lo the next 11
+__device__ __forceinline__ void split2(F2 xy, uint32_t* hi, uint32_t* lo) {
+  const float2 f = unpack(xy);
+  const float hx = __uint_as_float(__float_as_uint(f.x) & 0xffffe000u);
+  const float hy = __uint_as_float(__float_as_uint(f.y) & 0xffffe000u);
+  const float2 r = unpack(fma2(f2(hx, hy), f2(-1.0f, -1.0f), xy));
+  *hi = h2_bits(__floats2half2_rn(hx, hy));
+  *lo = h2_bits(__floats2half2_rn(r.x, r.y));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The loads of v have arrived (v as operands: no use may move above this).
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                 "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]),
+                 "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                 "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Four lanes with element k of row i each (i = 0..3 in x[i], k = lane & 3) change
+// to row k's elements in each lane.  Its own inverse.
+__device__ __forceinline__ void exchange4(float4 (&x)[4], int lane) {
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(i & o)) {
+        const bool up = lane & o;
+        float4 s = up ? x[i] : x[i + o];
+        s.x = __shfl_xor_sync(0xffffffffu, s.x, o);
+        s.y = __shfl_xor_sync(0xffffffffu, s.y, o);
+        s.z = __shfl_xor_sync(0xffffffffu, s.z, o);
+        s.w = __shfl_xor_sync(0xffffffffu, s.w, o);
+        if (up)
+          x[i] = s;
+        else
+          x[i + o] = s;
+      }
+}
+// Operand descriptor of V, 128-byte swizzle: a 128-byte row holds 64 of the N
+// columns, 1024 bytes from eight keys to the next eight, HALF to the next 64
+// columns.
+__device__ __forceinline__ uint64_t desc_v(uint32_t smem_addr, uint32_t half) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(half >> 4) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <int N>
+__device__ __forceinline__ void set_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// The two warps of 32 query rows (halves of the keys) meet.
+__device__ __forceinline__ void pair_sync(int warp) {
+  asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Element offset of the K row of a sequence's `pos`, -1 without one.
+__device__ __noinline__ int64_t key_offset(const CacheArgs& a, int s, int hk, int pos, int D) {
+  const int bs = static_cast<int>(a.bs), j = pos / bs;
+  const int64_t blk = a.block_tables[static_cast<int64_t>(s) * a.max_blocks + j];
+  if (blk < 0 || blk >= a.num_blocks) return -1;
+  return ((((blk * a.num_layers + a.layer) * 2) * a.hkv + hk) * a.bs + (pos - j * bs)) * D;
+}
+
+// Byte of a tile's 16-byte chunk c (of D / 8) of a key's row.
+template <int D>
+__device__ __forceinline__ uint32_t tile_byte(int key, int c) {
+  return (D == 128 ? static_cast<uint32_t>(c >> 3) * CacheLayout<D>::HALF : 0u) + static_cast<uint32_t>(key) * 128 +
+         (static_cast<uint32_t>((c & 7) ^ (key & 7)) << 4);
+}
+
+// A pair of 16-bit values: ones in the exponent, as sign bits.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  constexpr uint32_t e = Kind<T>::kBf16 ? 0x7f807f80u : 0x7c007c00u, one = Kind<T>::kBf16 ? 0x00800080u : 0x04000400u;
+  return ((w & e) + one) & 0x80008000u;
+}
+
+// V rows that not every query row sees: those that are not there become zeros (a
+// probability of 0 times what happens to stand in them must be 0), and so do
+// elements that are not finite, whose keys are noted for the rows that see them.
+template <int D, typename T>
+__device__ __noinline__ void clean_v(uint8_t* tile, uint32_t* note, int lane) {
+  constexpr int CPR = D / 8;
+  const uint32_t range = note[kRange];
+  const int hi = static_cast<int>((range >> 8) & 0xff), from = (range & kMissing) ? 0 : static_cast<int>(range & 0xff);
+  if (lane < 4) note[kPois + lane] = 0;
+  __syncwarp();
+  for (int i = from * CPR + lane; i < kTK * CPR; i += 32) {
+    const int key = i / CPR;
+    uint4* at = reinterpret_cast<uint4*>(tile + tile_byte<D>(key, i % CPR));
+    if (key >= hi || !((note[kThere + (key >> 5)] >> (key & 31)) & 1)) {
+      *at = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    uint4 v = *at;
+    const uint32_t bx = not_finite2<T>(v.x), by = not_finite2<T>(v.y), bz = not_finite2<T>(v.z), bw = not_finite2<T>(v.w);
+    if (bx | by | bz | bw) {
+      auto keep = [](uint32_t w, uint32_t b) {
+        return w & ~((b & 0x8000u ? 0xffffu : 0u) | (b & 0x80000000u ? 0xffff0000u : 0u));
+      };
+      *at = make_uint4(keep(v.x, bx), keep(v.y, by), keep(v.z, bz), keep(v.w, bw));
+      atomicOr(note + kPois + (key >> 5), 1u << (key & 31));
+    }
+  }
+  __syncwarp();
+}
+
+// BOX: copies by TMA, `box` pool rows each (block sizes that are multiples of
+// eight); otherwise row by row.
+template <int D, typename T, bool BOX>
+__global__ void __launch_bounds__(cache_threads<T>(), 1)
+cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
+  using L = CacheLayout<D>;
+  constexpr int NST = L::NST, kThreads = cache_threads<T>();
+  constexpr bool kBf16 = Kind<T>::kBf16;
+  extern __shared__ uint8_t smem_raw[];
+  // aligned by an offset, so that the compiler still sees shared memory (a
+  // pointer rounded as an integer makes every access a generic one)
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint32_t* const notes = reinterpret_cast<uint32_t*>(smem + L::META);
+  float* const max_s = reinterpret_cast<float*>(smem + L::MAX);
+  uint64_t* kraw = reinterpret_cast<uint64_t*>(smem + L::BAR);
+  uint64_t* vraw = kraw + NST;
+  uint64_t* kfull = vraw + NST;         // bf16: widened; fp16: kraw itself counts
+  uint64_t* vfull = kfull + NST;
+  uint64_t* kempty = vfull + NST;
+  uint64_t* vempty = kempty + NST;
+  uint64_t* sfull = vempty + NST;       // [2]
+  uint64_t* pready = sfull + 2;         // [2]
+  uint64_t* ofull = pready + 2;
+  uint64_t* oempty = ofull + 1;
+  uint64_t* qready = oempty + 1;
+  uint64_t* drain = qready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int64_t scan_s[kThreads / 32];
+  __shared__ Walk walk_s[kThreads / 32], start_s;
+  __shared__ SplitItem cut_s;
+  __shared__ Piece piece_s[kRowWarps];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&kraw[i], 1);
+      mbar_init(&vraw[i], 1);
+      mbar_init(&kfull[i], 4);
+      mbar_init(&vfull[i], kBf16 ? 4 : 1);
+      mbar_init(&kempty[i], 1);
+      mbar_init(&vempty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pready[i], kRowWarps);
+    }
+    mbar_init(ofull, 1);
+    mbar_init(oempty, kRowWarps);
+    mbar_init(qready, kRowWarps);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, L::COLS);
+    tmem_relinquish();
+  }
+  if (BOX && warp == kCopyWarp && lane == 0) prefetch_tmap(&map);
+  tc_fence_before();
+  grid_dep_wait();
+
+  // Q into L2 while the memory is idle: behind the K/V copies a row takes
+  // thousands of cycles
+  {
+    const int64_t bytes = a.total * a.hq * D * 4, each = (bytes / gridDim.x + 15) & ~int64_t(15);
+    const int64_t lo = each * blockIdx.x;
+    if (lo < bytes)
+      prefetch_range_l2(reinterpret_cast<const uint8_t*>(a.q) + lo,
+                        static_cast<size_t>(min(each, bytes - lo)), tid, kThreads);
+  }
+
+  // The line: its length, and the place where this CTA's share starts.
+  int64_t u0 = 0, q = 0, r = 0;                   // q units a CTA, one more for the first r
+  {
+    SeqWork w = {};
+    int64_t v = 0, inc = 0, carry = 0;
+    auto scan = [&](int b, bool first) {          // of kThreads sequences from b on
+      w = {};
+      v = 0;
+      if (b + tid < a.num_seqs) {
+        w = seq_work(a, b + tid);
+        v = units_of(a, w);
+        if (first && blockIdx.x == 0 && w.bad) raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
+      }
+      inc = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      __syncthreads();
+      if (lane == 31) scan_s[warp] = inc;
+      __syncthreads();
+      const int warps = min(kThreads / 32, (a.num_seqs - b + 31) / 32);
+      int64_t before = carry;
+      for (int i = 0; i < warps; ++i) {
+        if (i < warp) before += scan_s[i];
+        carry += scan_s[i];
+      }
+      inc += before;
+    };
+    auto find = [&](int b) {
+      if (v > 0 && u0 >= inc - v && u0 < inc) {
+        const int64_t rel = u0 - (inc - v);
+        int lo = 0, hi = w.nqt - 1;               // the last row tile that starts at or before rel
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (units_before(a, w, mid) <= rel)
+            lo = mid;
+          else
+            hi = mid - 1;
+        }
+        const int64_t in = rel - units_before(a, w, lo);
+        const int len = w.pre + min(w.nq, (lo + 1) * a.npt) + a.item_cost;
+        const int hk = static_cast<int>((in >> 32) ? in / len : static_cast<uint32_t>(in) / static_cast<uint32_t>(len));
+        start_s.w = w;
+        start_s.s = b + tid;
+        start_s.qt = lo;
+        start_s.hk = hk;
+        start_s.u = u0 - (in - static_cast<int64_t>(hk) * len);
+        start_s.u0 = u0;
+        start_s.u1 = u0 + q + (blockIdx.x < r ? 1 : 0);
+      }
+    };
+    if (tid == 0) start_s.u = start_s.u1 = 0;
+    for (int b = 0; b < a.num_seqs; b += kThreads) scan(b, true);
+    // a share is a tile at least, so that every CTA between an item's first and last
+    // has a piece of it
+    const int64_t U = carry, G = max(min(static_cast<int64_t>(gridDim.x), U / kTK), int64_t(1));
+    q = (U >> 32) ? U / G : static_cast<uint32_t>(U) / static_cast<uint32_t>(G);
+    r = U - q * G;
+    u0 = blockIdx.x * q + min(static_cast<int64_t>(blockIdx.x), r);
+    if (blockIdx.x < G) {
+      if (a.num_seqs <= kThreads) {
+        find(0);
+      } else {
+        carry = 0;
+        for (int b = 0; b < a.num_seqs; b += kThreads) scan(b, false), find(b);
+      }
+    }
+  }
+  __syncthreads();
+  // the next kernel's CTAs may take TMEM before they wait for this one: not
+  // before this CTA has its own
+  grid_dep_launch();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Walk* const wk = &walk_s[warp];
+  if (lane == 0) *wk = start_s;
+  if (tid == 0) cut_s.first = 0, cut_s.last = -1;
+  __syncwarp();
+  Piece pc = {};
+
+  // Bounded wait of the whole warp; gives up for all roles together, and from then on
+  // at once: the row warps go through their steps to the end all the same, because
+  // their pairs meet in each.
+  bool dead = false;
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (dead) return false;
+    bool ok = false;
+    for (uint32_t i = 0; i < (1u << 16); ++i) {
+      ok = mbar_poll64(bar, parity);
+      if (ok || *abort_flag) break;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) {
+      *abort_flag = 1;
+      dead = true;
+    }
+    return ok;
+  };
+
+  if (warp >= kRowWarps) {
+  set_regs_dec<kBf16 ? 72 : 104>();
+  if (warp == kMmaWarp) {
+    // ---------------- MMAs ----------------
+    constexpr uint32_t id_s = idesc_f16_f32(kRows, kTK);
+    constexpr uint32_t id_o = idesc_f16_f32(kRows, D) | (1u << 16);   // B: keys along K
+    const uint32_t kbase = smem_u32(smem + L::K_OFF), vbase = smem_u32(smem + L::V_OFF);
+    uint64_t* const kready = kBf16 ? kfull : kraw;
+    int n = 0, seg = 0;
+    bool ok = true;
+    auto scores = [&](int m) -> bool {              // S of tile m into buffer m & 1
+      const int st = m % NST;
+      if (!wait(kready + st, (m / NST) & 1)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t d = tmem + L::S_COL + static_cast<uint32_t>(m & 1) * kTK;
+        const uint64_t kd = desc_k_sw128(kbase + st * L::TILE);
+        // the small terms first: the tensor core cuts low bits off at every step,
+        // relative to the sum so far
+#pragma unroll
+        for (int term = 1; term >= 0; --term)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_f16_ts(d, tmem + L::Q_COL + term * (D / 2) + 8 * k, kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
+                       (term == 0 || k > 0) ? 1u : 0u);
+        mma_commit(&kempty[st]);
+        mma_commit(&sfull[m & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    while (ok && next_piece(a, wk, &pc)) {
+      if (!(ok = wait(qready, seg & 1))) break;
+      ++seg;
+      tc_fence_after();
+      const int cnt = pc.t1 - pc.t0;
+      if (!(ok = scores(n))) break;
+      if (cnt > 1 && !(ok = scores(n + 1))) break;
+#pragma unroll 1
+      for (int i = 0; i < cnt; ++i) {
+        const int m = n + i, st = m % NST;
+        if (!(ok = wait(&vfull[st], (m / NST) & 1) && wait(&pready[m & 1], (m >> 1) & 1) &&
+                   (m == 0 || wait(oempty, (m - 1) & 1))))
+          break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t d = tmem + L::O_COL;
+          const uint32_t p = tmem + L::S_COL + static_cast<uint32_t>(m & 1) * kTK;
+          const uint64_t vd = desc_v(vbase + st * L::TILE, L::HALF);
+#pragma unroll
+          for (int term = 1; term >= 0; --term)
+#pragma unroll
+            for (int k = 0; k < kTK / 16; ++k)
+              mma_f16_ts(d, p + 16 * k + 8 * term, vd + k * (2048 / 16), id_o, (term == 0 || k > 0) ? 1u : 0u);
+          mma_commit(&vempty[st]);
+          mma_commit(ofull);
+        }
+        __syncwarp();
+        // over P of this tile, which the products before it in the pipe have read
+        if (i + 2 < cnt && !(ok = scores(m + 2))) break;
+      }
+      n += cnt;
+    }
+    // nothing of this CTA's is in flight when its TMEM goes
+    if (elect_one()) mma_commit(drain);
+    __syncwarp();
+    mbar_wait(drain, 0);
+  } else if (warp == kCopyWarp || warp == kCopyWarp + 1) {
+    // ---------------- K (one warp) / V (the next) rows into shared memory ----------------
+    const int kv = warp - kCopyWarp;
+    uint64_t* const raw = kv ? vraw : kraw;
+    uint64_t* const freed = kv ? vempty : kempty;
+    uint8_t* const base = smem + (kv ? L::V_OFF : L::K_OFF);
+    // A lane has the boxes lane & 15 of a tile (of the columns 64 (lane >> 4) on), or
+    // its keys lane + 32 h: table column, place in the block and table entry, the
+    // entry fetched one tile ahead.  A tile's lookups are additions.
+    constexpr int NH = BOX ? 1 : 4;
+    const int bs = static_cast<int>(a.bs), dj = kTK / bs, dr = kTK - dj * bs;
+    const int box = BOX ? a.box : 1, nbox = kTK / box;
+    const int mine = BOX ? (lane & 15) : lane;
+    const bool use = !BOX || (mine < nbox && lane < D / 4);
+    const uint32_t rows_per_block = static_cast<uint32_t>(a.num_layers * 2 * a.hkv * a.bs);
+    bool have = next_piece(a, wk, &pc), bad = false;
+    int t = 0, done = 0, sent = 0;                // sent: row by row, tiles that are announced
+    uint32_t row0 = 0;                            // of the piece's layer and head in block 0
+    const int32_t* table = nullptr;
+    int col[NH], rest[NH], blk[NH];
+    auto begin = [&]() {
+      t = pc.t0;
+      row0 = static_cast<uint32_t>(((a.layer * 2 + kv) * a.hkv + pc.hk) * a.bs);
+      table = a.block_tables + static_cast<int64_t>(pc.s) * a.max_blocks;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const int pos = t * kTK + (mine + 32 * h) * box;
+        col[h] = pos / bs;
+        rest[h] = pos - col[h] * bs;
+      }
+    };
+    auto fetch = [&]() {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        blk[h] = -1;
+        if (have && use && t * kTK + (mine + 32 * h) * box < pc.keys) {
+          blk[h] = table[col[h]];
+          if (blk[h] < 0) blk[h] = INT32_MAX;
+        }
+      }
+    };
+    auto announce = [&]() {                       // row by row: a tile's copies have landed
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(raw + sent % NST);
+      ++sent;
+    };
+    if (have) begin();
+    fetch();
+    while (have) {
+      uint32_t row[NH], there[NH];
+      bool lost = false;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const bool on = blk[h] >= 0 && blk[h] < a.num_blocks;
+        lost = lost || (blk[h] >= 0 && !on);
+        row[h] = on ? static_cast<uint32_t>(blk[h]) * rows_per_block + row0 + static_cast<uint32_t>(rest[h]) : 0xffffffffu;
+        there[h] = __ballot_sync(0xffffffffu, on);
+      }
+      lost = __any_sync(0xffffffffu, lost);
+      bad = bad || lost;
+      const int lo = min(max(pc.kmin - t * kTK, 0), kTK), hi = min(max(pc.keys - t * kTK, 0), kTK);
+      if (++t < pc.t1) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          col[h] += dj;
+          rest[h] += dr;
+          if (rest[h] >= bs) rest[h] -= bs, ++col[h];
+        }
+      } else {
+        have = next_piece(a, wk, &pc);
+        if (have) begin();
+      }
+      fetch();
+      const int st = done % NST;
+      uint32_t* const note = notes + (done % kMeta) * L::META_WORDS;
+      if (done >= NST && !wait(freed + st, ((done / NST) - 1) & 1)) break;
+      // both warps the same
+      uint32_t word = 0xffffffffu;
+      if (BOX) {
+        if (lost && lane < 4) {
+          word = 0;
+          for (int i = 0; i < 32; ++i) word |= ((there[0] >> ((32 * lane + i) / box)) & 1u) << i;
+        }
+      } else {
+        word = lane == 0 ? there[0] : lane == 1 ? there[NH > 1 ? 1 : 0] : lane == 2 ? there[NH > 2 ? 2 : 0] : there[NH > 3 ? 3 : 0];
+      }
+      if (lane < 4) note[kThere + lane] = word;
+      if (lane == 0) note[kRange] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8 | (lost ? kMissing : 0) | (have ? 0 : kLast);
+      __syncwarp();
+      if (BOX) {
+        if (lane == 0) mbar_arrive_expect_tx(raw + st, static_cast<uint32_t>(__popc(there[0]) * box) * 128u);
+        __syncwarp();
+        if (row[0] != 0xffffffffu)
+          tma_load_2d(base + st * L::TILE + (lane >> 4) * L::HALF + mine * box * 128, &map, raw + st, (lane >> 4) * 64,
+                      static_cast<int32_t>(row[0]));
+      } else {
+        constexpr int CPR = D / 8, RPI = 32 / CPR;    // rows an instruction covers
+        const uint32_t dst = smem_u32(base + st * L::TILE);
+        const T* const pool = static_cast<const T*>(a.pool);
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll 4
+          for (int i = 0; i < 32 / RPI; ++i) {
+            const int k = i * RPI + lane / CPR, c = lane % CPR;
+            const uint32_t at = __shfl_sync(0xffffffffu, row[h], k);
+            if (at != 0xffffffffu)
+              copy16(dst + tile_byte<D>(32 * h + k, c), pool + static_cast<int64_t>(at) * D + c * 8);
+          }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (done - sent == kLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+          announce();
+        }
+      }
+      ++done;
+    }
+    if (BOX) {
+      // after an abort, let the copies still in flight land before the CTA exits
+      if (*abort_flag)
+        for (int i = max(0, done - NST); i < done; ++i) mbar_wait(raw + i % NST, (i / NST) & 1);
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      while (sent < done) announce();
+    }
+    if (bad && lane == 0) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
+  } else if (!kBf16) {
+    // ---------------- V rows that not every query row sees ----------------
+    bool more = next_piece(a, wk, &pc);
+#pragma unroll 1
+    for (int n = 0; more; ++n) {
+      const int st = n % NST;
+      uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
+      if (!wait(vraw + st, (n / NST) & 1)) break;
+      const uint32_t range = note[kRange];
+      if ((range & 0xff) < kTK || (range & kMissing)) {
+        clean_v<D, T>(smem + L::V_OFF + st * L::TILE, note, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      more = !(range & kLast);
+      if (lane == 0) mbar_arrive(vfull + st);
+    }
+  }
+  } else {
+    // ---------------- rows ----------------
+    set_regs_inc<kBf16 ? 184 : 200>();
+    const int hw = warp >> 2, row = (warp & 3) * 32 + lane;      // half, query row
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    constexpr int DH = D / 2;                       // columns of O per half
+    int n = 0;
+    const Piece& ps = piece_s[warp];                // of the rare paths
+    while (next_piece(a, wk, &pc)) {
+      __syncwarp();
+      if (lane == 0) piece_s[warp] = pc;
+      __syncwarp();
+      const int t0 = pc.t0, t1 = pc.t1;
+      const int rows = min(a.npt, pc.nq - pc.node0) * a.g;       // live ones of the tile
+      const bool live = row < rows;
+      // the row's place in q and out
+      auto row_at = [&](int R) -> int64_t {
+        const int node = R / a.g;
+        return ((ps.a0 + ps.node0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
+      };
+      float qinv;
+      // Q: hi / lo terms of the half's columns into TMEM.  Four lanes load 64
+      // bytes of a row, for the rows of the four, and exchange them
+      {
+        const float* qp[4];
+        float m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int R = (row & ~3) + k;
+          qp[k] = R < rows ? a.q + row_at(R) + (lane & 3) * 4 : nullptr;
+          m[k] = 0.0f;
+        }
+        auto quad = [&](int k, int c) {
+          return qp[k] ? *reinterpret_cast<const float4*>(qp[k] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        float4 v[DH / 4];
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {      // the other half's for the maximum alone
+#pragma unroll
+          for (int c = 0; c < DH / 4; ++c) v[c] = quad(c & 3, (hw ^ half) * DH + (c >> 2) * 16);
+#pragma unroll
+          for (int c = 0; c < DH / 4; ++c)
+            m[c & 3] = amax3(amax3(m[c & 3], v[c].x, v[c].y), v[c].z, v[c].w);
+        }
+        // the four lanes' maxima of the lane's row
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) m[k] = amax3(m[k], __shfl_xor_sync(0xffffffffu, m[k], o), 0.0f);
+        const float top = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
+        float qs;
+        pow2_scale(top, &qs, &qinv);
+#pragma unroll
+        for (int c0 = 0; c0 < DH / 4; c0 += 8) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int c = c0; c < c0 + 8; c += 4) {
+            float4 x[4] = {v[c], v[c + 1], v[c + 2], v[c + 3]};
+            exchange4(x, lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = (c - c0 + k) * 2;
+              split2(mul2(f2(x[k].x, x[k].y), f2(qs, qs)), &hi[at], &lo[at]);
+              split2(mul2(f2(x[k].z, x[k].w), f2(qs, qs)), &hi[at + 1], &lo[at + 1]);
+            }
+          }
+          tmem_st_32x32b_x16(lanes + L::Q_COL + (hw * DH + c0 * 4) / 2, hi);
+          tmem_st_32x32b_x16(lanes + L::Q_COL + DH + (hw * DH + c0 * 4) / 2, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qready);
+      }
+      const float cq = qinv * (a.scale * 1.44269504088896340736f);   // to powers of two
+      if ((warp & 3) * 32 >= rows) {
+        // no row of the warp's is live (Q, and so S and P, are zeros): it only keeps step
+#pragma unroll 1
+        for (int t = t0; t <= t1; ++t, ++n) {
+          if (t < t1) {
+            wait(&sfull[n & 1], (n >> 1) & 1);
+            if (lane == 0) mbar_arrive(&pready[n & 1]);
+          }
+          if (t > t0) {
+            wait(ofull, (n - 1) & 1);
+            if (lane == 0) mbar_arrive(oempty);
+          }
+        }
+        --n;
+        continue;
+      }
+      const int limit = live ? pc.pre + pc.node0 + row / a.g : -1;   // the last key that the row sees
+      // running state: the reference that the sums stand at (in powers of two;
+      // it follows the maximum once that is 2^8 above it, so most tiles
+      // rescale nothing), the half's sum
+      float mref = -INFINITY, l = 0.0f;
+      F2 acc[DH / 2];
+#pragma unroll
+      for (int c = 0; c < DH / 2; ++c) acc[c] = f2(0.f, 0.f);
+      // of the tile whose P V is still to be added
+      float corr_p = 1.0f;
+      bool rare_p = false;
+
+      // softmax of tile t, then the addition of tile t - 1's P V
+#pragma unroll 1
+      for (int t = t0; t <= t1; ++t, ++n) {
+        float corr = 1.0f;
+        bool rare = false;
+        if (t < t1) {
+          const int b = n & 1;
+          wait(&sfull[b], (n >> 1) & 1);
+          tc_fence_after();
+          const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK + 64 * hw;   // the half's scores
+          float xa[32], xb[32];
+          tmem_ld_32x32b_x32(sc, xa);
+          tmem_ld_32x32b_x32(sc + 32, xb);
+          const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
+          const bool special = (t + 1) * kTK > pc.kmin || (*const_cast<const volatile uint32_t*>(note + kRange) & kMissing);
+          tmem_wait_ld(xa);
+          tmem_wait_ld(xb);
+          if (__builtin_expect(special, 0)) {
+            wait(&vfull[n % NST], (n / NST) & 1);    // the notes on V
+            const int cnt = limit + 1 - t * kTK;     // keys of the tile that come before the row's end
+            auto seen = [&](int i) -> uint32_t {
+              const int k = cnt - 32 * i;
+              return note[kThere + i] & (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1);
+            };
+            const uint32_t wa = seen(2 * hw), wb = seen(2 * hw + 1);
+            const uint32_t any = note[kPois] | note[kPois + 1] | note[kPois + 2] | note[kPois + 3];
+            if (any)
+#pragma unroll 1
+              for (int i = 0; i < 4; ++i) rare = rare || (seen(i) & note[kPois + i]) != 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              xa[j] = (wa >> j) & 1 ? xa[j] : -INFINITY;
+              xb[j] = (wb >> j) & 1 ? xb[j] : -INFINITY;
+            }
+          }
+          float m0 = max3(xa[0], xa[1], xa[2]), m1 = max3(xb[0], xb[1], xb[2]);
+#pragma unroll
+          for (int j = 3; j + 1 < 32; j += 2) {
+            m0 = max3(m0, xa[j], xa[j + 1]);
+            m1 = max3(m1, xb[j], xb[j + 1]);
+          }
+          const float m = max3(m0, m1, fmaxf(xa[31], xb[31]));
+          // both halves take the whole row's maximum
+          float* const mx = max_s + (n & 1) * 2 * kRows + row;
+          mx[hw * kRows] = m;
+          pair_sync(warp);
+          const float mc = fmaxf(m, mx[(hw ^ 1) * kRows]) * cq;
+          if (mc > mref + 8.0f) {
+            corr = ex2(mref - mc);
+            mref = mc;
+          }
+          // P = 2^(x c - ref), up to 2^14: its terms are fp16
+          const float ref = mref == -INFINITY ? 0.0f : mref - 6.0f;
+          const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
+          F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+          auto probs = [&](float (&x)[32], uint32_t at) {
+            uint32_t pt[32];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float2 e = unpack(fma2(f2(x[j], x[j + 1]), c2, nref));
+              const F2 p = f2(ex2(e.x), ex2(e.y));
+              s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], p);
+              const int k = (j >> 4) * 16 + ((j & 15) >> 1);
+              split2(p, &pt[k], &pt[k + 8]);
+            }
+            tmem_st_32x32b_x32(at, pt);
+          };
+          probs(xa, sc);
+          probs(xb, sc + 32);
+          const float2 sa = unpack(s2[0]), sb = unpack(s2[1]);
+          l = fmaf(l, corr, (sa.x + sa.y) + (sb.x + sb.y));
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pready[b]);
+        }
+        if (t > t0) {
+          wait(ofull, (n - 1) & 1);
+          tc_fence_after();
+          const uint32_t o = lanes + L::O_COL + hw * DH;
+          if (__any_sync(0xffffffffu, corr_p != 1.0f)) {
+#pragma unroll
+            for (int c = 0; c < DH / 2; ++c) acc[c] = mul2(acc[c], f2(corr_p, corr_p));
+          }
+#pragma unroll
+          for (int i = 0; i < DH; i += 32) {
+            float v[32];
+            tmem_ld_32x32b_x32(o + i, v);
+            tmem_wait_ld(v);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) acc[i / 2 + c] = add2(acc[i / 2 + c], f2(v[2 * c], v[2 * c + 1]));
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(oempty);
+          if (__builtin_expect(rare_p, 0)) {
+            // V elements that are not finite: to the rows that see them
+            const uint32_t* const note = notes + ((n - 1) % kMeta) * L::META_WORDS;
+            const int cnt = limit + 1 - (t - 1) * kTK;
+#pragma unroll 1
+            for (int k = 0; k < min(cnt, kTK); ++k) {
+              if (!((note[kPois + (k >> 5)] >> (k & 31)) & 1)) continue;
+              const int64_t at = key_offset(a, ps.s, ps.hk, (t - 1) * kTK + k, D);
+              if (at < 0) continue;
+              const T* vp = static_cast<const T*>(a.pool) + at + a.hkv * a.bs * D + hw * DH;
+#pragma unroll
+              for (int c = 0; c < DH / 2; ++c) {
+                const float v0 = widen(vp[2 * c]), v1 = widen(vp[2 * c + 1]);
+                acc[c] = add2(acc[c], f2(isfinite(v0) ? 0.0f : v0, isfinite(v1) ? 0.0f : v1));
+              }
+            }
+          }
+          __syncwarp();
+        }
+        corr_p = corr;
+        rare_p = rare;
+      }
+      --n;                                          // the round after the last tile
+
+      // the halves' sums; the maxima's place in it is free: the last tile's is the other one
+      {
+        float* const mx = max_s + (n & 1) * 2 * kRows + row;
+        mx[hw * kRows] = l;
+        pair_sync(warp);
+        l += mx[(hw ^ 1) * kRows];
+        pair_sync(warp);
+      }
+      if (t0 == 0 && t1 == ps.ntiles) {
+        const float inv = 1.0f / l;
+        float* op[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int R = (row & ~3) + k;
+          op[k] = R < rows ? a.out + row_at(R) + hw * DH + (lane & 3) * 4 : nullptr;
+        }
+#pragma unroll
+        for (int c = 0; c < DH; c += 16) {
+          float4 x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 p = unpack(acc[c / 2 + 2 * k]), u = unpack(acc[c / 2 + 2 * k + 1]);
+            x[k] = make_float4(p.x * inv, p.y * inv, u.x * inv, u.y * inv);
+            if (l == 0.0f) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          exchange4(x, lane);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (op[k]) *reinterpret_cast<float4*>(op[k] + c) = x[k];
+        }
+      } else {
+        float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * part_floats<D>();
+        if (live) {
+          if (hw == 0) {
+            part[row] = mref;
+            part[kRows + row] = l;
+          }
+#pragma unroll
+          for (int c = 0; c < DH; c += 4) {
+            const float2 p = unpack(acc[c / 2]), u = unpack(acc[c / 2 + 1]);
+            reinterpret_cast<float4*>(part + 2 * kRows)[(hw * DH + c) / 4 * kRows + row] = make_float4(p.x, p.y, u.x, u.y);
+          }
+        }
+        if (t0 == 0 && tid == 0) {                 // the share's last piece: joined from here on
+          const int64_t x = ps.u + static_cast<int64_t>(ps.ntiles - 1) * kTK;   // the item's last tile
+          cut_s.first = static_cast<int>(blockIdx.x);
+          cut_s.last = static_cast<int>(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
+          cut_s.row0 = static_cast<int>(ps.a0 + ps.node0);
+          cut_s.rows = rows;
+          cut_s.hk = ps.hk;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    if (*abort_flag) {
+      raise_flag(a.flags, KSH_FLAG_TIMEOUT);
+      cut_s.last = -1;
+    }
+    a.items[blockIdx.x] = cut_s;
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::COLS);
+  }
+}
+
+// Joins the pieces of an item cut between CTAs, in key order:
+// M = max m, out = sum acc 2^(m - M) / sum l 2^(m - M), in one pass over the
+// pieces with the running M, two at a time.
+constexpr int kMergeThreads = 256, kMergeChunks = 16, kMergePieces = 2;
+
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads) cache_merge_kernel(CacheArgs a) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const SplitItem it = a.items[blockIdx.x];
+  if (it.last < it.first) return;
+  for (int i = blockIdx.y * kMergeThreads + threadIdx.x; i < kRows * (D / 4);
+       i += kMergeThreads * kMergeChunks) {
+    const int r = i % kRows, c4 = i / kRows;
+    if (r >= it.rows) continue;
+    const float* p0 = a.part + (static_cast<int64_t>(it.first) * 2 + 1) * part_floats<D>();
+    auto piece = [&](int c) {
+      return c == it.first ? p0 : a.part + static_cast<int64_t>(c) * 2 * part_floats<D>();
+    };
+    float M = -INFINITY, L = 0.0f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = it.first; c0 <= it.last; c0 += kMergePieces) {
+      float m[kMergePieces], l[kMergePieces];
+      float4 v[kMergePieces];
+#pragma unroll
+      for (int u = 0; u < kMergePieces; ++u) {
+        const float* p = piece(min(c0 + u, it.last));
+        m[u] = p[r];
+        l[u] = p[kRows + r];
+        v[u] = reinterpret_cast<const float4*>(p + 2 * kRows)[c4 * kRows + r];
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < kMergePieces; ++u) top = fmaxf(top, m[u]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float w0 = ex2(M - ref);
+      M = top;
+      L *= w0;
+      A = make_float4(A.x * w0, A.y * w0, A.z * w0, A.w * w0);
+#pragma unroll
+      for (int u = 0; u < kMergePieces; ++u) {
+        if (c0 + u > it.last) break;
+        const float w = ex2(m[u] - ref);
+        L = fmaf(l[u], w, L);
+        A.x = fmaf(v[u].x, w, A.x);
+        A.y = fmaf(v[u].y, w, A.y);
+        A.z = fmaf(v[u].z, w, A.z);
+        A.w = fmaf(v[u].w, w, A.w);
+      }
+    }
+    const int node = r / a.g;
+    float* op = a.out + ((static_cast<int64_t>(it.row0) + node) * a.hq +
+                         static_cast<int64_t>(it.hk) * a.g + (r - node * a.g)) * D;
+    const float inv = 1.0f / L;
+    float4 v = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+    if (L == 0.0f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    reinterpret_cast<float4*>(op)[c4] = v;
+  }
+}
+
+template <int D, typename T, bool BOX>
+int launch_cache_tc(const CacheArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
+  using L = CacheLayout<D>;
+  auto kern = cache_attn_tc_kernel<D, T, BOX>;
+  if (set_smem_optin(reinterpret_cast<const void*>(kern), L::BYTES) != KSH_OK) return KSH_ERR_CUDA;
+  const int rc = launch(kern, dim3(static_cast<unsigned>(grid)), dim3(cache_threads<T>()), L::BYTES, st, a, map);
+  if (rc != KSH_OK || grid == 1) return rc;
+  return launch(cache_merge_kernel<D>, dim3(static_cast<unsigned>(grid - 1), kMergeChunks),
+                dim3(kMergeThreads), 0, st, a);
+}
+
+template <int D, typename T>
+int launch_cache_tc(CacheArgs& a, int grid, cudaStream_t st) {
+  CUtensorMap map = {};
+  if (a.bs % 8 != 0) return launch_cache_tc<D, T, false>(a, map, grid, st);
+  a.box = 8;
+  while (a.box < kTK && a.bs % (2 * a.box) == 0) a.box *= 2;
+  const uint64_t rows = static_cast<uint64_t>(a.num_blocks) * a.num_layers * 2 * a.hkv * a.bs;
+  if (!make_tensor_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, a.pool, D, rows, D * 2, 64, static_cast<uint32_t>(a.box),
+                          CU_TENSOR_MAP_SWIZZLE_128B))
+    return KSH_ERR_CUDA;
+  return launch_cache_tc<D, T, true>(a, map, grid, st);
+}
+
+int64_t items_bytes() { return (static_cast<int64_t>(num_sms()) * sizeof(SplitItem) + 255) / 256 * 256; }
+
 }  // namespace
 }  // namespace ksh
 
@@ -97,7 +1207,8 @@ using namespace ksh;
 extern "C" int64_t ksh_cache_attention_workspace_size(int64_t num_seqs, int64_t hq, int64_t hkv,
                                                       int64_t d, int64_t max_q_len) {
   if (num_seqs <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || d <= 0 || max_q_len < 0) return 0;
-  return 256;
+  if (d != 64 && d != 128) return 256;
+  return items_bytes() + 2 * (d == 64 ? part_floats<64>() : part_floats<128>()) * 4 * num_sms();
 }
 
 extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, int64_t d,
@@ -116,7 +1227,7 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
   KSH_CHECK_ARG(pool_type == KSH_TYPE_F16 || pool_type == KSH_TYPE_BF16);
   if (num_seqs == 0 || total == 0 || max_q_len == 0) return KSH_OK;
   KSH_CHECK_ARG(q && pool && block_tables && q_start && prefix_lens && out);
-  if (d > 256 || hq > 65535 || num_seqs > 65535) return KSH_ERR_UNSUPPORTED;
+  if (d > 256) return KSH_ERR_UNSUPPORTED;
   CacheArgs a = {};
   a.q = q;
   a.pool = pool;
@@ -139,6 +1250,30 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
   a.max_q = static_cast<int>(max_q_len);
   a.scale = static_cast<float>(1.0 / sqrt(static_cast<double>(d)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Tensor cores: rows of the pool are numbered in 32 bits (2^31 rows of 64
+  // halves are 256 GB), a tile holds the heads of at least one token
+  const bool fast = pool_type == KSH_TYPE_F16 && (d == 64 || d == 128) && a.g <= kRows &&
+      ((reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
+      static_cast<double>(num_blocks) * 2.0 * static_cast<double>(num_layers) * static_cast<double>(hkv) *
+              static_cast<double>(block_size) <= static_cast<double>(INT32_MAX) &&
+      tensor_map_encoder_available();
+  if (fast) {
+    if (!workspace || workspace_bytes < ksh_cache_attention_workspace_size(num_seqs, hq, hkv, d, max_q_len))
+      return KSH_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return KSH_ERR_ALIGN;
+    a.items = static_cast<SplitItem*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + items_bytes());
+    a.npt = kRows / a.g;
+    // No more CTAs than there can be tiles; an item's start counts only where there
+    // are several tiles a CTA.
+    const double tiles = static_cast<double>(num_seqs) * static_cast<double>(hkv) *
+                         static_cast<double>((max_q_len + a.npt - 1) / a.npt) *
+                         static_cast<double>(std::max<int64_t>(1, (max_total_len + kTK - 1) / kTK));
+    const int grid = static_cast<int>(std::min<double>(num_sms(), tiles));
+    a.item_cost = tiles >= 4.0 * num_sms() ? kItemCost : 0;
+    return d == 64 ? launch_cache_tc<64, __half>(a, grid, st) : launch_cache_tc<128, __half>(a, grid, st);
+  }
+  if (hq > 65535 || num_seqs > 65535) return KSH_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(max_q_len), static_cast<unsigned>(hq), static_cast<unsigned>(num_seqs));
   return pool_type == KSH_TYPE_F16 ? launch(cache_attn_simple_kernel<__half>, grid, dim3(32), 0, st, a)
                                    : launch(cache_attn_simple_kernel<__nv_bfloat16>, grid, dim3(32), 0, st, a);
