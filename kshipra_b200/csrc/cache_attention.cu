@@ -439,6 +439,85 @@ __device__ __noinline__ void clean_v(uint8_t* tile, uint32_t* note, int lane) {
   __syncwarp();
 }
 
+// bf16 to fp16 in place, 16 keys: exact times a power of two that brings the
+// largest into fp16's range (elements below 2^-28 of it lose bits), which is 1
+// where that already lies in [2^-7, 2^15).  Keys from `hi` on and those not in
+// `there` become zeros where the tile is not whole; in `clean` (V) so do elements
+// that are not finite, whose keys are returned.
+template <int D>
+__device__ __forceinline__ uint32_t widen16(uint8_t* tile, int key0, bool whole, bool clean, int hi, uint32_t there, int lane,
+                                            float* inv, bool* scaled) {
+  constexpr int CPR = D / 8, N = kKeyGroup * CPR / 32, RPI = 32 / CPR;
+  uint4 v[N];
+  uint32_t at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    at[i] = tile_byte<D>(key0 + i * RPI + lane / CPR, lane % CPR);
+    v[i] = *reinterpret_cast<const uint4*>(tile + at[i]);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = i * RPI + lane / CPR;
+      if (key0 + k >= hi || !((there >> k) & 1)) v[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  auto amax2 = [](uint32_t x, uint32_t y) {         // magnitudes; NaN wins; the signs are not of use
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+  };
+  auto top_of = [&]() {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = amax2(amax2(amax2(m, v[i].x), amax2(v[i].y, v[i].z)), v[i].w);
+    return __reduce_max_sync(0xffffffffu, max(m & 0x7fffu, (m >> 16) & 0x7fffu));
+  };
+  uint32_t top = top_of(), pois = 0;
+  if (__builtin_expect(top >= 0x7f80u, 0)) {
+    // the largest of the others; in `clean` these go
+    uint4 was[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      was[i] = v[i];
+      auto drop = [](uint32_t w) {
+        const uint32_t b = not_finite2<__nv_bfloat16>(w);
+        return w & ~((b & 0x8000u ? 0xffffu : 0u) | (b & 0x80000000u ? 0xffff0000u : 0u));
+      };
+      v[i] = make_uint4(drop(v[i].x), drop(v[i].y), drop(v[i].z), drop(v[i].w));
+      const uint32_t who = __ballot_sync(0xffffffffu, v[i].x != was[i].x || v[i].y != was[i].y || v[i].z != was[i].z || v[i].w != was[i].w);
+#pragma unroll
+      for (int k = 0; k < RPI; ++k)
+        if ((who >> (k * CPR)) & ((CPR == 32 ? 0u : 1u << CPR) - 1)) pois |= 1u << (i * RPI + k);
+    }
+    top = top_of();
+    if (!clean) {
+      pois = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = was[i];
+    }
+  }
+  const int e = static_cast<int>(top >> 7);
+  float s = 1.0f;
+  *inv = 1.0f;
+  if (e < 120 || e > 141) {
+    // just into the range: P takes the inverse scales relative to the tile's largest,
+    // so a group must not seem small beside one that is scaled less (zeros: the smallest)
+    const int to = e < 120 ? 247 - e : 268 - e;
+    s = __uint_as_float(static_cast<uint32_t>(to) << 23);
+    *inv = __uint_as_float(static_cast<uint32_t>(254 - to) << 23);
+    *scaled = *scaled || top != 0;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    auto wide = [&](uint32_t w) {
+      return h2_bits(__floats2half2_rn(__uint_as_float(w << 16) * s, __uint_as_float(w & 0xffff0000u) * s));
+    };
+    *reinterpret_cast<uint4*>(tile + at[i]) = make_uint4(wide(v[i].x), wide(v[i].y), wide(v[i].z), wide(v[i].w));
+  }
+  return pois;
+}
+
 // BOX: copies by TMA, `box` pool rows each (block sizes that are multiples of
 // eight); otherwise row by row.
 template <int D, typename T, bool BOX>
@@ -805,7 +884,45 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       while (sent < done) announce();
     }
     if (bad && lane == 0) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
-  } else if (!kBf16) {
+  } else if (kBf16) {
+    // ---------------- bf16: K and V to fp16, 32 keys a warp ----------------
+    const int pw = warp - kPrepWarp;
+    if (pw < 4) {
+      bool more = next_piece(a, wk, &pc);
+#pragma unroll 1
+      for (int n = 0; more; ++n) {
+        const int st = n % NST;
+        uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
+        bool scaled = false;
+        if (!wait(kraw + st, (n / NST) & 1)) break;
+        const uint32_t range = note[kRange], there = note[kThere + pw];
+        const bool whole = (range & 0xff) >= kTK && !(range & kMissing);
+        const int hi = static_cast<int>((range >> 8) & 0xff);
+        more = !(range & kLast);
+        uint32_t pois = 0;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          if (kv && !wait(vraw + st, (n / NST) & 1)) break;
+          uint8_t* const tile = smem + (kv ? L::V_OFF : L::K_OFF) + st * L::TILE;
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            float inv;
+            const uint32_t p = widen16<D>(tile, 32 * pw + 16 * g, whole, kv && !whole, hi, there >> (16 * g), lane, &inv, &scaled);
+            pois |= kv ? p << (16 * g) : 0u;
+            if (lane == 0) note[(kv ? kVinv : kKinv) + 2 * pw + g] = __float_as_uint(inv);
+          }
+          if (lane == 0 && kv) {
+            note[kPois + pw] = pois;
+            reinterpret_cast<uint8_t*>(note + kScaled)[pw] = scaled;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive((kv ? vfull : kfull) + st);
+        }
+        if (dead) break;
+      }
+    }
+  } else {
     // ---------------- V rows that not every query row sees ----------------
     bool more = next_piece(a, wk, &pc);
 #pragma unroll 1
@@ -923,17 +1040,18 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
       for (int c = 0; c < DH / 2; ++c) acc[c] = f2(0.f, 0.f);
       // of the tile whose P V is still to be added
-      float corr_p = 1.0f;
+      float corr_p = 1.0f, vs_p = 1.0f;
       bool rare_p = false;
 
       // softmax of tile t, then the addition of tile t - 1's P V
 #pragma unroll 1
       for (int t = t0; t <= t1; ++t, ++n) {
-        float corr = 1.0f;
+        float corr = 1.0f, vs = 1.0f;
         bool rare = false;
         if (t < t1) {
           const int b = n & 1;
           wait(&sfull[b], (n >> 1) & 1);
+          if (kBf16) wait(&vfull[n % NST], (n / NST) & 1);   // the notes on V
           tc_fence_after();
           const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK + 64 * hw;   // the half's scores
           float xa[32], xb[32];
@@ -941,10 +1059,23 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           tmem_ld_32x32b_x32(sc + 32, xb);
           const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
           const bool special = (t + 1) * kTK > pc.kmin || (*const_cast<const volatile uint32_t*>(note + kRange) & kMissing);
+          const uint32_t scaled = kBf16 ? note[kScaled] : 0u;
+          const float* const kinv = reinterpret_cast<const float*>(note + kKinv);
+          const float* const vinv = reinterpret_cast<const float*>(note + kVinv);
           tmem_wait_ld(xa);
           tmem_wait_ld(xb);
+          if (kBf16 && __builtin_expect(scaled != 0, 0)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              xa[j] *= kinv[4 * hw + (j >> 4)];
+              xb[j] *= kinv[4 * hw + 2 + (j >> 4)];
+            }
+            vs = vinv[0];
+#pragma unroll
+            for (int j = 1; j < kKeyGroups; ++j) vs = fmaxf(vs, vinv[j]);
+          }
           if (__builtin_expect(special, 0)) {
-            wait(&vfull[n % NST], (n / NST) & 1);    // the notes on V
+            if (!kBf16) wait(&vfull[n % NST], (n / NST) & 1);    // the notes on V
             const int cnt = limit + 1 - t * kTK;     // keys of the tile that come before the row's end
             auto seen = [&](int i) -> uint32_t {
               const int k = cnt - 32 * i;
@@ -981,20 +1112,26 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           const float ref = mref == -INFINITY ? 0.0f : mref - 6.0f;
           const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
           F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-          auto probs = [&](float (&x)[32], uint32_t at) {
+          // bf16: V's scales relative to the tile's largest
+          const float up = kBf16 ? __uint_as_float((254u << 23) - __float_as_uint(vs)) : 1.0f;
+          auto probs = [&](float (&x)[32], uint32_t at, int group) {
             uint32_t pt[32];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               const float2 e = unpack(fma2(f2(x[j], x[j + 1]), c2, nref));
-              const F2 p = f2(ex2(e.x), ex2(e.y));
+              F2 p = f2(ex2(e.x), ex2(e.y));
               s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], p);
+              if (kBf16) {
+                const float f = vinv[group + (j >> 4)] * up;
+                p = mul2(p, f2(f, f));
+              }
               const int k = (j >> 4) * 16 + ((j & 15) >> 1);
               split2(p, &pt[k], &pt[k + 8]);
             }
             tmem_st_32x32b_x32(at, pt);
           };
-          probs(xa, sc);
-          probs(xb, sc + 32);
+          probs(xa, sc, 4 * hw);
+          probs(xb, sc + 32, 4 * hw + 2);
           const float2 sa = unpack(s2[0]), sb = unpack(s2[1]);
           l = fmaf(l, corr, (sa.x + sa.y) + (sb.x + sb.y));
           tmem_wait_st();
@@ -1016,7 +1153,10 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
             tmem_ld_32x32b_x32(o + i, v);
             tmem_wait_ld(v);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) acc[i / 2 + c] = add2(acc[i / 2 + c], f2(v[2 * c], v[2 * c + 1]));
+            for (int c = 0; c < 16; ++c) {
+              const F2 x = f2(v[2 * c], v[2 * c + 1]);
+              acc[i / 2 + c] = kBf16 ? fma2(x, f2(vs_p, vs_p), acc[i / 2 + c]) : add2(acc[i / 2 + c], x);
+            }
           }
           tc_fence_before();
           __syncwarp();
@@ -1041,6 +1181,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           __syncwarp();
         }
         corr_p = corr;
+        vs_p = vs;
         rare_p = rare;
       }
       --n;                                          // the round after the last tile
@@ -1252,7 +1393,7 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Tensor cores: rows of the pool are numbered in 32 bits (2^31 rows of 64
   // halves are 256 GB), a tile holds the heads of at least one token
-  const bool fast = pool_type == KSH_TYPE_F16 && (d == 64 || d == 128) && a.g <= kRows &&
+  const bool fast = (d == 64 || d == 128) && a.g <= kRows &&
       ((reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
       static_cast<double>(num_blocks) * 2.0 * static_cast<double>(num_layers) * static_cast<double>(hkv) *
               static_cast<double>(block_size) <= static_cast<double>(INT32_MAX) &&
@@ -1271,7 +1412,9 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
                          static_cast<double>(std::max<int64_t>(1, (max_total_len + kTK - 1) / kTK));
     const int grid = static_cast<int>(std::min<double>(num_sms(), tiles));
     a.item_cost = tiles >= 4.0 * num_sms() ? kItemCost : 0;
-    return d == 64 ? launch_cache_tc<64, __half>(a, grid, st) : launch_cache_tc<128, __half>(a, grid, st);
+    if (pool_type == KSH_TYPE_F16)
+      return d == 64 ? launch_cache_tc<64, __half>(a, grid, st) : launch_cache_tc<128, __half>(a, grid, st);
+    return d == 64 ? launch_cache_tc<64, __nv_bfloat16>(a, grid, st) : launch_cache_tc<128, __nv_bfloat16>(a, grid, st);
   }
   if (hq > 65535 || num_seqs > 65535) return KSH_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(max_q_len), static_cast<unsigned>(hq), static_cast<unsigned>(num_seqs));
