@@ -109,42 +109,47 @@ __global__ void __launch_bounds__(32) cache_attn_simple_kernel(CacheArgs a) {
 
 constexpr int kTK = 128;                 // keys per tile
 constexpr int kRows = 128;               // query rows per tile (MMA M)
-constexpr int kRowWarps = 8;
-constexpr int kMmaWarp = kRowWarps, kCopyWarp = kMmaWarp + 1, kPrepWarp = kCopyWarp + 2;
+constexpr int kRowWarps = 8, kSumWarp = kRowWarps, kSumWarps = 4;
+constexpr int kMmaWarp = kSumWarp + kSumWarps, kCopyWarp = kMmaWarp + 2;     // even and odd tiles; K and V
+constexpr int kThreads = 32 * (kCopyWarp + 2);
+// registers a thread, of 128 at launch: rows, sums, the other roles
+constexpr int kRowRegs = 112, kSumRegs = 176, kRegs = 112;
 constexpr int kItemCost = 512;
 constexpr int kMeta = 16;                // tiles whose notes are kept: more than the stages let run apart
-constexpr int kLag = 2;                  // row by row: tiles on their way behind the one announced
-constexpr int kKeyGroup = 16, kKeyGroups = kTK / kKeyGroup;   // keys that share a scale (bf16)
-
+// Tiles (pieces) that the row warps can be ahead of the sum warps, and more
+constexpr int kRing = 4;
 // floats of one partial state: m [128], l [128], acc [D / 4][128][4]
 template <int D>
 constexpr int64_t part_floats() { return 2 * kRows + static_cast<int64_t>(D) * kRows; }
 
+// 16-bit terms of a query and of a probability: two of 11 bits, three of 8
 template <typename T>
 struct Kind {
   static constexpr bool kBf16 = false;
-  static constexpr int PREP = 1;                     // warps
+  static constexpr int TERMS = 2;
 };
 template <>
 struct Kind<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
-  static constexpr int PREP = 5;                     // one idle: whole warpgroups
+  static constexpr int TERMS = 3;
 };
-template <typename T>
-constexpr int cache_threads() { return 32 * (kPrepWarp + Kind<T>::PREP); }
 
-template <int D>
+template <int D, typename T>
 struct CacheLayout {
+  static constexpr bool LOW = Kind<T>::TERMS == 3;   // third terms stand in shared memory
   static constexpr int HALF = kTK * 128;             // bytes of 64 columns of a tile
   static constexpr int TILE = kTK * D * 2;
-  static constexpr int NST = D == 128 ? 3 : 6;       // stages of K and of V
-  static constexpr int K_OFF = 0, V_OFF = NST * TILE;
+  // stages of K and of V; the third terms of Q and P (128 rows x D, 128 rows x 128 keys)
+  static constexpr int NST = D == 128 ? (LOW ? 2 : 3) : (LOW ? 5 : 6);
+  static constexpr int K_OFF = 0, V_OFF = NST * TILE, QLOW = V_OFF + NST * TILE, PLOW = QLOW + (LOW ? TILE : 0);
   // notes on a tile: range, four words of keys that are there, four of keys whose
-  // V is not finite, scaled, inverse scales of K and V
-  static constexpr int META = V_OFF + NST * TILE, META_WORDS = 10 + 2 * kKeyGroups;
+  // V is not finite
+  static constexpr int META = PLOW + (LOW ? 2 * HALF : 0), META_WORDS = 9;
   static constexpr int MAX = META + kMeta * META_WORDS * 4;       // row maxima of the halves [2][2][128]
-  static constexpr int BAR = MAX + 4 * kRows * 4;
-  static constexpr int NBAR = 6 * NST + 2 * 2 + 4;
+  static constexpr int CORR = MAX + 4 * kRows * 4;                // what the sums are rescaled by [kRing][128]
+  static constexpr int FIN = CORR + kRing * kRows * 4;            // a piece's reference and the halves' sums [kRing][3][128]
+  static constexpr int BAR = FIN + kRing * 3 * kRows * 4;
+  static constexpr int NBAR = 5 * NST + 5 * 2 + 1;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int BYTES = MISC + 64 + 1024;
   // TMEM columns: two S, whose place P takes (16 keys: eight columns of hi and
@@ -154,7 +159,7 @@ struct CacheLayout {
   static_assert(BYTES <= 222 * 1024, "shared memory");
 };
 // words of a tile's notes
-constexpr int kRange = 0, kThere = 1, kPois = 5, kScaled = 9, kKinv = 10, kVinv = 10 + kKeyGroups;
+constexpr int kRange = 0, kThere = 1, kPois = 5;
 // the range word: keys that all rows see | keys that are read << 8, and these bits
 constexpr uint32_t kMissing = 1u << 16, kLast = 1u << 17;
 
@@ -187,6 +192,8 @@ __device__ __forceinline__ int64_t units_of(const CacheArgs& a, const SeqWork& w
   return w.nqt == 0 ? 0 : units_before(a, w, w.nqt - 1) + a.hkv * (static_cast<int64_t>(w.pre) + w.nq + a.item_cost);
 }
 
+// (Out of line, as what is called from several roles or seldom: with all of it inline
+// the code is 180 KB, and a role that comes to an item's start waits for instructions.)
 // The items of one CTA's share [u0, u1) of the line, one after the other; tile t of
 // the item that starts at u belongs to the share that holds u + t * kTK.  Each warp
 // keeps its own walk in shared memory (registers are for the tiles).
@@ -261,6 +268,41 @@ __device__ __forceinline__ bool mbar_poll64(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Whether a phase is over, without waiting: the answer is used some way on (a
+// wait that need not wait takes 150 to 250 cycles).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Of four barriers at once, a bit each.
+__device__ __forceinline__ uint32_t mbar_test4(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2,
+                                               uint64_t* b3, uint32_t p3) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r, s;\n\t.reg .u32 x;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 s, [%7], %8;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "selp.u32 x, 2, 0, q;\n\t"
+      "or.b32 %0, %0, x;\n\t"
+      "selp.u32 x, 4, 0, r;\n\t"
+      "or.b32 %0, %0, x;\n\t"
+      "selp.u32 x, 8, 0, s;\n\t"
+      "or.b32 %0, %0, x;\n\t}"
+      : "=&r"(r)
+      : "r"(smem_u32(b0)), "r"(p0), "r"(smem_u32(b1)), "r"(p1), "r"(smem_u32(b2)), "r"(p2), "r"(smem_u32(b3)), "r"(p3)
+      : "memory");
+  return r;
+}
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 // largest |x|; NaN wins
 __device__ __forceinline__ float amax3(float a, float b, float c) {
@@ -305,14 +347,28 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   return r;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// x = hi + lo as fp16 pairs: hi the leading 11 bits, lo the next 11
-__device__ __forceinline__ void split2(F2 xy, uint32_t* hi, uint32_t* lo) {
-  const float2 f = unpack(xy);
-  const float hx = __uint_as_float(__float_as_uint(f.x) & 0xffffe000u);
-  const float hy = __uint_as_float(__float_as_uint(f.y) & 0xffffe000u);
-  const float2 r = unpack(fma2(f2(hx, hy), f2(-1.0f, -1.0f), xy));
-  *hi = h2_bits(__floats2half2_rn(hx, hy));
-  *lo = h2_bits(__floats2half2_rn(r.x, r.y));
+// x as a sum of pairs of 16-bit terms: fp16 hi (the leading 11 bits) + lo (the next
+// 11), bf16 hi + lo + low (eight each).
+template <typename T>
+__device__ __forceinline__ void split(F2 xy, uint32_t* hi, uint32_t* lo, uint32_t* low) {
+  constexpr uint32_t kKeep = Kind<T>::kBf16 ? 0xffff0000u : 0xffffe000u;
+  auto cut = [](float2 f) {
+    return make_float2(__uint_as_float(__float_as_uint(f.x) & kKeep), __uint_as_float(__float_as_uint(f.y) & kKeep));
+  };
+  auto less = [](F2 a, float2 b) { return fma2(f2(b.x, b.y), f2(-1.0f, -1.0f), a); };
+  const float2 h = cut(unpack(xy));
+  const F2 r = less(xy, h);
+  if constexpr (Kind<T>::kBf16) {
+    const float2 m = cut(unpack(r)), t = unpack(less(r, m));
+    *hi = __byte_perm(__float_as_uint(h.x), __float_as_uint(h.y), 0x7632);
+    *lo = __byte_perm(__float_as_uint(m.x), __float_as_uint(m.y), 0x7632);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(t.x, t.y);
+    *low = *reinterpret_cast<const uint32_t*>(&b);
+  } else {
+    const float2 t = unpack(r);
+    *hi = h2_bits(__floats2half2_rn(h.x, h.y));
+    *lo = h2_bits(__floats2half2_rn(t.x, t.y));
+  }
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float m;
@@ -333,6 +389,14 @@ __device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
                  "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
                  "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
                  "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                 "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
                :
                : "memory");
 }
@@ -379,6 +443,11 @@ template <int N>
 __device__ __forceinline__ void set_regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // The two warps of 32 query rows (halves of the keys) meet.
 __device__ __forceinline__ void pair_sync(int warp) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
@@ -388,7 +457,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 }
 
 // Element offset of the K row of a sequence's `pos`, -1 without one.
-__device__ __noinline__ int64_t key_offset(const CacheArgs& a, int s, int hk, int pos, int D) {
+__device__ __forceinline__ int64_t key_offset(const CacheArgs& a, int s, int hk, int pos, int D) {
   const int bs = static_cast<int>(a.bs), j = pos / bs;
   const int64_t blk = a.block_tables[static_cast<int64_t>(s) * a.max_blocks + j];
   if (blk < 0 || blk >= a.num_blocks) return -1;
@@ -398,7 +467,7 @@ __device__ __noinline__ int64_t key_offset(const CacheArgs& a, int s, int hk, in
 // Byte of a tile's 16-byte chunk c (of D / 8) of a key's row.
 template <int D>
 __device__ __forceinline__ uint32_t tile_byte(int key, int c) {
-  return (D == 128 ? static_cast<uint32_t>(c >> 3) * CacheLayout<D>::HALF : 0u) + static_cast<uint32_t>(key) * 128 +
+  return (D == 128 ? static_cast<uint32_t>(c >> 3) * CacheLayout<D, __half>::HALF : 0u) + static_cast<uint32_t>(key) * 128 +
          (static_cast<uint32_t>((c & 7) ^ (key & 7)) << 4);
 }
 
@@ -439,92 +508,43 @@ __device__ __noinline__ void clean_v(uint8_t* tile, uint32_t* note, int lane) {
   __syncwarp();
 }
 
-// bf16 to fp16 in place, 16 keys: exact times a power of two that brings the
-// largest into fp16's range (elements below 2^-28 of it lose bits), which is 1
-// where that already lies in [2^-7, 2^15).  Keys from `hi` on and those not in
-// `there` become zeros where the tile is not whole; in `clean` (V) so do elements
-// that are not finite, whose keys are returned.
-template <int D>
-__device__ __forceinline__ uint32_t widen16(uint8_t* tile, int key0, bool whole, bool clean, int hi, uint32_t there, int lane,
-                                            float* inv, bool* scaled) {
-  constexpr int CPR = D / 8, N = kKeyGroup * CPR / 32, RPI = 32 / CPR;
-  uint4 v[N];
-  uint32_t at[N];
+// Adds the elements that are not finite of tile t's noted V rows (the first cnt keys
+// are a row's) to O, 16 columns at a time.
+template <int D, typename T>
+__device__ __forceinline__ void add_rare(const CacheArgs& a, const Piece& p, uint32_t oc, const uint32_t* note, int t, int cnt) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 16) {
+    float v[16];
+    tmem_ld_32x32b_x16(oc + c0, v);
+    tmem_wait_ld(v);
+#pragma unroll 1
+    for (int k = 0; k < cnt; ++k) {
+      if (!((note[kPois + (k >> 5)] >> (k & 31)) & 1)) continue;
+      const int64_t at = key_offset(a, p.s, p.hk, t * kTK + k, D);
+      if (at < 0) continue;
+      const T* vp = static_cast<const T*>(a.pool) + at + a.hkv * a.bs * D + c0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    at[i] = tile_byte<D>(key0 + i * RPI + lane / CPR, lane % CPR);
-    v[i] = *reinterpret_cast<const uint4*>(tile + at[i]);
-  }
-  if (!whole) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int k = i * RPI + lane / CPR;
-      if (key0 + k >= hi || !((there >> k) & 1)) v[i] = make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < 16; ++c) {
+        const float x = widen(vp[c]);
+        v[c] += isfinite(x) ? 0.0f : x;
+      }
     }
+    uint32_t bits[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) bits[c] = __float_as_uint(v[c]);
+    __syncwarp();
+    tmem_st_32x32b_x16(oc + c0, bits);
   }
-  auto amax2 = [](uint32_t x, uint32_t y) {         // magnitudes; NaN wins; the signs are not of use
-    uint32_t r;
-    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
-    return r;
-  };
-  auto top_of = [&]() {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = amax2(amax2(amax2(m, v[i].x), amax2(v[i].y, v[i].z)), v[i].w);
-    return __reduce_max_sync(0xffffffffu, max(m & 0x7fffu, (m >> 16) & 0x7fffu));
-  };
-  uint32_t top = top_of(), pois = 0;
-  if (__builtin_expect(top >= 0x7f80u, 0)) {
-    // the largest of the others; in `clean` these go
-    uint4 was[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      was[i] = v[i];
-      auto drop = [](uint32_t w) {
-        const uint32_t b = not_finite2<__nv_bfloat16>(w);
-        return w & ~((b & 0x8000u ? 0xffffu : 0u) | (b & 0x80000000u ? 0xffff0000u : 0u));
-      };
-      v[i] = make_uint4(drop(v[i].x), drop(v[i].y), drop(v[i].z), drop(v[i].w));
-      const uint32_t who = __ballot_sync(0xffffffffu, v[i].x != was[i].x || v[i].y != was[i].y || v[i].z != was[i].z || v[i].w != was[i].w);
-#pragma unroll
-      for (int k = 0; k < RPI; ++k)
-        if ((who >> (k * CPR)) & ((CPR == 32 ? 0u : 1u << CPR) - 1)) pois |= 1u << (i * RPI + k);
-    }
-    top = top_of();
-    if (!clean) {
-      pois = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = was[i];
-    }
-  }
-  const int e = static_cast<int>(top >> 7);
-  float s = 1.0f;
-  *inv = 1.0f;
-  if (e < 120 || e > 141) {
-    // just into the range: P takes the inverse scales relative to the tile's largest,
-    // so a group must not seem small beside one that is scaled less (zeros: the smallest)
-    const int to = e < 120 ? 247 - e : 268 - e;
-    s = __uint_as_float(static_cast<uint32_t>(to) << 23);
-    *inv = __uint_as_float(static_cast<uint32_t>(254 - to) << 23);
-    *scaled = *scaled || top != 0;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    auto wide = [&](uint32_t w) {
-      return h2_bits(__floats2half2_rn(__uint_as_float(w << 16) * s, __uint_as_float(w & 0xffff0000u) * s));
-    };
-    *reinterpret_cast<uint4*>(tile + at[i]) = make_uint4(wide(v[i].x), wide(v[i].y), wide(v[i].z), wide(v[i].w));
-  }
-  return pois;
+  tmem_wait_st();
 }
 
 // BOX: copies by TMA, `box` pool rows each (block sizes that are multiples of
 // eight); otherwise row by row.
 template <int D, typename T, bool BOX>
-__global__ void __launch_bounds__(cache_threads<T>(), 1)
+__global__ void __launch_bounds__(kThreads, 1)
 cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
-  using L = CacheLayout<D>;
-  constexpr int NST = L::NST, kThreads = cache_threads<T>();
+  using L = CacheLayout<D, T>;
+  constexpr int NST = L::NST;
   constexpr bool kBf16 = Kind<T>::kBf16;
   extern __shared__ uint8_t smem_raw[];
   // aligned by an offset, so that the compiler still sees shared memory (a
@@ -532,43 +552,43 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint32_t* const notes = reinterpret_cast<uint32_t*>(smem + L::META);
   float* const max_s = reinterpret_cast<float*>(smem + L::MAX);
+  float* const corr_s = reinterpret_cast<float*>(smem + L::CORR);
+  float* const fin_s = reinterpret_cast<float*>(smem + L::FIN);
   uint64_t* kraw = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* vraw = kraw + NST;
-  uint64_t* kfull = vraw + NST;         // bf16: widened; fp16: kraw itself counts
-  uint64_t* vfull = kfull + NST;
+  uint64_t* vfull = vraw + NST;         // cleaned, or as it came
   uint64_t* kempty = vfull + NST;
   uint64_t* vempty = kempty + NST;
   uint64_t* sfull = vempty + NST;       // [2]
   uint64_t* pready = sfull + 2;         // [2]
-  uint64_t* ofull = pready + 2;
-  uint64_t* oempty = ofull + 1;
-  uint64_t* qready = oempty + 1;
-  uint64_t* drain = qready + 1;
+  uint64_t* oempty = pready + 2;        // [2]: the MMA warps' tiles alternate
+  uint64_t* qready = oempty + 2;        // [2]
+  uint64_t* ofull = qready + 2;
+  uint64_t* drain = ofull + 1;          // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int64_t scan_s[kThreads / 32];
   __shared__ Walk walk_s[kThreads / 32], start_s;
   __shared__ SplitItem cut_s;
-  __shared__ Piece piece_s[kRowWarps];
+  __shared__ Piece piece_s[kRowWarps + kSumWarps];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&kraw[i], 1);
       mbar_init(&vraw[i], 1);
-      mbar_init(&kfull[i], 4);
-      mbar_init(&vfull[i], kBf16 ? 4 : 1);
+      mbar_init(&vfull[i], 1);
       mbar_init(&kempty[i], 1);
       mbar_init(&vempty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pready[i], kRowWarps);
+      mbar_init(&oempty[i], kSumWarps);
+      mbar_init(&qready[i], kRowWarps);
+      mbar_init(&drain[i], 1);
     }
     mbar_init(ofull, 1);
-    mbar_init(oempty, kRowWarps);
-    mbar_init(qready, kRowWarps);
-    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -691,89 +711,132 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
     return ok;
   };
 
-  if (warp >= kRowWarps) {
-  set_regs_dec<kBf16 ? 72 : 104>();
-  if (warp == kMmaWarp) {
+  // The same for three barriers, whose answers come together; *fourth: whether that
+  // one's phase is over, too.
+  auto wait3 = [&](uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2, uint64_t* b3, uint32_t p3,
+                   bool* fourth) -> bool {
+    if (dead) return false;
+    bool ok = false;
+    uint32_t all = 0;
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+      all = mbar_test4(b0, p0, b1, p1, b2, p2, b3, p3);
+      ok = (all & 7) == 7;
+      if (ok || ((i & 63) == 63 && *abort_flag)) break;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    *fourth = __all_sync(0xffffffffu, all & 8);
+    if (!ok) {
+      *abort_flag = 1;
+      dead = true;
+    }
+    return ok;
+  };
+
+  if (warp >= kMmaWarp) {
+  set_regs_dec<kRegs>();
+  if (warp < kCopyWarp) {
     // ---------------- MMAs ----------------
-    constexpr uint32_t id_s = idesc_f16_f32(kRows, kTK);
-    constexpr uint32_t id_o = idesc_f16_f32(kRows, D) | (1u << 16);   // B: keys along K
+    // One warp for the even tiles and one for the odd: a wait takes 300 cycles beside
+    // MMAs even where there is nothing to wait for, and now the other warp's run
+    // meanwhile.  S and P of a tile are one warp's, so they follow one another.
+    constexpr uint32_t kType = kBf16 ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t id_s = idesc_f16_f32(kRows, kTK) | kType;
+    constexpr uint32_t id_o = idesc_f16_f32(kRows, D) | kType | (1u << 16);   // B: keys along K
     const uint32_t kbase = smem_u32(smem + L::K_OFF), vbase = smem_u32(smem + L::V_OFF);
-    uint64_t* const kready = kBf16 ? kfull : kraw;
+    const int b = warp - kMmaWarp;
+    const uint32_t sp = tmem + L::S_COL + static_cast<uint32_t>(b) * kTK;
     int n = 0, seg = 0;
     bool ok = true;
-    auto scores = [&](int m) -> bool {              // S of tile m into buffer m & 1
+    auto scores = [&](int m) {                      // S of tile m
       const int st = m % NST;
-      if (!wait(kready + st, (m / NST) & 1)) return false;
-      tc_fence_after();
       if (elect_one()) {
-        const uint32_t d = tmem + L::S_COL + static_cast<uint32_t>(m & 1) * kTK;
         const uint64_t kd = desc_k_sw128(kbase + st * L::TILE);
         // the small terms first: the tensor core cuts low bits off at every step,
         // relative to the sum so far
+        if (L::LOW)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_f16(sp, desc_k_sw128(smem_u32(smem + L::QLOW)) + (k / 4) * (L::HALF / 16) + 2 * (k % 4),
+                    kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s, k > 0 ? 1u : 0u);
 #pragma unroll
         for (int term = 1; term >= 0; --term)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            mma_f16_ts(d, tmem + L::Q_COL + term * (D / 2) + 8 * k, kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
-                       (term == 0 || k > 0) ? 1u : 0u);
+            mma_f16_ts(sp, tmem + L::Q_COL + term * (D / 2) + 8 * k, kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
+                       (L::LOW || term == 0 || k > 0) ? 1u : 0u);
         mma_commit(&kempty[st]);
-        mma_commit(&sfull[m & 1]);
+        mma_commit(&sfull[b]);
       }
       __syncwarp();
-      return true;
     };
     while (ok && next_piece(a, wk, &pc)) {
-      if (!(ok = wait(qready, seg & 1))) break;
+      const int first = n + ((n & 1) ^ b);          // the piece's first tile of this warp
+      n += pc.t1 - pc.t0;
+      if (first >= n) continue;
+      if (!(ok = wait(&qready[b], seg & 1) && wait(&kraw[first % NST], (first / NST) & 1))) break;
       ++seg;
       tc_fence_after();
-      const int cnt = pc.t1 - pc.t0;
-      if (!(ok = scores(n))) break;
-      if (cnt > 1 && !(ok = scores(n + 1))) break;
+      scores(first);
 #pragma unroll 1
-      for (int i = 0; i < cnt; ++i) {
-        const int m = n + i, st = m % NST;
-        if (!(ok = wait(&vfull[st], (m / NST) & 1) && wait(&pready[m & 1], (m >> 1) & 1) &&
-                   (m == 0 || wait(oempty, (m - 1) & 1))))
+      for (int m = first; m < n; m += 2) {
+        const int st = m % NST;
+        const bool more = m + 2 < n;
+        uint64_t* const k2 = &kraw[(m + 2) % NST];
+        const uint32_t k2p = ((m + 2) / NST) & 1;
+        bool k_there;
+        // m == 0: O is free, pready twice
+        if (!(ok = wait3(&pready[b], (m >> 1) & 1, &vfull[st], (m / NST) & 1, m == 0 ? &pready[b] : &oempty[b ^ 1],
+                         m == 0 ? 0 : ((m - 1) >> 1) & 1, k2, k2p, &k_there)))
           break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t d = tmem + L::O_COL;
-          const uint32_t p = tmem + L::S_COL + static_cast<uint32_t>(m & 1) * kTK;
           const uint64_t vd = desc_v(vbase + st * L::TILE, L::HALF);
+          if (L::LOW)
+#pragma unroll
+            for (int k = 0; k < kTK / 16; ++k)
+              mma_f16(tmem + L::O_COL, desc_k_sw128(smem_u32(smem + L::PLOW)) + (k / 4) * (L::HALF / 16) + 2 * (k % 4),
+                      vd + k * (2048 / 16), id_o, k > 0 ? 1u : 0u);
 #pragma unroll
           for (int term = 1; term >= 0; --term)
 #pragma unroll
             for (int k = 0; k < kTK / 16; ++k)
-              mma_f16_ts(d, p + 16 * k + 8 * term, vd + k * (2048 / 16), id_o, (term == 0 || k > 0) ? 1u : 0u);
+              mma_f16_ts(tmem + L::O_COL, sp + 16 * k + 8 * term, vd + k * (2048 / 16), id_o,
+                         (L::LOW || term == 0 || k > 0) ? 1u : 0u);
           mma_commit(&vempty[st]);
           mma_commit(ofull);
         }
         __syncwarp();
         // over P of this tile, which the products before it in the pipe have read
-        if (i + 2 < cnt && !(ok = scores(m + 2))) break;
+        if (more) {
+          if (!k_there && !(ok = wait(k2, k2p))) break;
+          tc_fence_after();
+          scores(m + 2);
+        }
       }
-      n += cnt;
     }
     // nothing of this CTA's is in flight when its TMEM goes
-    if (elect_one()) mma_commit(drain);
+    if (elect_one()) mma_commit(&drain[b]);
     __syncwarp();
-    mbar_wait(drain, 0);
-  } else if (warp == kCopyWarp || warp == kCopyWarp + 1) {
+    mbar_wait(&drain[b], 0);
+  } else {
     // ---------------- K (one warp) / V (the next) rows into shared memory ----------------
     const int kv = warp - kCopyWarp;
-    uint64_t* const raw = kv ? vraw : kraw;
     uint64_t* const freed = kv ? vempty : kempty;
-    uint8_t* const base = smem + (kv ? L::V_OFF : L::K_OFF);
+    uint64_t* const raw = kv ? vraw : kraw;
+    // V's tiles that every query row sees need no more than to arrive
+    const bool clean = kv != 0;
     // A lane has the boxes lane & 15 of a tile (of the columns 64 (lane >> 4) on), or
     // its keys lane + 32 h: table column, place in the block and table entry, the
     // entry fetched one tile ahead.  A tile's lookups are additions.
     constexpr int NH = BOX ? 1 : 4;
+    constexpr int kLag = NST > 2 ? 2 : 1;         // row by row: tiles on their way behind the one announced
     const int bs = static_cast<int>(a.bs), dj = kTK / bs, dr = kTK - dj * bs;
     const int box = BOX ? a.box : 1, nbox = kTK / box;
     const int mine = BOX ? (lane & 15) : lane;
     const bool use = !BOX || (mine < nbox && lane < D / 4);
     const uint32_t rows_per_block = static_cast<uint32_t>(a.num_layers * 2 * a.hkv * a.bs);
     bool have = next_piece(a, wk, &pc), bad = false;
+    uint32_t cleans = 0;
     int t = 0, done = 0, sent = 0;                // sent: row by row, tiles that are announced
     uint32_t row0 = 0;                            // of the piece's layer and head in block 0
     const int32_t* table = nullptr;
@@ -799,10 +862,16 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         }
       }
     };
+    // V with rows that not every query row sees, once it has landed
+    auto cleaned = [&](int i) {
+      uint32_t* const note = notes + (i % kMeta) * L::META_WORDS;
+      if ((note[kRange] & 0xff) < kTK || (note[kRange] & kMissing)) clean_v<D, T>(smem + L::V_OFF + (i % NST) * L::TILE, note, lane);
+    };
     auto announce = [&]() {                       // row by row: a tile's copies have landed
+      if (clean) cleaned(sent);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(raw + sent % NST);
+      if (lane == 0) mbar_arrive((clean ? vfull : raw) + sent % NST);
       ++sent;
     };
     if (have) begin();
@@ -848,24 +917,34 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       if (lane < 4) note[kThere + lane] = word;
       if (lane == 0) note[kRange] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8 | (lost ? kMissing : 0) | (have ? 0 : kLast);
       __syncwarp();
+      uint8_t* const tile = smem + (kv ? L::V_OFF : L::K_OFF) + st * L::TILE;
       if (BOX) {
-        if (lane == 0) mbar_arrive_expect_tx(raw + st, static_cast<uint32_t>(__popc(there[0]) * box) * 128u);
+        const bool whole = lo == kTK && !lost;
+        uint64_t* const bar = (clean && whole ? vfull : raw) + st;
+        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(__popc(there[0]) * box) * 128u);
         __syncwarp();
         if (row[0] != 0xffffffffu)
-          tma_load_2d(base + st * L::TILE + (lane >> 4) * L::HALF + mine * box * 128, &map, raw + st, (lane >> 4) * 64,
-                      static_cast<int32_t>(row[0]));
+          tma_load_2d(tile + (lane >> 4) * L::HALF + mine * box * 128, &map, bar, (lane >> 4) * 64, static_cast<int32_t>(row[0]));
+        if (clean && !whole) {
+          // (vraw's phases count these tiles alone)
+          mbar_wait(vraw + st, (cleans >> st) & 1);
+          cleans ^= 1u << st;
+          cleaned(done);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(vfull + st);
+        }
       } else {
         constexpr int CPR = D / 8, RPI = 32 / CPR;    // rows an instruction covers
-        const uint32_t dst = smem_u32(base + st * L::TILE);
-        const T* const pool = static_cast<const T*>(a.pool);
+        const uint32_t dst = smem_u32(tile);
+        const T* const src = static_cast<const T*>(a.pool);
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll 4
           for (int i = 0; i < 32 / RPI; ++i) {
             const int k = i * RPI + lane / CPR, c = lane % CPR;
             const uint32_t at = __shfl_sync(0xffffffffu, row[h], k);
-            if (at != 0xffffffffu)
-              copy16(dst + tile_byte<D>(32 * h + k, c), pool + static_cast<int64_t>(at) * D + c * 8);
+            if (at != 0xffffffffu) copy16(dst + tile_byte<D>(32 * h + k, c), src + static_cast<int64_t>(at) * D + c * 8);
           }
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (done - sent == kLag) {
@@ -878,75 +957,20 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
     if (BOX) {
       // after an abort, let the copies still in flight land before the CTA exits
       if (*abort_flag)
-        for (int i = max(0, done - NST); i < done; ++i) mbar_wait(raw + i % NST, (i / NST) & 1);
+        for (int i = max(0, done - NST); i < done; ++i) mbar_wait((clean ? vfull : raw) + i % NST, (i / NST) & 1);
     } else {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.wait_all;" ::: "memory");
       while (sent < done) announce();
     }
     if (bad && lane == 0) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
-  } else if (kBf16) {
-    // ---------------- bf16: K and V to fp16, 32 keys a warp ----------------
-    const int pw = warp - kPrepWarp;
-    if (pw < 4) {
-      bool more = next_piece(a, wk, &pc);
-#pragma unroll 1
-      for (int n = 0; more; ++n) {
-        const int st = n % NST;
-        uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
-        bool scaled = false;
-        if (!wait(kraw + st, (n / NST) & 1)) break;
-        const uint32_t range = note[kRange], there = note[kThere + pw];
-        const bool whole = (range & 0xff) >= kTK && !(range & kMissing);
-        const int hi = static_cast<int>((range >> 8) & 0xff);
-        more = !(range & kLast);
-        uint32_t pois = 0;
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv) {
-          if (kv && !wait(vraw + st, (n / NST) & 1)) break;
-          uint8_t* const tile = smem + (kv ? L::V_OFF : L::K_OFF) + st * L::TILE;
-#pragma unroll 1
-          for (int g = 0; g < 2; ++g) {
-            float inv;
-            const uint32_t p = widen16<D>(tile, 32 * pw + 16 * g, whole, kv && !whole, hi, there >> (16 * g), lane, &inv, &scaled);
-            pois |= kv ? p << (16 * g) : 0u;
-            if (lane == 0) note[(kv ? kVinv : kKinv) + 2 * pw + g] = __float_as_uint(inv);
-          }
-          if (lane == 0 && kv) {
-            note[kPois + pw] = pois;
-            reinterpret_cast<uint8_t*>(note + kScaled)[pw] = scaled;
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive((kv ? vfull : kfull) + st);
-        }
-        if (dead) break;
-      }
-    }
-  } else {
-    // ---------------- V rows that not every query row sees ----------------
-    bool more = next_piece(a, wk, &pc);
-#pragma unroll 1
-    for (int n = 0; more; ++n) {
-      const int st = n % NST;
-      uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
-      if (!wait(vraw + st, (n / NST) & 1)) break;
-      const uint32_t range = note[kRange];
-      if ((range & 0xff) < kTK || (range & kMissing)) {
-        clean_v<D, T>(smem + L::V_OFF + st * L::TILE, note, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      more = !(range & kLast);
-      if (lane == 0) mbar_arrive(vfull + st);
-    }
   }
-  } else {
+  } else if (warp < kRowWarps) {
     // ---------------- rows ----------------
-    set_regs_inc<kBf16 ? 184 : 200>();
+    set_regs_dec<kRowRegs>();
     const int hw = warp >> 2, row = (warp & 3) * 32 + lane;      // half, query row
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     constexpr int DH = D / 2;                       // columns of O per half
-    int n = 0;
+    int n = 0, seg = 0;
     const Piece& ps = piece_s[warp];                // of the rare paths
     while (next_piece(a, wk, &pc)) {
       __syncwarp();
@@ -975,11 +999,11 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         auto quad = [&](int k, int c) {
           return qp[k] ? *reinterpret_cast<const float4*>(qp[k] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
         };
-        float4 v[DH / 4];
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {      // the other half's for the maximum alone
+        for (int half = 0; half < 2; ++half) {       // all of the row for its maximum
+          float4 v[DH / 4];
 #pragma unroll
-          for (int c = 0; c < DH / 4; ++c) v[c] = quad(c & 3, (hw ^ half) * DH + (c >> 2) * 16);
+          for (int c = 0; c < DH / 4; ++c) v[c] = quad(c & 3, half * DH + (c >> 2) * 16);
 #pragma unroll
           for (int c = 0; c < DH / 4; ++c)
             m[c & 3] = amax3(amax3(m[c & 3], v[c].x, v[c].y), v[c].z, v[c].w);
@@ -990,45 +1014,48 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) m[k] = amax3(m[k], __shfl_xor_sync(0xffffffffu, m[k], o), 0.0f);
         const float top = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
-        float qs;
-        pow2_scale(top, &qs, &qinv);
+        float qs = 1.0f;
+        qinv = 1.0f;
+        if (!kBf16) pow2_scale(top, &qs, &qinv);
+#pragma unroll 1
+        for (int c = hw * DH; c < hw * DH + DH; c += 16) {
+          float4 x[4];
+          uint32_t hi[8], lo[8], low[8];
 #pragma unroll
-        for (int c0 = 0; c0 < DH / 4; c0 += 8) {
-          uint32_t hi[16], lo[16];
+          for (int k = 0; k < 4; ++k) x[k] = quad(k, c);
+          exchange4(x, lane);
 #pragma unroll
-          for (int c = c0; c < c0 + 8; c += 4) {
-            float4 x[4] = {v[c], v[c + 1], v[c + 2], v[c + 3]};
-            exchange4(x, lane);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int at = (c - c0 + k) * 2;
-              split2(mul2(f2(x[k].x, x[k].y), f2(qs, qs)), &hi[at], &lo[at]);
-              split2(mul2(f2(x[k].z, x[k].w), f2(qs, qs)), &hi[at + 1], &lo[at + 1]);
-            }
+          for (int k = 0; k < 4; ++k) {
+            split<T>(mul2(f2(x[k].x, x[k].y), f2(qs, qs)), &hi[2 * k], &lo[2 * k], &low[2 * k]);
+            split<T>(mul2(f2(x[k].z, x[k].w), f2(qs, qs)), &hi[2 * k + 1], &lo[2 * k + 1], &low[2 * k + 1]);
           }
-          tmem_st_32x32b_x16(lanes + L::Q_COL + (hw * DH + c0 * 4) / 2, hi);
-          tmem_st_32x32b_x16(lanes + L::Q_COL + DH + (hw * DH + c0 * 4) / 2, lo);
+          if (L::LOW) {
+            *reinterpret_cast<uint4*>(smem + L::QLOW + tile_byte<D>(row, c / 8)) = make_uint4(low[0], low[1], low[2], low[3]);
+            *reinterpret_cast<uint4*>(smem + L::QLOW + tile_byte<D>(row, c / 8 + 1)) = make_uint4(low[4], low[5], low[6], low[7]);
+          }
+          tmem_st_32x32b_x8(lanes + L::Q_COL + c / 2, hi);
+          tmem_st_32x32b_x8(lanes + L::Q_COL + (D + c) / 2, lo);
         }
         tmem_wait_st();
+        if (L::LOW) fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(qready);
+        if (lane == 0) {                            // to the MMA warps that have tiles of the piece
+          mbar_arrive(&qready[n & 1]);
+          if (t1 - t0 > 1) mbar_arrive(&qready[(n & 1) ^ 1]);
+        }
       }
       const float cq = qinv * (a.scale * 1.44269504088896340736f);   // to powers of two
       if ((warp & 3) * 32 >= rows) {
         // no row of the warp's is live (Q, and so S and P, are zeros): it only keeps step
 #pragma unroll 1
-        for (int t = t0; t <= t1; ++t, ++n) {
-          if (t < t1) {
-            wait(&sfull[n & 1], (n >> 1) & 1);
-            if (lane == 0) mbar_arrive(&pready[n & 1]);
-          }
-          if (t > t0) {
-            wait(ofull, (n - 1) & 1);
-            if (lane == 0) mbar_arrive(oempty);
-          }
+        for (int t = t0; t < t1; ++t, ++n) {
+          wait(&sfull[n & 1], (n >> 1) & 1);
+          // (bf16: in step with O, as the warps with rows are)
+          if (L::LOW && n > 0) wait(ofull, (n - 1) & 1);
+          if (lane == 0) mbar_arrive(&pready[n & 1]);
         }
-        --n;
+        ++seg;
         continue;
       }
       const int limit = live ? pc.pre + pc.node0 + row / a.g : -1;   // the last key that the row sees
@@ -1036,200 +1063,179 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       // it follows the maximum once that is 2^8 above it, so most tiles
       // rescale nothing), the half's sum
       float mref = -INFINITY, l = 0.0f;
-      F2 acc[DH / 2];
-#pragma unroll
-      for (int c = 0; c < DH / 2; ++c) acc[c] = f2(0.f, 0.f);
-      // of the tile whose P V is still to be added
-      float corr_p = 1.0f, vs_p = 1.0f;
-      bool rare_p = false;
-
-      // softmax of tile t, then the addition of tile t - 1's P V
+      bool s_there = false;                         // seen a tile ahead
 #pragma unroll 1
-      for (int t = t0; t <= t1; ++t, ++n) {
-        float corr = 1.0f, vs = 1.0f;
-        bool rare = false;
-        if (t < t1) {
-          const int b = n & 1;
-          wait(&sfull[b], (n >> 1) & 1);
-          if (kBf16) wait(&vfull[n % NST], (n / NST) & 1);   // the notes on V
-          tc_fence_after();
-          const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK + 64 * hw;   // the half's scores
-          float xa[32], xb[32];
-          tmem_ld_32x32b_x32(sc, xa);
-          tmem_ld_32x32b_x32(sc + 32, xb);
-          const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
-          const bool special = (t + 1) * kTK > pc.kmin || (*const_cast<const volatile uint32_t*>(note + kRange) & kMissing);
-          const uint32_t scaled = kBf16 ? note[kScaled] : 0u;
-          const float* const kinv = reinterpret_cast<const float*>(note + kKinv);
-          const float* const vinv = reinterpret_cast<const float*>(note + kVinv);
-          tmem_wait_ld(xa);
-          tmem_wait_ld(xb);
-          if (kBf16 && __builtin_expect(scaled != 0, 0)) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              xa[j] *= kinv[4 * hw + (j >> 4)];
-              xb[j] *= kinv[4 * hw + 2 + (j >> 4)];
-            }
-            vs = vinv[0];
-#pragma unroll
-            for (int j = 1; j < kKeyGroups; ++j) vs = fmaxf(vs, vinv[j]);
-          }
-          if (__builtin_expect(special, 0)) {
-            if (!kBf16) wait(&vfull[n % NST], (n / NST) & 1);    // the notes on V
-            const int cnt = limit + 1 - t * kTK;     // keys of the tile that come before the row's end
-            auto seen = [&](int i) -> uint32_t {
-              const int k = cnt - 32 * i;
-              return note[kThere + i] & (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1);
-            };
-            const uint32_t wa = seen(2 * hw), wb = seen(2 * hw + 1);
-            const uint32_t any = note[kPois] | note[kPois + 1] | note[kPois + 2] | note[kPois + 3];
-            if (any)
-#pragma unroll 1
-              for (int i = 0; i < 4; ++i) rare = rare || (seen(i) & note[kPois + i]) != 0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              xa[j] = (wa >> j) & 1 ? xa[j] : -INFINITY;
-              xb[j] = (wb >> j) & 1 ? xb[j] : -INFINITY;
-            }
-          }
-          float m0 = max3(xa[0], xa[1], xa[2]), m1 = max3(xb[0], xb[1], xb[2]);
-#pragma unroll
-          for (int j = 3; j + 1 < 32; j += 2) {
-            m0 = max3(m0, xa[j], xa[j + 1]);
-            m1 = max3(m1, xb[j], xb[j + 1]);
-          }
-          const float m = max3(m0, m1, fmaxf(xa[31], xb[31]));
-          // both halves take the whole row's maximum
-          float* const mx = max_s + (n & 1) * 2 * kRows + row;
-          mx[hw * kRows] = m;
-          pair_sync(warp);
-          const float mc = fmaxf(m, mx[(hw ^ 1) * kRows]) * cq;
-          if (mc > mref + 8.0f) {
-            corr = ex2(mref - mc);
-            mref = mc;
-          }
-          // P = 2^(x c - ref), up to 2^14: its terms are fp16
-          const float ref = mref == -INFINITY ? 0.0f : mref - 6.0f;
-          const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
-          F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-          // bf16: V's scales relative to the tile's largest
-          const float up = kBf16 ? __uint_as_float((254u << 23) - __float_as_uint(vs)) : 1.0f;
-          auto probs = [&](float (&x)[32], uint32_t at, int group) {
-            uint32_t pt[32];
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float2 e = unpack(fma2(f2(x[j], x[j + 1]), c2, nref));
-              F2 p = f2(ex2(e.x), ex2(e.y));
-              s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], p);
-              if (kBf16) {
-                const float f = vinv[group + (j >> 4)] * up;
-                p = mul2(p, f2(f, f));
-              }
-              const int k = (j >> 4) * 16 + ((j & 15) >> 1);
-              split2(p, &pt[k], &pt[k + 8]);
-            }
-            tmem_st_32x32b_x32(at, pt);
+      for (int t = t0; t < t1; ++t, ++n) {
+        const int b = n & 1;
+        if (!__all_sync(0xffffffffu, s_there)) wait(&sfull[b], (n >> 1) & 1);
+        tc_fence_after();
+        const uint32_t sc = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK + 64 * hw;   // the half's scores
+        float xa[32], xb[32];
+        tmem_ld_32x32b_x32(sc, xa);
+        tmem_ld_32x32b_x32(sc + 32, xb);
+        float corr = 1.0f;
+        const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
+        const bool special = (t + 1) * kTK > pc.kmin || (*const_cast<const volatile uint32_t*>(note + kRange) & kMissing);
+        tmem_wait_ld(xa);
+        tmem_wait_ld(xb);
+        if (__builtin_expect(special, 0)) {
+          const int cnt = limit + 1 - t * kTK;     // keys of the tile that come before the row's end
+          auto seen = [&](int i) -> uint32_t {
+            const int k = cnt - 32 * i;
+            return note[kThere + i] & (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1);
           };
-          probs(xa, sc, 4 * hw);
-          probs(xb, sc + 32, 4 * hw + 2);
-          const float2 sa = unpack(s2[0]), sb = unpack(s2[1]);
-          l = fmaf(l, corr, (sa.x + sa.y) + (sb.x + sb.y));
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pready[b]);
-        }
-        if (t > t0) {
-          wait(ofull, (n - 1) & 1);
-          tc_fence_after();
-          const uint32_t o = lanes + L::O_COL + hw * DH;
-          if (__any_sync(0xffffffffu, corr_p != 1.0f)) {
+          const uint32_t wa = seen(2 * hw), wb = seen(2 * hw + 1);
 #pragma unroll
-            for (int c = 0; c < DH / 2; ++c) acc[c] = mul2(acc[c], f2(corr_p, corr_p));
+          for (int j = 0; j < 32; ++j) {
+            xa[j] = (wa >> j) & 1 ? xa[j] : -INFINITY;
+            xb[j] = (wb >> j) & 1 ? xb[j] : -INFINITY;
           }
+        }
+        float m0 = max3(xa[0], xa[1], xa[2]), m1 = max3(xb[0], xb[1], xb[2]);
 #pragma unroll
-          for (int i = 0; i < DH; i += 32) {
-            float v[32];
-            tmem_ld_32x32b_x32(o + i, v);
+        for (int j = 3; j + 1 < 32; j += 2) {
+          m0 = max3(m0, xa[j], xa[j + 1]);
+          m1 = max3(m1, xb[j], xb[j + 1]);
+        }
+        const float m = max3(m0, m1, fmaxf(xa[31], xb[31]));
+        // both halves take the whole row's maximum
+        float* const mx = max_s + (n & 1) * 2 * kRows + row;
+        mx[hw * kRows] = m;
+        pair_sync(warp);
+        const float mc = fmaxf(m, mx[(hw ^ 1) * kRows]) * cq;
+        if (mc > mref + 8.0f) {
+          corr = ex2(mref - mc);
+          mref = mc;
+        }
+        // P = 2^(x c - ref): up to 2^14 in fp16 terms, 2^8 in bf16
+        const float ref = mref == -INFINITY ? 0.0f : kBf16 ? mref : mref - 6.0f;
+        const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
+        F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+        uint32_t low[L::LOW ? 32 : 1];
+        const bool low_free = L::LOW && n > 0 && mbar_test(ofull, (n - 1) & 1);
+        auto probs = [&](const float (&x)[32], int j0, int group) {    // 16 keys
+          uint32_t pt[16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 e = unpack(fma2(f2(x[j0 + j], x[j0 + j + 1]), c2, nref));
+            const F2 p = f2(ex2(e.x), ex2(e.y));
+            s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], p);
+            split<T>(p, &pt[j / 2], &pt[j / 2 + 8], &low[L::LOW ? 8 * group + j / 2 : 0]);
+          }
+          tmem_st_32x32b_x16(sc + 16 * group, pt);
+        };
+        if (hw == 0) corr_s[(n % kRing) * kRows + row] = corr;
+        probs(xa, 0, 0);
+        probs(xa, 16, 1);
+        probs(xb, 0, 2);
+        s_there = t + 1 < t1 && mbar_test(&sfull[b ^ 1], ((n + 1) >> 1) & 1);
+        probs(xb, 16, 3);
+        const float2 sa = unpack(s2[0]), sb = unpack(s2[1]);
+        l = fmaf(l, corr, (sa.x + sa.y) + (sb.x + sb.y));
+        if (t + 1 == t1) {
+          float* const fin = fin_s + (seg % kRing) * 3 * kRows + row;
+          fin[hw * kRows] = l;
+          if (hw == 0) fin[2 * kRows] = mref;
+        }
+        if constexpr (L::LOW) {                      // where the tile before's third terms have been read
+          if (n > 0 && !__all_sync(0xffffffffu, low_free)) wait(ofull, (n - 1) & 1);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(smem + L::PLOW + tile_byte<kTK>(row, 8 * hw + c)) =
+                make_uint4(low[4 * c], low[4 * c + 1], low[4 * c + 2], low[4 * c + 3]);
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[b]);
+      }
+      ++seg;
+    }
+  } else {
+    // ---------------- sums ----------------
+    // Every tile's P V added into fp32 registers (a long context added up inside the
+    // tensor core would lose low bits at each step); a thread has a row.
+    set_regs_inc<kSumRegs>();
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t oc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + L::O_COL;
+    int n = 0, seg = 0;
+    const Piece& ps = piece_s[kRowWarps + (warp & 3)];
+    bool ok = true;
+    while (ok && next_piece(a, wk, &pc)) {
+      __syncwarp();
+      if (lane == 0) piece_s[kRowWarps + (warp & 3)] = pc;
+      __syncwarp();
+      const int t0 = pc.t0, t1 = pc.t1;
+      const int rows = min(a.npt, pc.nq - pc.node0) * a.g;
+      const bool live = row < rows, some = (warp & 3) * 32 < rows;
+      auto row_at = [&](int R) -> int64_t {
+        const int node = R / a.g;
+        return ((ps.a0 + ps.node0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
+      };
+      F2 acc[D / 2];
+#pragma unroll
+      for (int c = 0; c < D / 2; ++c) acc[c] = f2(0.f, 0.f);
+#pragma unroll 1
+      for (int t = t0; t < t1; ++t, ++n) {
+        if (!(ok = wait(ofull, n & 1))) break;
+        const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
+        if (some) {
+          tc_fence_after();
+          const float corr = corr_s[(n % kRing) * kRows + row];
+          if (__builtin_expect((t + 1) * kTK > pc.kmin || (note[kRange] & kMissing), 0)) {
+            // V elements that are not finite went in as zeros: to the rows that see them
+            if (note[kPois] | note[kPois + 1] | note[kPois + 2] | note[kPois + 3])
+              add_rare<D, T>(a, ps, oc, note, t, live ? min(pc.pre + pc.node0 + row / a.g + 1 - t * kTK, kTK) : 0);
+          }
+          if (__any_sync(0xffffffffu, corr != 1.0f)) {
+#pragma unroll
+            for (int c = 0; c < D / 2; ++c) acc[c] = mul2(acc[c], f2(corr, corr));
+          }
+          constexpr int C = 32;                      // columns a load, as registers allow
+          float v[C];
+#pragma unroll
+          for (int i = 0; i < D; i += C) {
+            tmem_ld_32x32b_x32(oc + i, v);
             tmem_wait_ld(v);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
+            for (int c = 0; c < C / 2; ++c) {
               const F2 x = f2(v[2 * c], v[2 * c + 1]);
-              acc[i / 2 + c] = kBf16 ? fma2(x, f2(vs_p, vs_p), acc[i / 2 + c]) : add2(acc[i / 2 + c], x);
+              acc[i / 2 + c] = add2(acc[i / 2 + c], x);
             }
           }
           tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(oempty);
-          if (__builtin_expect(rare_p, 0)) {
-            // V elements that are not finite: to the rows that see them
-            const uint32_t* const note = notes + ((n - 1) % kMeta) * L::META_WORDS;
-            const int cnt = limit + 1 - (t - 1) * kTK;
-#pragma unroll 1
-            for (int k = 0; k < min(cnt, kTK); ++k) {
-              if (!((note[kPois + (k >> 5)] >> (k & 31)) & 1)) continue;
-              const int64_t at = key_offset(a, ps.s, ps.hk, (t - 1) * kTK + k, D);
-              if (at < 0) continue;
-              const T* vp = static_cast<const T*>(a.pool) + at + a.hkv * a.bs * D + hw * DH;
-#pragma unroll
-              for (int c = 0; c < DH / 2; ++c) {
-                const float v0 = widen(vp[2 * c]), v1 = widen(vp[2 * c + 1]);
-                acc[c] = add2(acc[c], f2(isfinite(v0) ? 0.0f : v0, isfinite(v1) ? 0.0f : v1));
-              }
-            }
-          }
-          __syncwarp();
         }
-        corr_p = corr;
-        vs_p = vs;
-        rare_p = rare;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&oempty[n & 1]);
       }
-      --n;                                          // the round after the last tile
-
-      // the halves' sums; the maxima's place in it is free: the last tile's is the other one
-      {
-        float* const mx = max_s + (n & 1) * 2 * kRows + row;
-        mx[hw * kRows] = l;
-        pair_sync(warp);
-        l += mx[(hw ^ 1) * kRows];
-        pair_sync(warp);
-      }
+      if (!ok) break;
+      const float* const fin = fin_s + (seg % kRing) * 3 * kRows + row;
+      ++seg;
+      if (!some) continue;
+      const float l = fin[0] + fin[kRows];
       if (t0 == 0 && t1 == ps.ntiles) {
-        const float inv = 1.0f / l;
-        float* op[4];
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (live) {
+          float* op = a.out + row_at(row);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int R = (row & ~3) + k;
-          op[k] = R < rows ? a.out + row_at(R) + hw * DH + (lane & 3) * 4 : nullptr;
-        }
-#pragma unroll
-        for (int c = 0; c < DH; c += 16) {
-          float4 x[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 p = unpack(acc[c / 2 + 2 * k]), u = unpack(acc[c / 2 + 2 * k + 1]);
-            x[k] = make_float4(p.x * inv, p.y * inv, u.x * inv, u.y * inv);
-            if (l == 0.0f) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = 0; c < D; c += 4) {
+            const float2 p = unpack(mul2(acc[c / 2], f2(inv, inv))), u = unpack(mul2(acc[c / 2 + 1], f2(inv, inv)));
+            *reinterpret_cast<float4*>(op + c) = make_float4(p.x, p.y, u.x, u.y);
           }
-          exchange4(x, lane);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (op[k]) *reinterpret_cast<float4*>(op[k] + c) = x[k];
         }
       } else {
         float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * part_floats<D>();
         if (live) {
-          if (hw == 0) {
-            part[row] = mref;
-            part[kRows + row] = l;
-          }
+          part[row] = fin[2 * kRows];
+          part[kRows + row] = l;
 #pragma unroll
-          for (int c = 0; c < DH; c += 4) {
+          for (int c = 0; c < D; c += 4) {
             const float2 p = unpack(acc[c / 2]), u = unpack(acc[c / 2 + 1]);
-            reinterpret_cast<float4*>(part + 2 * kRows)[(hw * DH + c) / 4 * kRows + row] = make_float4(p.x, p.y, u.x, u.y);
+            reinterpret_cast<float4*>(part + 2 * kRows)[c / 4 * kRows + row] = make_float4(p.x, p.y, u.x, u.y);
           }
         }
-        if (t0 == 0 && tid == 0) {                 // the share's last piece: joined from here on
+        if (t0 == 0 && warp == kSumWarp && lane == 0) {                 // the share's last piece: joined from here on
           const int64_t x = ps.u + static_cast<int64_t>(ps.ntiles - 1) * kTK;   // the item's last tile
           cut_s.first = static_cast<int>(blockIdx.x);
           cut_s.last = static_cast<int>(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
@@ -1316,10 +1322,10 @@ __global__ void __launch_bounds__(kMergeThreads) cache_merge_kernel(CacheArgs a)
 
 template <int D, typename T, bool BOX>
 int launch_cache_tc(const CacheArgs& a, const CUtensorMap& map, int grid, cudaStream_t st) {
-  using L = CacheLayout<D>;
+  using L = CacheLayout<D, T>;
   auto kern = cache_attn_tc_kernel<D, T, BOX>;
   if (set_smem_optin(reinterpret_cast<const void*>(kern), L::BYTES) != KSH_OK) return KSH_ERR_CUDA;
-  const int rc = launch(kern, dim3(static_cast<unsigned>(grid)), dim3(cache_threads<T>()), L::BYTES, st, a, map);
+  const int rc = launch(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), L::BYTES, st, a, map);
   if (rc != KSH_OK || grid == 1) return rc;
   return launch(cache_merge_kernel<D>, dim3(static_cast<unsigned>(grid - 1), kMergeChunks),
                 dim3(kMergeThreads), 0, st, a);
