@@ -244,6 +244,19 @@ class ContinuousEngine:
         self.waiting_queue.insert(0, victim)
         self.active_sequences.pop(victim.req_id, None)
 
+    def compact(self) -> None:
+        """Moves the blocks in use to the front of the pool (``PrefixCache.compact``)
+        and renumbers the block tables of the requests that run.  Call it between
+        steps; copies of a swap that are under way are waited for."""
+        pool = self.cache.allocator.pool
+        if pool.is_cuda:
+            torch.cuda.current_stream(pool.device).wait_stream(self._side_stream(pool.device))
+        to = self.cache.compact()
+        for req in self.active_sequences.values():
+            req.block_table = [to[b] for b in req.block_table]
+            if hasattr(req, "_own_blocks"):
+                req._own_blocks = [to[b] for b in req._own_blocks]
+
     def _side_stream(self, device) -> "torch.cuda.Stream":
         s = getattr(self, "_swap_stream", None)
         if s is None:

@@ -1402,8 +1402,7 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
   const bool fast = (d == 64 || d == 128) && a.g <= kRows &&
       ((reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
       static_cast<double>(num_blocks) * 2.0 * static_cast<double>(num_layers) * static_cast<double>(hkv) *
-              static_cast<double>(block_size) <= static_cast<double>(INT32_MAX) &&
-      tensor_map_encoder_available();
+              static_cast<double>(block_size) <= static_cast<double>(INT32_MAX);
   if (fast) {
     if (!workspace || workspace_bytes < ksh_cache_attention_workspace_size(num_seqs, hq, hkv, d, max_q_len))
       return KSH_ERR_WORKSPACE;

@@ -38,6 +38,7 @@ from . import _lib
 from ._lib import call, ptr, stream_ptr
 from .chunked_prefill import AttentionWorkspace, paged_attention
 from .config import ModelConfig
+from .kv_cache import POOL_TYPES, CacheWorkspace, cache_attention, rope_cache_write
 from .prefix_cache import BlockAllocator
 from .speculative import tree_attention
 from .tensor_parallel import (down_col_range, gate_up_row_ranges, merge_argmax, o_col_range,
@@ -106,13 +107,22 @@ class KshipraModel:
     def __init__(self, hf_model=None, device: torch.device = None, quantize: Optional[str] = None,
                  *, config: Optional[ModelConfig] = None,
                  state_dict: Optional[Dict[str, torch.Tensor]] = None, group_size: int = 128,
-                 tp: Optional[tuple] = None) -> None:
+                 tp: Optional[tuple] = None, kv_dtype: torch.dtype = torch.float32) -> None:
         """``tp=(rank, world, group)`` builds rank's tensor-parallel shard: heads,
         intermediate rows and lm_head vocabulary split over ``world`` ranks
         (one process per GPU), row-parallel sums all-reduced over ``group``
-        (a torch.distributed NCCL group; None = the default group)."""
+        (a torch.distributed NCCL group; None = the default group).
+
+        ``kv_dtype`` is the element type of the pools that ``new_pool`` and
+        ``generate`` make: fp32, or fp16 / bf16 for a cache of half the bytes.
+        ``forward``, ``prefill`` and ``run_batch`` go by the pool they are given.
+        A state dict with ``self_attn.q_norm.weight`` / ``k_norm.weight`` [head_dim]
+        gives a model whose queries and keys are normed per head before the
+        rotation."""
         if quantize not in (None, "int8", "int4"):
             raise ValueError(f"quantize must be None, 'int8' or 'int4', got {quantize!r}")
+        if kv_dtype not in POOL_TYPES:
+            raise ValueError(f"kv_dtype must be one of {[str(t) for t in POOL_TYPES]}, got {kv_dtype}")
         if device is None or torch.device(device).type != "cuda":
             if not torch.cuda.is_available():
                 raise _lib.KshipraLibraryError("KshipraModel runs on CUDA only (no CPU path)")
@@ -129,6 +139,7 @@ class KshipraModel:
         self.model = hf_model
         self.cfg = config
         self.quantize = quantize
+        self.kv_dtype = kv_dtype
         self.group_size = group_size
         self.tp_rank, self.tp_world, self.tp_group = (0, 1, None) if tp is None else tp
         self.tp = tp_shape(config, self.tp_rank, self.tp_world,
@@ -147,6 +158,7 @@ class KshipraModel:
         self.flags = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._lin_ws = Workspace()
         self._attn_ws = AttentionWorkspace()
+        self._cache_ws = CacheWorkspace()
         self._lm_ws: Optional[torch.Tensor] = None
         self._lm_hl = None
         self.lm_tc = True            # > 16 lm_head rows on the tensor-core kernel
@@ -232,6 +244,11 @@ class KshipraModel:
                 if self.tp_world > 1:
                     bias = torch.cat([bias[a:b] for a, b in qkv_rows])
                 L.qkv.bias = bias.contiguous()
+            L.q_norm, L.k_norm = (g(p + f"self_attn.{k}.weight").contiguous() if p + f"self_attn.{k}.weight" in sd else None
+                                  for k in ("q_norm", "k_norm"))
+            for w in (L.q_norm, L.k_norm):
+                if w is not None and tuple(w.shape) != (self.head_dim,):
+                    raise ValueError(f"norms of queries and keys must be [{self.head_dim}], got {tuple(w.shape)}")
             del wq, wk, wv
             L.o = self._shard_cols(self._pack(g(p + "self_attn.o_proj.weight")),
                                    *o_col_range(self.cfg, tpr))
@@ -307,8 +324,11 @@ class KshipraModel:
         s = stream_ptr()
         hid, xn, qkv, q, attn, h = (acts[k] for k in ("hidden", "xn", "qkv", "q", "attn", "h"))
         nb, L, _, hkv, bs, d = pool.shape
-        if pool.dtype != torch.float32 or not pool.is_contiguous():
-            raise ValueError("the pool must be a contiguous fp32 CUDA tensor")
+        if pool.dtype not in POOL_TYPES or not pool.is_contiguous():
+            raise ValueError("the pool must be a contiguous fp32, fp16 or bf16 CUDA tensor")
+        half = pool.dtype != torch.float32
+        if half and tree is not None:
+            raise ValueError("drafted trees need an fp32 pool")
         rc, rs = self._rope_tables()
         call("ksh_embedding", ptr(ids), T, ptr(self.embed), self.vocab_size, self.hidden, ptr(hid),
              ptr(self.flags), s)
@@ -316,7 +336,8 @@ class KshipraModel:
         # decode step (one token per sequence, position == prefix length): the
         # fused RoPE + K/V write + attention kernel
         fused = (tree is None and max_q_len == 1 and T == num_seqs and self.fused_decode
-                 and bs % 16 == 0
+                 and bs % 16 == 0 and not half
+                 and all(Ly.q_norm is None and Ly.k_norm is None for Ly in self.layers)
                  and d in (64, 128) and self.n_heads // self.n_kv_heads in _DECODE_GROUPS[d])
         if fused:   # key-split partial states (zeroed once; the kernels leave the counters at 0)
             dec_ws = attn_ws.decode(int(_lib.lib().ksh_decode_attention_workspace_size(
@@ -330,10 +351,17 @@ class KshipraModel:
                      i, bs, ptr(block_tables), block_tables.shape[1], max_total_len, ptr(attn),
                      ptr(dec_ws), dec_ws.numel(), ptr(self.flags), s)
             else:
-                call("ksh_rope_kv_write", ptr(qkv), T, self.n_heads, self.n_kv_heads,
-                     self.head_dim, ptr(positions), ptr(slots), ptr(rc), ptr(rs), rc.shape[0],
-                     ptr(q), ptr(pool), nb, L, i, bs, ptr(self.flags), s)
-                if tree is None:
+                if half or Ly.q_norm is not None or Ly.k_norm is not None:
+                    rope_cache_write(qkv, pool, i, positions, slots, rc, rs, q_norm=Ly.q_norm,
+                                     k_norm=Ly.k_norm, eps=eps, out=q, flags=self.flags)
+                else:
+                    call("ksh_rope_kv_write", ptr(qkv), T, self.n_heads, self.n_kv_heads,
+                         self.head_dim, ptr(positions), ptr(slots), ptr(rc), ptr(rs), rc.shape[0],
+                         ptr(q), ptr(pool), nb, L, i, bs, ptr(self.flags), s)
+                if half:
+                    cache_attention(q, pool, i, block_tables, q_start, prefix_lens, max_q_len,
+                                    max_total_len, attn, self.flags, ws=self._cache_ws)
+                elif tree is None:
                     paged_attention(q, pool, i, block_tables, q_start, prefix_lens, max_q_len,
                                     max_total_len, attn, self.flags, ws=attn_ws)
                 else:
@@ -479,7 +507,7 @@ class KshipraModel:
     def new_pool(self, num_blocks: int, block_size: int) -> BlockAllocator:
         return BlockAllocator(num_blocks=num_blocks, block_size=block_size, num_layers=self.n_layers,
                               num_kv_heads=self.n_kv_heads, head_dim=self.head_dim,
-                              dtype=torch.float32, device=self.device)
+                              dtype=self.kv_dtype, device=self.device)
 
     @torch.inference_mode()
     def prefill(self, prompt_ids: Sequence[int], pool: torch.Tensor, block_table: List[int],

@@ -206,3 +206,36 @@ class PrefixCache:
             if self.tree.evict(num_blocks) < num_blocks:
                 raise OutOfBlocksError("Not enough evictable memory to satisfy request")
             return [self.allocator.alloc() for _ in range(num_blocks)]
+
+    def compact(self) -> List[int]:
+        """Moves the blocks in use to the front of the pool, in every layer, and
+        the free ones behind them (the lowest is allocated first).
+
+        Returns each block's new id (its own where it did not move).  The tree's
+        nodes are renumbered here; block tables that a caller holds are its own
+        to renumber (``ContinuousEngine.compact`` does).  The pool is moved on its
+        device's current stream."""
+        alloc = self.allocator
+        nb = alloc.num_blocks
+        refs = torch.ones(nb, dtype=torch.int32)
+        if alloc.free_blocks:
+            refs[torch.tensor(alloc.free_blocks, dtype=torch.int64)] = 0
+        if alloc.pool.is_cuda:
+            from .kv_cache import compact_pages
+            dev = alloc.pool.device
+            none = torch.zeros((0, 1), dtype=torch.int32, device=dev)
+            _, _, page_map, _ = compact_pages(alloc.pool, none, refs.to(dev))
+            to = page_map.tolist()
+        else:
+            used = int(refs.sum())
+            holes = iter(b for b in range(used) if not refs[b])
+            to = [next(holes) if b >= used and refs[b] else b for b in range(nb)]
+            moved = [b for b in range(nb) if to[b] != b]
+            alloc.pool[[to[b] for b in moved]] = alloc.pool[moved]
+        stack = [self.tree.root]
+        while stack:
+            node = stack.pop()
+            node.block_ids = [to[b] for b in node.block_ids]
+            stack.extend(node.children.values())
+        alloc.free_blocks = list(range(nb - 1, int(refs.sum()) - 1, -1))
+        return to

@@ -481,6 +481,8 @@ class SpeculativeDecoder:
                  generator: Optional[torch.Generator] = None):
         if temperature > 0 and model.tp_world > 1:
             raise ValueError("sampling needs the whole vocabulary on one GPU")
+        if getattr(model, "kv_dtype", torch.float32) != torch.float32:
+            raise ValueError("drafted trees need an fp32 pool (kv_dtype)")
         self.m = model
         self.proposer = proposer if proposer is not None else PromptLookup()
         self.block_size = block_size
