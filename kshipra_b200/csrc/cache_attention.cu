@@ -113,7 +113,7 @@ constexpr int kRowWarps = 8, kSumWarp = kRowWarps, kSumWarps = 4;
 constexpr int kMmaWarp = kSumWarp + kSumWarps, kCopyWarp = kMmaWarp + 2;     // even and odd tiles; K and V
 constexpr int kThreads = 32 * (kCopyWarp + 2);
 // registers a thread, of 128 at launch: rows, sums, the other roles
-constexpr int kRowRegs = 112, kSumRegs = 176, kRegs = 112;
+constexpr int kRowRegs = 120, kSumRegs = 192, kRegs = 80;
 constexpr int kItemCost = 512;
 constexpr int kMeta = 16;                // tiles whose notes are kept: more than the stages let run apart
 // Tiles (pieces) that the row warps can be ahead of the sum warps, and more
@@ -687,6 +687,9 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Walk* const wk = &walk_s[warp];
+  // a row's token in the tile (rows are few: exact)
+  const float per = 1.0f / static_cast<float>(a.g);
+  auto token_of = [&](int R) { return static_cast<int>((static_cast<float>(R) + 0.5f) * per); };
   if (lane == 0) *wk = start_s;
   if (tid == 0) cut_s.first = 0, cut_s.last = -1;
   __syncwarp();
@@ -753,14 +756,19 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         const uint64_t kd = desc_k_sw128(kbase + st * L::TILE);
         // the small terms first: the tensor core cuts low bits off at every step,
         // relative to the sum so far
-        if (L::LOW)
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_f16(sp, desc_k_sw128(smem_u32(smem + L::QLOW)) + (k / 4) * (L::HALF / 16) + 2 * (k % 4),
-                    kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s, k > 0 ? 1u : 0u);
-#pragma unroll
+        if (L::LOW) {
+          const uint64_t qd = desc_k_sw128(smem_u32(smem + L::QLOW));
+#pragma unroll 2
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k / 4) * (L::HALF / 16) + 2 * (k % 4);
+            mma_f16(sp, qd + at, kd + at, id_s, k > 0 ? 1u : 0u);
+          }
+        }
+        // (loops, not 32 instructions in a row: with as many descriptors in registers
+        // the warp spills, and issues late)
+#pragma unroll 1
         for (int term = 1; term >= 0; --term)
-#pragma unroll
+#pragma unroll 2
           for (int k = 0; k < D / 16; ++k)
             mma_f16_ts(sp, tmem + L::Q_COL + term * (D / 2) + 8 * k, kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
                        (L::LOW || term == 0 || k > 0) ? 1u : 0u);
@@ -791,14 +799,15 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         tc_fence_after();
         if (elect_one()) {
           const uint64_t vd = desc_v(vbase + st * L::TILE, L::HALF);
-          if (L::LOW)
-#pragma unroll
+          if (L::LOW) {
+            const uint64_t pd = desc_k_sw128(smem_u32(smem + L::PLOW));
+#pragma unroll 2
             for (int k = 0; k < kTK / 16; ++k)
-              mma_f16(tmem + L::O_COL, desc_k_sw128(smem_u32(smem + L::PLOW)) + (k / 4) * (L::HALF / 16) + 2 * (k % 4),
-                      vd + k * (2048 / 16), id_o, k > 0 ? 1u : 0u);
-#pragma unroll
+              mma_f16(tmem + L::O_COL, pd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), vd + k * (2048 / 16), id_o, k > 0 ? 1u : 0u);
+          }
+#pragma unroll 1
           for (int term = 1; term >= 0; --term)
-#pragma unroll
+#pragma unroll 2
             for (int k = 0; k < kTK / 16; ++k)
               mma_f16_ts(tmem + L::O_COL, sp + 16 * k + 8 * term, vd + k * (2048 / 16), id_o,
                          (L::LOW || term == 0 || k > 0) ? 1u : 0u);
@@ -981,60 +990,63 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       const bool live = row < rows;
       // the row's place in q and out
       auto row_at = [&](int R) -> int64_t {
-        const int node = R / a.g;
+        const int node = token_of(R);
         return ((ps.a0 + ps.node0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
       };
-      float qinv;
-      // Q: hi / lo terms of the half's columns into TMEM.  Four lanes load 64
-      // bytes of a row, for the rows of the four, and exchange them
+      const bool some = (warp & 3) * 32 < rows;
+      float qinv = 1.0f;
+      // Q: the half's columns as terms into TMEM (zeros for rows that are not live).
+      // Four lanes load 64 bytes of a row, for the rows of the four, and exchange
+      // them: one trip to memory, 1500 cycles beside the copies.
       {
-        const float* qp[4];
-        float m[4];
+        float4 v[DH / 4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int R = (row & ~3) + k;
-          qp[k] = R < rows ? a.q + row_at(R) + (lane & 3) * 4 : nullptr;
-          m[k] = 0.0f;
-        }
-        auto quad = [&](int k, int c) {
-          return qp[k] ? *reinterpret_cast<const float4*>(qp[k] + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {       // all of the row for its maximum
-          float4 v[DH / 4];
-#pragma unroll
-          for (int c = 0; c < DH / 4; ++c) v[c] = quad(c & 3, half * DH + (c >> 2) * 16);
-#pragma unroll
-          for (int c = 0; c < DH / 4; ++c)
-            m[c & 3] = amax3(amax3(m[c & 3], v[c].x, v[c].y), v[c].z, v[c].w);
-        }
-        // the four lanes' maxima of the lane's row
-#pragma unroll
-        for (int o = 1; o <= 2; o <<= 1)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) m[k] = amax3(m[k], __shfl_xor_sync(0xffffffffu, m[k], o), 0.0f);
-        const float top = (lane & 2) ? ((lane & 1) ? m[3] : m[2]) : ((lane & 1) ? m[1] : m[0]);
+        for (int c = 0; c < DH / 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
         float qs = 1.0f;
-        qinv = 1.0f;
-        if (!kBf16) pow2_scale(top, &qs, &qinv);
-#pragma unroll 1
-        for (int c = hw * DH; c < hw * DH + DH; c += 16) {
-          float4 x[4];
-          uint32_t hi[8], lo[8], low[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = quad(k, c);
-          exchange4(x, lane);
+        if (some) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            split<T>(mul2(f2(x[k].x, x[k].y), f2(qs, qs)), &hi[2 * k], &lo[2 * k], &low[2 * k]);
-            split<T>(mul2(f2(x[k].z, x[k].w), f2(qs, qs)), &hi[2 * k + 1], &lo[2 * k + 1], &low[2 * k + 1]);
+            const int R = (row & ~3) + k;
+            if (R < rows) {
+              const float* qp = a.q + row_at(R) + hw * DH + (lane & 3) * 4;
+#pragma unroll
+              for (int c = 0; c < DH / 16; ++c) v[4 * c + k] = *reinterpret_cast<const float4*>(qp + 16 * c);
+            }
           }
+          float top = 0.0f;
+#pragma unroll
+          for (int c = 0; c < DH / 4; c += 4) {
+            float4 x[4] = {v[c], v[c + 1], v[c + 2], v[c + 3]};
+            exchange4(x, lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (!kBf16) top = amax3(amax3(top, x[k].x, x[k].y), x[k].z, x[k].w);
+              v[c + k] = x[k];
+            }
+          }
+          if (!kBf16) {                              // the halves' maxima
+            float* const mx = max_s + (n & 1) * 2 * kRows + row;
+            mx[hw * kRows] = top;
+            pair_sync(warp);
+            pow2_scale(amax3(top, mx[(hw ^ 1) * kRows], 0.0f), &qs, &qinv);
+            pair_sync(warp);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < DH / 4; c += 4) {
+          uint32_t hi[8], lo[8], low[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            split<T>(mul2(f2(v[c + k].x, v[c + k].y), f2(qs, qs)), &hi[2 * k], &lo[2 * k], &low[2 * k]);
+            split<T>(mul2(f2(v[c + k].z, v[c + k].w), f2(qs, qs)), &hi[2 * k + 1], &lo[2 * k + 1], &low[2 * k + 1]);
+          }
+          const int at = hw * DH + 4 * c;            // column
           if (L::LOW) {
-            *reinterpret_cast<uint4*>(smem + L::QLOW + tile_byte<D>(row, c / 8)) = make_uint4(low[0], low[1], low[2], low[3]);
-            *reinterpret_cast<uint4*>(smem + L::QLOW + tile_byte<D>(row, c / 8 + 1)) = make_uint4(low[4], low[5], low[6], low[7]);
+            *reinterpret_cast<uint4*>(smem + L::QLOW + tile_byte<D>(row, at / 8)) = make_uint4(low[0], low[1], low[2], low[3]);
+            *reinterpret_cast<uint4*>(smem + L::QLOW + tile_byte<D>(row, at / 8 + 1)) = make_uint4(low[4], low[5], low[6], low[7]);
           }
-          tmem_st_32x32b_x8(lanes + L::Q_COL + c / 2, hi);
-          tmem_st_32x32b_x8(lanes + L::Q_COL + (D + c) / 2, lo);
+          tmem_st_32x32b_x8(lanes + L::Q_COL + at / 2, hi);
+          tmem_st_32x32b_x8(lanes + L::Q_COL + (D + at) / 2, lo);
         }
         tmem_wait_st();
         if (L::LOW) fence_proxy_async_smem();
@@ -1046,7 +1058,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         }
       }
       const float cq = qinv * (a.scale * 1.44269504088896340736f);   // to powers of two
-      if ((warp & 3) * 32 >= rows) {
+      if (!some) {
         // no row of the warp's is live (Q, and so S and P, are zeros): it only keeps step
 #pragma unroll 1
         for (int t = t0; t < t1; ++t, ++n) {
@@ -1058,7 +1070,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         ++seg;
         continue;
       }
-      const int limit = live ? pc.pre + pc.node0 + row / a.g : -1;   // the last key that the row sees
+      const int limit = live ? pc.pre + pc.node0 + token_of(row) : -1;   // the last key that the row sees
       // running state: the reference that the sums stand at (in powers of two;
       // it follows the maximum once that is 2^8 above it, so most tiles
       // rescale nothing), the half's sum
@@ -1170,7 +1182,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       const int rows = min(a.npt, pc.nq - pc.node0) * a.g;
       const bool live = row < rows, some = (warp & 3) * 32 < rows;
       auto row_at = [&](int R) -> int64_t {
-        const int node = R / a.g;
+        const int node = token_of(R);
         return ((ps.a0 + ps.node0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
       };
       F2 acc[D / 2];
@@ -1186,7 +1198,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           if (__builtin_expect((t + 1) * kTK > pc.kmin || (note[kRange] & kMissing), 0)) {
             // V elements that are not finite went in as zeros: to the rows that see them
             if (note[kPois] | note[kPois + 1] | note[kPois + 2] | note[kPois + 3])
-              add_rare<D, T>(a, ps, oc, note, t, live ? min(pc.pre + pc.node0 + row / a.g + 1 - t * kTK, kTK) : 0);
+              add_rare<D, T>(a, ps, oc, note, t, live ? min(pc.pre + pc.node0 + token_of(row) + 1 - t * kTK, kTK) : 0);
           }
           if (__any_sync(0xffffffffu, corr != 1.0f)) {
 #pragma unroll
