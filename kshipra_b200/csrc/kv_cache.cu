@@ -61,10 +61,14 @@ __device__ __forceinline__ int64_t slot_offset(const WriteArgs& a, int64_t slot)
   return (((blk * a.num_layers + a.layer) * 2) * a.hkv * a.bs + (slot - blk * a.bs)) * a.d;
 }
 
-constexpr int kWriteThreads = 256;
+constexpr int kWriteThreads = 128;
 
 // D / 8 threads for each head of a token, four of the first half's elements
 // and the four that they rotate with each; a norm's sum by shuffles among them.
+// HBM bound.  2048 rows, 32 / 8 heads of 128, bf16, norms (93 MB): WRITEUS us, WRITEPC % of
+// measured HBM, inputs in turn; with 256 threads a CTA 23.4, 512 28; two or four
+// heads a thread, which share the angles' loads, 21 (at 256 threads 23 and 26); stores
+// past L2 would save 1 us here and cost the attention, which reads q next.
 template <int D, typename T>
 __global__ void __launch_bounds__(kWriteThreads) rope_write_kernel(WriteArgs a) {
   constexpr int TPH = D / 8, HALF = D / 2;
@@ -86,8 +90,8 @@ __global__ void __launch_bounds__(kWriteThreads) rope_write_kernel(WriteArgs a) 
   float4 x1 = make_float4(0.f, 0.f, 0.f, 0.f), x2 = x1;
   if (on) {
     const float* src = a.qkv + (t * heads + h) * D + j;
-    x1 = *reinterpret_cast<const float4*>(src);
-    x2 = *reinterpret_cast<const float4*>(src + HALF);
+    x1 = __ldcs(reinterpret_cast<const float4*>(src));          // read once
+    x2 = __ldcs(reinterpret_cast<const float4*>(src + HALF));
   }
   if (a.q_norm || a.k_norm) {      // the same for every thread
     float ss = x1.x * x1.x;
@@ -470,8 +474,11 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
   }
 }
 
-// Whole pages in pieces of 256 x kMoveUnroll units, over a grid of resident CTAs.
-constexpr int kMoveUnroll = 4;
+// Whole pages in pieces of 256 x kMoveUnroll units.  HBM bound: 100 pages of 2 MB (400
+// MB moved) in MOVEUS us with the tables, MOVEPC % of measured HBM.  Many small CTAs in turn
+// rather than eight resident ones an SM with larger pieces (81): a CTA that waits for
+// its loads leaves its place to another.
+constexpr int kMoveUnroll = 2;
 
 template <typename U>
 __global__ void __launch_bounds__(256) compact_move_kernel(const int32_t* scratch, int half, int64_t page_units, int pieces, U* pool) {
@@ -627,7 +634,7 @@ extern "C" int ksh_compact_pages(void* pool, int pool_type, int64_t num_blocks, 
   if (pieces > INT32_MAX) return KSH_ERR_UNSUPPORTED;
   const int rc = launch(compact_kernel, dim3(kPageCtas), dim3(kPageThreads), 0, st, a);
   if (rc != KSH_OK || num_blocks < 2) return rc;
-  const int grid = static_cast<int>(std::min<int64_t>(num_blocks / 2 * pieces, 8LL * num_sms()));
+  const int grid = static_cast<int>(std::min<int64_t>(num_blocks / 2 * pieces, 64LL * num_sms()));
   auto move = [&](auto* p) {
     using U = std::remove_pointer_t<decltype(p)>;
     return launch(compact_move_kernel<U>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, st, scratch,

@@ -192,15 +192,21 @@ def fork_pages(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
         raise ValueError("lens must have one entry per sequence, ref_counts one per page")
     if max_blocks < 1:
         raise ValueError("block_tables need a column")
-    tables = lens.new_empty((N, max_blocks))
-    new_lens = lens.new_empty(N)
-    refs = lens.new_empty(nb)
-    slots = torch.empty(N, dtype=torch.int64, device=pool.device)
-    scratch = lens.new_empty(S + 3 * N + 1)
+    # one allocation for the int32 outputs and the scratch (a tensor of its own takes
+    # twice a view's time, and the host's time is most of a small call's)
+    at_lens = N * max_blocks
+    at_refs = at_lens + N
+    scratch = S + 3 * N + 1
+    buf = lens.new_empty(at_refs + nb + scratch)
+    tables = buf.as_strided((N, max_blocks), (max_blocks, 1))
+    new_lens = buf.as_strided((N,), (1,), at_lens)
+    refs = buf.as_strided((nb,), (1,), at_refs)
+    slots = torch.empty_like(parents, dtype=torch.int64)
+    base = buf.data_ptr()
     _run(pool.device, "ksh_fork_pages", pool.data_ptr(), kind, nb, L, hkv, bs, d,
          block_tables.data_ptr(), max_blocks, lens.data_ptr(), S, parents.data_ptr(), N,
-         ref_counts.data_ptr(), tables.data_ptr(), new_lens.data_ptr(), slots.data_ptr(),
-         refs.data_ptr(), scratch.data_ptr(), scratch.numel(), _flags(flags, at))
+         ref_counts.data_ptr(), base, base + 4 * at_lens, slots.data_ptr(), base + 4 * at_refs,
+         base + 4 * (at_refs + nb), scratch, _flags(flags, at))
     return tables, new_lens, slots, refs
 
 
@@ -217,12 +223,15 @@ def compact_pages(pool: torch.Tensor, block_tables: torch.Tensor, ref_counts: to
     _need(block_tables, "block_tables", torch.int32, 2, at)
     if _need(ref_counts, "ref_counts", torch.int32, 1, at).shape[0] != nb:
         raise ValueError("ref_counts must have one entry per page")
-    tables = torch.empty_like(block_tables)
-    refs = torch.empty_like(ref_counts)
-    page_map = torch.empty_like(ref_counts)
-    used = ref_counts.new_empty(1)
-    scratch = ref_counts.new_empty(nb + 2)
+    rows, cols = block_tables.shape
+    n = rows * cols
+    buf = ref_counts.new_empty(n + 3 * nb + 3)             # one allocation, as in fork_pages
+    tables = buf.as_strided((rows, cols), (cols, 1))
+    refs = buf.as_strided((nb,), (1,), n)
+    page_map = buf.as_strided((nb,), (1,), n + nb)
+    used = buf.as_strided((1,), (1,), n + 2 * nb)
+    base = buf.data_ptr()
     _run(pool.device, "ksh_compact_pages", pool.data_ptr(), kind, nb, L, hkv, bs, d,
-         block_tables.data_ptr(), block_tables.numel(), ref_counts.data_ptr(), tables.data_ptr(),
-         refs.data_ptr(), page_map.data_ptr(), used.data_ptr(), scratch.data_ptr(), scratch.numel())
+         block_tables.data_ptr(), n, ref_counts.data_ptr(), base, base + 4 * n, base + 4 * (n + nb),
+         base + 4 * (n + 2 * nb), base + 4 * (n + 2 * nb + 1), nb + 2)
     return tables, refs, page_map, used
