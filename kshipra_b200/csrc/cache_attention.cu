@@ -140,7 +140,7 @@ struct CacheLayout {
   static constexpr int HALF = kTK * 128;             // bytes of 64 columns of a tile
   static constexpr int TILE = kTK * D * 2;
   // stages of K and of V; the third terms of Q and P (128 rows x D, 128 rows x 128 keys)
-  static constexpr int NST = D == 128 ? (LOW ? 2 : 3) : (LOW ? 5 : 6);
+  static constexpr int NST = D == 128 ? (LOW ? 2 : 3) : (LOW ? 4 : 6);
   static constexpr int K_OFF = 0, V_OFF = NST * TILE, QLOW = V_OFF + NST * TILE, PLOW = QLOW + (LOW ? TILE : 0);
   // notes on a tile: range, four words of keys that are there, four of keys whose
   // V is not finite
@@ -148,7 +148,8 @@ struct CacheLayout {
   static constexpr int MAX = META + kMeta * META_WORDS * 4;       // row maxima of the halves [2][2][128]
   static constexpr int CORR = MAX + 4 * kRows * 4;                // what the sums are rescaled by [kRing][128]
   static constexpr int FIN = CORR + kRing * kRows * 4;            // a piece's reference and the halves' sums [kRing][3][128]
-  static constexpr int BAR = FIN + kRing * 3 * kRows * 4;
+  static constexpr int FOLD = FIN + kRing * 3 * kRows * 4;        // 32 rows of O on their way to another warp
+  static constexpr int BAR = FOLD + 32 * D * 4;
   static constexpr int NBAR = 5 * NST + 5 * 2 + 1;
   static constexpr int MISC = BAR + NBAR * 8;
   static constexpr int BYTES = MISC + 64 + 1024;
@@ -448,6 +449,8 @@ __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+// The warps of the sums meet.
+__device__ __forceinline__ void sums_sync() { asm volatile("bar.sync 5, 128;" ::: "memory"); }
 // The two warps of 32 query rows (halves of the keys) meet.
 __device__ __forceinline__ void pair_sync(int warp) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
@@ -508,17 +511,18 @@ __device__ __noinline__ void clean_v(uint8_t* tile, uint32_t* note, int lane) {
   __syncwarp();
 }
 
-// Adds the elements that are not finite of tile t's noted V rows (the first cnt keys
+// Adds the elements that are not finite of tile t's noted V rows (keys from .. cnt - 1
 // are a row's) to O, 16 columns at a time.
 template <int D, typename T>
-__device__ __forceinline__ void add_rare(const CacheArgs& a, const Piece& p, uint32_t oc, const uint32_t* note, int t, int cnt) {
+__device__ __forceinline__ void add_rare(const CacheArgs& a, const Piece& p, uint32_t oc, const uint32_t* note, int t, int from,
+                                         int cnt) {
 #pragma unroll 1
   for (int c0 = 0; c0 < D; c0 += 16) {
     float v[16];
     tmem_ld_32x32b_x16(oc + c0, v);
     tmem_wait_ld(v);
 #pragma unroll 1
-    for (int k = 0; k < cnt; ++k) {
+    for (int k = from; k < cnt; ++k) {
       if (!((note[kPois + (k >> 5)] >> (k & 31)) & 1)) continue;
       const int64_t at = key_offset(a, p.s, p.hk, t * kTK + k, D);
       if (at < 0) continue;
@@ -554,6 +558,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
   float* const max_s = reinterpret_cast<float*>(smem + L::MAX);
   float* const corr_s = reinterpret_cast<float*>(smem + L::CORR);
   float* const fin_s = reinterpret_cast<float*>(smem + L::FIN);
+  float4* const fold_s = reinterpret_cast<float4*>(smem + L::FOLD);
   uint64_t* kraw = reinterpret_cast<uint64_t*>(smem + L::BAR);
   uint64_t* vraw = kraw + NST;
   uint64_t* vfull = vraw + NST;         // cleaned, or as it came
@@ -696,8 +701,8 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
   Piece pc = {};
 
   // Bounded wait of the whole warp; gives up for all roles together, and from then on
-  // at once: the row warps go through their steps to the end all the same, because
-  // their pairs meet in each.
+  // at once: the row and sum warps go through their steps to the end all the same,
+  // because they meet in them.
   bool dead = false;
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     if (dead) return false;
@@ -758,7 +763,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         // relative to the sum so far
         if (L::LOW) {
           const uint64_t qd = desc_k_sw128(smem_u32(smem + L::QLOW));
-#pragma unroll 2
+#pragma unroll 8
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t at = (k / 4) * (L::HALF / 16) + 2 * (k % 4);
             mma_f16(sp, qd + at, kd + at, id_s, k > 0 ? 1u : 0u);
@@ -768,7 +773,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         // the warp spills, and issues late)
 #pragma unroll 1
         for (int term = 1; term >= 0; --term)
-#pragma unroll 2
+#pragma unroll 8
           for (int k = 0; k < D / 16; ++k)
             mma_f16_ts(sp, tmem + L::Q_COL + term * (D / 2) + 8 * k, kd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), id_s,
                        (L::LOW || term == 0 || k > 0) ? 1u : 0u);
@@ -801,13 +806,13 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           const uint64_t vd = desc_v(vbase + st * L::TILE, L::HALF);
           if (L::LOW) {
             const uint64_t pd = desc_k_sw128(smem_u32(smem + L::PLOW));
-#pragma unroll 2
+#pragma unroll 8
             for (int k = 0; k < kTK / 16; ++k)
               mma_f16(tmem + L::O_COL, pd + (k / 4) * (L::HALF / 16) + 2 * (k % 4), vd + k * (2048 / 16), id_o, k > 0 ? 1u : 0u);
           }
 #pragma unroll 1
           for (int term = 1; term >= 0; --term)
-#pragma unroll 2
+#pragma unroll 8
             for (int k = 0; k < kTK / 16; ++k)
               mma_f16_ts(tmem + L::O_COL, sp + 16 * k + 8 * term, vd + k * (2048 / 16), id_o,
                          (L::LOW || term == 0 || k > 0) ? 1u : 0u);
@@ -987,13 +992,17 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       __syncwarp();
       const int t0 = pc.t0, t1 = pc.t1;
       const int rows = min(a.npt, pc.nq - pc.node0) * a.g;       // live ones of the tile
-      const bool live = row < rows;
+      // Up to 32 rows (decoding) stand in the lanes four times, a quarter of the keys
+      // each with its own softmax state: the chain of a tile is a quarter as long.
+      const bool fold = rows <= 32;
+      const int qrow = fold ? lane : row;
+      const bool live = qrow < rows;
       // the row's place in q and out
       auto row_at = [&](int R) -> int64_t {
         const int node = token_of(R);
         return ((ps.a0 + ps.node0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
       };
-      const bool some = (warp & 3) * 32 < rows;
+      const bool some = fold || (warp & 3) * 32 < rows;
       float qinv = 1.0f;
       // Q: the half's columns as terms into TMEM (zeros for rows that are not live).
       // Four lanes load 64 bytes of a row, for the rows of the four, and exchange
@@ -1006,7 +1015,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         if (some) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int R = (row & ~3) + k;
+            const int R = (qrow & ~3) + k;
             if (R < rows) {
               const float* qp = a.q + row_at(R) + hw * DH + (lane & 3) * 4;
 #pragma unroll
@@ -1070,12 +1079,90 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         ++seg;
         continue;
       }
-      const int limit = live ? pc.pre + pc.node0 + token_of(row) : -1;   // the last key that the row sees
+      const int limit = live ? pc.pre + pc.node0 + token_of(qrow) : -1;   // the last key that the row sees
       // running state: the reference that the sums stand at (in powers of two;
       // it follows the maximum once that is 2^8 above it, so most tiles
       // rescale nothing), the half's sum
       float mref = -INFINITY, l = 0.0f;
       bool s_there = false;                         // seen a tile ahead
+      if (fold) {
+        const int part = warp & 3;                   // the keys 32 part on are the pair's
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t, ++n) {
+          const int b = n & 1;
+          if (!__all_sync(0xffffffffu, s_there)) wait(&sfull[b], (n >> 1) & 1);
+          tc_fence_after();
+          const uint32_t sb = lanes + L::S_COL + static_cast<uint32_t>(b) * kTK, own = sb + 32 * part + 16 * hw;
+          float x[16];
+          tmem_ld_32x32b_x16(own, x);
+          float corr = 1.0f;
+          const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
+          const bool special = (t + 1) * kTK > pc.kmin || (*const_cast<const volatile uint32_t*>(note + kRange) & kMissing);
+          tmem_wait_ld(x);
+          if (__builtin_expect(special, 0)) {
+            const int k = limit + 1 - t * kTK - 32 * part;
+            const uint32_t seen = (note[kThere + part] & (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1)) >> (16 * hw);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = (seen >> j) & 1 ? x[j] : -INFINITY;
+          }
+          float m = max3(x[0], x[1], x[2]);
+#pragma unroll
+          for (int j = 3; j + 1 < 16; j += 2) m = max3(m, x[j], x[j + 1]);
+          float* const mx = max_s + (n & 1) * 2 * kRows + row;
+          mx[hw * kRows] = fmaxf(m, x[15]);
+          pair_sync(warp);
+          const float mc = fmaxf(mx[0], mx[kRows]) * cq;
+          if (mc > mref + 8.0f) {
+            corr = ex2(mref - mc);
+            mref = mc;
+          }
+          const float ref = mref == -INFINITY ? 0.0f : kBf16 ? mref : mref - 6.0f;
+          const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
+          F2 s2 = f2(0.f, 0.f);
+          if (hw == 0) corr_s[(n % kRing) * kRows + row] = corr;
+          const bool low_free = L::LOW && n > 0 && mbar_test(ofull, (n - 1) & 1);
+          s_there = t + 1 < t1 && mbar_test(&sfull[b ^ 1], ((n + 1) >> 1) & 1);
+          uint32_t pt[16], low[8];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 e = unpack(fma2(f2(x[j], x[j + 1]), c2, nref));
+            const F2 p = f2(ex2(e.x), ex2(e.y));
+            s2 = add2(s2, p);
+            split<T>(p, &pt[j / 2], &pt[j / 2 + 8], &low[j / 2]);
+          }
+          tmem_st_32x32b_x16(own, pt);
+          // zeros for the other quarters' keys
+#pragma unroll
+          for (int j = 0; j < 16; ++j) pt[j] = 0;
+#pragma unroll 1
+          for (int g = 4 * hw; g < 4 * hw + 4; ++g)
+            if ((g >> 1) != part) tmem_st_32x32b_x16(sb + 16 * g, pt);
+          const float2 sum = unpack(s2);
+          l = fmaf(l, corr, sum.x + sum.y);
+          if (t + 1 == t1) {
+            float* const fin = fin_s + (seg % kRing) * 3 * kRows + row;
+            fin[hw * kRows] = l;
+            if (hw == 0) fin[2 * kRows] = mref;
+          }
+          if constexpr (L::LOW) {
+            if (n > 0 && !__all_sync(0xffffffffu, low_free)) wait(ofull, (n - 1) & 1);
+            uint8_t* const ps = smem + L::PLOW;
+            if (t == t0)                             // they stay zeros for the rest of the piece
+              for (int c = 8 * hw; c < 8 * hw + 8; ++c)
+                if ((c >> 2) != part) *reinterpret_cast<uint4*>(ps + tile_byte<kTK>(row, c)) = make_uint4(0, 0, 0, 0);
+            const int c = 4 * part + 2 * hw;
+            *reinterpret_cast<uint4*>(ps + tile_byte<kTK>(row, c)) = make_uint4(low[0], low[1], low[2], low[3]);
+            *reinterpret_cast<uint4*>(ps + tile_byte<kTK>(row, c + 1)) = make_uint4(low[4], low[5], low[6], low[7]);
+            fence_proxy_async_smem();
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pready[b]);
+        }
+        ++seg;
+        continue;
+      }
 #pragma unroll 1
       for (int t = t0; t < t1; ++t, ++n) {
         const int b = n & 1;
@@ -1173,14 +1260,15 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
     const uint32_t oc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + L::O_COL;
     int n = 0, seg = 0;
     const Piece& ps = piece_s[kRowWarps + (warp & 3)];
-    bool ok = true;
-    while (ok && next_piece(a, wk, &pc)) {
+    while (next_piece(a, wk, &pc)) {
       __syncwarp();
       if (lane == 0) piece_s[kRowWarps + (warp & 3)] = pc;
       __syncwarp();
       const int t0 = pc.t0, t1 = pc.t1;
       const int rows = min(a.npt, pc.nq - pc.node0) * a.g;
-      const bool live = row < rows, some = (warp & 3) * 32 < rows;
+      const bool fold = rows <= 32;
+      const int part = warp & 3, qrow = fold ? lane : row;
+      const bool live = qrow < rows, some = fold || part * 32 < rows;
       auto row_at = [&](int R) -> int64_t {
         const int node = token_of(R);
         return ((ps.a0 + ps.node0 + node) * a.hq + static_cast<int64_t>(ps.hk) * a.g + (R - node * a.g)) * D;
@@ -1190,7 +1278,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       for (int c = 0; c < D / 2; ++c) acc[c] = f2(0.f, 0.f);
 #pragma unroll 1
       for (int t = t0; t < t1; ++t, ++n) {
-        if (!(ok = wait(ofull, n & 1))) break;
+        wait(ofull, n & 1);
         const uint32_t* const note = notes + (n % kMeta) * L::META_WORDS;
         if (some) {
           tc_fence_after();
@@ -1198,7 +1286,8 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           if (__builtin_expect((t + 1) * kTK > pc.kmin || (note[kRange] & kMissing), 0)) {
             // V elements that are not finite went in as zeros: to the rows that see them
             if (note[kPois] | note[kPois + 1] | note[kPois + 2] | note[kPois + 3])
-              add_rare<D, T>(a, ps, oc, note, t, live ? min(pc.pre + pc.node0 + token_of(row) + 1 - t * kTK, kTK) : 0);
+              add_rare<D, T>(a, ps, oc, note, t, fold ? 32 * part : 0,
+                             live ? min(pc.pre + pc.node0 + token_of(qrow) + 1 - t * kTK, fold ? 32 * part + 32 : kTK) : 0);
           }
           if (__any_sync(0xffffffffu, corr != 1.0f)) {
 #pragma unroll
@@ -1221,15 +1310,49 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&oempty[n & 1]);
       }
-      if (!ok) break;
       const float* const fin = fin_s + (seg % kRing) * 3 * kRows + row;
       ++seg;
       if (!some) continue;
-      const float l = fin[0] + fin[kRows];
+      float l = fin[0] + fin[kRows], ref = fin[2 * kRows];
+      if (fold) {
+        // the quarters' states, joined like an item's pieces
+        const float* const all = fin - row + lane;
+        float top = all[2 * kRows];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) top = fmaxf(top, all[2 * kRows + 32 * k]);
+        const float at = top == -INFINITY ? 0.0f : top, mine = ex2(ref - at);
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) l = fmaf(all[32 * k] + all[kRows + 32 * k], ex2(all[2 * kRows + 32 * k] - at), l);
+        ref = top;
+#pragma unroll
+        for (int c = 0; c < D / 2; ++c) acc[c] = mul2(acc[c], f2(mine, mine));
+#pragma unroll 1
+        for (int k = 1; k < 4; ++k) {
+          if (part == k) {
+#pragma unroll
+            for (int c = 0; c < D / 4; ++c) {
+              const float2 p = unpack(acc[2 * c]), u = unpack(acc[2 * c + 1]);
+              fold_s[c * 32 + lane] = make_float4(p.x, p.y, u.x, u.y);
+            }
+          }
+          sums_sync();
+          if (part == 0) {
+#pragma unroll
+            for (int c = 0; c < D / 4; ++c) {
+              const float4 v = fold_s[c * 32 + lane];
+              acc[2 * c] = add2(acc[2 * c], f2(v.x, v.y));
+              acc[2 * c + 1] = add2(acc[2 * c + 1], f2(v.z, v.w));
+            }
+          }
+          sums_sync();
+        }
+        if (part != 0) continue;
+      }
       if (t0 == 0 && t1 == ps.ntiles) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (live) {
-          float* op = a.out + row_at(row);
+          float* op = a.out + row_at(qrow);
 #pragma unroll
           for (int c = 0; c < D; c += 4) {
             const float2 p = unpack(mul2(acc[c / 2], f2(inv, inv))), u = unpack(mul2(acc[c / 2 + 1], f2(inv, inv)));
@@ -1237,14 +1360,14 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           }
         }
       } else {
-        float* part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * part_floats<D>();
+        float* state = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * part_floats<D>();
         if (live) {
-          part[row] = fin[2 * kRows];
-          part[kRows + row] = l;
+          state[qrow] = ref;
+          state[kRows + qrow] = l;
 #pragma unroll
           for (int c = 0; c < D; c += 4) {
             const float2 p = unpack(acc[c / 2]), u = unpack(acc[c / 2 + 1]);
-            reinterpret_cast<float4*>(part + 2 * kRows)[c / 4 * kRows + row] = make_float4(p.x, p.y, u.x, u.y);
+            reinterpret_cast<float4*>(state + 2 * kRows)[c / 4 * kRows + qrow] = make_float4(p.x, p.y, u.x, u.y);
           }
         }
         if (t0 == 0 && warp == kSumWarp && lane == 0) {                 // the share's last piece: joined from here on
