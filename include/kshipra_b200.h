@@ -452,11 +452,14 @@ int ksh_rope_cache_write(const float* qkv, int64_t m, int64_t hq, int64_t hkv, i
  * q_start[s] .. q_start[s + 1] - 1 of q [total, hq, d], whose K/V stand at
  * positions prefix_lens[s] .. of its block table; row i attends positions
  * 0 .. prefix + i.  Softmax statistics and sums are fp32.  What a row may not
- * see does not reach it, NaN and infinity included; a row that sees a K or V
- * element that is not finite gives NaN or infinity.  Rows of q that no sequence
- * covers are not written; a row whose pages are all missing gives zeros.
- * max_q_len and max_total_len are host-side upper bounds (a longer sequence
- * raises KSH_FLAG_BAD_LENGTH, its rows past the bound are not written).  d <= 256.
+ * see does not reach it, NaN and infinity included; a row that sees a V element
+ * that is not finite gives NaN or infinity in that column, one that sees such a K
+ * element in general NaN.  Rows of q that no sequence covers are not written; a
+ * row whose pages are all missing gives zeros.  max_q_len is a host-side upper bound of
+ * a sequence's rows (a longer one raises KSH_FLAG_BAD_LENGTH and its rows past the
+ * bound are not written), max_total_len, of a sequence's positions, only sizes the
+ * launch.  A sequence that does not fit its table raises KSH_FLAG_BAD_LENGTH; its
+ * rows are not specified.  d <= 256.
  * The workspace, of ksh_cache_attention_workspace_size bytes and 256-byte
  * aligned, needs no initialisation. */
 int64_t ksh_cache_attention_workspace_size(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d,

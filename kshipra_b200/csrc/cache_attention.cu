@@ -5,6 +5,51 @@
 // attends positions 0 .. prefix + i:
 //     o = sum_j exp(q.k_j / sqrt(D) - m) v_j / sum_j exp(q.k_j / sqrt(D) - m)
 // with the running maximum m.  q and o are fp32, K and V fp16 or bf16.
+//
+// Head dimensions 64 and 128 (cache_attn_tc_kernel): K and V go to the tensor cores
+// as they stand in the cache, TMA boxes of pool rows straight into the MMAs'
+// operand layout.  q and P, which are fp32, go in as sums of 16-bit terms of the
+// cache's type (fp16: two of 11 bits, q with a power of two per row; bf16: three of
+// 8), so a product costs two or three MMAs and the result has fp32's accuracy
+// (relative L2 error against 64 bits 3e-7 to 9e-7; the same in fp32 torch 8e-7 to
+// 3.4e-6).  Rounding q and P to one 16-bit term each would cost 2^-9 to 2^-12.
+//
+// One persistent CTA per SM.  An item is (sequence, row tile of up to 128 rows =
+// tokens x heads of a kv head, kv head); its 128-key tiles end at the last token's
+// position, so masked tiles are not read.  All items' keys form one line that is cut
+// into equal shares, one per CTA, so that uneven lengths leave no SM idle; an item
+// cut between CTAs leaves its (m, l, acc) pieces in the workspace and
+// cache_merge_kernel joins them in key order (the same bits in every run).  One
+// token of a sequence is an item of few rows.  Warps of a CTA:
+//   14, 15  K and V tiles into shared memory, and V's rows that not every query row
+//           sees cleaned of what may stand in them
+//   12, 13  MMAs, one warp for the even tiles and one for the odd: S = Q K^T (A = Q in
+//           TMEM), O = P V (A = P in TMEM, over S)
+//   0..7    rows: thread = query row and half of the tile's keys (up to 32 rows:
+//           an eighth): softmax in 32 bits, P's terms into TMEM
+//   8..11   sums: thread = query row: every tile's P V added into fp32 registers (a
+//           long context added up inside the tensor core would lose low bits at each
+//           step), results and pieces written
+//
+// What bounds it: with two terms a tile of 128 rows, 128 keys and D = 128 is 2.05 K
+// tensor cycles, with three 3.07 K, and 64 KB of K and V, 2.3 to 2.9 K cycles of the
+// SM's share of HBM.  Measured (back to back from a graph; in long runs the power limit
+// holds the clock at 1.5 GHz and adds 10 to 15 %):
+//   64 sequences x 4096 keys, one token each, 32 / 8 heads of 128, fp16 (1.08 GB): 210
+//   us, 5.1 TB/s, 79 % of measured HBM; tensor pipe 70 % active.  bf16 265 to 315.
+//   2048 tokens behind 4096, the same heads, fp16: 287 us, 600 TFLOP/s of attention and
+//   twice that of MMAs; tensor pipe 66 % active.
+//   3 sequences of up to 31000 keys with chunks of up to 200, bf16: 310 to 335 us.
+//   24 sequences of up to 2000 keys, chunks of up to 301 among single tokens, 14 / 2
+//   heads of 64, bf16: 91 us.  One sequence x 540 keys: 15.4 us, of which the second
+//   launch takes 4.
+// In a tile the longest chain is P V (1.0 K), its sums (1.2 K) and the waits between
+// them (0.3 K each: with MMAs in flight an mbarrier's answer takes that long).  No
+// faster, for the fp16 cases above: the sums in the row warps (10 % slower), sixteen row
+// warps with a quarter each (15 %), one MMA warp (its waits add up to 1.5 K cycles a
+// tile, 20 %), one warp for S and one for P V with Q in shared memory (30 %: the MMAs'
+// reads then fill it), O in two halves (5 to 10 %); bf16 widened to fp16 in shared memory by
+// four more warps and two terms (25 %).
 
 #include <cuda_bf16.h>
 #include <math.h>
@@ -112,8 +157,13 @@ constexpr int kRows = 128;               // query rows per tile (MMA M)
 constexpr int kRowWarps = 8, kSumWarp = kRowWarps, kSumWarps = 4;
 constexpr int kMmaWarp = kSumWarp + kSumWarps, kCopyWarp = kMmaWarp + 2;     // even and odd tiles; K and V
 constexpr int kThreads = 32 * (kCopyWarp + 2);
-// registers a thread, of 128 at launch: rows, sums, the other roles
+// registers a thread, of 128 at launch: rows, sums, the other roles (the sums spill
+// below 176, which costs 50 %)
 constexpr int kRowRegs = 120, kSumRegs = 192, kRegs = 80;
+// An item's start (its Q, an empty pipeline) takes about four tiles' time; counted so
+// in the line, the CTAs with more items are not the last ones.  24 sequences of
+// chunks and single tokens: 91 us, 160 with 128 keys, 122 with 1024.  Where there are
+// few tiles a CTA it would only put more tiles into some of them.
 constexpr int kItemCost = 512;
 constexpr int kMeta = 16;                // tiles whose notes are kept: more than the stages let run apart
 // Tiles (pieces) that the row warps can be ahead of the sum warps, and more
@@ -161,8 +211,9 @@ struct CacheLayout {
 };
 // words of a tile's notes
 constexpr int kRange = 0, kThere = 1, kPois = 5;
-// the range word: keys that all rows see | keys that are read << 8, and these bits
-constexpr uint32_t kMissing = 1u << 16, kLast = 1u << 17;
+// the range word: keys that all rows see | keys that are read << 8, and whether pages
+// are missing
+constexpr uint32_t kMissing = 1u << 16;
 
 // One sequence's share of the work.
 struct SeqWork {
@@ -929,7 +980,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
         word = lane == 0 ? there[0] : lane == 1 ? there[NH > 1 ? 1 : 0] : lane == 2 ? there[NH > 2 ? 2 : 0] : there[NH > 3 ? 3 : 0];
       }
       if (lane < 4) note[kThere + lane] = word;
-      if (lane == 0) note[kRange] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8 | (lost ? kMissing : 0) | (have ? 0 : kLast);
+      if (lane == 0) note[kRange] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8 | (lost ? kMissing : 0);
       __syncwarp();
       uint8_t* const tile = smem + (kv ? L::V_OFF : L::K_OFF) + st * L::TILE;
       if (BOX) {

@@ -136,7 +136,8 @@ def cache_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_table
     holding the new tokens' own K/V too; block_tables int32 [S, max_blocks]; rows
     q_start[s] .. q_start[s + 1] - 1 (int32 [S + 1]) are sequence s's, at positions
     prefix_lens[s] (int32 [S]) and on, and attend every position up to their own.
-    ``max_q_len`` and ``max_total_len`` bound a sequence's rows and positions.
+    ``max_q_len`` bounds a sequence's rows, ``max_total_len`` (its positions) only
+    sizes the launch.
     Returns fp32 [T, Hq, D]; rows of q that no sequence covers are not written."""
     at = _need(q, "q", torch.float32, 3).get_device()
     kind = _pool(pool, (1, 2), at)
