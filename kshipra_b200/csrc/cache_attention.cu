@@ -226,7 +226,7 @@ __device__ __forceinline__ SeqWork seq_work(const CacheArgs& a, int s) {
   SeqWork w = {};
   const int64_t a0 = a.q_start[s], n = a.q_start[s + 1] - a0;
   const int pre = a.prefix[s];
-  const int64_t cap = min(a.max_blocks * a.bs, static_cast<int64_t>(INT32_MAX - 2 * kTK));
+  const int64_t cap = min(a.max_blocks * a.bs, static_cast<int64_t>(INT32_MAX - 2 * kTK - kItemCost));
   w.a0 = a0;
   w.bad = a0 < 0 || n < 0 || a0 + n > a.total || n > a.max_q || pre < 0 || max(pre, 0) + max(n, int64_t(0)) > cap;
   if (a0 < 0 || n <= 0 || a0 >= a.total) return w;
@@ -1034,7 +1034,8 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
     set_regs_dec<kRowRegs>();
     const int hw = warp >> 2, row = (warp & 3) * 32 + lane;      // half, query row
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    constexpr int DH = D / 2;                       // columns of O per half
+    constexpr int DH = D / 2;                       // columns of Q per half
+    constexpr float kRefShift = kBf16 ? 8.0f : -6.0f;
     int n = 0, seg = 0;
     const Piece& ps = piece_s[warp];                // of the rare paths
     while (next_piece(a, wk, &pc)) {
@@ -1167,7 +1168,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
             corr = ex2(mref - mc);
             mref = mc;
           }
-          const float ref = mref == -INFINITY ? 0.0f : kBf16 ? mref : mref - 6.0f;
+          const float ref = mref == -INFINITY ? 0.0f : mref + kRefShift;
           const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
           F2 s2 = f2(0.f, 0.f);
           if (hw == 0) corr_s[(n % kRing) * kRows + row] = corr;
@@ -1257,8 +1258,9 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           corr = ex2(mref - mc);
           mref = mc;
         }
-        // P = 2^(x c - ref): up to 2^14 in fp16 terms, 2^8 in bf16
-        const float ref = mref == -INFINITY ? 0.0f : kBf16 ? mref : mref - 6.0f;
+        // P = 2^(x c - ref): up to 2^14 in fp16 terms, which keeps them above fp16's
+        // smallest; up to 1 in bf16, whose V may be as large as fp32
+        const float ref = mref == -INFINITY ? 0.0f : mref + kRefShift;
         const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
         F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
         uint32_t low[L::LOW ? 32 : 1];
@@ -1599,7 +1601,7 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
     // No more CTAs than there can be tiles; an item's start counts only where there
     // are several tiles a CTA.
     const double tiles = static_cast<double>(num_seqs) * static_cast<double>(hkv) *
-                         static_cast<double>((max_q_len + a.npt - 1) / a.npt) *
+                         static_cast<double>((std::min(max_q_len, total) + a.npt - 1) / a.npt) *
                          static_cast<double>(std::max<int64_t>(1, (max_total_len + kTK - 1) / kTK));
     const int grid = static_cast<int>(std::min<double>(num_sms(), tiles));
     a.item_cost = tiles >= 4.0 * num_sms() ? kItemCost : 0;
@@ -1608,7 +1610,7 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
     return d == 64 ? launch_cache_tc<64, __nv_bfloat16>(a, grid, st) : launch_cache_tc<128, __nv_bfloat16>(a, grid, st);
   }
   if (hq > 65535 || num_seqs > 65535) return KSH_ERR_UNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>(max_q_len), static_cast<unsigned>(hq), static_cast<unsigned>(num_seqs));
+  const dim3 grid(static_cast<unsigned>(std::min(max_q_len, total)), static_cast<unsigned>(hq), static_cast<unsigned>(num_seqs));
   return pool_type == KSH_TYPE_F16 ? launch(cache_attn_simple_kernel<__half>, grid, dim3(32), 0, st, a)
                                    : launch(cache_attn_simple_kernel<__nv_bfloat16>, grid, dim3(32), 0, st, a);
 }

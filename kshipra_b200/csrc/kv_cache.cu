@@ -568,7 +568,7 @@ extern "C" int ksh_fork_pages(void* pool, int pool_type, int64_t num_blocks, int
   KSH_CHECK_ARG(eb != 0 && num_blocks > 0 && num_blocks <= INT32_MAX / 2 && num_layers > 0 && hkv > 0 && block_size > 0 &&
                 block_size <= INT32_MAX && d > 0 && max_blocks > 0 && max_blocks <= INT32_MAX / 64 && num_seqs >= 0 &&
                 num_seqs <= INT32_MAX / 8 && n >= 0);
-  KSH_CHECK_ARG(pool && block_tables && lens && ref_counts && new_ref);
+  KSH_CHECK_ARG(pool && ref_counts && new_ref && (num_seqs == 0 || (block_tables && lens)));
   KSH_CHECK_ARG(n == 0 || (parents && new_tables && new_lens && slots));
   if (n > 65535) return KSH_ERR_UNSUPPORTED;
   if (!scratch || scratch_ints < ksh_fork_pages_scratch_ints(num_seqs, n)) return KSH_ERR_WORKSPACE;

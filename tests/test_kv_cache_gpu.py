@@ -731,6 +731,68 @@ def test_refusals():
         kv.compact_pages(pool.cpu(), table, refs)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16), (96, F16)])
+def test_attention_without_any_new_token(d, dtype):
+    b = Batch([(50, 0), (0, 0), (7, 0)], 4, 2, d, 16, dtype, tail_rows=3)
+    f = new_flags()
+    out = torch.full_like(b.q, 7.0)
+    kv.cache_attention(b.q, b.pool, 0, b.table, b.q_start, b.prefix, 5, 60, out=out, flags=f)
+    assert (out == 7).all() and int(f) == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_bf16_values_near_the_largest(d):
+    """Sums stay in range where the values nearly fill it."""
+    b = Batch([(40, 3), (9, 1)], 4, 2, d, 16, BF16)
+    b.pool[:, :, 1] = (b.pool[:, :, 1].float().abs().clamp(max=3.0) * 2.0 ** 118).to(BF16)
+    b.q *= 8.0                                               # the maximum rises as tiles go by
+    want = b.want()
+    got = b.run().double()
+    assert float((got - want).abs().max() / want.abs().max()) < 1e-5
+
+
+def test_attention_loose_bounds():
+    """max_q_len and max_total_len far above what comes."""
+    for d in (64, 96):
+        b = Batch([(40, 3), (9, 1)], 4, 2, d, 16, F16)
+        b.max_q, b.max_total = 2 ** 31 - 1, 2 ** 40
+        b.check(b.run())
+
+
+def test_fork_from_nothing():
+    pool = torch.randn(6, 1, 2, 1, 4, 8, device="cuda").half()
+    none = torch.empty((0, 3), dtype=torch.int32, device="cuda")
+    refs = i32([1, 0, 0, 2, 0, 0])
+    f = new_flags()
+    t, n, s, r = kv.fork_pages(pool, none, i32([]), i32([-1, -1]), refs, flags=f)
+    assert t.tolist() == [[0] * 3] * 2 and n.tolist() == [0, 0] and s.tolist() == [-1, -1] and torch.equal(r, refs)
+    assert int(f) == 0
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Forks and attentions of two batches on streams of their own."""
+    bs = [Batch([(300, 20), (77, 1)], 8, 2, 128, 16, F16, seed=i) for i in range(2)]
+    cases = [fork_case([37, 40, 64, 33], 8, 16, 100, seed=i) for i in range(2)]
+    wants = [fork_want(c[0], c[1], c[2], [0, 0, 2, 3, 3], c[3]) for c in cases]
+    lens, parents = i32([37, 40, 64, 33]), i32([0, 0, 2, 3, 3])
+    torch.cuda.synchronize()
+    streams, got, forked = [torch.cuda.Stream() for _ in range(2)], [], []
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, bs[i].run()))
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            forked.append(kv.fork_pages(cases[i][0], cases[i][1], lens, parents, cases[i][3]))
+    torch.cuda.synchronize()
+    for i, out in got:
+        bs[i].check(out)
+    for c, f, w in zip(cases, forked, wants):
+        for x, y in zip(f, w):
+            assert x.tolist() == y
+        assert torch.equal(c[0], w[4])
+
+
 def test_empty_calls():
     b = Batch([(20, 3)], 4, 2, 64, 16, F16)
     none = b.q[:0].contiguous()
