@@ -476,9 +476,9 @@ int ksh_cache_attention(const float* q, int64_t total, int64_t hq, int64_t d, co
  * with lens[S] tokens cached, and gets a row of new_tables [n, max_blocks]
  * (padded with 0), new_lens[i] = lens[parent] and slots[i], the slot of its
  * next token.  Whole pages are shared.  The page that the next token goes to is
- * the parent's for the first of its children; for the others it is a free page
- * into which the filled rows are copied, in every layer, and where a page
- * begins a free one for each.  ref_counts[nb] counts, for each page, the rows
+ * the parent's for the first child that continues in it, where no row but the S
+ * holds it; for the others it is a free page into which the filled rows are
+ * copied, in every layer, and where a page begins a free one for each.  ref_counts[nb] counts, for each page, the rows
  * (of all tables, these or others) that hold it; new_ref is what it is after the
  * S sequences have given up theirs and the children hold theirs.  Free pages
  * (count 0 then) are taken from the lowest number up in the children's order.

@@ -80,13 +80,13 @@ __global__ void __launch_bounds__(kWriteThreads) rope_write_kernel(WriteArgs a) 
   const int h = on ? static_cast<int>(unit - t * heads) : 0;
   const bool rot = h < a.hq + a.hkv;
   const float* nw = h < a.hq ? a.q_norm : rot ? a.k_norm : nullptr;
+  grid_dep_wait();
+  grid_dep_launch();
   float4 w1, w2;
   if (nw) {
     w1 = *reinterpret_cast<const float4*>(nw + j);
     w2 = *reinterpret_cast<const float4*>(nw + HALF + j);
   }
-  grid_dep_wait();
-  grid_dep_launch();
   float4 x1 = make_float4(0.f, 0.f, 0.f, 0.f), x2 = x1;
   if (on) {
     const float* src = a.qkv + (t * heads + h) * D + j;
@@ -255,8 +255,9 @@ __device__ __forceinline__ int cluster_scan(int count, int* cnt_s, int gw, int l
 
 // Children i = 0 .. n - 1 continue sequences parents[i].  A child's pages
 // before the one that its next token goes to are its parent's; that one is the
-// parent's for the first of its children, and a fresh one (with the filled rows
-// copied) for the others and where a page begins.
+// parent's for the first of the children that would write into it, where no other
+// row holds it, and a fresh one (with the filled rows copied) for the others and
+// where a page begins.
 __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads) fork_kernel(ForkArgs a) {
   __shared__ int cnt_s[2][kPageWarps];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -311,9 +312,21 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
     }
   }
   cluster_sync();
-  // the page that the next token goes to: kept, or fresh; fresh ones are numbered in
-  // the children's order.  A warp has a run of children.
+  // A warp has a run of children.  A page that is being filled and that nobody holds
+  // now goes to the first child whose parent held it: the least of i - n stands in for
+  // its count until the child takes it.
   const int per = (a.n + kPageWarps - 1) / kPageWarps;
+  for (int i = gw * per + lane; i < min(a.n, (gw + 1) * per); i += 32) {
+    const int p = parent(i);
+    if (p < 0 || __ldcg(first + p) != i) continue;
+    const int ln = length(p), full = ln / bs;
+    if (full >= M || ln == full * bs) continue;
+    const int page = a.tables[static_cast<int64_t>(p) * M + full];
+    if (page >= 0 && page < a.num_blocks && __ldcg(a.new_ref + page) <= 0) atomicMin(a.new_ref + page, i - a.n);
+  }
+  cluster_sync();
+  // the page that the next token goes to: kept, or fresh; fresh ones are numbered in
+  // the children's order.
   int count = 0;
   for (int i = gw * per + lane; i - lane < min(a.n, (gw + 1) * per); i += 32) {
     bool fresh = false;
@@ -324,17 +337,20 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
         const int ln = length(p), full = ln / bs, r = ln - full * bs;
         if (full >= M) {
           raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
-        } else if (r > 0 && __ldcg(first + p) == i) {
-          const int page = a.tables[static_cast<int64_t>(p) * M + full];
-          a.new_tables[static_cast<int64_t>(i) * M + full] = page;
-          if (page >= 0 && page < a.num_blocks) {
-            atomicAdd(a.new_ref + page, 1);
+        } else {
+          const bool mine = r > 0 && __ldcg(first + p) == i;
+          const int page = mine ? a.tables[static_cast<int64_t>(p) * M + full] : 0;
+          if (page < 0 || page >= a.num_blocks) {
+            a.new_tables[static_cast<int64_t>(i) * M + full] = page;
+          } else if (mine && __ldcg(a.new_ref + page) == i - a.n) {
+            a.new_tables[static_cast<int64_t>(i) * M + full] = page;
+            a.new_ref[page] = 1;
             a.slots[i] = static_cast<int64_t>(page) * bs + r;
             state = -2;                                // settled
+          } else {
+            fresh = true;
+            state = r;
           }
-        } else {
-          fresh = true;
-          state = r;
         }
       }
       rest[i] = state;

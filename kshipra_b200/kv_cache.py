@@ -23,6 +23,7 @@ given.
 from __future__ import annotations
 
 import functools
+import threading
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -57,6 +58,7 @@ class CacheWorkspace:
 
     def __init__(self):
         self.bufs: Dict[tuple, torch.Tensor] = {}
+        self.lock = threading.Lock()          # held over a call's launches: threads may share a stream
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
         idx = device.index
@@ -159,10 +161,11 @@ def cache_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_table
     elif _need(out, "out", torch.float32, 3, at).shape != q.shape:
         raise ValueError("out must have q's shape")
     dev = q.device
-    buf = ws.get(_workspace_bytes(S, hq, hkv, d, max_q_len), dev)
-    _run(dev, "ksh_cache_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), kind, nb, L, layer, hkv,
-         bs, block_tables.data_ptr(), max_blocks, q_start.data_ptr(), prefix_lens.data_ptr(), S,
-         max_q_len, max_total_len, out.data_ptr(), buf.data_ptr(), buf.numel(), _flags(flags, at))
+    with ws.lock:
+        buf = ws.get(_workspace_bytes(S, hq, hkv, d, max_q_len), dev)
+        _run(dev, "ksh_cache_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), kind, nb, L, layer,
+             hkv, bs, block_tables.data_ptr(), max_blocks, q_start.data_ptr(), prefix_lens.data_ptr(),
+             S, max_q_len, max_total_len, out.data_ptr(), buf.data_ptr(), buf.numel(), _flags(flags, at))
     return out
 
 
@@ -176,9 +179,9 @@ def fork_pages(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
     the old sequences, parents int32 [N] which of them each new one continues
     (negative: none), ref_counts int32 [nb] how many rows of all tables hold each
     page.  Whole pages are shared; the page that the next token goes to stays with
-    the parent's first child and is copied for the others (its filled rows, in
-    every layer of the pool, in place), and where a page begins each child gets a
-    free one: the lowest pages whose count is 0 once the old sequences gave up
+    the first child that continues in it, where no row but the old ones holds it,
+    and is copied for the others (its filled rows, in every layer of the pool, in
+    place), and where a page begins each child gets a free one: the lowest pages whose count is 0 once the old sequences gave up
     theirs.  With parents 0 .. S - 1 the call only grows the sequences, with
     negative ones it frees them.  Returns (block_tables [N, max_blocks], lens [N],
     slots int64 [N] of the next tokens, ref_counts [nb]); without a page left a slot is

@@ -13,6 +13,8 @@ products, a sum), and a stored value by half a step of its type beside that.
 Pages are exact.
 """
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -804,3 +806,80 @@ def test_empty_calls():
     assert kv.rope_cache_write(torch.empty(0, 512, device="cuda"), b.pool, 0, i64([]), i64([]), cos, sin).shape[0] == 0
     t, n, s, r = kv.fork_pages(b.pool, b.table, i32([23]), i32([]), i32([1] * b.pool.shape[0]))
     assert t.shape[0] == 0 and r.sum() == b.pool.shape[0] - 2
+
+
+def shared_fork_want(pool, table, lens, parents, refs):
+    """fork_want where rows may hold the same page while it fills: it stays with the
+    first child that continues in it if nobody else is left to hold it."""
+    pool, table, refs = pool.clone(), table.tolist(), refs.tolist()
+    b, m = pool.shape[4], len(table[0])
+    for row, ln in zip(table, lens):
+        for page in row[:-(-ln // b)]:
+            refs[page] -= 1
+    out = [[0] * m if p < 0 else table[p][:lens[p] // b] + [0] * (m - lens[p] // b) for p in parents]
+    for i, p in enumerate(parents):
+        for page in [] if p < 0 else table[p][:lens[p] // b]:
+            refs[page] += 1
+    last = [-1 if p < 0 or lens[p] // b >= m else lens[p] // b for p in parents]
+    kept = {}
+    for i, p in enumerate(parents):
+        if last[i] >= 0 and lens[p] % b and refs[table[p][last[i]]] == 0:
+            kept.setdefault(table[p][last[i]], i)
+    for page, i in kept.items():
+        refs[page], out[i][last[i]] = 1, page
+    free = iter([i for i, r in enumerate(refs) if r == 0])
+    for i, p in enumerate(parents):
+        if last[i] >= 0 and i not in kept.values():
+            page, rest = next(free), lens[p] % b
+            refs[page], out[i][last[i]] = 1, page
+            pool[page, :, :, :, :rest] = pool[table[p][last[i]], :, :, :, :rest]
+    slots = [-1 if last[i] < 0 else out[i][last[i]] * b + lens[p] % b for i, p in enumerate(parents)]
+    return out, [0 if p < 0 else lens[p] for p in parents], slots, refs, pool
+
+
+@pytest.mark.parametrize("lens,parents,outside", [
+    ([37, 37, 37, 37], [0, 1, 2, 3], 0), ([37, 37, 37, 37], [3, 1, 1, 0, 2], 0), ([37], [0], 1), ([37], [0, 0], 1),
+    ([37, 37], [1], 0), ([37, 48, 37], [1, 0, 2], 0), ([37, 48, 41], [0, 2], 0), ([37, 48], [-1, 0], 2), ([37, 35], [1, 0, 0], 0),
+], ids=lambda x: None)
+def test_fork_of_pages_that_several_rows_fill(lens, parents, outside):
+    """Rows of one prompt, repeated: no two children write into one page."""
+    row = [5, 9, 2, 0]
+    table = i32([row] * len(lens))
+    refs = [0] * 24
+    for ln in lens:
+        for page in row[:-(-ln // 16)]:
+            refs[page] += 1
+    refs[2] += outside
+    refs = i32(refs)
+    pool = torch.randn(24, 2, 2, 2, 16, 64, generator=torch.Generator("cuda").manual_seed(0), device="cuda").half()
+    want = shared_fork_want(pool, table, lens, parents, refs)
+    f = new_flags()
+    got = kv.fork_pages(pool, table, i32(lens), i32(parents), refs, flags=f)
+    assert int(f) == 0
+    for x, y in zip(got, want):
+        assert x.tolist() == y
+    assert torch.equal(pool, want[4])
+    slots = [s for s in got[2].tolist() if s >= 0]
+    assert len({s // 16 for s in slots}) == len(slots)
+
+
+def test_two_threads_on_one_stream():
+    """Each call's launches stay together: both use the stream's workspace."""
+    bs = [Batch([(5000 + 900 * i, 20), (77, 1)], 8, 2, 128, 16, F16, seed=i) for i in range(2)]
+    want = [b.run() for b in bs]
+    got, stream = [[], []], torch.cuda.current_stream()
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            for _ in range(60):
+                got[i].append(bs[i].run())
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 60 and all(torch.equal(x, want[i]) for x in got[i])
