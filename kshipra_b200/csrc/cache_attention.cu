@@ -55,6 +55,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cstring>
+#include <type_traits>
 
 #include "tc_common.cuh"
 
@@ -93,59 +95,162 @@ struct SplitItem {
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Any head dimension up to 256 and any alignment: one warp per (row, head), keys
-// one after the other.
-template <typename T>
-__global__ void __launch_bounds__(32) cache_attn_simple_kernel(CacheArgs a) {
-  const int lane = threadIdx.x, i = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
+// Any head dimension up to 256 and any alignment: a CTA per (row, head), whose warps
+// take 16 keys at a time each, four of them in flight, and join their states at the
+// end.  VEC: elements a load takes, four where dimension and pool allow; PER: elements a
+// lane has.  Bound by instructions and, with few rows, by a warp's trips to memory.  16 /
+// 4 heads, fp16: one sequence x 540 keys 23 us with D = 96, 32 with D = 256 (a warp for
+// all keys, one after the other: 525); 64 x 4096 keys 540 and 1180 (7000 and 7750), four
+// sequences' chunks of 128 behind 1000 655 and 1070.  With two elements a load 25, 57,
+// 510 and 3380, 740 and 2650; a group's heads side by side in the grid save nothing.
+constexpr int kAnyWarps = 8, kAnyRun = 16, kAnyKeys = 4, kAnyMax = 256;
+
+template <typename T, int VEC, int PER>
+__global__ void __launch_bounds__(kAnyWarps * 32) cache_attn_any_kernel(CacheArgs a) {
+  using Raw = std::conditional_t<VEC == 4, uint2, uint16_t>;
+  constexpr int kLoads = PER / VEC;
+  __shared__ float m_s[kAnyWarps], l_s[kAnyWarps], acc_s[kAnyWarps][kAnyMax];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.y;
+  const int64_t row = blockIdx.x;
   grid_dep_wait();
   grid_dep_launch();
-  const int64_t a0 = a.q_start[s], n = a.q_start[s + 1] - a0;
-  const int64_t pre = max(a.prefix[s], 0);
   const int64_t cap = a.max_blocks * a.bs;
-  if (lane == 0 && (a0 < 0 || n < 0 || a0 + n > a.total || n > a.max_q || a.prefix[s] < 0 || pre + n > cap))
-    raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
-  if (i >= n || a0 < 0 || a0 + i >= a.total) return;
-  const int d = a.d;
-  const int64_t end = min(pre + i + 1, cap);
-  const float* q = a.q + ((a0 + i) * a.hq + h) * d;
-  const int hk = h / a.g;
-  const T* pool = static_cast<const T*>(a.pool);
-  constexpr int kPer = 8;
-  float acc[kPer];
+  if (row == 0 && h == 0) {
+    for (int s = tid; s < a.num_seqs; s += kAnyWarps * 32) {
+      const int64_t a0 = a.q_start[s], n = a.q_start[s + 1] - a0;
+      if (a0 < 0 || n < 0 || a0 + n > a.total || n > a.max_q || a.prefix[s] < 0 || max(a.prefix[s], 0) + max(n, int64_t(0)) > cap)
+        raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
+    }
+  }
+  int s = 0, past = a.num_seqs;                   // the last sequence that starts at or before the row
+  while (past - s > 1) {
+    const int mid = s + (past - s) / 2;
+    if (a.q_start[mid] <= row)
+      s = mid;
+    else
+      past = mid;
+  }
+  const int64_t i = row - a.q_start[s];
+  if (i < 0 || i >= a.max_q || row >= a.q_start[s + 1]) return;
+  const int d = a.d, hk = h / a.g;
+  const int64_t end = min(static_cast<int64_t>(max(a.prefix[s], 0)) + i + 1, cap);
+  const int32_t* const table = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
+  const uint32_t bs = static_cast<uint32_t>(a.bs);
+  const float* const q = a.q + (row * a.hq + h) * d;
+  const T* const kpool = static_cast<const T*>(a.pool) + ((a.layer * 2) * a.hkv + hk) * a.bs * d + lane * VEC;
+  const int64_t page = a.num_layers * 2 * a.hkv * a.bs * d, to_v = a.hkv * a.bs * d;
+  float qv[PER], acc[PER];
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+  for (int e = 0; e < PER; ++e) {
+    const int c = (e / VEC * 32 + lane) * VEC + e % VEC;
+    qv[e] = c < d ? q[c] * a.scale : 0.0f;
+    acc[e] = 0.0f;
+  }
   float m = -INFINITY, l = 0.0f;
   bool bad = false;
-  for (int64_t pos = 0; pos < end; ++pos) {
-    const int64_t b = pos / a.bs;
-    const int64_t blk = a.block_tables[static_cast<int64_t>(s) * a.max_blocks + b];
-    if (blk < 0 || blk >= a.num_blocks) {
-      bad = true;
-      continue;
+  auto value = [](Raw r, int e) {
+    uint16_t b;
+    if constexpr (VEC == 4)
+      b = static_cast<uint16_t>((e % 4 < 2 ? r.x : r.y) >> (e % 2 * 16));
+    else
+      b = r;
+    T t;
+    memcpy(&t, &b, 2);
+    return widen(t);
+  };
+  for (int64_t p0 = warp * kAnyRun; p0 < end; p0 += kAnyWarps * kAnyRun) {
+    // a lane finds one key's place
+    int64_t mine = -1;
+    if (lane < kAnyRun && p0 + lane < end) {
+      const uint32_t pos = static_cast<uint32_t>(p0 + lane), b = pos / bs;   // below 2^32: two int32 lengths
+      const int64_t blk = table[b];
+      if (blk >= 0 && blk < a.num_blocks)
+        mine = blk * page + static_cast<int64_t>(pos - b * bs) * d;
+      else
+        bad = true;
     }
-    const T* k = pool + ((((blk * a.num_layers + a.layer) * 2) * a.hkv + hk) * a.bs + (pos - b * a.bs)) * d;
-    const T* v = k + a.hkv * a.bs * d;
-    float dot = 0.0f;
-    for (int c = lane; c < d; c += 32) dot = fmaf(q[c], widen(k[c]), dot);
-    const float x = warp_sum(dot) * a.scale;
-    const float mn = fmaxf(m, x), ms = mn == -INFINITY ? 0.0f : mn;
-    const float p = expf(x - ms), corr = expf(m - ms);
-    l = fmaf(l, corr, p);
+    const int run = static_cast<int>(min(end - p0, static_cast<int64_t>(kAnyRun)));
+#pragma unroll 1
+    for (int u0 = 0; u0 < run; u0 += kAnyKeys) {
+      Raw k[kAnyKeys][kLoads], v[kAnyKeys][kLoads];
+      bool on[kAnyKeys];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int c = lane + 32 * e;
-      if (c < d) acc[e] = fmaf(acc[e], corr, p * widen(v[c]));
+      for (int u = 0; u < kAnyKeys; ++u) {
+        const int64_t at = __shfl_sync(0xffffffffu, mine, u0 + u);
+        on[u] = at >= 0;
+#pragma unroll
+        for (int e = 0; e < kLoads; ++e) {
+          const bool there = on[u] && (e * 32 + lane) * VEC < d;
+          k[u][e] = there ? *reinterpret_cast<const Raw*>(kpool + at + e * 32 * VEC) : Raw{};
+          v[u][e] = there ? *reinterpret_cast<const Raw*>(kpool + at + to_v + e * 32 * VEC) : Raw{};
+        }
+      }
+      float x[kAnyKeys];
+#pragma unroll
+      for (int u = 0; u < kAnyKeys; ++u) {
+        x[u] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[u] = fmaf(qv[e], value(k[u][e / VEC], e), x[u]);
+      }
+      // four sums over the warp at once: a lane ends with that of key lane >> 3
+      float y = lane & 16 ? x[2] : x[0], z = lane & 16 ? x[3] : x[1];
+      y += __shfl_xor_sync(0xffffffffu, lane & 16 ? x[0] : x[2], 16);
+      z += __shfl_xor_sync(0xffffffffu, lane & 16 ? x[1] : x[3], 16);
+      const float w = __shfl_xor_sync(0xffffffffu, lane & 8 ? y : z, 8);
+      y = (lane & 8 ? z : y) + w;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < kAnyKeys; ++u) {
+        x[u] = __shfl_sync(0xffffffffu, y, 8 * u);
+        if (!on[u]) x[u] = -INFINITY;
+        top = fmaxf(top, x[u]);
+      }
+      const float ref = top == -INFINITY ? 0.0f : top;
+      if (top > m) {
+        const float corr = expf(m - ref);
+        m = top;
+        l *= corr;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] *= corr;
+      }
+#pragma unroll
+      for (int u = 0; u < kAnyKeys; ++u) {
+        const float p = expf(x[u] - ref);
+        l += p;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = fmaf(p, value(v[u][e / VEC], e), acc[e]);
+      }
     }
-    m = mn;
   }
-  if (bad && lane == 0) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
-  float* o = a.out + ((a0 + i) * a.hq + h) * d;
+  if (bad) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
+  if (lane == 0) m_s[warp] = m, l_s[warp] = l;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const int c = lane + 32 * e;
-    if (c < d) o[c] = l == 0.0f ? 0.0f : acc[e] / l;
+  for (int e = 0; e < PER; ++e) acc_s[warp][(e / VEC * 32 + lane) * VEC + e % VEC] = acc[e];
+  __syncthreads();
+  if (tid >= d) return;
+  float top = -INFINITY, sum = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kAnyWarps; ++w) top = fmaxf(top, m_s[w]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int w = 0; w < kAnyWarps; ++w) {
+    const float f = expf(m_s[w] - ref);
+    sum = fmaf(l_s[w], f, sum);
+    o = fmaf(acc_s[w][tid], f, o);
   }
+  a.out[(row * a.hq + h) * d + tid] = sum == 0.0f ? 0.0f : o / sum;
+}
+
+template <typename T>
+int launch_cache_any(const CacheArgs& a, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.total), static_cast<unsigned>(a.hq)), block(kAnyWarps * 32);
+  auto go = [&](auto kern) { return launch(kern, grid, block, 0, st, a); };
+  if (a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.pool) & 7) == 0)
+    return a.d <= 128 ? go(cache_attn_any_kernel<T, 4, 4>) : go(cache_attn_any_kernel<T, 4, 8>);
+  return a.d <= 128 ? go(cache_attn_any_kernel<T, 1, 4>) : go(cache_attn_any_kernel<T, 1, 8>);
 }
 
 // ---------------------------------------------------------------------------
@@ -1610,7 +1715,5 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
     return d == 64 ? launch_cache_tc<64, __nv_bfloat16>(a, grid, st) : launch_cache_tc<128, __nv_bfloat16>(a, grid, st);
   }
   if (hq > 65535 || num_seqs > 65535) return KSH_ERR_UNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>(std::min(max_q_len, total)), static_cast<unsigned>(hq), static_cast<unsigned>(num_seqs));
-  return pool_type == KSH_TYPE_F16 ? launch(cache_attn_simple_kernel<__half>, grid, dim3(32), 0, st, a)
-                                   : launch(cache_attn_simple_kernel<__nv_bfloat16>, grid, dim3(32), 0, st, a);
+  return pool_type == KSH_TYPE_F16 ? launch_cache_any<__half>(a, st) : launch_cache_any<__nv_bfloat16>(a, st);
 }

@@ -883,3 +883,26 @@ def test_two_threads_on_one_stream():
     torch.cuda.synchronize()
     for i in range(2):
         assert len(got[i]) == 60 and all(torch.equal(x, want[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("d,block", [(255, 7), (256, 16), (130, 16), (12, 1), (1, 3), (80, 24), (112, 10), (134, 64)])
+def test_attention_other_dimensions(d, block, dtype):
+    """Lengths around the warps' runs of 16 keys and the CTA's of 128, and long ones."""
+    b = Batch([(0, 1), (15, 1), (0, 18), (16, 1), (126, 4), (0, 0), (1500, 1), (700, 33), (31, 1)], 6, 2, d, block, dtype, layers=2,
+              seed=d, first_row=1, tail_rows=2)
+    out = torch.full_like(b.q, 7.0)
+    b.run(out=out)
+    assert (out[:1] == 7).all() and (out[-2:] == 7).all()
+    b.check(out)
+    assert torch.equal(b.run()[1:-2], out[1:-2])
+
+
+def test_attention_other_dimensions_many_sequences():
+    rs = np.random.RandomState(4)
+    b = Batch([(int(rs.randint(0, 90)), int(rs.choice([0, 1, 1, 1, 9]))) for _ in range(700)], 4, 2, 96, 16, F16)
+    b.check(b.run())
+    f = new_flags()
+    b.prefix[[3, 699]] = -1
+    b.run(flags=f)
+    assert int(f) == BAD_LENGTH
