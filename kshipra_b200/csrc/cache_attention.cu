@@ -1637,7 +1637,498 @@ int launch_cache_tc(CacheArgs& a, int grid, cudaStream_t st) {
   return launch_cache_tc<D, T, true>(a, map, grid, st);
 }
 
-int64_t items_bytes() { return (static_cast<int64_t>(num_sms()) * sizeof(SplitItem) + 255) / 256 * 256; }
+// ---------------------------------------------------------------------------
+// Few rows (decoding): up to 16 rows of q, all heads of a group, a sequence
+// ---------------------------------------------------------------------------
+// The tiles above do their products for 128 rows, however few there are.  Here a warp
+// works alone: 16 keys of a (sequence, kv head) a step, K and V by cp.async into its own
+// ring in shared memory, S = Q K^T and O = P V as 16 x 8 x 16 products (q's terms in
+// registers; S's accumulators are P's operand), each step's P V added in fp32.  No warp
+// waits for another.  The line of all items' steps is cut into equal shares, one per
+// warp, and cache_rows_merge_kernel joins the pieces in key order.
+
+constexpr int kFewRows = 16, kFewKeys = 16, kFewWarps = 8;
+constexpr int kFewShare = 4;             // steps that a share has at least
+template <int D>
+constexpr int kFewStages = 3 * 128 / D;
+template <int D>
+constexpr int kFewStage = kFewKeys * D * 2 * 2;                  // bytes of K and V
+template <int D>
+constexpr int64_t few_floats() { return 2 * kFewRows + static_cast<int64_t>(D) * kFewRows; }
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (Kind<T>::kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void load_8x8x4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// 16 bytes, zeros where there is nothing to copy.
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(CacheArgs a) {
+  constexpr int NST = kFewStages<D>, KS = D / 16, TERMS = Kind<T>::TERMS;
+  constexpr int CPR = D / 8, RPI = 32 / CPR;                      // 16-byte chunks of a row, rows an instruction copies
+  constexpr float kRefShift = Kind<T>::kBf16 ? 8.0f : -6.0f;
+  extern __shared__ __align__(128) uint8_t few_smem[];
+  __shared__ int64_t scan_s[kFewWarps];
+  __shared__ int start_s[kFewWarps][3];
+  __shared__ uint32_t there_s[kFewWarps][NST];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hkv = static_cast<int>(a.hkv), g = a.g;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  // ---- the line, and where the warps' shares start ----
+  const int64_t me = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;    // few shares: one an SM
+  int64_t v = 0, inc = 0, carry = 0, q = 0, r = 0, G = 1;
+  auto scan = [&](int b, bool flag) {
+    v = 0;
+    if (b + tid < a.num_seqs) {
+      const SeqWork w = seq_work(a, b + tid);
+      if (flag && blockIdx.x == 0 && w.bad) raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
+      if (w.nq > 0) v = static_cast<int64_t>(hkv) * ((w.pre + w.nq + kFewKeys - 1) / kFewKeys);
+    }
+    inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    __syncthreads();
+    if (lane == 31) scan_s[warp] = inc;
+    __syncthreads();
+    int64_t before = carry;
+#pragma unroll
+    for (int i = 0; i < kFewWarps; ++i) {
+      if (i < warp) before += scan_s[i];
+      carry += scan_s[i];
+    }
+    inc += before;
+  };
+  auto start_of = [&](int64_t i) { return i * q + min(i, r); };
+  auto find = [&](int b) {
+    if (v == 0) return;
+    const int64_t per = v / hkv;
+#pragma unroll 1
+    for (int w = 0; w < kFewWarps; ++w) {
+      const int64_t i = static_cast<int64_t>(w) * gridDim.x + blockIdx.x, at = start_of(i) - (inc - v);
+      if (i >= G || at < 0 || at >= v) continue;
+      start_s[w][0] = b + tid;
+      start_s[w][1] = static_cast<int>(at / per);
+      start_s[w][2] = static_cast<int>(at % per);
+    }
+  };
+  for (int b = 0; b < a.num_seqs; b += kFewWarps * 32) scan(b, true);
+  const int64_t U = carry;
+  G = max(min(static_cast<int64_t>(gridDim.x) * kFewWarps, U / kFewShare), int64_t(1));
+  q = U / G;
+  r = U - q * G;
+  if (a.num_seqs <= kFewWarps * 32) {
+    find(0);
+  } else {
+    carry = 0;
+    for (int b = 0; b < a.num_seqs; b += kFewWarps * 32) scan(b, false), find(b);
+  }
+  __syncthreads();
+  SplitItem cut = {};
+  cut.last = -1;
+  int64_t left = me < G ? start_of(me + 1) - start_of(me) : 0;     // steps still to be computed
+  if (left > 0) {
+    // ---- copies: the place that is copied next, and its table entries ----
+    const uint32_t bs = static_cast<uint32_t>(a.bs);
+    const uint32_t rows_per_block = static_cast<uint32_t>(a.num_layers * 2 * a.hkv * a.bs);
+    const int64_t to_v = a.hkv * a.bs * D;
+    const uint32_t ring = smem_u32(few_smem) + static_cast<uint32_t>(warp) * NST * kFewStage<D>;
+    const int chunk = lane % CPR, sub = lane / CPR;
+    int ls = start_s[warp][0], lhk = start_s[warp][1], lt = start_s[warp][2];
+    int64_t lleft = left;
+    int lkeys;
+    {
+      const SeqWork w = seq_work(a, ls);
+      lkeys = w.pre + w.nq;
+    }
+    int blk = -1;                                 // of key lane & 15: -1 behind the end
+    uint32_t rest = 0;
+    bool bad = false;
+    auto fetch = [&]() {
+      const int pos = lt * kFewKeys + (lane & 15);
+      blk = -1;
+      if (lleft > 0 && pos < lkeys) {
+        const uint32_t j = static_cast<uint32_t>(pos) / bs;
+        rest = static_cast<uint32_t>(pos) - j * bs;
+        blk = a.block_tables[static_cast<int64_t>(ls) * a.max_blocks + j];
+        if (blk < 0) blk = INT32_MAX;
+      }
+    };
+    auto issue = [&](int st) {
+      if (lleft > 0) {
+        const bool on = blk >= 0 && blk < a.num_blocks;
+        bad = bad || (blk >= 0 && !on);
+        const uint32_t row = on ? static_cast<uint32_t>(blk) * rows_per_block + rest +
+                                      static_cast<uint32_t>((a.layer * 2 * hkv + lhk) * a.bs)
+                                : 0xffffffffu;
+        const uint32_t there = __ballot_sync(0xffffffffu, on) & 0xffffu;
+        if (lane == 0) there_s[warp][st] = there;
+        const uint32_t kd = ring + static_cast<uint32_t>(st) * kFewStage<D>;
+#pragma unroll
+        for (int i = 0; i < kFewKeys / RPI; ++i) {
+          const int key = i * RPI + sub;
+          const uint32_t at = __shfl_sync(0xffffffffu, row, key);
+          const bool is = at != 0xffffffffu;
+          const T* src = static_cast<const T*>(a.pool) + (is ? static_cast<int64_t>(at) * D + chunk * 8 : 0);
+          const uint32_t dst = kd + static_cast<uint32_t>(key) * (D * 2) + (static_cast<uint32_t>(chunk ^ (key & 7)) << 4);
+          copy16_or_zero(dst, src, is);
+          copy16_or_zero(dst + kFewKeys * D * 2, is ? src + to_v : src, is);
+        }
+        --lleft;
+        if (++lt * kFewKeys >= lkeys) {
+          lt = 0;
+          if (++lhk == hkv) {
+            lhk = 0;
+            if (lleft > 0) {
+              SeqWork w;
+              do w = seq_work(a, ++ls);
+              while (w.nq == 0 && ls + 1 < a.num_seqs);
+              lkeys = w.pre + w.nq;
+            }
+          }
+        }
+        fetch();
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch();
+#pragma unroll 1
+    for (int i = 0; i < NST - 1; ++i) issue(i);
+
+    // ---- products ----
+    int s = start_s[warp][0], hk = start_s[warp][1], t = start_s[warp][2];
+    SeqWork w = seq_work(a, s);
+    int st = 0, rows = 0, steps = 0, t0 = 0, lim0 = -1, lim1 = -1;
+    const int r0 = lane >> 2, c0 = (lane & 3) * 2;                // rows r0 and r0 + 8, columns c0 and c0 + 1 of eight
+    uint32_t qa[TERMS][KS][4];
+    float acc[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, cq0 = 0.0f, cq1 = 0.0f;
+    auto row_at = [&](int R) -> int64_t {
+      const int node = R / g;
+      return ((w.a0 + node) * a.hq + static_cast<int64_t>(hk) * g + (R - node * g)) * D;
+    };
+    bool fresh = true;
+    for (; left > 0; --left) {
+      if (fresh) {                                // an item begins, or the share inside one
+        fresh = false;
+        rows = w.nq * g;
+        steps = (w.pre + w.nq + kFewKeys - 1) / kFewKeys;
+        t0 = t;
+        lim0 = r0 < rows ? w.pre + r0 / g : -1;
+        lim1 = r0 + 8 < rows ? w.pre + (r0 + 8) / g : -1;
+        float2 x[KS][4];
+        float top0 = 0.0f, top1 = 0.0f, s0 = 1.0f, s1 = 1.0f, i0 = 1.0f, i1 = 1.0f;
+        const float* const p0 = a.q + (r0 < rows ? row_at(r0) : 0) + c0;
+        const float* const p1 = a.q + (r0 + 8 < rows ? row_at(r0 + 8) : 0) + c0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const float2 zero = make_float2(0.f, 0.f);
+          x[k][0] = r0 < rows ? *reinterpret_cast<const float2*>(p0 + 16 * k) : zero;
+          x[k][1] = r0 + 8 < rows ? *reinterpret_cast<const float2*>(p1 + 16 * k) : zero;
+          x[k][2] = r0 < rows ? *reinterpret_cast<const float2*>(p0 + 16 * k + 8) : zero;
+          x[k][3] = r0 + 8 < rows ? *reinterpret_cast<const float2*>(p1 + 16 * k + 8) : zero;
+        }
+        if constexpr (!Kind<T>::kBf16) {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            top0 = amax3(amax3(top0, x[k][0].x, x[k][0].y), x[k][2].x, x[k][2].y);
+            top1 = amax3(amax3(top1, x[k][1].x, x[k][1].y), x[k][3].x, x[k][3].y);
+          }
+#pragma unroll
+          for (int o = 1; o <= 2; o <<= 1) {
+            top0 = amax3(top0, __shfl_xor_sync(0xffffffffu, top0, o), 0.0f);
+            top1 = amax3(top1, __shfl_xor_sync(0xffffffffu, top1, o), 0.0f);
+          }
+          pow2_scale(top0, &s0, &i0);
+          pow2_scale(top1, &s1, &i1);
+        }
+        cq0 = i0 * (a.scale * 1.44269504088896340736f);
+        cq1 = i1 * (a.scale * 1.44269504088896340736f);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float sc = e & 1 ? s1 : s0;
+            uint32_t low;
+            split<T>(mul2(f2(x[k][e].x, x[k][e].y), f2(sc, sc)), &qa[0][k][e], &qa[1][k][e], &low);
+            if constexpr (TERMS == 3) qa[2][k][e] = low;
+          }
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.0f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
+      __syncwarp();
+      issue(st == 0 ? NST - 1 : st - 1);          // the stage of the step before
+      const uint32_t kd = ring + static_cast<uint32_t>(st) * kFewStage<D>, vd = kd + kFewKeys * D * 2;
+      const uint32_t there = there_s[warp][st];
+      // S: a chain per term and eight keys
+      float sc[TERMS][2][4];
+#pragma unroll
+      for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[i][0][e] = sc[i][1][e] = 0.0f;
+      {
+        const int key = (lane >> 4) * 8 + (lane & 7), c = (lane >> 3) & 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t b[4];
+          load_8x8x4<false>(b, kd + static_cast<uint32_t>(key) * (D * 2) + (static_cast<uint32_t>((2 * k + c) ^ (key & 7)) << 4));
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) {
+            mma_16816<T>(sc[i][0], qa[i][k], b[0], b[1]);
+            mma_16816<T>(sc[i][1], qa[i][k], b[2], b[3]);
+          }
+        }
+      }
+      float x[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y = sc[1][n][e];
+          if constexpr (TERMS == 3) y += sc[2][n][e];
+          x[n][e] = sc[0][n][e] + y;
+        }
+      const bool some_hidden = (t + 1) * kFewKeys > w.pre + 1, special = some_hidden || there != 0xffffu;
+      if (special) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 8 * n + c0 + (e & 1);
+            const bool see = ((there >> k) & 1) && t * kFewKeys + k <= (e < 2 ? lim0 : lim1);
+            if (!see) x[n][e] = -INFINITY;
+          }
+      }
+      float mc0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+      float mc1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        mc0 = fmaxf(mc0, __shfl_xor_sync(0xffffffffu, mc0, o));
+        mc1 = fmaxf(mc1, __shfl_xor_sync(0xffffffffu, mc1, o));
+      }
+      mc0 *= cq0;
+      mc1 *= cq1;
+      // the reference follows the maximum once that is 2^8 above it
+      const bool up0 = mc0 > m0 + 8.0f, up1 = mc1 > m1 + 8.0f;
+      if (__any_sync(0xffffffffu, up0 || up1)) {
+        const float f0 = up0 ? ex2(m0 - mc0) : 1.0f, f1 = up1 ? ex2(m1 - mc1) : 1.0f;
+        if (up0) m0 = mc0;
+        if (up1) m1 = mc1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          acc[n][0] *= f0;
+          acc[n][1] *= f0;
+          acc[n][2] *= f1;
+          acc[n][3] *= f1;
+        }
+      }
+      const float ref0 = m0 == -INFINITY ? 0.0f : m0 + kRefShift, ref1 = m1 == -INFINITY ? 0.0f : m1 + kRefShift;
+      uint32_t pa[TERMS][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[n][e] = ex2(fmaf(x[n][e], e < 2 ? cq0 : cq1, -(e < 2 ? ref0 : ref1)));
+        l0 += x[n][0] + x[n][1];
+        l1 += x[n][2] + x[n][3];
+        uint32_t low0, low1;
+        split<T>(f2(x[n][0], x[n][1]), &pa[0][2 * n], &pa[1][2 * n], &low0);
+        split<T>(f2(x[n][2], x[n][3]), &pa[0][2 * n + 1], &pa[1][2 * n + 1], &low1);
+        if constexpr (TERMS == 3) pa[2][2 * n] = low0, pa[2][2 * n + 1] = low1;
+      }
+      // V that some row does not see and that is not finite must not meet that row's 0
+      bool rare = false;
+      if (some_hidden && w.nq > 1) {
+        uint32_t f = 0;
+        for (int i = lane; i < kFewKeys * CPR; i += 32) {
+          uint4 y;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w) : "r"(vd + 16 * i));
+          f |= not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w);
+        }
+        rare = __any_sync(0xffffffffu, f != 0);
+      }
+      if (!rare) {
+        const int key = ((lane >> 3) & 1) * 8 + (lane & 7), c = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < D / 8; n += 2) {
+          uint32_t b[4];
+          load_8x8x4<true>(b, vd + static_cast<uint32_t>(key) * (D * 2) + (static_cast<uint32_t>((n + c) ^ (key & 7)) << 4));
+          float o[2][4] = {};
+#pragma unroll
+          for (int i = TERMS - 1; i >= 0; --i) {   // the small terms first
+            mma_16816<T>(o[0], pa[i], b[0], b[1]);
+            mma_16816<T>(o[1], pa[i], b[2], b[3]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[n][e] += o[0][e];
+            acc[n + 1][e] += o[1][e];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kFewKeys; ++k) {
+          const int from = (lane & ~3) + (k % 8) / 2;
+          const float q0 = __shfl_sync(0xffffffffu, x[k / 8][k % 2], from), q1 = __shfl_sync(0xffffffffu, x[k / 8][2 + k % 2], from);
+          const int pos = t * kFewKeys + k;
+          const bool on = (there >> k) & 1;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            uint32_t y;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(y) : "r"(vd + k * (D * 2) + ((n ^ (k & 7)) << 4) + c0 * 2));
+            T e[2];
+            memcpy(e, &y, 4);
+            const float va = widen(e[0]), vb = widen(e[1]);
+            if (on && pos <= lim0) acc[n][0] = fmaf(q0, va, acc[n][0]), acc[n][1] = fmaf(q0, vb, acc[n][1]);
+            if (on && pos <= lim1) acc[n][2] = fmaf(q1, va, acc[n][2]), acc[n][3] = fmaf(q1, vb, acc[n][3]);
+          }
+        }
+      }
+      st = st + 1 == NST ? 0 : st + 1;
+      ++t;
+      if (t < steps && left > 1) continue;
+      // ---- the piece t0 .. t - 1 of the item is done ----
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+      }
+      if (t0 == 0 && t == steps) {
+        const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
+        float* const o0 = a.out + (r0 < rows ? row_at(r0) : 0) + c0;
+        float* const o1 = a.out + (r0 + 8 < rows ? row_at(r0 + 8) : 0) + c0;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          if (r0 < rows) *reinterpret_cast<float2*>(o0 + 8 * n) = make_float2(acc[n][0] * i0, acc[n][1] * i0);
+          if (r0 + 8 < rows) *reinterpret_cast<float2*>(o1 + 8 * n) = make_float2(acc[n][2] * i1, acc[n][3] * i1);
+        }
+      } else {
+        float* const part = a.part + (me * 2 + (t0 > 0 ? 0 : 1)) * few_floats<D>();
+        float* const o0 = part + 2 * kFewRows + r0 * D + c0;
+        if ((lane & 3) == 0) {
+          part[r0] = m0, part[r0 + 8] = m1;
+          part[kFewRows + r0] = l0, part[kFewRows + r0 + 8] = l1;
+        }
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          if (r0 < rows) *reinterpret_cast<float2*>(o0 + 8 * n) = make_float2(acc[n][0], acc[n][1]);
+          if (r0 + 8 < rows) *reinterpret_cast<float2*>(o0 + 8 * D + 8 * n) = make_float2(acc[n][2], acc[n][3]);
+        }
+        if (t0 == 0) {                            // the share's last piece: joined from here on
+          const int64_t x = start_of(me + 1) - 1 + (steps - t);     // the item's last step
+          cut.first = static_cast<int>(me);
+          cut.last = static_cast<int>(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
+          cut.row0 = static_cast<int>(w.a0);
+          cut.rows = rows;
+          cut.hk = hk;
+        }
+      }
+      fresh = true;
+      t = 0;
+      if (++hk == hkv) {
+        hk = 0;
+        if (left > 1) {
+          do w = seq_work(a, ++s);
+          while (w.nq == 0 && s + 1 < a.num_seqs);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (bad) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
+  }
+  if (lane == 0) a.items[me] = cut;
+}
+
+// Joins the pieces of an item cut between warps, in key order; a CTA an item.
+template <int D>
+__global__ void __launch_bounds__(D) cache_rows_merge_kernel(CacheArgs a) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const SplitItem it = a.items[blockIdx.x];
+  if (it.last < it.first) return;
+  constexpr int kPieces = 4;
+  for (int i = threadIdx.x; i < it.rows * (D / 4); i += D) {
+    const int row = i / (D / 4), c = i % (D / 4);
+    float M = -INFINITY, L = 0.0f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = it.first; p0 <= it.last; p0 += kPieces) {
+      float m[kPieces], l[kPieces];
+      float4 v[kPieces];
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int p = min(p0 + u, it.last);
+        const float* part = a.part + (static_cast<int64_t>(p) * 2 + (p == it.first ? 1 : 0)) * few_floats<D>();
+        m[u] = part[row];
+        l[u] = part[kFewRows + row];
+        v[u] = reinterpret_cast<const float4*>(part + 2 * kFewRows + row * D)[c];
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) top = fmaxf(top, m[u]);
+      const float ref = top == -INFINITY ? 0.0f : top, w0 = ex2(M - ref);
+      M = top;
+      L *= w0;
+      A = make_float4(A.x * w0, A.y * w0, A.z * w0, A.w * w0);
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        if (p0 + u > it.last) break;
+        const float w = ex2(m[u] - ref);
+        L = fmaf(l[u], w, L);
+        A = make_float4(fmaf(v[u].x, w, A.x), fmaf(v[u].y, w, A.y), fmaf(v[u].z, w, A.z), fmaf(v[u].w, w, A.w));
+      }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const int node = row / a.g;
+    float* out = a.out + ((static_cast<int64_t>(it.row0) + node) * a.hq + static_cast<int64_t>(it.hk) * a.g + (row - node * a.g)) * D;
+    reinterpret_cast<float4*>(out)[c] = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+  }
+}
+
+template <int D, typename T>
+int launch_cache_rows(const CacheArgs& a, int grid, cudaStream_t st) {
+  constexpr int kBytes = kFewWarps * kFewStages<D> * kFewStage<D>;
+  auto kern = cache_attn_rows_kernel<D, T>;
+  if (set_smem_optin(reinterpret_cast<const void*>(kern), kBytes) != KSH_OK) return KSH_ERR_CUDA;
+  const int rc = launch(kern, dim3(static_cast<unsigned>(grid)), dim3(kFewWarps * 32), kBytes, st, a);
+  if (rc != KSH_OK) return rc;
+  return launch(cache_rows_merge_kernel<D>, dim3(static_cast<unsigned>(grid * kFewWarps - 1)), dim3(D), 0, st, a);
+}
+
+static_assert(few_floats<64>() * kFewWarps == part_floats<64>() && few_floats<128>() * kFewWarps == part_floats<128>(), "workspace");
+
+int64_t items_bytes() { return (static_cast<int64_t>(num_sms()) * kFewWarps * sizeof(SplitItem) + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace ksh
@@ -1703,6 +2194,14 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
     a.items = static_cast<SplitItem*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + items_bytes());
     a.npt = kRows / a.g;
+    if (max_q_len * a.g <= kFewRows) {
+      const double shares = static_cast<double>(num_seqs) * static_cast<double>(hkv) *
+                            static_cast<double>(std::max<int64_t>(1, (max_total_len + kFewKeys * kFewShare - 1) / (kFewKeys * kFewShare)));
+      const int grid = static_cast<int>(std::min<double>(num_sms(), shares));
+      if (pool_type == KSH_TYPE_F16)
+        return d == 64 ? launch_cache_rows<64, __half>(a, grid, st) : launch_cache_rows<128, __half>(a, grid, st);
+      return d == 64 ? launch_cache_rows<64, __nv_bfloat16>(a, grid, st) : launch_cache_rows<128, __nv_bfloat16>(a, grid, st);
+    }
     // No more CTAs than there can be tiles; an item's start counts only where there
     // are several tiles a CTA.
     const double tiles = static_cast<double>(num_seqs) * static_cast<double>(hkv) *

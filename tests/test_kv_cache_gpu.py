@@ -906,3 +906,145 @@ def test_attention_other_dimensions_many_sequences():
     b.prefix[[3, 699]] = -1
     b.run(flags=f)
     assert int(f) == BAD_LENGTH
+
+
+# ---- few rows a sequence: a path of their own (rows = tokens x heads of a group up to 16) ----
+
+FEW = [[(0, 1)], [(540, 1)], [(15, 1), (16, 1), (31, 1), (0, 1), (63, 1), (64, 1), (65, 1)], [(4100, 1), (0, 1), (0, 0), (900, 1)],
+       [(3, 2), (0, 2), (500, 1), (2000, 2), (0, 0), (14, 2), (15, 2), (0, 0)], [(int(x), 1) for x in range(0, 1200, 9)],
+       [(20000, 1)], [(0, 0), (0, 0), (77, 1)]]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("d,heads,kv_heads,block", [(64, 14, 2, 16), (128, 32, 8, 16), (128, 8, 8, 10), (64, 8, 1, 64), (128, 3, 1, 1),
+                                                    (64, 5, 5, 7)])
+@pytest.mark.parametrize("lengths", range(len(FEW)))
+def test_few_rows(lengths, d, heads, kv_heads, block, dtype):
+    b = Batch(FEW[lengths], heads, kv_heads, d, block, dtype, layers=2, seed=lengths, first_row=1, tail_rows=2)
+    out = torch.full_like(b.q, 7.0)
+    f = new_flags()
+    b.run(out=out, flags=f)
+    assert int(f) == 0 and (out[:1] == 7).all() and (out[-2:] == 7).all()
+    b.check(out)
+    assert torch.equal(b.run()[1:-2], out[1:-2])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("d,heads,kv_heads,new", [(64, 16, 1, 1), (128, 32, 2, 1), (128, 4, 4, 16), (64, 4, 2, 8), (128, 12, 4, 5),
+                                                  (64, 9, 3, 5), (64, 17, 1, 1), (128, 6, 3, 9)])
+def test_few_rows_of_several_tokens(d, heads, kv_heads, new, dtype):
+    """Groups and chunks that fill the 16 rows, or pass them by one."""
+    rs = np.random.RandomState(new)
+    b = Batch([(int(rs.randint(0, 700)), int(rs.randint(1, new + 1))) for _ in range(30)] + [(3000, new), (0, new), (16, new)],
+              heads, kv_heads, d, 16, dtype, seed=new)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), float("-inf"), 6e4])
+def test_few_rows_pages_behind_the_end_hold_anything(d, dtype, junk):
+    b = Batch([(40, 1), (130, 2), (0, 3), (127, 1), (250, 4)], 4, 2, d, 24, dtype)
+    want = b.want()
+    for s, (p, n) in enumerate(zip(b.pre, b.new)):
+        end = p + n
+        page = int(b.table[s, (end - 1) // 24])
+        b.pool[page, :, :, :, (end - 1) % 24 + 1:] = junk
+    b.pool[b.unused] = junk
+    b.check(b.run(), want)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, F16), (64, BF16), (128, BF16)])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), float("-inf")])
+def test_few_rows_later_tokens_do_not_reach_earlier_ones(d, dtype, where, junk):
+    """What the last token of each chunk brings is seen by its own row alone."""
+    b = Batch([(100, 5), (3, 8), (0, 2), (14, 3)], 4, 2, d, 16, dtype)
+    want = b.want()
+    last = torch.zeros(b.total, dtype=torch.bool, device="cuda")
+    for s, (p, n) in enumerate(zip(b.pre, b.new)):
+        end = p + n - 1
+        b.pool[int(b.table[s, end // 16]), 0, 0 if where == "k" else 1, :, end % 16, 3] = junk
+        last[int(b.qs[s]) + n - 1] = True
+    got = b.run()
+    want[last] = float("nan")
+    diff = (got.double() - want)[~last]
+    assert torch.isfinite(got[~last]).all()
+    assert float(diff.norm()) <= 1e-5 * float(want[~last].norm())
+    if where == "v":
+        assert not torch.isfinite(got[last][..., 3]).any() and torch.isfinite(got[last][..., :3]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+def test_few_rows_missing_pages_and_bad_lengths(d, dtype):
+    b = Batch([(100, 3), (50, 1), (10, 2)], 4, 2, d, 16, dtype)
+    want = b.want()
+    good, b.table = b.table, b.table.clone()
+    b.table[0, 2] = 10 ** 6
+    b.table[1] = -1
+    f = new_flags()
+    got = b.run(flags=f)
+    b.table = good
+    assert int(f) == BAD_BLOCK and (got[3] == 0).all()
+    on = torch.ones(103, dtype=torch.bool, device="cuda")
+    on[32:48] = False
+    k, v = b.seq(0).repeat_interleave(b.g, 1)[:, :, on]
+    x = torch.einsum("nhd,hkd->hnk", b.q[:3].double(), k) / d ** 0.5
+    hide = torch.ones(3, 87, dtype=torch.bool, device="cuda").triu(85)
+    want[:3] = torch.einsum("hnk,hkd->nhd", torch.softmax(x.masked_fill(hide, float("-inf")), -1), v)
+    want[3] = 0
+    b.check(got, want)
+    for bad in (10 ** 6, -4):
+        b.prefix[1] = bad
+        f.zero_()
+        b.run(flags=f)
+        assert int(f) == BAD_LENGTH
+    b.prefix[1] = 50
+    b.max_q = 2                                              # rows past the bound stay
+    f.zero_()
+    out = torch.full_like(b.q, 7.0)
+    b.run(flags=f, out=out)
+    assert int(f) == BAD_LENGTH and (out[2] == 7).all()
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, F16), (128, BF16)])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-6, 1e3])
+def test_few_rows_q_scales(d, dtype, scale):
+    b = Batch([(70, 1), (1300, 1)], 4, 2, d, 16, dtype, q_scale=scale)
+    if scale > 1:
+        b.pool[:, :, 0] = (b.pool[:, :, 0].float() * (2.0 / scale)).to(dtype)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+def test_few_rows_many_sequences(d, dtype):
+    rs = np.random.RandomState(3)
+    b = Batch([(int(rs.randint(0, 90)), int(rs.choice([0, 1, 1, 1, 4]))) for _ in range(1300)], 8, 2, d, 16, dtype)
+    b.check(b.run())
+
+
+def test_few_rows_loose_bounds_and_captured():
+    b = Batch([(4000, 1), (90, 1), (300, 1)], 8, 2, 128, 16, F16)
+    b.check(b.run())
+    for b.max_total in (0, 1, 2 ** 40):
+        b.check(b.run())
+    b.max_total = 4001
+    out = torch.empty_like(b.q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b.run(out=out)
+    for p in ([17, 90, 299], [4000, 0, 5]):
+        b.pre = p
+        b.prefix.copy_(i32(p))
+        out.zero_()
+        g.replay()
+        b.check(out)
+
+
+def test_few_rows_offsets_past_32_bits():
+    b = Batch([(300, 1), (77, 2)], 8, 8, 128, 16, F16)
+    nb = (1 << 31) // (2 * 8 * 16 * 128) + 600
+    pool = torch.empty((nb, 1, 2, 8, 16, 128), dtype=F16, device="cuda")
+    n = b.pool.shape[0]
+    pool[nb - n:] = b.pool
+    b.check(kv.cache_attention(b.q, pool, 0, b.table + (nb - n), b.q_start, b.prefix, 2, 301), b.want())
