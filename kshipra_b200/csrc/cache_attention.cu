@@ -1642,10 +1642,10 @@ int launch_cache_tc(CacheArgs& a, int grid, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // The tiles above do their products for 128 rows, however few there are.  Here a warp
 // works alone: 16 keys of a (sequence, kv head) a step, K and V by cp.async into its own
-// ring in shared memory, S = Q K^T and O = P V as 16 x 8 x 16 products (q's terms in
-// registers; S's accumulators are P's operand), each step's P V added in fp32.  No warp
-// waits for another.  The line of all items' steps is cut into equal shares, one per
-// warp, and cache_rows_merge_kernel joins the pieces in key order.
+// ring in shared memory, S^T = K Q^T and O^T = V^T P^T as 16 x 8 x 16 products of eight
+// rows (q's terms in registers, P's transposed by movmatrix), each step's P V added in
+// fp32.  No warp waits for another.  The line of all items' steps is cut into equal
+// shares, one per warp, and cache_rows_merge_kernel joins the pieces in key order.
 
 constexpr int kFewRows = 16, kFewKeys = 16, kFewWarps = 8;
 constexpr int kFewShare = 4;             // steps that a share has at least
@@ -1680,12 +1680,18 @@ __device__ __forceinline__ void load_8x8x4(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 // 16 bytes, zeros where there is nothing to copy.
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-template <int D, typename T>
+// NT: eights of rows.
+template <int D, typename T, int NT>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(CacheArgs a) {
   constexpr int NST = kFewStages<D>, KS = D / 16, TERMS = Kind<T>::TERMS;
   constexpr int CPR = D / 8, RPI = 32 / CPR;                      // 16-byte chunks of a row, rows an instruction copies
@@ -1825,10 +1831,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
     // ---- products ----
     int s = start_s[warp][0], hk = start_s[warp][1], t = start_s[warp][2];
     SeqWork w = seq_work(a, s);
-    int st = 0, rows = 0, steps = 0, t0 = 0, lim0 = -1, lim1 = -1;
-    const int r0 = lane >> 2, c0 = (lane & 3) * 2;                // rows r0 and r0 + 8, columns c0 and c0 + 1 of eight
-    uint32_t qa[TERMS][KS][4];
-    float acc[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, cq0 = 0.0f, cq1 = 0.0f;
+    int st = 0, rows = 0, steps = 0, t0 = 0;
+    // a lane's place in a product: row of eight, and columns c0 and c0 + 1 of eight
+    const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+    constexpr int PAR = 2 / NT;                   // chains of a term's sums
+    uint32_t qb[TERMS][KS][NT][2];
+    float acc[D / 16][NT][4], m[NT][2], l[NT][2], cq[NT][2];     // (d, rows), by columns: rows 8 n + c0, 8 n + c0 + 1
+    int lim[NT][2];
     auto row_at = [&](int R) -> int64_t {
       const int node = R / g;
       return ((w.a0 + node) * a.hq + static_cast<int64_t>(hk) * g + (R - node * g)) * D;
@@ -1840,133 +1849,134 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
         rows = w.nq * g;
         steps = (w.pre + w.nq + kFewKeys - 1) / kFewKeys;
         t0 = t;
-        lim0 = r0 < rows ? w.pre + r0 / g : -1;
-        lim1 = r0 + 8 < rows ? w.pre + (r0 + 8) / g : -1;
-        float2 x[KS][4];
-        float top0 = 0.0f, top1 = 0.0f, s0 = 1.0f, s1 = 1.0f, i0 = 1.0f, i1 = 1.0f;
-        const float* const p0 = a.q + (r0 < rows ? row_at(r0) : 0) + c0;
-        const float* const p1 = a.q + (r0 + 8 < rows ? row_at(r0 + 8) : 0) + c0;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const float2 zero = make_float2(0.f, 0.f);
-          x[k][0] = r0 < rows ? *reinterpret_cast<const float2*>(p0 + 16 * k) : zero;
-          x[k][1] = r0 + 8 < rows ? *reinterpret_cast<const float2*>(p1 + 16 * k) : zero;
-          x[k][2] = r0 < rows ? *reinterpret_cast<const float2*>(p0 + 16 * k + 8) : zero;
-          x[k][3] = r0 + 8 < rows ? *reinterpret_cast<const float2*>(p1 + 16 * k + 8) : zero;
+        for (int n = 0; n < NT; ++n) {
+          const int R = 8 * n + r0;
+          float2 x[KS][2];
+          const float* const p = a.q + (R < rows ? row_at(R) : 0) + c0;
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              x[k][e] = R < rows ? *reinterpret_cast<const float2*>(p + 16 * k + 8 * e) : make_float2(0.f, 0.f);
+          float sc = 1.0f, inv = 1.0f;
+          if constexpr (!Kind<T>::kBf16) {
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) top = amax3(amax3(top, x[k][0].x, x[k][0].y), x[k][1].x, x[k][1].y);
+#pragma unroll
+            for (int o = 1; o <= 2; o <<= 1) top = amax3(top, __shfl_xor_sync(0xffffffffu, top, o), 0.0f);
+            pow2_scale(top, &sc, &inv);
+          }
+          inv *= a.scale * 1.44269504088896340736f;                // to powers of two
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t low;
+              split<T>(mul2(f2(x[k][e].x, x[k][e].y), f2(sc, sc)), &qb[0][k][n][e], &qb[1][k][n][e], &low);
+              if constexpr (TERMS == 3) qb[2][k][n][e] = low;
+            }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            cq[n][j] = __shfl_sync(0xffffffffu, inv, (c0 + j) * 4);
+            lim[n][j] = 8 * n + c0 + j < rows ? w.pre + (8 * n + c0 + j) / g : -1;    // the last key that the row sees
+            m[n][j] = -INFINITY;
+            l[n][j] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
         }
-        if constexpr (!Kind<T>::kBf16) {
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            top0 = amax3(amax3(top0, x[k][0].x, x[k][0].y), x[k][2].x, x[k][2].y);
-            top1 = amax3(amax3(top1, x[k][1].x, x[k][1].y), x[k][3].x, x[k][3].y);
-          }
-#pragma unroll
-          for (int o = 1; o <= 2; o <<= 1) {
-            top0 = amax3(top0, __shfl_xor_sync(0xffffffffu, top0, o), 0.0f);
-            top1 = amax3(top1, __shfl_xor_sync(0xffffffffu, top1, o), 0.0f);
-          }
-          pow2_scale(top0, &s0, &i0);
-          pow2_scale(top1, &s1, &i1);
-        }
-        cq0 = i0 * (a.scale * 1.44269504088896340736f);
-        cq1 = i1 * (a.scale * 1.44269504088896340736f);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float sc = e & 1 ? s1 : s0;
-            uint32_t low;
-            split<T>(mul2(f2(x[k][e].x, x[k][e].y), f2(sc, sc)), &qa[0][k][e], &qa[1][k][e], &low);
-            if constexpr (TERMS == 3) qa[2][k][e] = low;
-          }
-        m0 = m1 = -INFINITY;
-        l0 = l1 = 0.0f;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
       }
       asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
       __syncwarp();
       issue(st == 0 ? NST - 1 : st - 1);          // the stage of the step before
       const uint32_t kd = ring + static_cast<uint32_t>(st) * kFewStage<D>, vd = kd + kFewKeys * D * 2;
       const uint32_t there = there_s[warp][st];
-      // S: a chain per term and eight keys
-      float sc[TERMS][2][4];
+      const int octet = lane >> 3, in8 = lane & 7;
+      float sc[TERMS][PAR][NT][4];
 #pragma unroll
-      for (int i = 0; i < TERMS; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[i][0][e] = sc[i][1][e] = 0.0f;
+      for (int i = 0; i < TERMS * PAR * NT * 4; ++i) (&sc[0][0][0][0])[i] = 0.0f;
       {
-        const int key = (lane >> 4) * 8 + (lane & 7), c = (lane >> 3) & 1;
+        const uint32_t at = kd + static_cast<uint32_t>((octet & 1) * 8 + in8) * (D * 2);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          uint32_t b[4];
-          load_8x8x4<false>(b, kd + static_cast<uint32_t>(key) * (D * 2) + (static_cast<uint32_t>((2 * k + c) ^ (key & 7)) << 4));
+          uint32_t ka[4];
+          load_8x8x4<false>(ka, at + (static_cast<uint32_t>((2 * k + (octet >> 1)) ^ in8) << 4));
 #pragma unroll
-          for (int i = 0; i < TERMS; ++i) {
-            mma_16816<T>(sc[i][0], qa[i][k], b[0], b[1]);
-            mma_16816<T>(sc[i][1], qa[i][k], b[2], b[3]);
-          }
+          for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<T>(sc[i][k % PAR][n], ka, qb[i][k][n][0], qb[i][k][n][1]);
         }
       }
-      float x[2][4];
+      const bool some_hidden = (t + 1) * kFewKeys > w.pre + 1, special = some_hidden || there != 0xffffu;
+      float x[NT][4];                             // keys r0 (+ 8 from element 2 on) of 16, rows 8 n + c0 (+ 1)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float y = sc[1][n][e];
-          if constexpr (TERMS == 3) y += sc[2][n][e];
-          x[n][e] = sc[0][n][e] + y;
+          float y[TERMS];
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) y[i] = PAR == 2 ? sc[i][0][n][e] + sc[i][PAR - 1][n][e] : sc[i][0][n][e];
+          if constexpr (TERMS == 3) y[1] += y[2];
+          x[n][e] = y[0] + y[1];
         }
-      const bool some_hidden = (t + 1) * kFewKeys > w.pre + 1, special = some_hidden || there != 0xffffu;
       if (special) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int k = 8 * n + c0 + (e & 1);
-            const bool see = ((there >> k) & 1) && t * kFewKeys + k <= (e < 2 ? lim0 : lim1);
-            if (!see) x[n][e] = -INFINITY;
+            const int k = r0 + (e >> 1) * 8;
+            if (!((there >> k) & 1) || t * kFewKeys + k > lim[n][e & 1]) x[n][e] = -INFINITY;
           }
       }
-      float mc0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-      float mc1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
-#pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        mc0 = fmaxf(mc0, __shfl_xor_sync(0xffffffffu, mc0, o));
-        mc1 = fmaxf(mc1, __shfl_xor_sync(0xffffffffu, mc1, o));
-      }
-      mc0 *= cq0;
-      mc1 *= cq1;
       // the reference follows the maximum once that is 2^8 above it
-      const bool up0 = mc0 > m0 + 8.0f, up1 = mc1 > m1 + 8.0f;
-      if (__any_sync(0xffffffffu, up0 || up1)) {
-        const float f0 = up0 ? ex2(m0 - mc0) : 1.0f, f1 = up1 ? ex2(m1 - mc1) : 1.0f;
-        if (up0) m0 = mc0;
-        if (up1) m1 = mc1;
-        l0 *= f0;
-        l1 *= f1;
+      bool up = false;
+      float mc[NT][2];
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          acc[n][0] *= f0;
-          acc[n][1] *= f0;
-          acc[n][2] *= f1;
-          acc[n][3] *= f1;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = fmaxf(x[n][j], x[n][2 + j]);
+#pragma unroll
+          for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          mc[n][j] = top * cq[n][j];
+          up = up || mc[n][j] > m[n][j] + 8.0f;
         }
+      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (!(mc[n][j] > m[n][j] + 8.0f)) continue;
+            const float f = ex2(m[n][j] - mc[n][j]);
+            m[n][j] = mc[n][j];
+            l[n][j] *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              acc[i][n][j] *= f;
+              acc[i][n][2 + j] *= f;
+            }
+          }
       }
-      const float ref0 = m0 == -INFINITY ? 0.0f : m0 + kRefShift, ref1 = m1 == -INFINITY ? 0.0f : m1 + kRefShift;
-      uint32_t pa[TERMS][4];
+      uint32_t pb[TERMS][NT][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < NT; ++n) {
+        const float ra = m[n][0] == -INFINITY ? 0.0f : m[n][0] + kRefShift, rb = m[n][1] == -INFINITY ? 0.0f : m[n][1] + kRefShift;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] = ex2(fmaf(x[n][e], e < 2 ? cq0 : cq1, -(e < 2 ? ref0 : ref1)));
-        l0 += x[n][0] + x[n][1];
-        l1 += x[n][2] + x[n][3];
-        uint32_t low0, low1;
-        split<T>(f2(x[n][0], x[n][1]), &pa[0][2 * n], &pa[1][2 * n], &low0);
-        split<T>(f2(x[n][2], x[n][3]), &pa[0][2 * n + 1], &pa[1][2 * n + 1], &low1);
-        if constexpr (TERMS == 3) pa[2][2 * n] = low0, pa[2][2 * n + 1] = low1;
+        for (int e = 0; e < 4; ++e) x[n][e] = ex2(fmaf(x[n][e], cq[n][e & 1], e & 1 ? -rb : -ra));
+        l[n][0] += x[n][0] + x[n][2];
+        l[n][1] += x[n][1] + x[n][3];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hi, lo, low;
+          split<T>(f2(x[n][2 * h], x[n][2 * h + 1]), &hi, &lo, &low);
+          pb[0][n][h] = transpose_8x8(hi);
+          pb[1][n][h] = transpose_8x8(lo);
+          if constexpr (TERMS == 3) pb[2][n][h] = transpose_8x8(low);
+        }
       }
       // V that some row does not see and that is not finite must not meet that row's 0
       bool rare = false;
@@ -1980,80 +1990,76 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
         rare = __any_sync(0xffffffffu, f != 0);
       }
       if (!rare) {
-        const int key = ((lane >> 3) & 1) * 8 + (lane & 7), c = lane >> 4;
+        const uint32_t at = vd + static_cast<uint32_t>((octet >> 1) * 8 + in8) * (D * 2);
 #pragma unroll
-        for (int n = 0; n < D / 8; n += 2) {
-          uint32_t b[4];
-          load_8x8x4<true>(b, vd + static_cast<uint32_t>(key) * (D * 2) + (static_cast<uint32_t>((n + c) ^ (key & 7)) << 4));
-          float o[2][4] = {};
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t va[4];
+          load_8x8x4<true>(va, at + (static_cast<uint32_t>((2 * i + (octet & 1)) ^ in8) << 4));
 #pragma unroll
-          for (int i = TERMS - 1; i >= 0; --i) {   // the small terms first
-            mma_16816<T>(o[0], pa[i], b[0], b[1]);
-            mma_16816<T>(o[1], pa[i], b[2], b[3]);
-          }
+          for (int n = 0; n < NT; ++n) {
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            acc[n][e] += o[0][e];
-            acc[n + 1][e] += o[1][e];
+            for (int k = TERMS - 1; k >= 0; --k) mma_16816<T>(o, va, pb[k][n][0], pb[k][n][1]);   // the small terms first
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][n][e] += o[e];
           }
         }
       } else {
 #pragma unroll
         for (int k = 0; k < kFewKeys; ++k) {
-          const int from = (lane & ~3) + (k % 8) / 2;
-          const float q0 = __shfl_sync(0xffffffffu, x[k / 8][k % 2], from), q1 = __shfl_sync(0xffffffffu, x[k / 8][2 + k % 2], from);
           const int pos = t * kFewKeys + k;
           const bool on = (there >> k) & 1;
+          float pr[NT][2];
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            uint32_t y;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(y) : "r"(vd + k * (D * 2) + ((n ^ (k & 7)) << 4) + c0 * 2));
-            T e[2];
-            memcpy(e, &y, 4);
-            const float va = widen(e[0]), vb = widen(e[1]);
-            if (on && pos <= lim0) acc[n][0] = fmaf(q0, va, acc[n][0]), acc[n][1] = fmaf(q0, vb, acc[n][1]);
-            if (on && pos <= lim1) acc[n][2] = fmaf(q1, va, acc[n][2]), acc[n][3] = fmaf(q1, vb, acc[n][3]);
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) pr[n][j] = __shfl_sync(0xffffffffu, x[n][k / 8 * 2 + j], k % 8 * 4 + (lane & 3));
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint16_t b;
+              asm volatile("ld.shared.u16 %0, [%1];"
+                           : "=h"(b)
+                           : "r"(vd + k * (D * 2) + (((2 * i + (e >> 1)) ^ (k & 7)) << 4) + r0 * 2));
+              T y;
+              memcpy(&y, &b, 2);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                if (on && pos <= lim[n][e & 1]) acc[i][n][e] = fmaf(pr[n][e & 1], widen(y), acc[i][n][e]);
+            }
         }
       }
       st = st + 1 == NST ? 0 : st + 1;
       ++t;
       if (t < steps && left > 1) continue;
       // ---- the piece t0 .. t - 1 of the item is done ----
+      const bool whole = t0 == 0 && t == steps;
+      float* const part = a.part + (me * 2 + (t0 > 0 ? 0 : 1)) * few_floats<D>();
 #pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-      }
-      if (t0 == 0 && t == steps) {
-        const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
-        float* const o0 = a.out + (r0 < rows ? row_at(r0) : 0) + c0;
-        float* const o1 = a.out + (r0 + 8 < rows ? row_at(r0 + 8) : 0) + c0;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          if (r0 < rows) *reinterpret_cast<float2*>(o0 + 8 * n) = make_float2(acc[n][0] * i0, acc[n][1] * i0);
-          if (r0 + 8 < rows) *reinterpret_cast<float2*>(o1 + 8 * n) = make_float2(acc[n][2] * i1, acc[n][3] * i1);
-        }
-      } else {
-        float* const part = a.part + (me * 2 + (t0 > 0 ? 0 : 1)) * few_floats<D>();
-        float* const o0 = part + 2 * kFewRows + r0 * D + c0;
-        if ((lane & 3) == 0) {
-          part[r0] = m0, part[r0 + 8] = m1;
-          part[kFewRows + r0] = l0, part[kFewRows + r0 + 8] = l1;
-        }
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          if (r0 < rows) *reinterpret_cast<float2*>(o0 + 8 * n) = make_float2(acc[n][0], acc[n][1]);
-          if (r0 + 8 < rows) *reinterpret_cast<float2*>(o0 + 8 * D + 8 * n) = make_float2(acc[n][2], acc[n][3]);
+          for (int o = 4; o <= 16; o <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], o);
+          const int R = 8 * n + c0 + j;
+          if (R >= rows) continue;
+          const float inv = !whole ? 1.0f : l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j];
+          float* const to = (whole ? a.out + row_at(R) : part + 2 * kFewRows + R * D) + r0;
+          if (!whole && r0 == 0) part[R] = m[n][j], part[kFewRows + R] = l[n][j];
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            to[16 * i] = acc[i][n][j] * inv;
+            to[16 * i + 8] = acc[i][n][2 + j] * inv;
+          }
         }
-        if (t0 == 0) {                            // the share's last piece: joined from here on
-          const int64_t x = start_of(me + 1) - 1 + (steps - t);     // the item's last step
-          cut.first = static_cast<int>(me);
-          cut.last = static_cast<int>(x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q);
-          cut.row0 = static_cast<int>(w.a0);
-          cut.rows = rows;
-          cut.hk = hk;
-        }
+      if (!whole && t0 == 0) {                    // the share's last piece: joined from here on
+        const int64_t at = start_of(me + 1) - 1 + (steps - t);     // the item's last step
+        cut.first = static_cast<int>(me);
+        cut.last = static_cast<int>(at < r * (q + 1) ? at / (q + 1) : r + (at - r * (q + 1)) / q);
+        cut.row0 = static_cast<int>(w.a0);
+        cut.rows = rows;
+        cut.hk = hk;
       }
       fresh = true;
       t = 0;
@@ -2071,42 +2077,65 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
   if (lane == 0) a.items[me] = cut;
 }
 
-// Joins the pieces of an item cut between warps, in key order; a CTA an item.
+// Joins the pieces of an item cut between warps, in key order: a CTA an item, its
+// threads in groups that take runs of the pieces (one long sequence has over a hundred).
+constexpr int kJoinThreads = 256;
+
 template <int D>
-__global__ void __launch_bounds__(D) cache_rows_merge_kernel(CacheArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) cache_rows_merge_kernel(CacheArgs a) {
+  __shared__ float m_s[kJoinThreads], l_s[kJoinThreads];
+  __shared__ float4 a_s[kJoinThreads];
   grid_dep_wait();
   grid_dep_launch();
   const SplitItem it = a.items[blockIdx.x];
   if (it.last < it.first) return;
   constexpr int kPieces = 4;
-  for (int i = threadIdx.x; i < it.rows * (D / 4); i += D) {
+  const int units = it.rows * (D / 4), groups = max(1, kJoinThreads / units), tid = threadIdx.x;
+  const int all = it.last - it.first + 1, per = (all + groups - 1) / groups, grp = tid / units;
+  for (int i = groups > 1 ? tid % units : tid; i < units; i += kJoinThreads) {    // (one trip where there are groups)
     const int row = i / (D / 4), c = i % (D / 4);
+    const int from = groups > 1 ? it.first + grp * per : it.first;
+    const int to = groups > 1 ? (grp < groups ? min(it.last, from + per - 1) : from - 1) : it.last;
     float M = -INFINITY, L = 0.0f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = it.first; p0 <= it.last; p0 += kPieces) {
-      float m[kPieces], l[kPieces];
-      float4 v[kPieces];
-#pragma unroll
-      for (int u = 0; u < kPieces; ++u) {
-        const int p = min(p0 + u, it.last);
-        const float* part = a.part + (static_cast<int64_t>(p) * 2 + (p == it.first ? 1 : 0)) * few_floats<D>();
-        m[u] = part[row];
-        l[u] = part[kFewRows + row];
-        v[u] = reinterpret_cast<const float4*>(part + 2 * kFewRows + row * D)[c];
-      }
+    auto add = [&](const float* m, const float* l, const float4* v, int n) {
       float top = M;
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) top = fmaxf(top, m[u]);
+      for (int u = 0; u < kPieces; ++u)
+        if (u < n) top = fmaxf(top, m[u]);
       const float ref = top == -INFINITY ? 0.0f : top, w0 = ex2(M - ref);
       M = top;
       L *= w0;
       A = make_float4(A.x * w0, A.y * w0, A.z * w0, A.w * w0);
 #pragma unroll
       for (int u = 0; u < kPieces; ++u) {
-        if (p0 + u > it.last) break;
+        if (u >= n) break;
         const float w = ex2(m[u] - ref);
         L = fmaf(l[u], w, L);
         A = make_float4(fmaf(v[u].x, w, A.x), fmaf(v[u].y, w, A.y), fmaf(v[u].z, w, A.z), fmaf(v[u].w, w, A.w));
+      }
+    };
+    for (int p0 = from; p0 <= to; p0 += kPieces) {
+      float m[kPieces], l[kPieces];
+      float4 v[kPieces];
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        if (p0 + u > to) break;
+        const float* part = a.part + (static_cast<int64_t>(p0 + u) * 2 + (p0 + u == it.first ? 1 : 0)) * few_floats<D>();
+        m[u] = part[row];
+        l[u] = part[kFewRows + row];
+        v[u] = reinterpret_cast<const float4*>(part + 2 * kFewRows + row * D)[c];
+      }
+      add(m, l, v, to - p0 + 1);
+    }
+    if (groups > 1) {
+      m_s[tid] = M, l_s[tid] = L, a_s[tid] = A;
+      __syncthreads();
+      if (grp > 0) return;
+      for (int k = 1; k < groups; ++k) {
+        const float m[kPieces] = {m_s[k * units + i]}, l[kPieces] = {l_s[k * units + i]};
+        const float4 v[kPieces] = {a_s[k * units + i]};
+        add(m, l, v, 1);
       }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -2119,11 +2148,13 @@ __global__ void __launch_bounds__(D) cache_rows_merge_kernel(CacheArgs a) {
 template <int D, typename T>
 int launch_cache_rows(const CacheArgs& a, int grid, cudaStream_t st) {
   constexpr int kBytes = kFewWarps * kFewStages<D> * kFewStage<D>;
-  auto kern = cache_attn_rows_kernel<D, T>;
-  if (set_smem_optin(reinterpret_cast<const void*>(kern), kBytes) != KSH_OK) return KSH_ERR_CUDA;
-  const int rc = launch(kern, dim3(static_cast<unsigned>(grid)), dim3(kFewWarps * 32), kBytes, st, a);
+  auto go = [&](auto kern) -> int {
+    if (set_smem_optin(reinterpret_cast<const void*>(kern), kBytes) != KSH_OK) return KSH_ERR_CUDA;
+    return launch(kern, dim3(static_cast<unsigned>(grid)), dim3(kFewWarps * 32), kBytes, st, a);
+  };
+  const int rc = static_cast<int64_t>(a.max_q) * a.g <= 8 ? go(cache_attn_rows_kernel<D, T, 1>) : go(cache_attn_rows_kernel<D, T, 2>);
   if (rc != KSH_OK) return rc;
-  return launch(cache_rows_merge_kernel<D>, dim3(static_cast<unsigned>(grid * kFewWarps - 1)), dim3(D), 0, st, a);
+  return launch(cache_rows_merge_kernel<D>, dim3(static_cast<unsigned>(grid * kFewWarps - 1)), dim3(kJoinThreads), 0, st, a);
 }
 
 static_assert(few_floats<64>() * kFewWarps == part_floats<64>() && few_floats<128>() * kFewWarps == part_floats<128>(), "workspace");
