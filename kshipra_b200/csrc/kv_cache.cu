@@ -309,6 +309,10 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
     if (lane == 0) {
       a.new_lens[i] = ln;
       if (p >= 0) atomicMin(first + p, i);
+      const int r = ln - full * bs;
+      if (p >= 0 && full >= M) raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
+      rest[i] = p < 0 || full >= M ? -1 : r;           // filled rows of the page that the next token goes to
+      dst[i] = p >= 0 && full < M && r > 0 ? a.tables[static_cast<int64_t>(p) * M + full] : -1;
     }
   }
   cluster_sync();
@@ -317,12 +321,10 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
   // its count until the child takes it.
   const int per = (a.n + kPageWarps - 1) / kPageWarps;
   for (int i = gw * per + lane; i < min(a.n, (gw + 1) * per); i += 32) {
-    const int p = parent(i);
-    if (p < 0 || __ldcg(first + p) != i) continue;
-    const int ln = length(p), full = ln / bs;
-    if (full >= M || ln == full * bs) continue;
-    const int page = a.tables[static_cast<int64_t>(p) * M + full];
-    if (page >= 0 && page < a.num_blocks && __ldcg(a.new_ref + page) <= 0) atomicMin(a.new_ref + page, i - a.n);
+    const int p = a.parents[i], page = __ldcg(dst + i);
+    const bool mine = __ldcg(rest + i) > 0 && __ldcg(first + p) == i, there = page >= 0 && page < a.num_blocks;
+    if (mine && there && __ldcg(a.new_ref + page) <= 0) atomicMin(a.new_ref + page, i - a.n);
+    src[i] = mine;
   }
   cluster_sync();
   // the page that the next token goes to: kept, or fresh; fresh ones are numbered in
@@ -331,30 +333,23 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
   for (int i = gw * per + lane; i - lane < min(a.n, (gw + 1) * per); i += 32) {
     bool fresh = false;
     if (i < min(a.n, (gw + 1) * per)) {
-      const int p = parent(i);
-      int state = -1;                                  // no page wanted
-      if (p >= 0) {
-        const int ln = length(p), full = ln / bs, r = ln - full * bs;
-        if (full >= M) {
-          raise_flag(a.flags, KSH_FLAG_BAD_LENGTH);
+      int state = __ldcg(rest + i);                    // -1: no page wanted, -2: settled
+      if (state < 0) {
+        a.slots[i] = -1;
+      } else {
+        const int page = __ldcg(dst + i);
+        const bool mine = __ldcg(src + i) != 0, there = page >= 0 && page < a.num_blocks;
+        const bool keep = mine && there && __ldcg(a.new_ref + page) == i - a.n;
+        fresh = !(mine && !there) && !keep;
+        if (fresh) {
+          a.slots[i] = there ? page : -1;              // what is copied, for now
         } else {
-          const bool mine = r > 0 && __ldcg(first + p) == i;
-          const int page = mine ? a.tables[static_cast<int64_t>(p) * M + full] : 0;
-          if (page < 0 || page >= a.num_blocks) {
-            a.new_tables[static_cast<int64_t>(i) * M + full] = page;
-          } else if (mine && __ldcg(a.new_ref + page) == i - a.n) {
-            a.new_tables[static_cast<int64_t>(i) * M + full] = page;
-            a.new_ref[page] = 1;
-            a.slots[i] = static_cast<int64_t>(page) * bs + r;
-            state = -2;                                // settled
-          } else {
-            fresh = true;
-            state = r;
-          }
+          a.new_tables[static_cast<int64_t>(i) * M + __ldcg(a.new_lens + i) / bs] = page;
+          if (keep) a.new_ref[page] = 1;
+          a.slots[i] = keep ? static_cast<int64_t>(page) * bs + state : -1;
+          rest[i] = keep ? -2 : -1;
         }
       }
-      rest[i] = state;
-      if (state == -1) a.slots[i] = -1;
     }
     count += __popc(__ballot_sync(0xffffffffu, fresh));
   }
@@ -381,7 +376,7 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
   }
   cluster_sync();
   for (int i = gw * per + lane; i - lane < min(a.n, (gw + 1) * per); i += 32) {
-    const bool here = i < min(a.n, (gw + 1) * per), fresh = here && rest[i] >= 0;
+    const bool here = i < min(a.n, (gw + 1) * per), fresh = here && __ldcg(rest + i) >= 0;
     const uint32_t who = __ballot_sync(0xffffffffu, fresh);
     const int k = rank_of + __popc(who & ((1u << lane) - 1));
     if (here) dst[i] = fresh && k < have ? __ldcg(src + k) : -1;
@@ -389,21 +384,16 @@ __global__ void __cluster_dims__(kPageCtas, 1, 1) __launch_bounds__(kPageThreads
   }
   cluster_sync();
   for (int i = gw * per + lane; i < min(a.n, (gw + 1) * per); i += 32) {
-    const int r = rest[i], page = dst[i];
-    src[i] = -1;
+    const int r = __ldcg(rest + i), page = __ldcg(dst + i), from = static_cast<int>(__ldcg(a.slots + i));
+    src[i] = r >= 0 && page >= 0 ? from : -1;
     if (r < 0) continue;
     if (page < 0) {
       raise_flag(a.flags, KSH_FLAG_NO_PAGE);
       a.slots[i] = -1;
       continue;
     }
-    const int p = a.parents[i], full = length(p) / bs;
-    a.new_tables[static_cast<int64_t>(i) * M + full] = page;
+    a.new_tables[static_cast<int64_t>(i) * M + __ldcg(a.new_lens + i) / bs] = page;
     a.slots[i] = static_cast<int64_t>(page) * bs + r;
-    if (r > 0) {
-      const int from = a.tables[static_cast<int64_t>(p) * M + full];
-      if (from >= 0 && from < a.num_blocks) src[i] = from;
-    }
   }
 }
 
