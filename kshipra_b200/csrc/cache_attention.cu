@@ -6,6 +6,10 @@
 //     o = sum_j exp(q.k_j / sqrt(D) - m) v_j / sum_j exp(q.k_j / sqrt(D) - m)
 // with the running maximum m.  q and o are fp32, K and V fp16 or bf16.
 //
+// Three kernels: calls whose sequences bring at most 16 rows (tokens x heads of a group)
+// of head dimension 64 or 128, as decoding does, go to cache_attn_rows_kernel, others of
+// these dimensions to cache_attn_tc_kernel, the rest to cache_attn_any_kernel.
+//
 // Head dimensions 64 and 128 (cache_attn_tc_kernel): K and V go to the tensor cores
 // as they stand in the cache, TMA boxes of pool rows straight into the MMAs'
 // operand layout.  q and P, which are fp32, go in as sums of 16-bit terms of the
@@ -35,14 +39,13 @@
 // tensor cycles, with three 3.07 K, and 64 KB of K and V, 2.3 to 2.9 K cycles of the
 // SM's share of HBM.  Measured (back to back from a graph; in long runs the power limit
 // holds the clock at 1.5 GHz and adds 10 to 15 %):
-//   64 sequences x 4096 keys, one token each, 32 / 8 heads of 128, fp16 (1.08 GB): 210
-//   us, 5.1 TB/s, 79 % of measured HBM; tensor pipe 70 % active.  bf16 265 to 315.
-//   2048 tokens behind 4096, the same heads, fp16: 287 us, 600 TFLOP/s of attention and
-//   twice that of MMAs; tensor pipe 66 % active.
+//   2048 tokens behind 4096, 32 / 8 heads of 128, fp16: 287 us, 600 TFLOP/s of attention
+//   and twice that of MMAs; tensor pipe 66 % active.
 //   3 sequences of up to 31000 keys with chunks of up to 200, bf16: 310 to 335 us.
 //   24 sequences of up to 2000 keys, chunks of up to 301 among single tokens, 14 / 2
-//   heads of 64, bf16: 91 us.  One sequence x 540 keys: 15.4 us, of which the second
-//   launch takes 4.
+//   heads of 64, bf16: 91 us.
+//   (Decoding by this kernel, too: 64 sequences x 4096 keys, 32 / 8 heads of 128, 214 us,
+//   bf16 265 to 315; tensor pipe 70 % active on rows that are mostly not there.)
 // In a tile the longest chain is P V (1.0 K), its sums (1.2 K) and the waits between
 // them (0.3 K each: with MMAs in flight an mbarrier's answer takes that long).  No
 // faster, for the fp16 cases above: the sums in the row warps (10 % slower), sixteen row
@@ -1646,9 +1649,18 @@ int launch_cache_tc(CacheArgs& a, int grid, cudaStream_t st) {
 // rows (q's terms in registers, P's transposed by movmatrix), each step's P V added in
 // fp32.  No warp waits for another.  The line of all items' steps is cut into equal
 // shares, one per warp, and cache_rows_merge_kernel joins the pieces in key order.
+// HBM bound.  us, and by cache_attn_tc_kernel: 64 sequences x 4096 keys, 32 / 8 heads of
+// 128, fp16 (1.08 GB) 172 (214), 97 % of measured HBM, tensor pipe 20 % active; bf16 170
+// (294); 128 / 8 heads 201 (248), four tokens each 199 (233), pages of ten tokens 170
+// (422); 14 / 2 heads of 64 41 (60); 256 sequences x 300 keys 65 (158), 4 x 1000 15 (27),
+// 1 x 30000 47 (49), 1 x 540, 14 / 2 heads of 64, 11.1 (15.4).  With the rows as the first
+// operand (16, half of them not there) 193 and 240: these products are issued at a
+// fraction of the tile kernel's rate.
 
 constexpr int kFewRows = 16, kFewKeys = 16, kFewWarps = 8;
-constexpr int kFewShare = 4;             // steps that a share has at least
+// Steps that a share has at least: with fewer more pieces are joined, with more fewer
+// warps work (1 x 540 keys: 1 24.5 us, 2 16.1, 4 13.5, 8 15.7).
+constexpr int kFewShare = 4;
 template <int D>
 constexpr int kFewStages = 3 * 128 / D;
 template <int D>
