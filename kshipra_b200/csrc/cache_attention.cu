@@ -98,6 +98,16 @@ struct SplitItem {
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+// What the probabilities (at most 1) of keys 0 .. last are scaled down by, and so their
+// sum: the power of two that keeps the sum of their products with values as large as
+// bf16's within fp32's range (fp16's leave 2^112 of room).  It costs no bits, except that
+// products of V below 2^-118 times the number of keys may become subnormal.
+template <typename T>
+__device__ __forceinline__ float head_room(uint32_t last) {
+  if (!std::is_same_v<T, __nv_bfloat16>) return 1.0f;
+  return __uint_as_float((95u + static_cast<uint32_t>(__clz(static_cast<int>(last)))) << 23);   // 2^-ceil(log2(last + 1))
+}
+
 // Any head dimension up to 256 and any alignment: a CTA per (row, head), whose warps
 // take 16 keys at a time each, four of them in flight, and join their states at the
 // end.  VEC: elements a load takes, four where dimension and pool allow; PER: elements a
@@ -151,6 +161,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) cache_attn_any_kernel(CacheArg
     acc[e] = 0.0f;
   }
   float m = -INFINITY, l = 0.0f;
+  float room = head_room<T>(static_cast<uint32_t>(end - 1));
   bool bad = false;
   auto value = [](Raw r, int e) {
     uint16_t b;
@@ -212,6 +223,12 @@ __global__ void __launch_bounds__(kAnyWarps * 32) cache_attn_any_kernel(CacheArg
         top = fmaxf(top, x[u]);
       }
       const float ref = top == -INFINITY ? 0.0f : top;
+      if constexpr (PER == 8 && std::is_same_v<T, __nv_bfloat16>) {
+        // made anew, as there is no register for it (64 x 4096 keys of 256 1157 us, held 1350)
+        uint32_t last = static_cast<uint32_t>(end) - 1;
+        asm volatile("" : "+r"(last));
+        room = head_room<T>(last);
+      }
       if (top > m) {
         const float corr = expf(m - ref);
         m = top;
@@ -221,11 +238,13 @@ __global__ void __launch_bounds__(kAnyWarps * 32) cache_attn_any_kernel(CacheArg
       }
 #pragma unroll
       for (int u = 0; u < kAnyKeys; ++u) {
-        const float p = expf(x[u] - ref);
-        l += p;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = fmaf(p, value(v[u][e / VEC], e), acc[e]);
+        x[u] = expf(x[u] - ref) * room;
+        l += x[u];
       }
+#pragma unroll
+      for (int u = 0; u < kAnyKeys; ++u)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = fmaf(x[u], value(v[u][e / VEC], e), acc[e]);
     }
   }
   if (bad) raise_flag(a.flags, KSH_FLAG_BAD_BLOCK);
@@ -1244,6 +1263,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
       // it follows the maximum once that is 2^8 above it, so most tiles
       // rescale nothing), the half's sum
       float mref = -INFINITY, l = 0.0f;
+      const float room = head_room<T>(static_cast<uint32_t>(pc.keys - 1));      // the same for all pieces of an item
       bool s_there = false;                         // seen a tile ahead
       if (fold) {
         const int part = warp & 3;                   // the keys 32 part on are the pair's
@@ -1286,7 +1306,8 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const float2 e = unpack(fma2(f2(x[j], x[j + 1]), c2, nref));
-            const F2 p = f2(ex2(e.x), ex2(e.y));
+            F2 p = f2(ex2(e.x), ex2(e.y));
+            if (kBf16) p = mul2(p, f2(room, room));
             s2 = add2(s2, p);
             split<T>(p, &pt[j / 2], &pt[j / 2 + 8], &low[j / 2]);
           }
@@ -1367,7 +1388,7 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
           mref = mc;
         }
         // P = 2^(x c - ref): up to 2^14 in fp16 terms, which keeps them above fp16's
-        // smallest; up to 1 in bf16, whose V may be as large as fp32
+        // smallest; up to 1 in bf16, times head_room, as V may be as large as fp32
         const float ref = mref == -INFINITY ? 0.0f : mref + kRefShift;
         const F2 nref = f2(-ref, -ref), c2 = f2(cq, cq);
         F2 s2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
@@ -1378,7 +1399,8 @@ cache_attn_tc_kernel(CacheArgs a, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const float2 e = unpack(fma2(f2(x[j0 + j], x[j0 + j + 1]), c2, nref));
-            const F2 p = f2(ex2(e.x), ex2(e.y));
+            F2 p = f2(ex2(e.x), ex2(e.y));
+            if (kBf16) p = mul2(p, f2(room, room));
             s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], p);
             split<T>(p, &pt[j / 2], &pt[j / 2 + 8], &low[L::LOW ? 8 * group + j / 2 : 0]);
           }
@@ -1850,6 +1872,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
     uint32_t qb[TERMS][KS][NT][2];
     float acc[D / 16][NT][4], m[NT][2], l[NT][2], cq[NT][2];     // (d, rows), by columns: rows 8 n + c0, 8 n + c0 + 1
     int lim[NT][2];
+    float room = 1.0f;
     auto row_at = [&](int R) -> int64_t {
       const int node = R / g;
       return ((w.a0 + node) * a.hq + static_cast<int64_t>(hk) * g + (R - node * g)) * D;
@@ -1860,6 +1883,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
         fresh = false;
         rows = w.nq * g;
         steps = (w.pre + w.nq + kFewKeys - 1) / kFewKeys;
+        room = head_room<T>(static_cast<uint32_t>(w.pre + w.nq - 1));
         t0 = t;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -1978,7 +2002,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) cache_attn_rows_kernel(Cach
       for (int n = 0; n < NT; ++n) {
         const float ra = m[n][0] == -INFINITY ? 0.0f : m[n][0] + kRefShift, rb = m[n][1] == -INFINITY ? 0.0f : m[n][1] + kRefShift;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] = ex2(fmaf(x[n][e], cq[n][e & 1], e & 1 ? -rb : -ra));
+        for (int e = 0; e < 4; ++e) {
+          x[n][e] = ex2(fmaf(x[n][e], cq[n][e & 1], e & 1 ? -rb : -ra));
+          if (Kind<T>::kBf16) x[n][e] *= room;
+        }
         l[n][0] += x[n][0] + x[n][2];
         l[n][1] += x[n][1] + x[n][3];
 #pragma unroll

@@ -1048,3 +1048,30 @@ def test_few_rows_offsets_past_32_bits():
     n = b.pool.shape[0]
     pool[nb - n:] = b.pool
     b.check(kv.cache_attention(b.q, pool, 0, b.table + (nb - n), b.q_start, b.prefix, 2, 301), b.want())
+
+
+# (the tile kernel with whole and with folded row tiles, the few-row kernel, the general kernel)
+LARGEST = [(64, 8, 2, [(600, 40), (3000, 1), (0, 1)]), (128, 4, 4, [(5, 130), (2000, 20)]), (64, 4, 2, [(3000, 1), (40, 1)]),
+           (128, 32, 8, [(700, 3), (9000, 1)]), (96, 4, 2, [(1500, 2), (0, 7)]), (33, 2, 1, [(900, 1)])]
+
+
+@pytest.mark.parametrize("scores", ["equal", "rising", "any"])
+@pytest.mark.parametrize("d,heads,kv_heads,seqs", LARGEST)
+def test_attention_bf16_means_of_the_largest_values(d, heads, kv_heads, seqs, scores):
+    """A mean of values is no larger than they are, however many keys add up to it:
+    thousands of keys whose V is bf16's largest, with scores that are all the same,
+    that rise by less than what the running reference follows (7.9 powers of two behind
+    the first 128 keys), or random ones with signs of V that differ."""
+    b = Batch(seqs, heads, kv_heads, d, 16, BF16)
+    top = torch.finfo(BF16).max
+    if scores == "any":
+        b.pool[:, :, 1] = torch.where(b.pool[:, :, 1] > -1.0, top, -top)
+    else:
+        b.pool[:, :, 1] = top
+        b.pool[:, :, 0] = 0.0
+        b.q.zero_()
+    if scores == "rising":
+        b.pool[:, :, 0, :, :, 0] = 1.0
+        b.pool[b.table[:, :8].long().reshape(-1), :, 0, :, :, 0] = 0.0      # (a page is one sequence's; spare entries name page 0)
+        b.q[:, :, 0] = 7.9 * np.log(2.0) * d ** 0.5
+    b.check(b.run())
