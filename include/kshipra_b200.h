@@ -459,7 +459,9 @@ int ksh_rope_cache_write(const float* qkv, int64_t m, int64_t hq, int64_t hkv, i
  * a sequence's rows (a longer one raises KSH_FLAG_BAD_LENGTH and its rows past the
  * bound are not written), max_total_len, of a sequence's positions, only sizes the
  * launch.  A sequence that does not fit its table raises KSH_FLAG_BAD_LENGTH; its
- * rows are not specified.  d <= 256.
+ * rows are not specified.  d <= 256; calls that the tensor cores do not take (d other than 64 and 128,
+ * more than 128 heads a group, tensors that are not 16-byte aligned, pools of 2^31 rows) have up to
+ * 65535 heads and 65535 sequences (KSH_ERR_UNSUPPORTED).
  * The workspace, of ksh_cache_attention_workspace_size bytes and 256-byte
  * aligned, needs no initialisation. */
 int64_t ksh_cache_attention_workspace_size(int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d,

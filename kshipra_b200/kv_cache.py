@@ -33,6 +33,7 @@ from ._lib import ptr, stream_ptr
 from .speculative import _flags, _need, _raw_stream, _run, _wrong_device
 
 POOL_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_SEQS = 65535             # sequences of one call of ksh_cache_attention's general kernel
 
 
 def _pool(t: torch.Tensor, types, dev: Optional[int] = None) -> int:
@@ -161,11 +162,17 @@ def cache_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_table
     elif _need(out, "out", torch.float32, 3, at).shape != q.shape:
         raise ValueError("out must have q's shape")
     dev = q.device
+    step = S
+    if S > MAX_SEQS and not (d in (64, 128) and hq // hkv <= 128 and pool.numel() // d < 1 << 31
+                             and (q.data_ptr() | pool.data_ptr() | out.data_ptr()) % 16 == 0):
+        step = MAX_SEQS                      # a call of the general kernel: runs of sequences
     with ws.lock:
         buf = ws.get(_workspace_bytes(S, hq, hkv, d, max_q_len), dev)
-        _run(dev, "ksh_cache_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), kind, nb, L, layer,
-             hkv, bs, block_tables.data_ptr(), max_blocks, q_start.data_ptr(), prefix_lens.data_ptr(),
-             S, max_q_len, max_total_len, out.data_ptr(), buf.data_ptr(), buf.numel(), _flags(flags, at))
+        for s in range(0, max(S, 1), max(step, 1)):
+            _run(dev, "ksh_cache_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), kind, nb, L, layer,
+                 hkv, bs, block_tables.data_ptr() + 4 * s * max_blocks, max_blocks, q_start.data_ptr() + 4 * s,
+                 prefix_lens.data_ptr() + 4 * s, min(step, S - s), max_q_len, max_total_len, out.data_ptr(),
+                 buf.data_ptr(), buf.numel(), _flags(flags, at))
     return out
 
 

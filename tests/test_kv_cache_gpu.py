@@ -1075,3 +1075,45 @@ def test_attention_bf16_means_of_the_largest_values(d, heads, kv_heads, seqs, sc
         b.pool[b.table[:, :8].long().reshape(-1), :, 0, :, :, 0] = 0.0      # (a page is one sequence's; spare entries name page 0)
         b.q[:, :, 0] = 7.9 * np.log(2.0) * d ** 0.5
     b.check(b.run())
+
+
+@pytest.mark.parametrize("d,group", [(80, 1), (64, 129)])
+def test_attention_more_sequences_than_one_general_call(d, group):
+    """The general kernel's calls are split into runs of sequences: 70000 of them, over a
+    few pages that they share, some empty, some of three rows, rows of no sequence before them."""
+    S, bs = 70000, 16
+    rs = np.random.RandomState(0)
+    new = rs.choice([0, 1, 1, 1, 3], S)
+    pre = rs.randint(0, 20, S)
+    qs = 5 + np.concatenate([[0], np.cumsum(new)])
+    table = rs.randint(0, 6, (S, 2))
+    g = torch.Generator(device="cuda").manual_seed(0)
+    pool = torch.randn(6, 1, 2, 1, bs, d, generator=g, device="cuda").half()
+    q = torch.randn(int(qs[-1]) + 2, group, d, generator=g, device="cuda")
+    out = torch.full_like(q, 7.0)
+    f = new_flags()
+    kv.cache_attention(q, pool, 0, i32(table), i32(qs), i32(pre), 3, 32, out=out, flags=f)
+    assert int(f) == 0 and (out[:5] == 7).all() and (out[int(qs[-1]):] == 7).all()
+    seq = np.repeat(np.arange(S), new)
+    last = i64(pre[seq] + np.arange(len(seq)) - (qs[:-1][seq] - 5))
+    rows = pool[i64(table)[i64(seq)], 0, :, 0].double()                        # [rows, 2 pages, K / V, bs, d]
+    top = float(pool[:, :, 1].abs().max())
+    for a in range(0, len(seq), 4096):
+        k, v = (rows[a:a + 4096, :, i].reshape(-1, 2 * bs, d) for i in (0, 1))
+        x = torch.einsum("nhd,nkd->nhk", q[5 + a:5 + a + k.shape[0]].double(), k) / d ** 0.5
+        hide = torch.arange(2 * bs, device="cuda") > last[a:a + 4096, None]
+        want = torch.einsum("nhk,nkd->nhd", torch.softmax(x.masked_fill(hide[:, None], -torch.inf), -1), v)
+        diff = out[5 + a:5 + a + k.shape[0]].double() - want
+        assert float(diff.norm()) <= 1e-5 * float(want.norm()) and float(diff.abs().max()) <= 8e-5 * top
+
+
+def test_attention_sequence_runs_report_bad_lengths():
+    S = 65540
+    pool = torch.zeros(1, 1, 2, 1, 4, 80, dtype=F16, device="cuda")
+    q = torch.ones(S, 1, 80, device="cuda")
+    for bad in (3, S - 1):
+        pre = np.zeros(S)
+        pre[bad] = 9                                          # past the table's one page
+        f = new_flags()
+        kv.cache_attention(q, pool, 0, i32(np.zeros((S, 1))), i32(np.arange(S + 1)), i32(pre), 1, 4, flags=f)
+        assert int(f) == BAD_LENGTH
