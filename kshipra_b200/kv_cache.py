@@ -79,13 +79,14 @@ _WS = CacheWorkspace()
 
 
 @functools.lru_cache(maxsize=None)
-def _workspace_bytes(seqs: int, hq: int, hkv: int, d: int, max_q_len: int) -> int:
-    return int(_lib.lib().ksh_cache_attention_workspace_size(seqs, hq, hkv, d, max_q_len))
+def _workspace_bytes(d: int) -> int:
+    """Of any call with this head dimension: the size depends on nothing else."""
+    return int(_lib.lib().ksh_cache_attention_workspace_size(1, 1, 1, d, 1))
 
 
 @functools.lru_cache(maxsize=None)
 def _largest_workspace() -> int:
-    return max(_workspace_bytes(1, 1, 1, d, 1) for d in (64, 128))
+    return max(_workspace_bytes(d) for d in (64, 128))
 
 
 def rope_cache_write(qkv: torch.Tensor, pool: torch.Tensor, layer: int, positions: torch.Tensor,
@@ -167,7 +168,7 @@ def cache_attention(q: torch.Tensor, pool: torch.Tensor, layer: int, block_table
                              and (q.data_ptr() | pool.data_ptr() | out.data_ptr()) % 16 == 0):
         step = MAX_SEQS                      # a call of the general kernel: runs of sequences
     with ws.lock:
-        buf = ws.get(_workspace_bytes(S, hq, hkv, d, max_q_len), dev)
+        buf = ws.get(_workspace_bytes(d), dev)
         for s in range(0, max(S, 1), max(step, 1)):
             _run(dev, "ksh_cache_attention", q.data_ptr(), T, hq, d, pool.data_ptr(), kind, nb, L, layer,
                  hkv, bs, block_tables.data_ptr() + 4 * s * max_blocks, max_blocks, q_start.data_ptr() + 4 * s,

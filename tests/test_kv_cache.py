@@ -163,3 +163,9 @@ def test_compaction_of_empty_and_full_pools():
     cache.allocator.free(taken[2])
     to = cache.compact()
     assert to[4] == taken[2] if taken[2] != 4 else to == list(range(5))
+
+
+def test_attention_workspace_size_depends_on_the_dimension_alone():
+    size = _lib.lib().ksh_cache_attention_workspace_size
+    for d in (64, 96, 128, 256):
+        assert {size(s, h, k, d, n) for s in (1, 7, 70000) for h, k in ((1, 1), (32, 8), (256, 1)) for n in (0, 1, 5000)} == {size(1, 1, 1, d, 1)}

@@ -1117,3 +1117,14 @@ def test_attention_sequence_runs_report_bad_lengths():
         f = new_flags()
         kv.cache_attention(q, pool, 0, i32(np.zeros((S, 1))), i32(np.arange(S + 1)), i32(pre), 1, 4, flags=f)
         assert int(f) == BAD_LENGTH
+
+
+def test_attention_keeps_nothing_for_each_batch():
+    """A server's calls differ in sequences and chunk lengths: the host's tables do not grow with them."""
+    for d in (64, 96):
+        seen = []
+        for n in range(1, 9):
+            b = Batch([(10 + n, n)] * n, 4, 2, d, 16, F16)
+            b.run()
+            seen.append(kv._workspace_bytes.cache_info().currsize)
+        assert seen[-1] == seen[0]
