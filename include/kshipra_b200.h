@@ -484,7 +484,9 @@ int ksh_cache_attention(const float* q, int64_t total, int64_t hq, int64_t d, co
  * (of all tables, these or others) that hold it; new_ref is what it is after the
  * S sequences have given up theirs and the children hold theirs.  Free pages
  * (count 0 then) are taken from the lowest number up in the children's order.
- * Without one left a child's slot is -1 and KSH_FLAG_NO_PAGE is raised.
+ * Without one left a child's slot is -1 and KSH_FLAG_NO_PAGE is raised; its row
+ * (like any whose slot is -1) holds its whole pages alone: go on with lens /
+ * block_size * block_size of it, since a later call gives up the pages of `lens`.
  * KSH_FLAG_BAD_LENGTH: a length that does not fit its row (slot -1 where the
  * next token has no place), KSH_FLAG_BAD_PARENT: a parent past S,
  * KSH_FLAG_BAD_BLOCK: a page outside the pool, or held more often than counted.

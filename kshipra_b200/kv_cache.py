@@ -193,7 +193,9 @@ def fork_pages(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
     theirs.  With parents 0 .. S - 1 the call only grows the sequences, with
     negative ones it frees them.  Returns (block_tables [N, max_blocks], lens [N],
     slots int64 [N] of the next tokens, ref_counts [nb]); without a page left a slot is
-    -1 and KSH_FLAG_NO_PAGE (512) raised."""
+    -1 and KSH_FLAG_NO_PAGE (512) raised.  A row whose slot is -1 takes no token and
+    holds its whole pages alone: pass lens // B * B of it to the next call, which gives
+    up the pages that its lens name."""
     kind = _pool(pool, (0, 1, 2))
     at = pool.get_device()
     nb, L, _, hkv, bs, d = pool.shape

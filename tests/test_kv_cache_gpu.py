@@ -1128,3 +1128,34 @@ def test_attention_keeps_nothing_for_each_batch():
             b.run()
             seen.append(kv._workspace_bytes.cache_info().currsize)
         assert seen[-1] == seen[0]
+
+
+@pytest.mark.parametrize("lens", [[20, 20], [16, 32], [20, 32]])
+def test_fork_goes_on_after_it_ran_out_of_pages(lens):
+    """Children without a page go on with their whole pages: counts stay those of the
+    rows, in a call that continues some of them and in one that frees them all."""
+    pool, table, _, refs = fork_case(lens, 4, 16, sum(-(-n // 16) for n in lens) + 2, shared=False)
+    outside = refs.clone()
+    for row, ln in zip(table.tolist(), lens):
+        for page in row[:-(-ln // 16)]:
+            outside[page] -= 1
+    f = new_flags()
+
+    def cut(t, n, s, r, written):
+        """The lengths that go into the next call; the counts are those of the rows and the pages for their next tokens."""
+        n = torch.where(s < 0, n // 16 * 16, n + written)
+        want = outside.clone()
+        for row, ln, slot in zip(t.tolist(), n.tolist(), s.tolist()):
+            for page in {*row[:-(-ln // 16)], *([slot // 16] if slot >= 0 else [])}:
+                want[page] += 1
+        assert r.tolist() == want.tolist()
+        return n
+
+    t, n, s, r = kv.fork_pages(pool, table, i32(lens), i32([0, 0, 0, 1, 1]), refs, flags=f)
+    assert int(f) == NO_PAGE and (s < 0).any() and (s >= 0).any()
+    n = cut(t, n, s, r, 1)
+    f.zero_()
+    t, n, s, r = kv.fork_pages(pool, t, n, i32([int((s < 0).nonzero()[0]), int((s >= 0).nonzero()[0])]), r, flags=f)
+    assert int(f) == 0 and (s >= 0).all()
+    n = cut(t, n, s, r, 1)
+    assert torch.equal(kv.fork_pages(pool, t, n, i32([]), r, flags=f)[3], outside) and int(f) == 0
