@@ -8,6 +8,9 @@ model's best two logits are further apart than 2e-3 of the largest (twice
 the bound); at closer calls a stream may take either and is left there.
 """
 
+import threading
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -303,3 +306,112 @@ def test_refusals():
     bad["model.layers.0.self_attn.q_norm.weight"] = torch.ones(7)
     with pytest.raises(ValueError):
         KshipraModel(config=cfg, state_dict=bad)
+
+
+def test_beam_search_ends_early_among_several_prompts():
+    """An ended beam competes with itself alone: against the plain search wherever no
+    choice of it is close, and at least one such search has a beam that ends early."""
+    cfg = TINY_LLAMA
+    sd = synthetic_state_dict(cfg, seed=4)
+    sd = {k: v * (6.0 if k == "lm_head.weight" else 1.0) for k, v in sd.items()}
+    km = KshipraModel(config=cfg, state_dict=sd, kv_dtype=F16)
+    plain = Plain(cfg, sd, F16)
+    beams = BeamDecoder(km, beams=3, block_size=4)
+    compared = 0
+    for n in (5, 12, 21, 30, 37, 44):
+        prompt = prompt_of(n, cfg.vocab, n)
+        eos = beams.generate([prompt], 5)[0][0][0][1]         # the best beam's second token ends it now
+        got = beams.generate([prompt], 5, eos_token_id=eos)[0]
+        want, clear = plain_beams(plain, prompt, 3, 5, eos)
+        if clear:
+            assert [t for t, _ in got] == [t for t, _, _ in want]
+            compared += any(len(t) < 5 and t[-1] == eos for t, _ in got)
+    assert compared > 0
+
+
+class Ranks:
+    """Ranks as threads that issue their kernels to one stream in turn: what a
+    collective takes from the others is there once all have come to it on the host."""
+
+    def __init__(self, n):
+        self.n, self.meet, self.parts, self.me = n, threading.Barrier(n, timeout=60), [None] * n, threading.local()
+
+    def run(self, fn):
+        def rank(r):
+            self.me.rank = r
+            try:
+                return fn(r)
+            except BaseException:
+                self.meet.abort()
+                raise
+        with ThreadPoolExecutor(self.n) as ex:
+            return [f.result() for f in [ex.submit(rank, r) for r in range(self.n)]]
+
+    def gather(self, t):
+        self.parts[self.me.rank] = t.clone()
+        self.meet.wait()
+        parts = list(self.parts)
+        self.meet.wait()
+        return parts
+
+    def all_reduce(self, t, group=None):
+        t.copy_(torch.stack(self.gather(t)).sum(0))
+
+    def all_gather_into_tensor(self, out, t, group=None):
+        out.copy_(torch.stack(self.gather(t)))
+
+
+@pytest.mark.parametrize("cfg,dtype,norm", [(TINY_LLAMA, F16, False), (TINY_LLAMA, BF16, True), (TINY_LLAMA, F32, True), (WIDE, F16, True)],
+                         ids=lambda x: getattr(x, "name", str(x)))
+def test_tensor_parallel_shards(cfg, dtype, norm, monkeypatch):
+    """Shards over pools of each type, with norms of queries and keys: chunks and a
+    single token give the whole model's logits."""
+    monkeypatch.setenv("KSH_PEER_AR", "0")
+    sd = synthetic_state_dict(cfg, seed=3)
+    sd = normed(cfg, sd) if norm else sd
+    ranks = Ranks(2)
+    monkeypatch.setattr(torch.distributed, "all_reduce", ranks.all_reduce)
+    monkeypatch.setattr(torch.distributed, "all_gather_into_tensor", ranks.all_gather_into_tensor)
+    prompt = prompt_of(40, cfg.vocab, 1)
+
+    def rank(r):
+        km = KshipraModel(config=cfg, state_dict=sd, kv_dtype=dtype, tp=(r, 2, None))
+        pool = km.new_pool(5, 8).pool
+        assert pool.dtype == dtype and pool.shape[3] == cfg.kv_heads // 2
+        rows, at = [], 0
+        for n in (21, 18, 1):
+            rows.append(km.forward(torch.tensor([prompt[at:at + n]]), torch.arange(at, at + n)[None], pool, [3, 0, 4, 1, 2],
+                                   [[3, 0, 4, 1, 2][i // 8] * 8 + i % 8 for i in range(at, at + n)], at)[0])
+            at += n
+        return torch.cat(rows)
+
+    got = ranks.run(rank)
+    want = Plain(cfg, sd, dtype).logits(prompt)
+    for x in got:
+        assert float((x.double() - want).abs().max()) <= RTOL * float(want.abs().max())
+    assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["fp16", "bf16", "fp32"])
+def test_prefix_cache_compacts_on_the_gpu_as_on_the_host(dtype):
+    caches = [PrefixCache(num_blocks=50, block_size=4, num_layers=2, num_kv_heads=2, head_dim=64, dtype=dtype, device=torch.device(dev))
+              for dev in ("cuda", "cpu")]
+    rs = np.random.RandomState(0)
+    data = torch.randn(caches[0].allocator.pool.shape, generator=torch.Generator().manual_seed(0)).to(dtype)
+    drop = [int(b) for b in rs.permutation(30)[:17]]
+    for c in caches:
+        c.allocator.pool.copy_(data)
+        held = c.allocate_blocks(30)
+        c.node = c.tree.insert(list(range(12)), [b for b in held if held.index(b) not in drop][:3], 0, c.tree.root)
+        for i in drop:
+            c.allocator.free(held[i])
+        c.before = set(held) - {held[i] for i in drop}
+        c.blocks = list(c.node.block_ids)
+        c.to = c.compact()
+    gpu, cpu = caches
+    assert gpu.to == cpu.to and gpu.to != list(range(50)) and gpu.allocator.free_blocks == cpu.allocator.free_blocks
+    for c in caches:
+        assert sorted(c.to[b] for b in c.before) == list(range(13))
+        assert c.node.block_ids == [c.to[b] for b in c.blocks]
+        for b in c.before:
+            assert torch.equal(c.allocator.pool[c.to[b]].cpu(), data[b])
