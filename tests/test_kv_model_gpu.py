@@ -415,3 +415,16 @@ def test_prefix_cache_compacts_on_the_gpu_as_on_the_host(dtype):
         assert c.node.block_ids == [c.to[b] for b in c.blocks]
         for b in c.before:
             assert torch.equal(c.allocator.pool[c.to[b]].cpu(), data[b])
+
+
+def test_drafted_trees_in_a_model_with_norms():
+    """Trees over an fp32 pool with norms of queries and keys: the model's greedy streams."""
+    cfg = TINY_LLAMA
+    sd = normed(cfg, synthetic_state_dict(cfg, seed=6))
+    km = KshipraModel(config=cfg, state_dict=sd)
+    plain = Plain(cfg, sd, F32)
+    a = prompt_of(11, cfg.vocab, 3)
+    prompts = [a * 4, a, prompt_of(33, cfg.vocab, 4)]
+    for p, toks in zip(prompts, SpeculativeDecoder(km).generate(prompts, 12)):
+        assert len(toks) == 12
+        same_stream(plain, p, toks)
