@@ -457,7 +457,7 @@ int ksh_rope_cache_write(const float* qkv, int64_t m, int64_t hq, int64_t hkv, i
  * element in general NaN.  Rows of q that no sequence covers are not written; a
  * row whose pages are all missing gives zeros.  max_q_len is a host-side upper bound of
  * a sequence's rows (a longer one raises KSH_FLAG_BAD_LENGTH and its rows past the
- * bound are not written), max_total_len, of a sequence's positions, only sizes the
+ * bound are not written; with max_q_len 0 nothing runs), max_total_len, of a sequence's positions, only sizes the
  * launch.  A sequence that does not fit its table raises KSH_FLAG_BAD_LENGTH; its
  * rows are not specified.  d <= 256; calls that the tensor cores do not take (d other than 64 and 128,
  * more than 128 heads a group, tensors that are not 16-byte aligned, pools of 2^31 rows) have up to

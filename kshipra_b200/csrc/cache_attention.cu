@@ -41,9 +41,15 @@
 // holds the clock at 1.5 GHz and adds 10 to 15 %):
 //   2048 tokens behind 4096, 32 / 8 heads of 128, fp16: 287 us, 600 TFLOP/s of attention
 //   and twice that of MMAs; tensor pipe 66 % active.
-//   3 sequences of up to 31000 keys with chunks of up to 200, bf16: 310 to 335 us.
+//   3 sequences of up to 31000 keys with chunks of up to 200, bf16: 300 to 345 us; 19 % of
+//   the tiles are of two sequences' single tokens, four rows of 128 in each.
 //   24 sequences of up to 2000 keys, chunks of up to 301 among single tokens, 14 / 2
-//   heads of 64, bf16: 91 us.
+//   heads of 64, bf16: 91 to 117 us, of which its tiles' and items' cycles (33 tiles and
+//   2.8 items an SM) explain 51 to 67.
+//   A chunk of 2048 beside 63 single tokens behind 4096, 32 / 8 heads of 128, fp16: 400 to
+//   440 us.
+//   All eight of these kernels spill, not in the MMA warps' loops (fp16 52 to 72 bytes
+//   stored, bf16 72 at D = 128 and 88 to 96 at D = 64).
 //   (Decoding by this kernel, too: 64 sequences x 4096 keys, 32 / 8 heads of 128, 214 us,
 //   bf16 265 to 315; tensor pipe 70 % active on rows that are mostly not there.)
 // In a tile the longest chain is P V (1.0 K), its sums (1.2 K) and the waits between
@@ -113,9 +119,12 @@ __device__ __forceinline__ float head_room(uint32_t last) {
 // end.  VEC: elements a load takes, four where dimension and pool allow; PER: elements a
 // lane has.  Bound by instructions and, with few rows, by a warp's trips to memory.  16 /
 // 4 heads, fp16: one sequence x 540 keys 23 us with D = 96, 32 with D = 256 (a warp for
-// all keys, one after the other: 525); 64 x 4096 keys 540 and 1180 (7000 and 7750), four
-// sequences' chunks of 128 behind 1000 655 and 1070.  With two elements a load 25, 57,
-// 510 and 3380, 740 and 2650; a group's heads side by side in the grid save nothing.
+// all keys, one after the other: 525); 64 x 4096 keys 540 and 1180 (7000 and 7750; bf16 440
+// and 1157), four sequences' chunks of 128 behind 1000 655 and 1070.  With two elements a
+// load 25, 57, 510 and 3380, 740 and 2650; a group's heads side by side in the grid save
+// nothing.  It is no kernel for long chunks, whose rows each read all of K and V: 2048
+// tokens behind 4096, 32 / 8 heads, 23 to 25 ms at D = 96 and 43 to 46 at 256 (0.28 by the
+// tiles at D = 128).
 constexpr int kAnyWarps = 8, kAnyRun = 16, kAnyKeys = 4, kAnyMax = 256;
 
 template <typename T, int VEC, int PER>
@@ -289,8 +298,13 @@ constexpr int kThreads = 32 * (kCopyWarp + 2);
 constexpr int kRowRegs = 120, kSumRegs = 192, kRegs = 80;
 // An item's start (its Q, an empty pipeline) takes about four tiles' time; counted so
 // in the line, the CTAs with more items are not the last ones.  24 sequences of
-// chunks and single tokens: 91 us, 160 with 128 keys, 122 with 1024.  Where there are
-// few tiles a CTA it would only put more tiles into some of them.
+// chunks and single tokens, D = 64, bf16: 91 us, 160 with 128 keys, 122 with 1024; counted
+// and not, D = 128, fp16: a chunk of 2048 beside 63 single tokens behind 4096 400 to 440 us
+// and 1010, one of 256 beside seven behind 8000 84 to 102 and 352.  It is left out of calls
+// with fewer than four tiles an SM, by the host's bound (sequences x longest chunk x longest
+// context, which a padded or captured call exceeds); measured there it would gain, too:
+// 4 x 1000 keys with chunks of 30 16.4 us (left out 20.3), 4000 keys with a chunk of 20 22
+// (27.6), eight chunks of 128 30 (57.7).
 constexpr int kItemCost = 512;
 constexpr int kMeta = 16;                // tiles whose notes are kept: more than the stages let run apart
 // Tiles (pieces) that the row warps can be ahead of the sum warps, and more
@@ -1671,11 +1685,15 @@ int launch_cache_tc(CacheArgs& a, int grid, cudaStream_t st) {
 // rows (q's terms in registers, P's transposed by movmatrix), each step's P V added in
 // fp32.  No warp waits for another.  The line of all items' steps is cut into equal
 // shares, one per warp, and cache_rows_merge_kernel joins the pieces in key order.
-// HBM bound.  us, and by cache_attn_tc_kernel: 64 sequences x 4096 keys, 32 / 8 heads of
-// 128, fp16 (1.08 GB) 172 (214), 97 % of measured HBM, tensor pipe 20 % active; bf16 170
-// (294); 128 / 8 heads 201 (248), four tokens each 199 (233), pages of ten tokens 170
-// (422); 14 / 2 heads of 64 41 (60); 256 sequences x 300 keys 65 (158), 4 x 1000 15 (27),
-// 1 x 30000 47 (49), 1 x 540, 14 / 2 heads of 64, 11.1 (15.4).  With the rows as the first
+// HBM bound where many sequences of 128 decode.  us, and by cache_attn_tc_kernel: 64
+// sequences x 4096 keys, 32 / 8 heads of 128, fp16 (1.08 GB) 172 (214), 97 % of measured HBM,
+// tensor pipe 20 % active; bf16 170 (294); 128 / 8 heads 201 (248), four tokens each 199 (233;
+// bf16 247), pages of ten tokens 170 (422); 256 sequences x 300 keys 65 (158), 4 x 1000 15 (27).
+// Not HBM bound: 64 x 4096, 14 / 2 heads of 64 (134 MB, 21 us of HBM) 38 to 40 (60): a step
+// is 4 KB, and its table entries are there one step ahead only; 1 x 30000, 32 / 8 heads of
+// 128 (123 MB, 19 us) 44 to 47 (49): some 149 pieces of each kv head are joined by one CTA;
+// 1 x 540, 14 / 2 heads of 64, 11.1 (15.4): start and two launches.  The kernel of bf16 at D =
+// 128 with 9 to 16 rows spills 134 bytes, the others nothing.  With the rows as the first
 // operand (16, half of them not there) 193 and 240: these products are issued at a
 // fraction of the tile kernel's rate.
 
@@ -2283,6 +2301,7 @@ extern "C" int ksh_cache_attention(const float* q, int64_t total, int64_t hq, in
       return d == 64 ? launch_cache_tc<64, __half>(a, grid, st) : launch_cache_tc<128, __half>(a, grid, st);
     return d == 64 ? launch_cache_tc<64, __nv_bfloat16>(a, grid, st) : launch_cache_tc<128, __nv_bfloat16>(a, grid, st);
   }
+  // (the grid numbers heads in 16 bits; the limit on sequences is the entry's, stated in its header)
   if (hq > 65535 || num_seqs > 65535) return KSH_ERR_UNSUPPORTED;
   return pool_type == KSH_TYPE_F16 ? launch_cache_any<__half>(a, st) : launch_cache_any<__nv_bfloat16>(a, st);
 }

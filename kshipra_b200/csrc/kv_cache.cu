@@ -65,10 +65,13 @@ constexpr int kWriteThreads = 128;
 
 // D / 8 threads for each head of a token, four of the first half's elements
 // and the four that they rotate with each; a norm's sum by shuffles among them.
-// HBM bound.  2048 rows, 32 / 8 heads of 128, bf16, norms (93 MB): 21.5 us, 67 % of
-// measured HBM, with other inputs in each call; with 256 threads a CTA 23.4, 512 28; two or four
-// heads a thread, which share the angles' loads, 21 (at 256 threads 23 and 26); stores
-// past L2 would save 1 us here and cost the attention, which reads q next.
+// 2048 rows, 32 / 8 heads of 128, bf16, norms (93 MB, 14.5 us of HBM): 21.5 us with other
+// inputs in each call, 18.5 replayed over eight sets of them, 16.5 over one that stays in
+// L2, so HBM is not what bounds it: a thread makes three trips to memory one after the
+// other, for its elements, for the position and its angles, for the slot.  With 256 threads a
+// CTA 23.4, 512 28; two or four heads a thread, which share the angles' loads, 21 (at 256
+// threads 23 and 26); stores past L2 would save 1 us here and cost the attention, which
+// reads q next.
 template <int D, typename T>
 __global__ void __launch_bounds__(kWriteThreads) rope_write_kernel(WriteArgs a) {
   constexpr int TPH = D / 8, HALF = D / 2;

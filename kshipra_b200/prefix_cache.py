@@ -209,7 +209,9 @@ class PrefixCache:
 
     def compact(self) -> List[int]:
         """Moves the blocks in use to the front of the pool, in every layer, and
-        the free ones behind them (the lowest is allocated first).
+        the free ones behind them (the lowest is allocated first): what is
+        allocated next lies in runs, which a swap copies at once, and the pool can
+        be saved or cut to the blocks in use.
 
         Returns each block's new id (its own where it did not move).  The tree's
         nodes are renumbered here; block tables that a caller holds are its own
